@@ -35,6 +35,7 @@ def require(t: torch.Tensor, name: str, device: torch.device,
 
 
 def require_optional(t: Optional[torch.Tensor], name: str, device: torch.device,
-                     shape: Optional[Sequence[int]] = None) -> None:
+                     shape: Optional[Sequence[int]] = None,
+                     dtype: torch.dtype = torch.float32) -> None:
     if t is not None:
-        require(t, name, device, shape)
+        require(t, name, device, shape, dtype)

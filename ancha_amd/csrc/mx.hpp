@@ -1,0 +1,224 @@
+// Microscaled (MX) operands of the gfx950 kernels: values in blocks of 32 along a row that share a
+// power of two. A block with largest magnitude a > 0 has the scale byte
+//   s = max(0, floor(log2 a) + 127 - E),   E = 8 for e4m3 ("fp8"), 2 for e2m1 ("fp4"),
+// and each value v the code of v / 2^(s - 127), rounded to nearest even and saturated at 448 / 6. The
+// division is exact, so the code is the only rounding. A block without a non-zero value has s = 0; one
+// with a NaN or an infinity has s = 255 and codes 0: the matrix cores and the decoder make every value
+// of it NaN.
+//
+// A row of dim values is stored as whole groups of 128: 128 (fp8) or 64 (fp4, two values to a byte,
+// the first in the low half) code bytes and 4 scale bytes each; what lies behind dim is zero.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/ancha_hip.h"
+#include "common.hpp"
+
+namespace ancha {
+namespace mx {
+
+constexpr int kBlock = 32, kGroup = 128;
+constexpr int kFp8 = ANCHA_HIP_MX_FP8, kFp4 = ANCHA_HIP_MX_FP4;
+constexpr int kF32 = ANCHA_HIP_F32, kF16 = ANCHA_HIP_F16, kBf16 = ANCHA_HIP_BF16;
+
+__host__ __device__ constexpr long groups(long dim) { return (dim + kGroup - 1) / kGroup; }
+__host__ __device__ constexpr long pitch(long dim, int format) {
+  return groups(dim) * (format == kFp8 ? 128 : 64);
+}
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+template <int TYPE>
+struct Stored {
+  typedef float type;
+};
+template <>
+struct Stored<kF16> {
+  typedef _Float16 type;
+};
+template <>
+struct Stored<kBf16> {
+  typedef __bf16 type;
+};
+
+// N consecutive values at `p`, of which the first `valid` exist (the others read as 0). Any alignment
+// of whole elements: gfx950 reads wide words from any address.
+template <int TYPE, int N>
+__device__ __forceinline__ void load_row(const void* base, long at, int valid, float* v) {
+  typedef typename Stored<TYPE>::type T;
+  const T* p = static_cast<const T*>(base) + at;
+  if (valid >= N) {
+    T t[N];
+    __builtin_memcpy(t, p, sizeof(t));
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = (float)t[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = i < valid ? (float)p[i] : 0.f;
+  }
+}
+
+template <int TYPE, int N>
+__device__ __forceinline__ void store_row(void* base, long at, int valid, const float* v) {
+  typedef typename Stored<TYPE>::type T;
+  T* p = static_cast<T*>(base) + at;
+  if (valid >= N) {
+    T t[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) t[i] = (T)v[i];
+    __builtin_memcpy(p, t, sizeof(t));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++)
+      if (i < valid) p[i] = (T)v[i];
+  }
+}
+
+// Magnitude of x as an unsigned number: ordered like |x|, infinities and NaN above every finite value
+// (the library is compiled without NaN semantics, so the comparison is made on the bits).
+__device__ __forceinline__ unsigned magnitude(float x) {
+  unsigned bits = __builtin_bit_cast(unsigned, x);
+  asm("" : "+v"(bits));
+  return bits & 0x7fffffffu;
+}
+
+// Lane exchanges within 16 lanes (DPP, no LDS): the neighbour, the other pair of four lanes, the other
+// four of eight and the other eight of sixteen (the last two reversed: for values equal within a quad).
+template <int CTRL>
+__device__ __forceinline__ unsigned dpp(unsigned x) {
+  return (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true);
+}
+constexpr int kSwap1 = 0xb1, kSwap2 = 0x4e, kMirror8 = 0x141, kMirror16 = 0x140;
+
+// Scale byte of a block whose largest magnitude has the bits `top`.
+__device__ __forceinline__ unsigned scale_byte(unsigned top, int format) {
+  const int e = (int)(top >> 23);
+  return e == 255 ? 255u : (unsigned)max(e - (format == kFp8 ? 8 : 2), 0);
+}
+
+// 2^(127 - s): what a value is multiplied by before it is rounded (0 for the byte of a NaN block).
+__device__ __forceinline__ float unscale(unsigned s) {
+  return s == 255u ? 0.f : __builtin_bit_cast(float, (254u - s) << 23);
+}
+
+// 2^(s - 127), NaN for s = 255.
+__device__ __forceinline__ float scale_value(unsigned s) {
+  return __builtin_bit_cast(float, s == 255u ? 0x7fc00000u : s == 0u ? 0x00400000u : s << 23);
+}
+
+// Codes of four values that are already divided by their block's scale.
+__device__ __forceinline__ unsigned codes_fp8(float a, float b, float c, float d) {
+  a = __builtin_amdgcn_fmed3f(a, -448.f, 448.f);
+  b = __builtin_amdgcn_fmed3f(b, -448.f, 448.f);
+  c = __builtin_amdgcn_fmed3f(c, -448.f, 448.f);
+  d = __builtin_amdgcn_fmed3f(d, -448.f, 448.f);
+  const int low = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, low, true);
+}
+
+// Codes of eight values (the conversion saturates).
+__device__ __forceinline__ unsigned codes_fp4(const float* v) {
+  unsigned r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, v[0], v[1], 1.f, 0);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], 1.f, 1);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[4], v[5], 1.f, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6], v[7], 1.f, 3);
+}
+
+// Eight consecutive values of a row held by one lane, a block by four neighbouring lanes, a group of
+// 128 by sixteen: rounds them, writes the codes of unit `unit` (eight values, counted from the start of
+// the codes) and, from one lane of sixteen, the group's four scale bytes. All sixteen lanes take part.
+__device__ __forceinline__ void store_codes(const float* v, int format, bool store, long unit,
+                                            uint8_t* codes, uint8_t* scales) {
+  unsigned top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i++) top = max(top, magnitude(v[i]));
+  top = max(top, dpp<kSwap1>(top));
+  top = max(top, dpp<kSwap2>(top));
+  const unsigned s = scale_byte(top, format);
+  const int lane = threadIdx.x & 15;
+  unsigned all = s << (8 * (lane >> 2));
+  all |= dpp<kMirror8>(all);
+  all |= dpp<kMirror16>(all);
+  const float f = unscale(s);
+  float q[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) q[i] = v[i] * f;
+  const bool none = s == 255u;
+  if (!store) return;
+  if (format == kFp8) {
+    const u32x2 c = {none ? 0u : codes_fp8(q[0], q[1], q[2], q[3]),
+                     none ? 0u : codes_fp8(q[4], q[5], q[6], q[7])};
+    *reinterpret_cast<u32x2*>(codes + unit * 8) = c;
+  } else {
+    *reinterpret_cast<unsigned*>(codes + unit * 4) = none ? 0u : codes_fp4(q);
+  }
+  if (lane == 0) *reinterpret_cast<unsigned*>(scales + (unit >> 4) * 4) = all;
+}
+
+// ---- parameter blocks and launchers (arguments checked by the entry points)
+
+struct RowParams {
+  const void* x;         // [rows][dim], row stride ldx
+  const void* residual;  // the same shape, row stride ldr, or null
+  const float* scale;    // [dim] or null
+  void* sum;             // [rows][dim] contiguous, with a residual (may be x or residual)
+  uint8_t* codes;
+  uint8_t* scales;
+  long ldx, ldr;
+  int rows, dim, type, format;
+  double eps;
+};
+hipError_t launch_quantize(const RowParams& p, hipStream_t stream);
+hipError_t launch_norm(const RowParams& p, hipStream_t stream);
+
+struct ValueParams {
+  const uint8_t* codes;
+  const uint8_t* scales;
+  void* out;  // [rows][dim] contiguous
+  int rows, dim, type, format;
+};
+hipError_t launch_values(const ValueParams& p, hipStream_t stream);
+
+// A weight [k][m] in e2m1 along k, as the matrix cores read it: for each strip of 64 columns and each
+// group of 128 k, four fragments of 1 KiB (16 columns: lane l has column l % 16, k 32 (l / 16) .. + 31
+// in 16 bytes); then, behind all of them, a dword per lane with the scale bytes of its four fragments.
+// m is filled up to whole 128 with zero columns, k to whole 128 with zeros.
+constexpr long kStripCodes = 4096, kStripScales = 256;  // bytes per strip and group
+__host__ __device__ constexpr long strips(long m) { return (m + 127) / 128 * 2; }
+__host__ __device__ constexpr long weight_bytes(long k, long m) {
+  return strips(m) * groups(k) * (kStripCodes + kStripScales);
+}
+
+struct WeightParams {
+  const void* x;  // element (k, m) at k * ldk + m * ldm
+  uint8_t* weight;
+  long ldk, ldm;
+  int k, m, type;
+};
+hipError_t launch_weight(const WeightParams& p, hipStream_t stream);
+
+struct WeightValueParams {
+  const uint8_t* weight;
+  void* out;  // [k][m] contiguous
+  int k, m, type;
+};
+hipError_t launch_weight_values(const WeightValueParams& p, hipStream_t stream);
+
+struct LinearParams {
+  const uint8_t* x;         // codes [n][pitch(k)]
+  const uint8_t* x_scales;  // [n][4 groups(k)]
+  const uint8_t* weight;
+  const float* bias;     // [m] or null
+  const float* rope;     // [4][tokens][64] or null
+  const void* residual;  // [n][m] contiguous, of `type`, or null
+  void* out;             // [n][m] contiguous, of `type`; with out_format the codes
+  uint8_t* out_scales;   // with out_format
+  int n, k, m, format;
+  int tokens, width, gelu;
+  int type, out_format;  // out_format 0: values of `type`
+};
+hipError_t launch_linear(const LinearParams& p, hipStream_t stream);
+
+}  // namespace mx
+}  // namespace ancha

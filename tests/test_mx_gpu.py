@@ -1,0 +1,502 @@
+"""The microscaled operators on the GPU against the 64-bit oracle.
+
+Quantisation, decoding and the norm (which the kernel evaluates in 64 bits) have to give the oracle's
+bytes. Products: every product of two codes is exact, sums are held in 32 bits. With S = sum_k |x w| and
+`steps` matrix instructions along k, each of which adds sixteen partial sums and its accumulator with at
+most one step (2^-23) of the largest, the product is within (steps + 1) 2^-22 S. An "fp8" operand under a
+16-bit result also loses what lies 13 bits below the largest of eight neighbouring products: at most
+8 x 2^-13 of it per eight. Then, in order: bias (one rounding, 2^-24), GELU (slope at most 1.13, erf to
+2^-22), rotation (two products: sqrt 2 and 2^-23), residual (2^-24) and the result's type (half its eps).
+"""
+import numpy as np
+import pytest
+import torch
+
+from ancha_amd import _native, fused, mx
+from ancha_amd import workload as W
+from oracle import mx as O
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def dev(a, gpu, dtype=torch.float32):
+    return torch.from_numpy(np.ascontiguousarray(a, dtype=np.float32)).to(gpu).to(dtype)
+
+
+def host(t):
+    return t.detach().cpu().double().numpy()
+
+
+def same_bytes(name, got, want):
+    codes, scales = got.codes.cpu().numpy(), got.scales.cpu().numpy()
+    assert np.array_equal(scales, want[1]), f"{name}: {(scales != want[1]).sum()} scale bytes differ"
+    assert np.array_equal(codes, want[0]), f"{name}: {(codes != want[0]).sum()} code bytes differ"
+
+
+def rows_of(shape, seed):
+    """Rows with large channels, blocks of very different size, zeros and exact ties."""
+    x = W.normal(shape, seed, 1.0)
+    rng = np.random.default_rng(seed)
+    x *= np.exp2(rng.integers(-12, 12, shape[:-1] + (1,))).astype(np.float32)
+    x[..., rng.random(shape[-1]) < 0.03] *= 20
+    x[..., rng.random(shape[-1]) < 0.1] = 0
+    tie = rng.random(shape) < 0.1
+    x[tie] = (rng.integers(-15, 16, shape) * 0.25)[tie]
+    return x
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "fp4"])
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("shape", [(1, 1), (3, 31), (2, 32), (5, 129), (7, 384), (2, 3, 512), (33, 1549),
+                                   (1, 8192), (4, 16500)])
+def test_quantize_and_values(gpu, shape, kind, fmt):
+    x = dev(rows_of(shape, 3), gpu, TYPES[kind])
+    got = mx.quantize(x, fmt)
+    assert got.shape == x.shape and got.format == fmt
+    flat = host(x).reshape(-1, shape[-1])
+    want = O.encode(flat, fmt)
+    same_bytes(f"{shape} {kind} {fmt}", got, want)
+    values = O.decode(*want, fmt, shape[-1]).reshape(shape)
+    for dtype in TYPES.values():
+        back = got.values(dtype)
+        assert back.shape == x.shape and back.dtype == dtype
+        assert torch.equal(back.cpu(), torch.from_numpy(values).to(dtype))
+
+
+def test_quantize_special_values(gpu):
+    inf, nan = np.inf, np.nan
+    x = np.zeros((8, 100), np.float32)
+    x[0, 5], x[1, 40], x[2, 99] = nan, inf, -inf
+    x[3, :] = 3.4e38
+    x[4, :] = 2.0 ** -149
+    x[4, 64:] = 2.0 ** -126
+    x[5, ::2] = -0.0
+    x[6, :3] = [1.0, -1.0, 2.0 ** -30]
+    x[7, :] = np.float32(2.0) ** 120
+    x[7, 33] = 1e-30
+    for fmt in ("fp8", "fp4"):
+        got = mx.quantize(dev(x, gpu), fmt)
+        want = O.encode(x, fmt)
+        same_bytes(fmt, got, want)
+        values = O.decode(*want, fmt, 100)
+        back = host(got.values())
+        assert np.array_equal(np.isnan(back), np.isnan(values))
+        ok = np.isfinite(values) & (np.abs(values) >= 2.0 ** -126)
+        assert np.array_equal(back[ok], values[ok])
+        assert (np.abs(back[~ok & ~np.isnan(values)]) <= 2.0 ** -126).all()
+    half = mx.quantize(dev(x, gpu).to(torch.float16), "fp8")  # 3.4e38 and 2^120 are infinite there
+    with np.errstate(over="ignore"):
+        same_bytes("f16", half, O.encode(x.astype(np.float16).astype(np.float64), "fp8"))
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "fp4"])
+def test_quantize_layouts(gpu, fmt):
+    base = dev(rows_of((40, 301), 5), gpu)
+    for name, x in (("columns 1..", base[:, 1:]), ("rows apart", base[::3, 2:131]),
+                    ("transposed", base.t()), ("one row", base[7:8, 3:]), ("broadcast", base[:1].expand(6, 301)),
+                    ("three axes", base[:, :300].reshape(40, 3, 100).transpose(0, 1))):
+        got = mx.quantize(x, fmt)
+        same_bytes(name, got, O.encode(host(x).reshape(-1, x.shape[-1]), fmt))
+    for shape in ((0, 64), (3, 0), (2, 0, 5)):
+        got = mx.quantize(torch.zeros(shape, device=gpu), fmt)
+        assert got.shape == shape and got.values().shape == shape
+    with pytest.raises(ValueError, match="float32, float16 or bfloat16"):
+        mx.quantize(base.double(), fmt)
+
+
+NORM_DIMS = [1, 31, 64, 200, 384, 500, 512, 1000, 1024, 1549, 2048, 4096, 5000, 8192, 8200, 20000]
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("dim", NORM_DIMS)
+def test_norms(gpu, dim, kind):
+    dtype = TYPES[kind]
+    rows = 37 if dim < 3000 else 5
+    x, r = dev(rows_of((rows, dim), 7) * 0.01, gpu, dtype), dev(W.normal((rows, dim), 8, 1.0), gpu, dtype)
+    x[0] = 0
+    g = dev(np.sqrt(dim) * (1 + 0.3 * W.normal((dim,), 9, 1.0)), gpu)
+    for fmt, eps, scale in (("fp8", 0.0, g), ("fp8", 1e-5, None), ("fp4", 1e-6, g)):
+        s = None if scale is None else host(scale)
+        same_bytes(f"norm {dim} {fmt}", mx.unit_norm(x, scale, eps, fmt),
+                   O.encode(O.unit_norm(host(x), s, eps), fmt))
+        got, total = mx.add_unit_norm(x, r, scale, eps, fmt)
+        h = (x.float() + r.float()).to(dtype)
+        assert torch.equal(total, h)
+        same_bytes(f"add norm {dim} {fmt}", got, O.encode(O.unit_norm(host(h), s, eps), fmt))
+
+
+def test_norm_special_rows(gpu):
+    for dim in (300, 700, 3000, 9000):
+        x = W.normal((6, dim), 11, 1.0)
+        x[1, 40], x[2, dim - 1], x[3] = np.inf, np.nan, 0
+        x[4], x[5] = 1e-30, 3e38
+        got = mx.unit_norm(dev(x, gpu))
+        want = O.encode(O.unit_norm(x), "fp8")
+        same_bytes(f"dim {dim}", got, want)
+        assert want[1][1, 40 // 32] == 255 and (want[1][2, :-(-dim // 32)] == 255).all()
+
+
+def test_norm_layouts_and_sums_in_place(gpu):
+    lib, stream = _native.lib(), torch.cuda.current_stream().cuda_stream
+    base, other = dev(rows_of((50, 700), 13), gpu), dev(W.normal((50, 800), 14, 2.0), gpu)
+    for rows, a, b in ((slice(None), 1, 3), (slice(0, 50, 2), 5, 0), (slice(9, 10), 2, 2)):
+        x, r = base[rows, a:a + 385], other[rows, b:b + 385]
+        got, total = mx.add_unit_norm(x, r)
+        assert torch.equal(total, x + r) and total.is_contiguous()
+        same_bytes("strided", got, O.encode(O.unit_norm(host(x + r)), "fp8"))
+    for dim in (384, 1549, 12000):
+        for place in ("x", "residual"):
+            x, r = dev(rows_of((9, dim), 15), gpu), dev(W.normal((9, dim), 16, 1.0), gpu)
+            want = x + r
+            out = mx.Tensor._empty((9, dim), "fp8", gpu)
+            total = x if place == "x" else r
+            rc = lib.ancha_hip_mx_norm(x.data_ptr(), 0, 9, dim, dim, r.data_ptr(), dim, None, 0.0, 8,
+                                       total.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), stream)
+            assert rc == _native.OK
+            assert torch.equal(total, want)
+            same_bytes(f"in place of {place}", out, O.encode(O.unit_norm(host(want)), "fp8"))
+    with pytest.raises(ValueError, match="residual must"):
+        mx.add_unit_norm(base, base[:, :5])
+    with pytest.raises(ValueError, match="residual must"):
+        mx.add_unit_norm(base, base.half())
+    with pytest.raises(ValueError, match="scale must"):
+        mx.unit_norm(base, torch.ones(3, device=gpu))
+    with pytest.raises(ValueError, match="eps"):
+        mx.unit_norm(base, eps=-1e-6)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("k,m", [(1, 1), (33, 5), (128, 64), (384, 1664), (129, 130), (1000, 77)])
+def test_weight(gpu, k, m, kind):
+    w = rows_of((m, k), 17) * 0.05
+    if k * m > 50:
+        w[0, 0] = np.inf
+    for name, t in (("in out", dev(w.T, gpu, TYPES[kind])), ("out in", dev(w, gpu, TYPES[kind]).t()),
+                    ("apart", dev(np.repeat(w, 2, 0), gpu, TYPES[kind])[::2].t())):
+        handle = mx.weight(t)
+        assert handle.shape == (k, m)
+        want = O.decode(*O.encode(host(t).T, "fp4"), "fp4", k).T
+        for dtype in TYPES.values():
+            got = handle.values(dtype)
+            assert got.shape == (k, m) and got.dtype == dtype
+            assert np.array_equal(host(got), host(torch.from_numpy(want).to(dtype)), equal_nan=True), name
+    with pytest.raises(ValueError, match=r"\[k, m\]"):
+        mx.weight(torch.zeros((2, 3, 4), device=gpu))
+    assert mx.weight(torch.zeros((0, 4), device=gpu)) is None
+
+
+# ---- products
+
+
+def problem(gpu, n, k, m, fmt, seed=21):
+    x = O.encode(rows_of((n, k), seed), fmt)
+    t = mx.Tensor(torch.from_numpy(x[0]).to(gpu), torch.from_numpy(x[1]).to(gpu), fmt, (n, k))
+    w = dev(W.normal((k, m), seed + 1, 1 / np.sqrt(k)), gpu)
+    handle = mx.weight(w)
+    return t, handle, O.decode(*x, fmt, k), host(handle.values())
+
+
+def product_bound(x, w, fmt, short):
+    """How far the product may be off the exact one (the head of this file)."""
+    k = x.shape[1]
+    steps = -(-k // 128)
+    off = (steps + 1) * 2.0 ** -22 * (np.abs(x) @ np.abs(w))
+    if short and fmt == "fp8":
+        for k0 in range(0, k, 8):
+            a, b = np.abs(x[:, k0:k0 + 8]), np.abs(w[k0:k0 + 8])
+            off += 8 * 2.0 ** -13 * (a[:, :, None] * b[None]).max(1)
+    return off
+
+
+def near(name, got, want, tol):
+    err = np.abs(got - want)
+    assert np.isfinite(got).all(), name
+    ratio = float((err / tol).max())
+    print(f"{name}: max|diff| {err.max():.3e}, worst diff/bound {ratio:.3f}", flush=True)
+    assert ratio <= 1.0, name
+
+
+def expected(x, w, fmt, short, bias=None, gelu=False, rotary=None, residual=None, dtype=torch.float32):
+    """The 64-bit result and how far the kernel's may be from it."""
+    off = product_bound(x, w, fmt, short) + 1e-37
+    y = x @ w
+    if bias is not None:
+        y = y + bias
+        off = off + 2.0 ** -24 * (np.abs(y) + off)
+    if gelu:
+        y = O.gelu(y)
+        off = 1.13 * off + 2.0 ** -21 * (np.abs(y) + off) + 2.0 ** -24 * np.abs(x @ w)
+    if rotary is not None:
+        width = rotary[1]
+        size = O.rotate(np.abs(y) + off, np.abs(rotary[0]), width)
+        rolled = O.rotate(off, np.abs(rotary[0]), width)
+        y = O.rotate(y, *rotary)
+        off = np.where(np.arange(y.shape[1]) < 2 * width, rolled + 2.0 ** -22 * size, off)
+    if residual is not None:
+        y = y + residual
+        off = off + 2.0 ** -24 * (np.abs(y) + off)
+    half = torch.finfo(dtype).eps / 2
+    return y, off + half * (np.abs(y) + off) + float(torch.finfo(dtype).smallest_normal) * half
+
+
+SIZES = [(1, 1, 1), (1, 32, 8), (3, 31, 5), (16, 128, 128), (17, 129, 130), (33, 384, 64), (70, 200, 1549),
+         (129, 512, 257), (300, 1000, 200), (260, 384, 640)]
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("fmt", ["fp8", "fp4"])
+@pytest.mark.parametrize("n,k,m", SIZES)
+def test_products(gpu, n, k, m, fmt, kind):
+    t, w, x, wv = problem(gpu, n, k, m, fmt)
+    got = mx.linear(t, w, dtype=TYPES[kind])
+    assert got.shape == (n, m) and got.dtype == TYPES[kind]
+    y, tol = expected(x, wv, fmt, kind != "f32", dtype=TYPES[kind])
+    near(f"{n}x{k}x{m} {fmt} {kind}", host(got), y, tol)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("fmt", ["fp8", "fp4"])
+@pytest.mark.parametrize("n,k,m", [(5, 96, 70), (64, 384, 256), (140, 640, 1549), (801, 128, 192)])
+def test_epilogues(gpu, n, k, m, fmt, kind):
+    dtype = TYPES[kind]
+    t, w, x, wv = problem(gpu, n, k, m, fmt, 31)
+    b, r = dev(W.normal((m,), 33, 1.0), gpu), dev(W.normal((n, m), 34, 2.0), gpu, dtype)
+    got = mx.linear(t, w, fused.Epilogue(bias=b, gelu=True, residual=r), dtype=dtype)
+    y, tol = expected(x, wv, fmt, kind != "f32", host(b), True, None, host(r), dtype)
+    near(f"bias gelu residual {n}x{k}x{m} {fmt} {kind}", host(got), y, tol)
+    got = mx.linear(t, w, fused.Epilogue(gelu=True), dtype=dtype)
+    y, tol = expected(x, wv, fmt, kind != "f32", gelu=True, dtype=dtype)
+    near(f"gelu {n}x{k}x{m} {fmt} {kind}", host(got), y, tol)
+    width = m // 128 * 64
+    if width:
+        tokens = max(d for d in range(1, 200) if n % d == 0)
+        table = W.axis_rope_packed(W.rope_freqs(), tokens)
+        got = mx.linear(t, w, fused.Epilogue(bias=b, rotary=(dev(table, gpu), width)), dtype=dtype)
+        y, tol = expected(x, wv, fmt, kind != "f32", host(b), False, (table.astype(np.float64), width), None,
+                          dtype)
+        near(f"rotary {n}x{k}x{m} {fmt} {kind}", host(got), y, tol)
+
+
+def check_codes(name, got, y, tol, fmt):
+    """Codes of a result that is known to within tol: the scale byte lies between those of the block's
+    largest magnitude less and plus tol, and under it each code between those of y - tol and y + tol."""
+    n, m = y.shape
+    full = O.padded(m)
+    scales = got.scales.cpu().numpy()
+    lo, hi = np.zeros((n, full)), np.zeros((n, full))
+    lo[:, :m], hi[:, :m] = y - tol, y + tol
+    size_lo = np.where((lo <= 0) & (hi >= 0), 0, np.minimum(np.abs(lo), np.abs(hi)))
+    size_hi = np.maximum(np.abs(lo), np.abs(hi))
+    block = lambda a: a.reshape(n, -1, O.BLOCK)  # noqa: E731
+    assert (scales >= O.scale_bytes(block(size_lo).max(2), fmt)).all(), name
+    assert (scales <= O.scale_bytes(block(size_hi).max(2), fmt)).all(), name
+    f = np.exp2(127.0 - scales)[:, :, None]
+    rounded = lambda a: (np.sign(block(a)) * O.grid(fmt)[O.nearest(block(a) * f, fmt)] / f)  # noqa: E731
+    values = block(np.pad(O.decode(got.codes.cpu().numpy(), scales, fmt, full), ((0, 0), (0, 0))))
+    assert (values >= rounded(lo)).all() and (values <= rounded(hi)).all(), name
+    exact = np.mean(values == rounded((lo + hi) / 2))
+    print(f"{name}: {exact:.6f} of the codes are those of the exact result", flush=True)
+
+
+@pytest.mark.parametrize("out", ["fp8", "fp4"])
+@pytest.mark.parametrize("fmt", ["fp8", "fp4"])
+@pytest.mark.parametrize("n,k,m", [(1, 64, 32), (3, 100, 33), (20, 384, 200), (130, 256, 1549), (257, 512, 384)])
+def test_results_in_codes(gpu, n, k, m, fmt, out):
+    t, w, x, wv = problem(gpu, n, k, m, fmt, 41)
+    b, r = dev(W.normal((m,), 43, 0.5), gpu), dev(W.normal((n, m), 44, 1.0), gpu)
+    for name, e, kw in (("bare", None, {}),
+                        ("bias gelu", fused.Epilogue(bias=b, gelu=True), {"bias": host(b), "gelu": True}),
+                        ("residual", fused.Epilogue(residual=r), {"residual": host(r)})):
+        got = mx.linear(t, w, e, format=out)
+        assert isinstance(got, mx.Tensor) and got.shape == (n, m) and got.format == out
+        y, tol = expected(x, wv, fmt, False, **kw)
+        check_codes(f"{name} {n}x{k}x{m} {fmt} -> {out}", got, y, tol, out)
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "fp4"])
+def test_products_not_finite(gpu, fmt):
+    """A NaN block of a row spoils that row alone, one of the weight its column alone; codes of a result
+    with a NaN mark its block alone."""
+    n, k, m = 40, 300, 150
+    x, w = W.normal((n, k), 51, 1.0), W.normal((k, m), 52, 0.1)
+    x[7, 130], x[39, 299], w[5, 70] = np.nan, np.inf, np.nan
+    t, handle = mx.quantize(dev(x, gpu), fmt), mx.weight(dev(w, gpu))
+    for dtype in TYPES.values():
+        bad = np.isnan(host(mx.linear(t, handle, dtype=dtype)))
+        want = np.zeros((n, m), bool)
+        want[[7, 39]], want[:, 70] = True, True
+        assert np.array_equal(bad, want)
+    got = mx.linear(t, handle, format="fp8")
+    marked = got.scales.cpu().numpy() == 255
+    want = np.zeros((n, 8), bool)
+    want[[7, 39], :5], want[:, 2] = True, True
+    assert np.array_equal(marked, want)
+    assert np.isnan(host(got.values())[0, 64:96]).all() and np.isfinite(host(got.values())[0, :64]).all()
+
+
+def test_zero_rows_and_empty_calls(gpu):
+    w = mx.weight(dev(W.normal((100, 70), 61, 1.0), gpu))
+    zero = mx.quantize(torch.zeros((5, 100), device=gpu), "fp8")
+    assert (mx.linear(zero, w) == 0).all()
+    none = mx.quantize(torch.zeros((0, 100), device=gpu))
+    assert mx.linear(none, w).shape == (0, 70) and mx.linear(none, w, format="fp4").shape == (0, 70)
+    three = mx.quantize(dev(W.normal((2, 3, 100), 62, 1.0), gpu), "fp4")
+    flat = mx.Tensor(three.codes, three.scales, "fp4", (6, 100))
+    assert torch.equal(mx.linear(three, w).reshape(6, 70), mx.linear(flat, w))
+
+
+def test_refusals(gpu):
+    x, w = mx.quantize(torch.ones((8, 100), device=gpu)), mx.weight(torch.ones((100, 256), device=gpu))
+    table = torch.zeros((4, 4, 64), device=gpu)
+    for t, width in ((torch.zeros((4, 3, 64), device=gpu), 64), (table, 32), (table, 192),
+                     (torch.zeros((3, 4, 64), device=gpu), 64), (torch.zeros((4, 0, 64), device=gpu), 64)):
+        assert mx.linear(x, w, fused.Epilogue(rotary=(t, width))) is None
+    for e, text in ((fused.Epilogue(bias=torch.zeros(255, device=gpu)), "bias must"),
+                    (fused.Epilogue(bias=torch.zeros(256, device=gpu).half()), "bias must"),
+                    (fused.Epilogue(residual=torch.zeros((8, 255), device=gpu)), "residual must"),
+                    (fused.Epilogue(residual=torch.zeros((8, 256), device=gpu).half()), "residual must"),
+                    (fused.Epilogue(rotary=(table.cpu(), 64)), "rotary table must")):
+        with pytest.raises(ValueError, match=text):
+            mx.linear(x, w, e)
+    with pytest.raises(ValueError, match="rows of 100"):
+        mx.linear(x, mx.weight(torch.ones((96, 256), device=gpu)))
+    with pytest.raises(ValueError, match="leave dtype"):
+        mx.linear(x, w, dtype=torch.float16, format="fp8")
+    with pytest.raises(ValueError, match="dtype must"):
+        mx.linear(x, w, dtype=torch.float64)
+    for codes, scales in (((8, 63), (8, 4)), ((8, 64), (8, 5)), ((7, 64), (7, 4))):
+        with pytest.raises(ValueError, match="must have shape"):
+            mx.Tensor(torch.zeros(codes, dtype=torch.uint8, device=gpu),
+                      torch.zeros(scales, dtype=torch.uint8, device=gpu), "fp4", (8, 100))
+    with pytest.raises(ValueError, match="uint8"):
+        mx.Tensor(torch.zeros((8, 64), device=gpu), torch.zeros((8, 4), device=gpu), "fp4", (8, 100))
+
+
+def test_unaligned_codes_and_operands(gpu):
+    """Codes that start off a 16-byte border are taken over; bias, residual and table may start anywhere."""
+    n, k, m = 20, 256, 200
+    t, w, x, wv = problem(gpu, n, k, m, "fp8", 71)
+    buf = torch.zeros(n * 256 + 3, dtype=torch.uint8, device=gpu)
+    buf[3:] = t.codes.reshape(-1)
+    off = mx.Tensor(buf[3:].view(n, 256), t.scales, "fp8", (n, k))
+    assert torch.equal(mx.linear(off, w), mx.linear(t, w))
+    b, r = dev(W.normal((m + 1,), 73, 1.0), gpu), dev(W.normal((n * m + 1,), 74, 1.0), gpu)
+    tab = dev(np.concatenate(([0.0], W.axis_rope_packed(W.rope_freqs(), 5).reshape(-1))), gpu)
+    one = mx.linear(t, w, fused.Epilogue(bias=b[1:], rotary=(tab[1:].view(4, 5, 64), 64),
+                                         residual=r[1:].view(n, m)))
+    two = mx.linear(t, w, fused.Epilogue(bias=b[1:].clone(), rotary=(tab[1:].view(4, 5, 64).clone(), 64),
+                                         residual=r[1:].view(n, m).clone()))
+    assert torch.equal(one, two)
+
+
+@pytest.mark.parametrize("n", [1, 5, 33, 200, 1000])
+def test_nothing_beyond_the_outputs(gpu, n):
+    """Writes end with the outputs, wherever the rows and columns end."""
+    lib, stream = _native.lib(), torch.cuda.current_stream().cuda_stream
+    k, m = 160, 333
+    t, w, _, _ = problem(gpu, n, k, m, "fp8", 81)
+    for kind, dtype in enumerate(TYPES.values()):
+        room = torch.full((n * m + 4096,), 7.0, dtype=dtype, device=gpu)
+        rc = lib.ancha_hip_mx_linear(t.codes.data_ptr(), t.scales.data_ptr(), n, k, 8, w._data.data_ptr(), m,
+                                     None, 0, None, 0, 0, None, kind, 0, room.data_ptr(), None, stream)
+        assert rc == _native.OK and (room[n * m:] == 7).all()
+        assert torch.equal(room[:n * m].view(n, m), mx.linear(t, w, dtype=dtype))
+    for fmt, bits in (("fp8", 8), ("fp4", 4)):
+        codes = torch.full((n * 48 * bits + 4096,), 7, dtype=torch.uint8, device=gpu)
+        scales = torch.full((n * 12 + 4096,), 7, dtype=torch.uint8, device=gpu)
+        rc = lib.ancha_hip_mx_linear(t.codes.data_ptr(), t.scales.data_ptr(), n, k, 8, w._data.data_ptr(), m,
+                                     None, 0, None, 0, 0, None, 0, bits, codes.data_ptr(), scales.data_ptr(),
+                                     stream)
+        want = mx.linear(t, w, format=fmt)
+        assert rc == _native.OK and (codes[n * 48 * bits:] == 7).all() and (scales[n * 12:] == 7).all()
+        assert torch.equal(codes[:n * 48 * bits].view(n, -1), want.codes)
+        assert torch.equal(scales[:n * 12].view(n, -1), want.scales)
+        rc = lib.ancha_hip_mx_quantize(room.data_ptr(), 2, n, 333, 333, bits, codes.data_ptr(),
+                                       scales.data_ptr(), stream)
+        assert rc == _native.OK and (codes[n * 48 * bits:] == 7).all() and (scales[n * 12:] == 7).all()
+
+
+def feed_forward(x, r, scale, up, down, b_in, b_out):
+    y, stream = mx.add_unit_norm(x, r, scale, eps=1e-6)
+    hidden = mx.linear(y, up, fused.Epilogue(bias=b_in, gelu=True), format="fp8")
+    return stream, hidden, mx.linear(hidden, down, fused.Epilogue(bias=b_out, residual=stream),
+                                     dtype=stream.dtype)
+
+
+@pytest.mark.parametrize("kind,rows,dim,inner", [("f32", 301, 384, 1536), ("bf16", 1, 512, 2048),
+                                                 ("f16", 60, 200, 333)])
+def test_feed_forward(gpu, kind, rows, dim, inner):
+    """Norm, both projections and the residual as a block runs them, against 64 bits over the codes that
+    each part hands to the next."""
+    dtype = TYPES[kind]
+    x, r = dev(W.normal((rows, dim), 91, 1.0), gpu, dtype), dev(W.normal((rows, dim), 92, 1.0), gpu, dtype)
+    scale = dev(np.sqrt(dim) * (1 + 0.2 * W.normal((dim,), 93, 1.0)), gpu)
+    up = mx.weight(dev(W.normal((dim, inner), 94, dim ** -0.5), gpu))
+    down = mx.weight(dev(W.normal((inner, dim), 95, inner ** -0.5), gpu))
+    b_in, b_out = dev(W.normal((inner,), 96, 0.1), gpu), dev(W.normal((dim,), 97, 0.1), gpu)
+    stream, hidden, out = feed_forward(x, r, scale, up, down, b_in, b_out)
+    h = (x.float() + r.float()).to(dtype)
+    assert torch.equal(stream, h)
+    codes = O.encode(O.unit_norm(host(h), host(scale), 1e-6), "fp8")
+    y, tol = expected(O.decode(*codes, "fp8", dim), host(up.values()), "fp8", False, host(b_in), True)
+    check_codes("hidden", hidden, y, tol, "fp8")
+    y, tol = expected(host(hidden.values()), host(down.values()), "fp8", kind != "f32", host(b_out),
+                      residual=host(stream), dtype=dtype)
+    near(f"out {kind}", host(out), y, tol)
+
+
+def test_feed_forward_in_a_graph_and_on_streams(gpu):
+    """The same run captured and replayed with new inputs between eager calls, and on a stream of its own."""
+    rows, dim, inner = 77, 384, 1536
+    up = mx.weight(dev(W.normal((dim, inner), 101, dim ** -0.5), gpu))
+    down = mx.weight(dev(W.normal((inner, dim), 102, inner ** -0.5), gpu))
+    scale, b_in, b_out = (dev(W.normal((c,), s, 1.0), gpu) for c, s in ((dim, 103), (inner, 104), (dim, 105)))
+    x, r = torch.empty((rows, dim), device=gpu), torch.empty((rows, dim), device=gpu)
+    args = (x, r, scale, up, down, b_in, b_out)
+
+    def load(seed):
+        x.copy_(dev(W.normal((rows, dim), seed, 1.0), gpu))
+        r.copy_(dev(W.normal((rows, dim), seed + 1, 1.0), gpu))
+
+    load(110)
+    feed_forward(*args)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        stream, hidden, out = feed_forward(*args)
+    side = torch.cuda.Stream()
+    for seed in (120, 130, 140):
+        load(seed)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = feed_forward(*args)
+        torch.cuda.synchronize()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = feed_forward(*args)
+        side.synchronize()
+        for a in (want, other):
+            assert torch.equal(stream, a[0]) and torch.equal(out, a[2])
+            assert torch.equal(hidden.codes, a[1].codes) and torch.equal(hidden.scales, a[1].scales)
+
+
+def test_offsets_past_32_bits(gpu):
+    """More than 2^32 bytes of codes and values in one call: the last rows equal those of a call on them
+    alone."""
+    dim, rows = 4096, (1 << 20) + 77
+    x = torch.empty((rows, dim), dtype=torch.bfloat16, device=gpu)
+    x[:1000] = dev(W.normal((1000, dim), 111, 1.0), gpu, torch.bfloat16)
+    x[1000:-1000] = 1.5
+    x[-1000:] = dev(W.normal((1000, dim), 112, 1.0), gpu, torch.bfloat16)
+    got, tail = mx.quantize(x, "fp8"), mx.quantize(x[-1000:].clone(), "fp8")
+    assert torch.equal(got.codes[-1000:], tail.codes) and torch.equal(got.scales[-1000:], tail.scales)
+    normed = mx.unit_norm(x)
+    assert torch.equal(normed.codes[-1000:], mx.unit_norm(x[-1000:].clone()).codes)
+    back = got.values(torch.bfloat16)
+    assert torch.equal(back[-1000:], tail.values(torch.bfloat16))
+    del x, back, normed
+    w = mx.weight(dev(W.normal((dim, 130), 113, 0.02), gpu))
+    y, z = mx.linear(got, w), mx.linear(tail, w)
+    assert torch.equal(y[-1000:], z)
