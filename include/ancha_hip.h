@@ -311,7 +311,8 @@ int ancha_hip_mx_values(const void *codes, const void *scales, size_t rows, size
                         int type, void *out, hipStream_t stream);
 
 /* A weight w [k][m] (element (i, j) at i * ldk + j * ldm) in e2m1 with blocks along k, laid out for
- * ancha_hip_mx_linear: ancha_hip_mx_weight_bytes(k, m) bytes (0: empty or too large), 16-byte aligned.
+ * ancha_hip_mx_linear: ancha_hip_mx_weight_bytes(k, m) bytes (0: empty, k > 2^23 or too large), 16-byte
+ * aligned.
  * Done once, when a model is loaded. */
 size_t ancha_hip_mx_weight_bytes(size_t k, size_t m);
 int ancha_hip_mx_weight(const void *w, int type, size_t k, size_t m, size_t ldk, size_t ldm,
