@@ -35,7 +35,6 @@ def require(t: torch.Tensor, name: str, device: torch.device,
 
 
 def require_optional(t: Optional[torch.Tensor], name: str, device: torch.device,
-                     shape: Optional[Sequence[int]] = None,
-                     dtype: torch.dtype = torch.float32) -> None:
+                     shape: Optional[Sequence[int]] = None) -> None:
     if t is not None:
-        require(t, name, device, shape, dtype)
+        require(t, name, device, shape)

@@ -125,6 +125,11 @@ __device__ __forceinline__ unsigned codes_fp4(const float* v) {
   return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6], v[7], 1.f, 3);
 }
 
+__device__ __forceinline__ unsigned codes_fp4x4(float a, float b, float c, float d) {
+  const unsigned r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, a, b, 1.f, 0);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, c, d, 1.f, 1);
+}
+
 // Eight consecutive values of a row held by one lane, a block by four neighbouring lanes, a group of
 // 128 by sixteen: rounds them, writes the codes of unit `unit` (eight values, counted from the start of
 // the codes) and, from one lane of sixteen, the group's four scale bytes. All sixteen lanes take part.

@@ -11,10 +11,16 @@
 // Where the result keeps more than that (fp32, and codes, which flip at a border), an e4m3 operand is
 // split into its values of at least 2 and those below (in units of the block's scale), each of which
 // fits, and multiplied in two passes: 7e-9.
+#include <algorithm>
+
+#include "buffer.hpp"
 #include "gemm.hpp"
 #include "mx.hpp"
 
 namespace ancha {
+
+int device_cus();
+
 namespace mx {
 namespace {
 
@@ -34,98 +40,284 @@ __device__ __forceinline__ f32x4 mfma(u32x4 w, unsigned ws, u32x8 x, unsigned xs
       a, __builtin_bit_cast(i32x8, x), acc, 4, FORMAT == kFp8 ? 0 : 4, B, (int)ws, 0, (int)xs);
 }
 
-// The e4m3 codes with the top exponent bit set (magnitude 2 or more, and NaN), or those without;
-// zeros (of either sign) in place of the others.
-__device__ __forceinline__ unsigned large_part(unsigned c) {
-  const unsigned t = c & 0x40404040u;
-  return c & (((t << 1) - (t >> 6)) | 0x80808080u);
-}
-__device__ __forceinline__ unsigned small_part(unsigned c) {
-  const unsigned t = c & 0x40404040u;
-  return c & ~((t << 1) - (t >> 6));
+// Four e4m3 codes, those with the top exponent bit set (magnitude 2 or more, and NaN) apart from the
+// others; zeros in place of those that went the other way. v_perm_b32's selectors 8 .. 11 spread the
+// sign of a byte over eight bits: of S1's bytes 1 and 3 (the codes shifted up by one), then of S0's.
+__device__ __forceinline__ void split(unsigned c, unsigned& large, unsigned& small) {
+  const unsigned mask = __builtin_amdgcn_perm(c << 9, c << 1, 0x090b080au);
+  large = c & mask;
+  small = c & ~mask;
 }
 
 constexpr bool kCodes(int out) { return out == kFp8 || out == kFp4; }
 
-// Four neighbouring columns c .. c + 3 of row r of the product through the epilogue; OUT is the type of
-// the result (and of the residual), or the format of its codes (fp32 residual). Columns of the filling
-// become 0, also in a NaN row.
+constexpr int kOutStage = 4096;  // LDS bytes per wave for one 16 x 64 tile on its way out
+
+// Where a workgroup's rows lie: buffers over them, so that rows behind the last one read as 0 and are
+// not written, or plain pointers (DIRECT) where a row is not whole groups of four columns or the rows
+// reach past 32-bit offsets.
 template <int OUT>
-__device__ __forceinline__ void finish(const LinearParams& p, long r, int c, float* v) {
-  constexpr int TYPE = kCodes(OUT) ? kF32 : OUT;
-  if (p.bias) {
-    float b[4];
-    load_row<kF32, 4>(p.bias, c < p.m ? c : 0, p.m - c, b);
+struct Rows {
+  static constexpr int kType = kCodes(OUT) ? kF32 : OUT;
+  static constexpr int kSize = kType == kF32 ? 4 : 2;  // of the residual and of uncoded results
+  rsrc_t out, residual;
+  long row0;
+  int rows;
+};
+
+template <int OUT>
+__device__ __forceinline__ Rows<OUT> rows_of(const LinearParams& p, long row0, int rows) {
+  Rows<OUT> d;
+  d.row0 = row0;
+  d.rows = rows;
+  const long row = kCodes(OUT) ? pitch(p.m, OUT) : (long)p.m * d.kSize;
+  d.out = make_rsrc(static_cast<uint8_t*>(p.out) + row0 * row, (unsigned)(rows * row));
+  const long span = (long)p.m * d.kSize;
+  d.residual = make_rsrc(p.residual ? static_cast<const uint8_t*>(p.residual) + row0 * span : p.out,
+                         p.residual ? (unsigned)(rows * span) : 0u);
+  return d;
+}
+
+__device__ __forceinline__ void unpack(u32x2 w, bool half, float* v) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) v[i] += b[i];
+  for (int i = 0; i < 4; i++) {
+    const unsigned short h = (unsigned short)(w[i / 2] >> (16 * (i & 1)));
+    v[i] = half ? (float)__builtin_bit_cast(_Float16, h) : (float)__builtin_bit_cast(__bf16, h);
+  }
+}
+
+// The residual of four neighbouring columns c .. of row r of the workgroup.
+template <int OUT, bool DIRECT>
+__device__ __forceinline__ void load_residual(const LinearParams& p, const Rows<OUT>& d, int r, int c,
+                                              float* v) {
+  constexpr int TYPE = Rows<OUT>::kType;
+  if constexpr (DIRECT) {
+    const bool here = r < d.rows && c < p.m;
+    load_row<TYPE, 4>(p.residual, here ? (d.row0 + r) * p.m + c : 0, here ? p.m - c : 0, v);
+  } else {
+    const unsigned off = c < p.m ? ((unsigned)r * (unsigned)p.m + c) * d.kSize : 0x80000000u;
+    if constexpr (TYPE == kF32) {
+      const float4 x = bload4<true>(d.residual, off);
+      v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+    } else {
+      unpack(__builtin_amdgcn_raw_buffer_load_b64(d.residual, off, 0, 0), TYPE == kF16, v);
+    }
+  }
+}
+
+template <int OUT, bool DIRECT>
+__device__ __forceinline__ void store_values(const LinearParams& p, const Rows<OUT>& d, int r, int c,
+                                             const float* v) {
+  if constexpr (DIRECT) {
+    if (r < d.rows && c < p.m) store_row<OUT, 4>(p.out, (d.row0 + r) * p.m + c, p.m - c, v);
+  } else {
+    const unsigned off = c < p.m ? ((unsigned)r * (unsigned)p.m + c) * d.kSize : 0x80000000u;
+    if constexpr (OUT == kF32) {
+      bstore4<true>(d.out, off, make_float4(v[0], v[1], v[2], v[3]));
+    } else {
+      typename Stored<OUT>::type t[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) t[i] = (typename Stored<OUT>::type)v[i];
+      u32x2 w;
+      __builtin_memcpy(&w, t, 8);
+      __builtin_amdgcn_raw_buffer_store_b64(w, d.out, off, 0, 0);
+    }
+  }
+}
+
+__device__ __forceinline__ unsigned bits_of(float x) {
+  unsigned bits = __builtin_bit_cast(unsigned, x);
+  asm("" : "+v"(bits));
+  return bits;
+}
+
+// Sixteen neighbouring values a lane, a block of 32 by lanes l and l ^ 16, to codes and the scale byte.
+// The largest magnitude is taken on the bits, as signed numbers (the largest positive value) and as
+// unsigned ones (the largest negative value, if there is one), a NaN above everything. The conversion
+// divides by the scale and, with saturate() in effect, stops at the largest value.
+template <int OUT>
+__device__ __forceinline__ unsigned encode16(const float* v, unsigned* codes) {
+  int positive = 0;
+  unsigned negative = 0;
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    const unsigned b = bits_of(v[i]);
+    positive = max(positive, (int)b);
+    negative = max(negative, b);
+  }
+  unsigned top = max((unsigned)positive, negative & 0x7fffffffu);
+  const auto both = __builtin_amdgcn_permlane16_swap(top, top, false, false);
+  top = max((unsigned)both[0], (unsigned)both[1]);
+  const unsigned s = scale_byte(top, OUT);
+  const float f = __builtin_bit_cast(float, s == 0u ? 0x00400000u : s << 23);
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int i = 0; i < (OUT == kFp8 ? 4 : 2); i++) {
+    unsigned c;
+    if constexpr (OUT == kFp8) {
+      s16x2 w = {0, 0};
+      w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, v[4 * i], v[4 * i + 1], f, false);
+      w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, v[4 * i + 2], v[4 * i + 3], f, true);
+      c = __builtin_bit_cast(unsigned, w);
+    } else {
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, v[8 * i], v[8 * i + 1], f, 0);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * i + 2], v[8 * i + 3], f, 1);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * i + 4], v[8 * i + 5], f, 2);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * i + 6], v[8 * i + 7], f, 3);
+    }
+    codes[i] = s == 255u ? 0u : c;
+  }
+  return s;
+}
+
+// Sets MODE.FP16_OVFL: conversions to e4m3 stop at 448 instead of turning into a NaN. Only behind the last
+// matrix instruction: with the mode set those no longer give a NaN for the scale byte 255.
+__device__ __forceinline__ void saturate() { __builtin_amdgcn_s_setreg(1 | 23 << 6 | 0 << 11, 1); }
+
+// Turns acc[t] of a 16 x 64 tile as the MFMAs leave it (lane l: row l % 16, columns 16 t + 4 (l / 16) ..
+// + 3) into sixteen neighbouring columns of the same row: lane l has columns 16 (l / 16) + 4 t .. + 3 in
+// v[4 t] .. (a transposition of four lane groups and four registers, by exchanges of half and quarter
+// waves).
+__device__ __forceinline__ void gather16(const f32x4* acc, float* v) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    unsigned x[4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+      const float y = acc[t][e];  // a bit cast of the vector's element itself takes element 0
+      x[t] = __builtin_bit_cast(unsigned, y);
+    }
+    const auto a = __builtin_amdgcn_permlane32_swap(x[0], x[2], false, false);
+    const auto b = __builtin_amdgcn_permlane32_swap(x[1], x[3], false, false);
+    const auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
+    const auto d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+    v[e] = __builtin_bit_cast(float, (unsigned)c[0]);
+    v[4 + e] = __builtin_bit_cast(float, (unsigned)c[1]);
+    v[8 + e] = __builtin_bit_cast(float, (unsigned)d[0]);
+    v[12 + e] = __builtin_bit_cast(float, (unsigned)d[1]);
+  }
+}
+
+// The epilogue of 16 rows r0 .. and a strip of 64 columns c0 .. to codes; bias[i]: column c0 + 16 (l / 16)
+// + i. Columns of the filling become 0, also in a NaN row.
+template <int OUT, bool DIRECT>
+__device__ __forceinline__ void finish_codes(const LinearParams& p, const Rows<OUT>& d, int r0, int c0,
+                                             const float* bias, const f32x4* acc) {
+  const int lane = threadIdx.x & 63, r = r0 + (lane & 15), c = c0 + 16 * (lane >> 4);
+  float v[16];
+  gather16(acc, v);
+#pragma unroll
+  for (int i = 0; i < 16; i++) v[i] += bias[i];
+  if (p.gelu)
+#pragma unroll
+    for (int i = 0; i < 16; i++) v[i] = gemm::gelu_fast(v[i]);
+  if (p.rope && c < 2 * p.width) {
+    const unsigned token = (unsigned)(d.row0 + r) % (unsigned)p.tokens;
+    const float* table = p.rope + (c < p.width ? 0 : 2) * (long)p.tokens * 64 + token * 64ul + (c & 63);
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+      float cs[4], sn[4];
+      __builtin_memcpy(cs, table + 4 * t, 16);
+      __builtin_memcpy(sn, table + (long)p.tokens * 64 + 4 * t, 16);
+      float* y = v + 4 * t;
+      const float4 z = rotate4(make_float4(y[0], y[1], y[2], y[3]), make_float4(cs[0], cs[1], cs[2], cs[3]),
+                               make_float4(sn[0], sn[1], sn[2], sn[3]));
+      y[0] = z.x, y[1] = z.y, y[2] = z.z, y[3] = z.w;
+    }
+  }
+  if (p.residual)
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+      float x[4];
+      load_residual<OUT, DIRECT>(p, d, r, c + 4 * t, x);
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[4 * t + i] += x[i];
+    }
+  if (c0 + 64 > p.m)
+#pragma unroll
+    for (int i = 0; i < 16; i++) v[i] = c + i < p.m ? v[i] : 0.f;
+  unsigned codes[4];
+  const unsigned s = encode16<OUT>(v, codes);
+  const unsigned width = 128u * (unsigned)groups(p.m);  // values of a stored row
+  const unsigned at = (unsigned)r * width + c;
+  if constexpr (OUT == kFp8)
+    __builtin_amdgcn_raw_buffer_store_b128(u32x4{codes[0], codes[1], codes[2], codes[3]}, d.out, at, 0, 0);
+  else
+    __builtin_amdgcn_raw_buffer_store_b64(u32x2{codes[0], codes[1]}, d.out, at >> 1, 0, 0);
+  if ((lane & 16) == 0 && r < d.rows)
+    p.out_scales[(d.row0 + r) * (long)(width >> 5) + (c >> 5)] = (uint8_t)s;
+}
+
+// The epilogue of 16 rows r0 .. of the workgroup and a strip of 64 columns c0 ..; acc[t] as the MFMAs
+// leave it: lane l has row l % 16, columns 16 t + 4 (l / 16) .. + 3. The tile passes through `st` (row of
+// 256 bytes, 16-byte chunk c of row r at c ^ r), so that sixteen lanes have a row's 64 neighbouring
+// columns: whole rows of the strip are read and written (in pieces of 64 bytes 96 120 x 384 -> 1536 in
+// fp32 took 297 us, in pieces of 256 it takes 186).
+template <int OUT, bool DIRECT>
+__device__ __forceinline__ void finish_tile(const LinearParams& p, const Rows<OUT>& d, int r0, int c0,
+                                            const float* bias, const f32x4* acc, const int* tokens,
+                                            uint8_t* st) {
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int c = c0 + 4 * r;
+  float x[4][4], v[4][4];
+  if (p.residual)
+#pragma unroll
+    for (int q = 0; q < 4; q++) load_residual<OUT, DIRECT>(p, d, r0 + 4 * q + g, c, x[q]);
+#pragma unroll
+  for (int t = 0; t < 4; t++) *reinterpret_cast<f32x4*>(st + r * 256 + (((4 * t + g) ^ r) << 4)) = acc[t];
+#pragma unroll
+  for (int q = 0; q < 4; q++) {
+    const int tr = 4 * q + g;
+    const f32x4 y = *reinterpret_cast<const f32x4*>(st + tr * 256 + ((r ^ tr) << 4));
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[q][i] = y[i] + bias[i];
   }
   if (p.gelu)
 #pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = OUT == kF32 ? gemm::gelu_erf(v[i]) : gemm::gelu_fast(v[i]);
+    for (int q = 0; q < 4; q++)
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        v[q][i] = OUT == kF32 ? gemm::gelu_erf(v[q][i]) : gemm::gelu_fast(v[q][i]);
   if (p.rope && c < 2 * p.width) {
-    const long t = (long)(r % p.tokens) * 64 + (c & 63);
-    const float* table = p.rope + (c < p.width ? 0 : 2) * (long)p.tokens * 64 + t;
-    float cs[4], sn[4];
-    __builtin_memcpy(cs, table, 16);
-    __builtin_memcpy(sn, table + (long)p.tokens * 64, 16);
-    const float4 y = rotate4(make_float4(v[0], v[1], v[2], v[3]), make_float4(cs[0], cs[1], cs[2], cs[3]),
-                             make_float4(sn[0], sn[1], sn[2], sn[3]));
-    v[0] = y.x, v[1] = y.y, v[2] = y.z, v[3] = y.w;
-  }
-  if (p.residual) {
-    float x[4];
-    load_row<TYPE, 4>(p.residual, c < p.m ? r * p.m + c : 0, p.m - c, x);
+    const float* table = p.rope + (c < p.width ? 0 : 2) * (long)p.tokens * 64 + (c & 63);
 #pragma unroll
-    for (int i = 0; i < 4; i++) v[i] += x[i];
+    for (int q = 0; q < 4; q++) {
+      float cs[4], sn[4];
+      const float* at = table + tokens[r0 + 4 * q + g] * 64l;
+      __builtin_memcpy(cs, at, 16);
+      __builtin_memcpy(sn, at + (long)p.tokens * 64, 16);
+      const float4 y = rotate4(make_float4(v[q][0], v[q][1], v[q][2], v[q][3]),
+                               make_float4(cs[0], cs[1], cs[2], cs[3]),
+                               make_float4(sn[0], sn[1], sn[2], sn[3]));
+      v[q][0] = y.x, v[q][1] = y.y, v[q][2] = y.z, v[q][3] = y.w;
+    }
   }
-  if (kCodes(OUT) && c + 3 >= p.m)
+  if (p.residual)
 #pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = c + i < p.m ? v[i] : 0.f;
+    for (int q = 0; q < 4; q++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[q][i] += x[q][i];
+#pragma unroll
+  for (int q = 0; q < 4; q++) store_values<OUT, DIRECT>(p, d, r0 + 4 * q + g, c, v[q]);
 }
 
-// The epilogue of a strip of 64 columns of one row: lane l has columns c0 + 16 t + 4 (l / 16) .. + 3 in
-// acc[t]. `here`: the row exists (the lanes of a row agree).
-template <int OUT>
-__device__ __forceinline__ void finish_strip(const LinearParams& p, long r, bool here, int c0,
-                                             const f32x4* acc) {
-  const int g = (threadIdx.x & 63) >> 4;
-  const long rr = here ? r : 0;
-  float v[4][4];
+// The epilogue of a wave: SM strips from column c0 on, TN tiles of 16 rows from r0 on.
+template <int OUT, bool DIRECT, int SM, int TN>
+__device__ __forceinline__ void finish_wave(const LinearParams& p, const Rows<OUT>& d, int r0, int c0,
+                                            const f32x4 (*acc)[SM][4], const int* tokens, uint8_t* st) {
+  constexpr int N = kCodes(OUT) ? 16 : 4;  // neighbouring columns of a lane
+  const int c = c0 + (kCodes(OUT) ? 16 * ((threadIdx.x & 63) >> 4) : 4 * (threadIdx.x & 15));
 #pragma unroll
-  for (int t = 0; t < 4; t++) {
-    const int c = c0 + 16 * t + 4 * g;
+  for (int i = 0; i < SM; i++) {
+    if (c0 + 64 * i >= 64 * (int)strips(p.m)) break;
+    float bias[N] = {};
+    if (p.bias) load_row<kF32, N>(p.bias, c + 64 * i < p.m ? c + 64 * i : 0, p.m - c - 64 * i, bias);
 #pragma unroll
-    for (int i = 0; i < 4; i++) v[t][i] = acc[t][i];
-    finish<OUT>(p, rr, c, v[t]);
-    if constexpr (!kCodes(OUT))
-      if (here && c < p.m) store_row<OUT, 4>(p.out, r * p.m + c, p.m - c, v[t]);
-  }
-  if constexpr (kCodes(OUT)) {
-    // A block of 32 columns: two tiles, in lanes l % 16 + {0, 16, 32, 48}.
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      unsigned top = 0;
-#pragma unroll
-      for (int i = 0; i < 8; i++) top = max(top, magnitude(v[2 * h + i / 4][i % 4]));
-      top = max(top, (unsigned)__shfl_xor((int)top, 16));
-      top = max(top, (unsigned)__shfl_xor((int)top, 32));
-      const unsigned s = scale_byte(top, OUT);
-      const float f = unscale(s);
-      const long block = rr * 4 * groups(p.m) + (c0 >> 5) + h;
-      if (here && g == 0) p.out_scales[block] = (uint8_t)s;
-#pragma unroll
-      for (int t = 0; t < 2; t++) {
-        float q[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) q[i] = i < 4 ? v[2 * h + t][i] * f : 0.f;
-        if (!here) continue;
-        if constexpr (OUT == kFp8)
-          *reinterpret_cast<unsigned*>(static_cast<uint8_t*>(p.out) + block * 32 + 16 * t + 4 * g) =
-              s == 255u ? 0u : codes_fp8(q[0], q[1], q[2], q[3]);
-        else
-          *reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(p.out) + block * 16 + 8 * t + 2 * g) =
-              s == 255u ? (uint16_t)0 : (uint16_t)codes_fp4(q);
-      }
+    for (int j = 0; j < TN; j++) {
+      if constexpr (kCodes(OUT))
+        finish_codes<OUT, DIRECT>(p, d, r0 + 16 * j, c0 + 64 * i, bias, acc[j][i]);
+      else
+        finish_tile<OUT, DIRECT>(p, d, r0 + 16 * j, c0 + 64 * i, bias, acc[j][i], tokens, st);
     }
   }
 }
@@ -181,25 +373,25 @@ __device__ __forceinline__ void barrier() {
 
 // A workgroup of WM x WN waves has 64 SM WM columns and 16 TN WN rows; a wave SM strips of 64 columns
 // and TN tiles of 16 rows, its accumulators in registers. Per step of 128 k both operands and their
-// scales go straight from memory to LDS, two steps ahead, in three buffers: one barrier per step, behind
-// which the buffer of the step before is free.
+// scales go straight from memory to LDS, ST - 1 steps ahead, in ST buffers: one barrier per step, behind
+// which the buffer of the step before is free. OCC: waves per SIMD that the registers leave room for.
 //
 // A row's 16-byte chunks lie in LDS at chunk ^ (row & 7) (e4m3: 128 bytes a row; e2m1: 64 bytes, chunk ^
 // (row / 2 & 3)), so that the eight lanes that are served together hit different banks; the loads to LDS
 // write in lane order, so the lanes choose their chunk in memory instead. Weight fragments are in lane
 // order already.
-template <int FORMAT, bool SPLIT, int OUT, int WM, int WN, int SM, int TN>
-__global__ __launch_bounds__(64 * WM * WN) void tile_kernel(LinearParams p, unsigned mtiles,
-                                                            unsigned ntiles) {
+template <int FORMAT, bool SPLIT, int OUT, int WM, int WN, int SM, int TN, int ST, int OCC>
+__global__ __launch_bounds__(64 * WM * WN, OCC) void tile_kernel(LinearParams p, unsigned mtiles,
+                                                            unsigned ntiles, int direct) {
   constexpr int W = WM * WN, STRIPS = WM * SM, ROWS = 16 * TN * WN;
   constexpr int kRow = FORMAT == kFp8 ? 128 : 64;           // bytes of a row and step
   constexpr int kX = ROWS * kRow, kW = STRIPS * (int)kStripCodes;
-  constexpr int kXS = kX + kW, kWS = kXS + ROWS * 4, kStage = kWS + STRIPS * (int)kStripScales;
+  constexpr int kXS = kX + kW, kWS = kXS + ROWS * 4, kStageBytes = kWS + STRIPS * (int)kStripScales;
   constexpr int PX = kX / 1024 / W, PW = kW / 1024 / W;     // 1 KiB pieces per wave
   constexpr int QX = ROWS / 64, Q = (QX + STRIPS + W - 1) / W;  // 256-byte pieces of scales
   static_assert(PX * W * 1024 == kX && PW * W * 1024 == kW && QX * 64 == ROWS, "whole pieces");
   constexpr int kLoads = PX + PW + Q;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[3][kStage];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[ST][kStageBytes];
   const int lane = threadIdx.x & 63, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % WM, wn = wave / WM;
@@ -277,16 +469,17 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(LinearParams p, unsi
     xa[0] = xa[1] = r * 64 + ((g ^ ((r >> 1) & 3)) << 4);
   }
 
-  load(0, lds[0]);
-  if (steps > 1) load(1, lds[1]);
+#pragma unroll
+  for (int s = 0; s < ST - 1; s++)
+    if (s < steps) load(s, lds[s]);
   int b = 0;
   for (int s = 0; s < steps; s++) {
-    if (s + 1 < steps)
-      wait_loads<kLoads>();
+    if (s + ST - 2 < steps)
+      wait_loads<(ST - 2) * kLoads>();
     else
       wait_loads<0>();
     barrier();
-    if (s + 2 < steps) load(s + 2, lds[b == 0 ? 2 : b - 1]);
+    if (s + ST - 1 < steps) load(s + ST - 1, lds[b == 0 ? ST - 1 : b - 1]);
     const uint8_t* from = lds[b];
     u32x4 a[SM][4];
     unsigned sa[SM];
@@ -308,47 +501,229 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(LinearParams p, unsi
       u32x8 large = operand<FORMAT>(lo, hi), small = large;
       if constexpr (SPLIT)
 #pragma unroll
-        for (int i = 0; i < 8; i++) small[i] = small_part(large[i]), large[i] = large_part(large[i]);
+        for (int i = 0; i < 8; i++) {
+          unsigned u, v;
+          split(large[i], u, v);
+          large[i] = u, small[i] = v;
+        }
 #pragma unroll
       for (int i = 0; i < SM; i++) multiply<FORMAT, SPLIT>(a[i], sa[i], large, small, sb, acc[j][i]);
     }
-    b = b == 2 ? 0 : b + 1;
+    b = b == ST - 1 ? 0 : b + 1;
   }
+  static_assert(W * kOutStage + ROWS * 4 <= ST * kStageBytes, "the way out fits the operands' buffers");
+  int* tokens = reinterpret_cast<int*>(&lds[0][0] + W * kOutStage);
+  const int rows = (int)min((long)ROWS, p.n - row0);
+  if (!kCodes(OUT)) {
+    // Every wave is done with the operands before the first one's results take their place.
+    wait_loads<0>();
+    barrier();
+  }
+  if (!kCodes(OUT) && p.rope) {
+    if ((int)threadIdx.x < ROWS) tokens[threadIdx.x] = (int)((unsigned)(row0 + threadIdx.x) % (unsigned)p.tokens);
+    __syncthreads();
+  }
+  if (kCodes(OUT)) saturate();
+  const Rows<OUT> d = rows_of<OUT>(p, row0, rows);
+  const int c0 = (strip0 + wm * SM) * 64;
+  if (direct)
+    finish_wave<OUT, true, SM, TN>(p, d, wn * TN * 16, c0, acc, tokens, &lds[0][0] + wave * kOutStage);
+  else
+    finish_wave<OUT, false, SM, TN>(p, d, wn * TN * 16, c0, acc, tokens, &lds[0][0] + wave * kOutStage);
+}
+
+// Whether the rows of a workgroup are written (and the residual read) through plain pointers.
+int direct_rows(const LinearParams& p, long rows) {
+  return p.m % 4 != 0 || rows * (p.m + 128l) * 4 >= 1l << 31 ||
+         (reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.residual)) % 4 != 0;
+}
+
+template <int FORMAT, bool SPLIT, int OUT, int WM, int WN, int SM, int TN, int ST, int OCC>
+void start_tiles(const LinearParams& p, hipStream_t stream) {
+  const unsigned mtiles = (unsigned)((strips(p.m) + WM * SM - 1) / (WM * SM));
+  const unsigned ntiles = (unsigned)(((long)p.n + 16 * TN * WN - 1) / (16 * TN * WN));
+  hipLaunchKernelGGL((tile_kernel<FORMAT, SPLIT, OUT, WM, WN, SM, TN, ST, OCC>), dim3(mtiles * ntiles),
+                     dim3(64 * WM * WN), 0, stream, p, mtiles, ntiles, direct_rows(p, 16 * TN * WN));
+}
+
+// Few rows: the weight is what has to be read. A workgroup has 32 columns and 16 TN rows; its waves (one
+// to sixteen) take the steps of 128 k in turn, straight from memory, and add up their sums in LDS. Then
+// eight threads have a row, four neighbouring columns each.
+constexpr int kFewColumns = 32, kFewWaves = 16;
+
+template <int FORMAT, bool SPLIT, int OUT, int TN>
+__global__ __launch_bounds__(64 * kFewWaves) void few_kernel(LinearParams p) {
+  constexpr int kRow = FORMAT == kFp8 ? 128 : 64;
+  constexpr int kPart = 16 * TN * kFewColumns * 4;  // bytes of one wave's sums
+  extern __shared__ __attribute__((aligned(16))) uint8_t part[];
+  const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int steps = (int)groups(p.k), nstrips = (int)strips(p.m);
+  const int strip = (int)blockIdx.x >> 1, half = (int)blockIdx.x & 1;
+  const long row0 = (long)blockIdx.y * (16 * TN);
+  const uint8_t* w = p.weight + (long)strip * steps * kStripCodes + half * 2048 + lane * 16;
+  const uint8_t* ws = p.weight + (long)nstrips * steps * kStripCodes +
+                      (long)strip * steps * kStripScales + lane * 4 + half * 2;
+  const uint8_t *x[TN], *xs[TN];
 #pragma unroll
   for (int j = 0; j < TN; j++) {
-    const long row = row0 + (wn * TN + j) * 16 + r;
+    const long row = min(row0 + 16 * j + r, (long)p.n - 1);
+    x[j] = p.x + row * steps * kRow + 16 * g;
+    xs[j] = p.x_scales + row * steps * 4 + g;
+  }
+  f32x4 acc[TN][2];
 #pragma unroll
-    for (int i = 0; i < SM; i++) {
-      const int strip = strip0 + wm * SM + i;
-      if (strip < nstrips) finish_strip<OUT>(p, row, row < p.n, strip * 64, acc[j][i]);
+  for (int j = 0; j < TN; j++) acc[j][0] = zero4(), acc[j][1] = zero4();
+  // Four of the wave's steps at a time, all their loads in flight together (steps behind the last are
+  // loaded again, not multiplied).
+  constexpr int U = 4;
+  for (int s0 = wave; s0 < steps; s0 += U * waves) {
+    u32x4 a[U][2], lo[U][TN], hi[U][TN];
+    unsigned sa[U], sb[U][TN];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const long s = min(s0 + u * waves, steps - 1);
+      a[u][0] = *reinterpret_cast<const u32x4*>(w + s * kStripCodes);
+      a[u][1] = *reinterpret_cast<const u32x4*>(w + s * kStripCodes + 1024);
+      sa[u] = *reinterpret_cast<const uint16_t*>(ws + s * kStripScales);
+#pragma unroll
+      for (int j = 0; j < TN; j++) {
+        lo[u][j] = *reinterpret_cast<const u32x4*>(x[j] + s * kRow);
+        hi[u][j] = FORMAT == kFp8 ? *reinterpret_cast<const u32x4*>(x[j] + s * kRow + 64) : lo[u][j];
+        sb[u][j] = xs[j][s * 4];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (s0 + u * waves >= steps) break;
+#pragma unroll
+      for (int j = 0; j < TN; j++) {
+        u32x8 large = operand<FORMAT>(lo[u][j], hi[u][j]), small = large;
+        if constexpr (SPLIT)
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            unsigned y, z;
+            split(large[i], y, z);
+            large[i] = y, small[i] = z;
+          }
+        acc[j][0] = mfma<FORMAT, 0>(a[u][0], sa[u], large, sb[u][j], acc[j][0]);
+        acc[j][1] = mfma<FORMAT, 1>(a[u][1], sa[u], large, sb[u][j], acc[j][1]);
+        if constexpr (SPLIT) {
+          acc[j][0] = mfma<FORMAT, 0>(a[u][0], sa[u], small, sb[u][j], acc[j][0]);
+          acc[j][1] = mfma<FORMAT, 1>(a[u][1], sa[u], small, sb[u][j], acc[j][1]);
+        }
+      }
+    }
+  }
+  // Row of 128 bytes, 16-byte chunk c of row r at c ^ (r & 7).
+#pragma unroll
+  for (int j = 0; j < TN; j++)
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+      *reinterpret_cast<f32x4*>(part + wave * kPart + (16 * j + r) * 128 + (((4 * t + g) ^ (r & 7)) << 4)) =
+          acc[j][t];
+  __syncthreads();
+  for (int i = (int)threadIdx.x; i < 16 * TN * 8; i += (int)blockDim.x) {
+    const int tr = i >> 3, c = (int)blockIdx.x * kFewColumns + 4 * (i & 7);
+    const long row = row0 + tr;
+    const bool here = row < p.n;
+    const uint8_t* at = part + tr * 128 + (((i & 7) ^ (tr & 7)) << 4);
+    f32x4 y = *reinterpret_cast<const f32x4*>(at);
+    for (int q = 1; q < waves; q++) y += *reinterpret_cast<const f32x4*>(at + q * kPart);
+    float v[4] = {y[0], y[1], y[2], y[3]}, b[4];
+    const int valid = here ? p.m - c : 0;
+    const long to = valid > 0 ? row * p.m + c : 0;
+    if (p.bias) {
+      load_row<kF32, 4>(p.bias, valid > 0 ? c : 0, valid, b);
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[e] += b[e];
+    }
+    if (p.gelu)
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[e] = OUT == kF32 ? gemm::gelu_erf(v[e]) : gemm::gelu_fast(v[e]);
+    if (p.rope && here && c < 2 * p.width) {
+      const float* table = p.rope + (c < p.width ? 0 : 2) * (long)p.tokens * 64 +
+                           (unsigned)row % (unsigned)p.tokens * 64ul + (c & 63);
+      float cs[4], sn[4];
+      __builtin_memcpy(cs, table, 16);
+      __builtin_memcpy(sn, table + (long)p.tokens * 64, 16);
+      const float4 z = rotate4(make_float4(v[0], v[1], v[2], v[3]), make_float4(cs[0], cs[1], cs[2], cs[3]),
+                               make_float4(sn[0], sn[1], sn[2], sn[3]));
+      v[0] = z.x, v[1] = z.y, v[2] = z.z, v[3] = z.w;
+    }
+    if (p.residual) {
+      load_row<Rows<OUT>::kType, 4>(p.residual, to, valid, b);
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[e] += b[e];
+    }
+    if constexpr (!kCodes(OUT)) {
+      if (valid > 0) store_row<OUT, 4>(p.out, to, valid, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[e] = e < valid ? v[e] : 0.f;
+      unsigned top = max(max(magnitude(v[0]), magnitude(v[1])), max(magnitude(v[2]), magnitude(v[3])));
+      top = max(top, dpp<kSwap1>(top));
+      top = max(top, dpp<kSwap2>(top));
+      top = max(top, dpp<kMirror8>(top));
+      const unsigned s = scale_byte(top, OUT);
+      const float f = unscale(s);
+      if (!here) continue;
+      const long unit = row * 32 * groups(p.m) + (c >> 2);  // four values
+      if ((i & 7) == 0) p.out_scales[unit >> 3] = (uint8_t)s;
+      uint8_t* out = static_cast<uint8_t*>(p.out);
+      if constexpr (OUT == kFp8)
+        *reinterpret_cast<unsigned*>(out + unit * 4) =
+            s == 255u ? 0u : codes_fp8(v[0] * f, v[1] * f, v[2] * f, v[3] * f);
+      else
+        *reinterpret_cast<uint16_t*>(out + unit * 2) =
+            s == 255u ? (uint16_t)0 : (uint16_t)codes_fp4x4(v[0] * f, v[1] * f, v[2] * f, v[3] * f);
     }
   }
 }
 
-template <int FORMAT, bool SPLIT, int OUT, int WM, int WN, int SM, int TN>
-void start_tiles(const LinearParams& p, hipStream_t stream) {
-  const unsigned mtiles = (unsigned)((strips(p.m) + WM * SM - 1) / (WM * SM));
-  const unsigned ntiles = (unsigned)(((long)p.n + 16 * TN * WN - 1) / (16 * TN * WN));
-  hipLaunchKernelGGL((tile_kernel<FORMAT, SPLIT, OUT, WM, WN, SM, TN>), dim3(mtiles * ntiles),
-                     dim3(64 * WM * WN), 0, stream, p, mtiles, ntiles);
+template <int FORMAT, bool SPLIT, int OUT, int TN>
+void start_few(const LinearParams& p, hipStream_t stream) {
+  const int waves = (int)std::min<long>(kFewWaves, groups(p.k));
+  // Codes have their filling written too.
+  const unsigned columns = kCodes(OUT) ? (unsigned)strips(p.m) * 2 : (unsigned)((p.m + 31l) / 32);
+  hipLaunchKernelGGL((few_kernel<FORMAT, SPLIT, OUT, TN>),
+                     dim3(columns, (unsigned)((p.n + 16l * TN - 1) / (16 * TN))), dim3(64 * waves),
+                     (size_t)waves * 16 * TN * kFewColumns * 4, stream, p);
+}
+
+template <int FORMAT, bool SPLIT, int OUT>
+void start(const LinearParams& p, hipStream_t stream) {
+  // Measured with each form forced, e4m3 -> bf16, us (n x k x m):
+  //   few rows / 64 x 64 tiles: 16 x 4096 x 4096 6.3 / 10.9, 64 x 4096 x 4096 9.8 / 11.0, 64 x 8192 x 8192
+  //   30.6 / 19.9, 64 x 2048 x 512 4.4 / 6.8; with 16 / 32 rows a workgroup where 16 already fill the
+  //   chip: 24 x 8192 x 8192 16.9 / 13.7 (e2m1 16.7 / 11.0);
+  //   64 x 64 / 128 x 128: 512 x 4096 x 4096 14.9 / 21.7, 4096 x 2048 x 512 9.2 / 12.9, 1024 x 4096 x 4096
+  //   26.2 / 25.5, 512 x 8192 x 8192 51.0 / 45.8;
+  //   128 rows x 128 / 256 columns: 2048 x 4096 x 4096 35.0 / 37.7, 4096 x 4096 x 4096 61.6 / 56.1,
+  //   8192 x 8192 x 8192 441 / 388; where 256 columns leave a tile mostly empty (96 120 x 1536 x 384, fp32
+  //   with bias and residual) 118 / 134.
+  const long cus = device_cus(), n = p.n, m = p.m;
+  const long columns = (m + 31) / 32, narrow = (m + 127) / 128, wide = (m + 255) / 256;
+  const long high = (n + 127) / 128;
+  if (n > 16 && columns >= cus && (n + 31) / 32 * columns <= cus)
+    start_few<FORMAT, SPLIT, OUT, 2>(p, stream);
+  else if ((n + 15) / 16 * columns <= 2 * cus)
+    start_few<FORMAT, SPLIT, OUT, 1>(p, stream);
+  else if (narrow * high * 4 < 3 * cus)
+    start_tiles<FORMAT, SPLIT, OUT, 1, 4, 1, 1, 3, 4>(p, stream);
+  else if (wide * 32 <= narrow * 17 && wide * high >= 2 * cus)
+    start_tiles<FORMAT, SPLIT, OUT, 1, 4, 4, 2, 2, 2>(p, stream);
+  else
+    start_tiles<FORMAT, SPLIT, OUT, 1, 4, 2, 2, 2, 3>(p, stream);
 }
 
 // The result's type or format picks the kernel: e4m3 rows are split for fp32 and for codes.
 template <int OUT>
 hipError_t linear_to(const LinearParams& p, hipStream_t stream) {
-  constexpr bool kSplit = OUT == kF32 || kCodes(OUT);
-  const bool wide = (long)((p.n + 255) / 256) * ((p.m + 255) / 256) >= 256;
-  if (p.format == kFp4) {
-    if (wide)
-      start_tiles<kFp4, false, OUT, 2, 4, 2, 4>(p, stream);
-    else
-      start_tiles<kFp4, false, OUT, 2, 2, 1, 4>(p, stream);
-  } else {
-    if (wide)
-      start_tiles<kFp8, kSplit, OUT, 2, 4, 2, 4>(p, stream);
-    else
-      start_tiles<kFp8, kSplit, OUT, 2, 2, 1, 4>(p, stream);
-  }
+  if (p.format == kFp4)
+    start<kFp4, false, OUT>(p, stream);
+  else
+    start<kFp8, OUT == kF32 || kCodes(OUT), OUT>(p, stream);
   return hipGetLastError();
 }
 

@@ -15,14 +15,13 @@ float32, float16 or bfloat16 in any row layout; nothing here is differentiable.
 """
 from __future__ import annotations
 
-import contextlib
 from typing import Optional, Sequence
 
 import torch
 
 from . import _native
-from ._tensors import require, require_optional
-from .fused import ATTENTION_HEAD_DIM, Epilogue, _ptr, _stream, _usable
+from ._tensors import require
+from .fused import ATTENTION_HEAD_DIM, Epilogue, _ptr, _usable
 
 BLOCK = 32
 _FORMATS = {"fp8": 8, "fp4": 4}
@@ -41,15 +40,18 @@ def _type(dtype: torch.dtype, what: str) -> int:
     return _TYPES[dtype]
 
 
-def _on(device: torch.device):
-    """The device of a call's tensors as the current one."""
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def _launch(index: int, name: str, *args) -> bool:
+    """Entry point ``name`` on the current stream of GPU ``index``, the one its tensors are on."""
+    fn = getattr(_native.lib(), name)
+    if index == torch._C._cuda_getDevice():
+        return _native.check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+    with torch.cuda.device(index):
+        return _native.check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
 
 
-def _bytes(t: torch.Tensor, name: str, shape: Sequence[int], align: int) -> torch.Tensor:
-    require(t, name, t.device, shape, torch.uint8)
+def _bytes(t: torch.Tensor, name: str, device: torch.device, shape: Sequence[int],
+           align: int) -> torch.Tensor:
+    require(t, name, device, shape, torch.uint8)
     t = t.contiguous()
     return t if t.data_ptr() % align == 0 else t.clone()
 
@@ -63,34 +65,52 @@ class Tensor:
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, format: str, shape: Sequence[int]):
         bits = _format(format)
-        self.shape = torch.Size(shape)
+        self.shape, self.format = torch.Size(shape), format
         if not self.shape:
             raise ValueError("a microscaled tensor has at least one axis")
-        rows, groups = self.shape[:-1].numel(), -(-self.shape[-1] // 128)
         for t in (codes, scales):
             if not isinstance(t, torch.Tensor) or not t.is_cuda:
                 raise ValueError("codes and scales must be tensors on a GPU")
-        self.codes = _bytes(codes, "codes", (rows, groups * 16 * bits), 16)
-        require(scales, "scales", codes.device, (rows, groups * 4), torch.uint8)
-        self.scales = _bytes(scales, "scales", (rows, groups * 4), 4)
-        self.format = format
+        self.rows, groups = self.shape[:-1].numel(), -(-self.shape[-1] // 128)
+        self._codes = _bytes(codes, "codes", codes.device, (self.rows, groups * 16 * bits), 16)
+        self._scales = _bytes(scales, "scales", codes.device, (self.rows, groups * 4), 4)
+        self._whole = None
 
     @classmethod
-    def _empty(cls, shape: Sequence[int], format: str, device: torch.device) -> "Tensor":
+    def _empty(cls, shape: torch.Size, rows: int, format: str, device: torch.device) -> "Tensor":
+        """Room for ``rows`` rows, codes and scales in one allocation."""
         self = cls.__new__(cls)
-        self.shape, self.format = torch.Size(shape), format
-        rows, groups = self.rows, -(-self.shape[-1] // 128)
-        self.codes = torch.empty((rows, groups * 16 * _FORMATS[format]), dtype=torch.uint8, device=device)
-        self.scales = torch.empty((rows, groups * 4), dtype=torch.uint8, device=device)
+        self.shape, self.rows, self.format = shape, rows, format
+        self._codes = self._scales = None
+        self._whole = torch.empty(rows * -(-shape[-1] // 128) * (16 * _FORMATS[format] + 4),
+                                  dtype=torch.uint8, device=device)
         return self
 
+    def _split(self) -> int:
+        return self.rows * -(-self.shape[-1] // 128) * 16 * _FORMATS[self.format]
+
+    def _pointers(self) -> tuple[int, int]:
+        if self._whole is None:
+            return self._codes.data_ptr(), self._scales.data_ptr()
+        at = self._whole.data_ptr()
+        return at, at + self._split()
+
     @property
-    def rows(self) -> int:
-        return self.shape[:-1].numel()
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            self._codes = self._whole[:self._split()].view(
+                self.rows, -(-self.shape[-1] // 128) * 16 * _FORMATS[self.format])
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            self._scales = self._whole[self._split():].view(self.rows, -(-self.shape[-1] // 128) * 4)
+        return self._scales
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return (self._codes if self._whole is None else self._whole).device
 
     def values(self, dtype: torch.dtype = torch.float32) -> Optional[torch.Tensor]:
         """The values that the codes stand for, ``shape`` in ``dtype`` (16 bits hold all but those at
@@ -98,12 +118,11 @@ class Tensor:
         kind = _type(dtype, "dtype")
         if not _usable():
             return None
-        out = torch.empty(self.shape, dtype=dtype, device=self.device)
-        with _on(self.device):
-            rc = _native.lib().ancha_hip_mx_values(
-                self.codes.data_ptr(), self.scales.data_ptr(), self.rows, self.shape[-1],
-                _FORMATS[self.format], kind, out.data_ptr(), _stream())
-        return out if _native.check(rc) else None
+        device = self.device
+        out = torch.empty(self.shape, dtype=dtype, device=device)
+        codes, scales = self._pointers()
+        return out if _launch(device.index, "ancha_hip_mx_values", codes, scales, self.rows,
+                              self.shape[-1], _FORMATS[self.format], kind, out.data_ptr()) else None
 
 
 class Weight:
@@ -122,26 +141,23 @@ class Weight:
         if not _usable():
             return None
         out = torch.empty(self.shape, dtype=dtype, device=self.device)
-        with _on(self.device):
-            rc = _native.lib().ancha_hip_mx_weight_values(
-                self._data.data_ptr(), *self.shape, kind, out.data_ptr(), _stream())
-        return out if _native.check(rc) else None
+        return out if _launch(self.device.index, "ancha_hip_mx_weight_values", self._data.data_ptr(),
+                              *self.shape, kind, out.data_ptr()) else None
 
 
-def _flat(t: torch.Tensor) -> torch.Tensor:
-    """t as [rows, dim] with neighbouring columns (a view where its layout allows one)."""
-    flat = t if t.dim() == 2 else t.reshape(-1, t.shape[-1]) if t.numel() else \
-        t.reshape(t.shape[:-1].numel(), t.shape[-1])
-    if flat.shape[0] > 1 and flat.stride(0) < flat.shape[1] or flat.shape[1] > 1 and flat.stride(1) != 1:
-        flat = flat.contiguous()
-    return flat
+def _rows(t: torch.Tensor, dim: int, rows: int) -> tuple[torch.Tensor, int]:
+    """t [..., dim] as ``rows`` rows of neighbouring columns (a view where its layout allows one) and
+    their stride."""
+    if t.is_contiguous():
+        return t, dim
+    flat = t if t.dim() == 2 else t.reshape(rows, dim)
+    stride = flat.stride()
+    if (rows > 1 and stride[0] < dim) or (dim > 1 and stride[1] != 1):
+        return flat.contiguous(), dim
+    return flat, stride[0] if rows > 1 else dim
 
 
-def _stride(flat: torch.Tensor) -> int:
-    return max(flat.stride(0), flat.shape[1]) if flat.shape[0] > 1 else flat.shape[1]
-
-
-def _rows_op(x: torch.Tensor, name: str) -> Optional[int]:
+def _input(x: torch.Tensor, name: str) -> Optional[int]:
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise ValueError(f"{name} must be a tensor on a GPU")
     if x.dim() == 0:
@@ -151,37 +167,40 @@ def _rows_op(x: torch.Tensor, name: str) -> Optional[int]:
 
 def quantize(x: torch.Tensor, format: str = "fp4") -> Optional[Tensor]:
     """``x`` [..., dim] in blocks of 32 along its last axis."""
-    bits, kind = _format(format), _rows_op(x, "x")
+    bits, kind = _format(format), _input(x, "x")
     if kind is None:
         return None
-    flat = _flat(x)
-    out = Tensor._empty(x.shape, format, x.device)
-    with _on(x.device):
-        rc = _native.lib().ancha_hip_mx_quantize(
-            flat.data_ptr(), kind, flat.shape[0], flat.shape[1], _stride(flat), bits,
-            out.codes.data_ptr(), out.scales.data_ptr(), _stream())
-    return out if _native.check(rc) else None
+    shape = x.shape
+    dim = shape[-1]
+    rows = shape[:-1].numel()
+    flat, ld = _rows(x, dim, rows)
+    out = Tensor._empty(shape, rows, format, x.device)
+    codes, scales = out._pointers()
+    return out if _launch(x.get_device(), "ancha_hip_mx_quantize", flat.data_ptr(), kind, rows, dim, ld,
+                          bits, codes, scales) else None
 
 
 def _norm(x, residual, scale, eps, format):
-    bits, kind = _format(format), _rows_op(x, "x")
+    bits, kind = _format(format), _input(x, "x")
     if kind is None:
         return None, None
-    dim = x.shape[-1]
-    require_optional(scale, "scale", x.device, (dim,))
-    flat, total, other = _flat(x), None, None
+    shape, device = x.shape, x.device
+    dim = shape[-1]
+    rows = shape[:-1].numel()
+    if scale is not None:
+        require(scale, "scale", device, (dim,))
+        scale = scale.contiguous()
+    flat, ld = _rows(x, dim, rows)
+    total, ldr = None, 0
     if residual is not None:
-        require(residual, "residual", x.device, x.shape, x.dtype)
-        other = _flat(residual)
-        total = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    out = Tensor._empty(x.shape, format, x.device)
-    s = None if scale is None else scale.contiguous()
-    with _on(x.device):
-        rc = _native.lib().ancha_hip_mx_norm(
-            flat.data_ptr(), kind, flat.shape[0], dim, _stride(flat), _ptr(other),
-            0 if other is None else _stride(other), _ptr(s), float(eps), bits, _ptr(total),
-            out.codes.data_ptr(), out.scales.data_ptr(), _stream())
-    return (out, total) if _native.check(rc) else (None, None)
+        require(residual, "residual", device, shape, x.dtype)
+        residual, ldr = _rows(residual, dim, rows)
+        total = torch.empty(shape, dtype=x.dtype, device=device)
+    out = Tensor._empty(shape, rows, format, device)
+    codes, scales = out._pointers()
+    done = _launch(device.index, "ancha_hip_mx_norm", flat.data_ptr(), kind, rows, dim, ld, _ptr(residual),
+                   ldr, _ptr(scale), float(eps), bits, _ptr(total), codes, scales)
+    return (out, total) if done else (None, None)
 
 
 def unit_norm(x: torch.Tensor, scale: Optional[torch.Tensor] = None, eps: float = 0.0,
@@ -207,7 +226,7 @@ def weight(w: torch.Tensor) -> Optional[Weight]:
     """The [k, m] weight ``w`` (Burn Linear layout as in :func:`ancha_amd.fused.linear`; the transposed
     view of a PyTorch [out, in] weight is as good) in e2m1 with blocks of 32 along k. Made once, when a
     model is loaded."""
-    kind = _rows_op(w, "w")
+    kind = _input(w, "w")
     if w.dim() != 2:
         raise ValueError(f"w must be [k, m], got {tuple(w.shape)}")
     if kind is None:
@@ -219,10 +238,8 @@ def weight(w: torch.Tensor) -> Optional[Weight]:
     if min(w.stride()) < 0 or (0 in w.stride()):
         w = w.contiguous()
     data = torch.empty(size, dtype=torch.uint8, device=w.device)
-    with _on(w.device):
-        rc = _native.lib().ancha_hip_mx_weight(w.data_ptr(), kind, k, m, *w.stride(), data.data_ptr(),
-                                               _stream())
-    return Weight(data, k, m) if _native.check(rc) else None
+    return Weight(data, k, m) if _launch(w.get_device(), "ancha_hip_mx_weight", w.data_ptr(), kind, k, m,
+                                         *w.stride(), data.data_ptr()) else None
 
 
 def linear(x: Tensor, w: Weight, epilogue: Optional[Epilogue] = None,
@@ -236,43 +253,44 @@ def linear(x: Tensor, w: Weight, epilogue: Optional[Epilogue] = None,
     the matrix cores' shorter sums (4e-6 of the result on normal data, far below the type's step)."""
     if not isinstance(x, Tensor) or not isinstance(w, Weight):
         raise ValueError("linear takes a microscaled Tensor and a Weight")
-    e = epilogue or Epilogue()
     kind = _type(dtype, "dtype")
     bits = 0 if format is None else _format(format)
     if bits and dtype != torch.float32:
         raise ValueError("an output in codes is taken from the float32 result: leave dtype alone")
-    n, (k, m) = x.rows, w.shape
+    n, device, (k, m) = x.rows, x.device, w.shape
     if x.shape[-1] != k:
         raise ValueError(f"x has rows of {x.shape[-1]}, the weight takes {k}")
-    if w.device != x.device:
-        raise ValueError(f"the weight must be on {x.device}, got {w.device}")
+    if w.device != device:
+        raise ValueError(f"the weight must be on {device}, got {w.device}")
     shape = x.shape[:-1] + (m,)
-    tokens = width = 0
-    table = None
-    if e.rotary is not None:
-        table, width = e.rotary
-        require(table, "rotary table", x.device)
-        if table.dim() != 3 or table.shape[0] != 4 or table.shape[2] != ATTENTION_HEAD_DIM:
-            return None
-        tokens = table.shape[1]
-        if tokens == 0 or n % tokens or width < 0 or width % 64 or 2 * width > m:
-            return None
-        table = table.contiguous()
-    require_optional(e.bias, "bias", x.device, (m,))
-    require_optional(e.residual, "residual", x.device, shape, dtype)
-    bias = None if e.bias is None else e.bias.contiguous()
-    residual = None if e.residual is None else e.residual.contiguous()
+    bias = residual = table = None
+    gelu = tokens = width = 0
+    if epilogue is not None:
+        bias, residual, gelu = epilogue.bias, epilogue.residual, int(epilogue.gelu)
+        if epilogue.rotary is not None:
+            table, width = epilogue.rotary
+            require(table, "rotary table", device)
+            if table.dim() != 3 or table.shape[0] != 4 or table.shape[2] != ATTENTION_HEAD_DIM:
+                return None
+            tokens = table.shape[1]
+            if tokens == 0 or n % tokens or width < 0 or width % 64 or 2 * width > m:
+                return None
+            table = table.contiguous()
+        if bias is not None:
+            require(bias, "bias", device, (m,))
+            bias = bias.contiguous()
+        if residual is not None:
+            require(residual, "residual", device, shape, dtype)
+            residual = residual.contiguous()
     if not _usable():
         return None
     if bits:
-        out = Tensor._empty(shape, format, x.device)
-        to, scales = out.codes.data_ptr(), out.scales.data_ptr()
+        out = Tensor._empty(shape, n, format, device)
+        to, to_scales = out._pointers()
     else:
-        out = torch.empty(shape, dtype=dtype, device=x.device)
-        to, scales = out.data_ptr(), None
-    with _on(x.device):
-        rc = _native.lib().ancha_hip_mx_linear(
-            x.codes.data_ptr(), x.scales.data_ptr(), n, k, _FORMATS[x.format], w._data.data_ptr(), m,
-            _ptr(bias), int(e.gelu), _ptr(table), tokens, width, _ptr(residual), kind, bits, to, scales,
-            _stream())
-    return out if _native.check(rc) else None
+        out = torch.empty(shape, dtype=dtype, device=device)
+        to, to_scales = out.data_ptr(), None
+    codes, scales = x._pointers()
+    return out if _launch(device.index, "ancha_hip_mx_linear", codes, scales, n, k, _FORMATS[x.format],
+                          w._data.data_ptr(), m, _ptr(bias), gelu, _ptr(table), tokens, width,
+                          _ptr(residual), kind, bits, to, to_scales) else None

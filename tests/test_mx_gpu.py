@@ -150,7 +150,7 @@ def test_norm_layouts_and_sums_in_place(gpu):
         for place in ("x", "residual"):
             x, r = dev(rows_of((9, dim), 15), gpu), dev(W.normal((9, dim), 16, 1.0), gpu)
             want = x + r
-            out = mx.Tensor._empty((9, dim), "fp8", gpu)
+            out = mx.Tensor._empty(torch.Size((9, dim)), 9, "fp8", gpu)
             total = x if place == "x" else r
             rc = lib.ancha_hip_mx_norm(x.data_ptr(), 0, 9, dim, dim, r.data_ptr(), dim, None, 0.0, 8,
                                        total.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), stream)
@@ -497,6 +497,7 @@ def test_offsets_past_32_bits(gpu):
     back = got.values(torch.bfloat16)
     assert torch.equal(back[-1000:], tail.values(torch.bfloat16))
     del x, back, normed
+    # The product of the last rows against 64 bits (a call on them alone may add up in another order).
     w = mx.weight(dev(W.normal((dim, 130), 113, 0.02), gpu))
-    y, z = mx.linear(got, w), mx.linear(tail, w)
-    assert torch.equal(y[-1000:], z)
+    y, tol = expected(host(tail.values()), host(w.values()), "fp8", False)
+    near("last rows", host(mx.linear(got, w)[-1000:]), y, tol)
