@@ -113,14 +113,14 @@ __device__ __forceinline__ void store_values(const LinearParams& p, const Rows<O
   } else {
     const unsigned off = c < p.m ? ((unsigned)r * (unsigned)p.m + c) * d.kSize : 0x80000000u;
     if constexpr (OUT == kF32) {
-      bstore4<true>(d.out, off, make_float4(v[0], v[1], v[2], v[3]));
+      bstore4<true, kStream>(d.out, off, make_float4(v[0], v[1], v[2], v[3]));
     } else {
       typename Stored<OUT>::type t[4];
 #pragma unroll
       for (int i = 0; i < 4; i++) t[i] = (typename Stored<OUT>::type)v[i];
       u32x2 w;
       __builtin_memcpy(&w, t, 8);
-      __builtin_amdgcn_raw_buffer_store_b64(w, d.out, off, 0, 0);
+      __builtin_amdgcn_raw_buffer_store_b64(w, d.out, off, 0, kStream);
     }
   }
 }

@@ -8,16 +8,31 @@ namespace {
 
 constexpr int kThreads = 256;
 
-template <int TYPE>
+// The unit of eight neighbouring values that a thread has: L threads side by side in a row, 256 / L rows a
+// workgroup, column pieces of 8 L along the grid's second axis.
+struct Unit {
+  unsigned row;
+  int col;
+  long at;  // among the units of the codes
+};
+template <int L>
+__device__ __forceinline__ Unit my_unit(int dim) {
+  Unit u;
+  u.row = blockIdx.x * (unsigned)(kThreads / L) + threadIdx.x / L;
+  const int c = (int)blockIdx.y * L + (int)threadIdx.x % L;
+  u.col = 8 * c;
+  u.at = (long)u.row * (16 * groups(dim)) + c;
+  return u;
+}
+
+template <int TYPE, int FORMAT, int L>
 __global__ __launch_bounds__(kThreads) void quantize_kernel(RowParams p) {
-  const unsigned per_row = 16u * (unsigned)groups(p.dim);
-  const unsigned unit = blockIdx.x * (unsigned)kThreads + threadIdx.x;
-  const unsigned row = unit / per_row;
-  const int col = 8 * (int)(unit - row * per_row);
-  const bool here = row < (unsigned)p.rows;
+  const Unit u = my_unit<L>(p.dim);
+  const bool here = u.row < (unsigned)p.rows && u.col < kGroup * (int)groups(p.dim);
+  const int valid = here ? p.dim - u.col : 0;
   float v[8];
-  load_row<TYPE, 8>(p.x, here ? (long)row * p.ldx + col : 0, here ? p.dim - col : 0, v);
-  store_codes(v, p.format, here, unit, p.codes, p.scales);
+  load_row<TYPE, 8>(p.x, valid > 0 ? (long)u.row * p.ldx + u.col : 0, valid, v);
+  store_codes(v, FORMAT, here, u.at, p.codes, p.scales);
 }
 
 // Sum over L lanes (a power of two up to 64) in 64 bits.
@@ -51,25 +66,63 @@ __device__ __forceinline__ float rounded(float x) {
   return (float)(typename Stored<TYPE>::type)x;
 }
 
-// One row by L threads, eight neighbouring values each, V times; a workgroup of 256 threads.
+// Eight values h of a row from column col on through the norm, rounded to odd; whole: all exist.
+__device__ __forceinline__ void normed(const RowParams& p, const float* h, double inv, int col, bool whole,
+                                       float* y) {
+  if (p.scale) {
+    float s[8];
+    load_row<kF32, 8>(p.scale, whole || col < p.dim ? col : 0, whole ? 8 : p.dim - col, s);
+#pragma unroll
+    for (int j = 0; j < 8; j++) y[j] = to_odd((double)h[j] * inv * (double)s[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) y[j] = to_odd((double)h[j] * inv);
+  }
+  // Behind the last value: zeros, also where inv is not finite.
+  if (!whole)
+#pragma unroll
+    for (int j = 0; j < 8; j++) y[j] = col + j < p.dim ? y[j] : 0.f;
+}
+
+// One row by L threads, eight neighbouring values each, V times; a workgroup of 256 threads. A piece of 8 L
+// columns that all exist is read and written without a mask (threads behind the last row read that one).
 template <int TYPE, int L, int V>
 __global__ __launch_bounds__(kThreads) void norm_kernel(RowParams p) {
   const int at = threadIdx.x % L;
-  const unsigned row = blockIdx.x * (unsigned)(kThreads / L) + threadIdx.x / L;
-  const bool here = row < (unsigned)p.rows;
+  const unsigned mine = blockIdx.x * (unsigned)(kThreads / L) + threadIdx.x / L;
+  const bool here = mine < (unsigned)p.rows;
+  const long row = here ? mine : p.rows - 1;
   const int padded = kGroup * (int)groups(p.dim);
+  typedef typename Stored<TYPE>::type T;
+  T x[V][8], r[V][8];  // all of the row's loads in flight before the first use
+#pragma unroll
+  for (int i = 0; i < V; i++) {
+    const int col = 8 * (at + L * i);
+    if (8 * L * (i + 1) <= p.dim) {
+      load_stored<TYPE, 8>(p.x, row * p.ldx + col, 8, x[i]);
+      if (p.residual) load_stored<TYPE, 8>(p.residual, row * p.ldr + col, 8, r[i]);
+    } else {
+      const int valid = p.dim - col;
+      load_stored<TYPE, 8>(p.x, row * p.ldx + (valid > 0 ? col : 0), valid, x[i]);
+      if (p.residual) load_stored<TYPE, 8>(p.residual, row * p.ldr + (valid > 0 ? col : 0), valid, r[i]);
+    }
+  }
   float h[V][8];
   double ss = 0.0;
 #pragma unroll
   for (int i = 0; i < V; i++) {
-    const int col = 8 * (at + L * i), valid = here ? p.dim - col : 0;
-    load_row<TYPE, 8>(p.x, valid > 0 ? (long)row * p.ldx + col : 0, valid, h[i]);
-    if (p.residual) {
-      float r[8];
-      load_row<TYPE, 8>(p.residual, valid > 0 ? (long)row * p.ldr + col : 0, valid, r);
+    const int col = 8 * (at + L * i);
 #pragma unroll
-      for (int j = 0; j < 8; j++) h[i][j] = rounded<TYPE>(h[i][j] + r[j]);
-      store_row<TYPE, 8>(p.sum, valid > 0 ? (long)row * p.dim + col : 0, valid, h[i]);
+    for (int j = 0; j < 8; j++) h[i][j] = (float)x[i][j];
+    if (p.residual) {
+#pragma unroll
+      for (int j = 0; j < 8; j++) h[i][j] = rounded<TYPE>(h[i][j] + (float)r[i][j]);
+      const int valid = here ? p.dim - col : 0;
+      if (8 * L * (i + 1) <= p.dim) {
+        if (here) store_row<TYPE, 8>(p.sum, row * p.dim + col, 8, h[i]);
+      } else {
+        store_row<TYPE, 8>(p.sum, row * p.dim + (valid > 0 ? col : 0), valid, h[i]);
+      }
     }
 #pragma unroll
     for (int j = 0; j < 8; j++) ss = __builtin_fma((double)h[i][j], (double)h[i][j], ss);
@@ -84,15 +137,12 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(RowParams p) {
     for (int w = 0; w < kThreads / 64; w++) ss += part[w];
   }
   const double inv = inverse_length(ss + (double)p.dim * p.eps);
-  const long first = (long)row * (padded / 8);
+  const long first = row * (padded / 8);
 #pragma unroll
   for (int i = 0; i < V; i++) {
     const int col = 8 * (at + L * i);
-    float s[8], y[8];
-    if (p.scale) load_row<kF32, 8>(p.scale, col < p.dim ? col : 0, p.dim - col, s);
-#pragma unroll
-    for (int j = 0; j < 8; j++)
-      y[j] = col + j < p.dim ? to_odd((double)h[i][j] * inv * (p.scale ? (double)s[j] : 1.0)) : 0.f;
+    float y[8];
+    normed(p, h[i], inv, col, 8 * L * (i + 1) <= p.dim, y);
     store_codes(y, p.format, here && col < padded, first + at + L * i, p.codes, p.scales);
   }
 }
@@ -129,27 +179,21 @@ __global__ __launch_bounds__(kThreads) void norm_long_kernel(RowParams p) {
   const void* from = p.residual ? p.sum : p.x;
   const long ld = p.residual ? p.dim : p.ldx;
   for (int col = 8 * threadIdx.x; col < padded; col += 8 * kThreads) {
-    float h[8], s[8], y[8];
+    float h[8], y[8];
     load_row<TYPE, 8>(from, col < p.dim ? (long)row * ld + col : 0, p.dim - col, h);
-    if (p.scale) load_row<kF32, 8>(p.scale, col < p.dim ? col : 0, p.dim - col, s);
-#pragma unroll
-    for (int j = 0; j < 8; j++)
-      y[j] = col + j < p.dim ? to_odd((double)h[j] * inv * (p.scale ? (double)s[j] : 1.0)) : 0.f;
+    normed(p, h, inv, col, col + 8 <= p.dim, y);
     store_codes(y, p.format, true, first + col / 8, p.codes, p.scales);
   }
 }
 
-template <int TYPE>
+template <int TYPE, int FORMAT, int L>
 __global__ __launch_bounds__(kThreads) void values_kernel(ValueParams p) {
-  const unsigned per_row = 16u * (unsigned)groups(p.dim);
-  const unsigned unit = blockIdx.x * (unsigned)kThreads + threadIdx.x;
-  const unsigned row = unit / per_row;
-  const int col = 8 * (int)(unit - row * per_row);
-  if (row >= (unsigned)p.rows || col >= p.dim) return;
-  const float f = scale_value(p.scales[unit >> 2]);
+  const Unit u = my_unit<L>(p.dim);
+  if (u.row >= (unsigned)p.rows || u.col >= p.dim) return;
+  const float f = scale_value(p.scales[u.at >> 2]);
   float v[8];
-  if (p.format == kFp8) {
-    const u32x2 c = *reinterpret_cast<const u32x2*>(p.codes + (long)unit * 8);
+  if constexpr (FORMAT == kFp8) {
+    const u32x2 c = *reinterpret_cast<const u32x2*>(p.codes + u.at * 8);
 #pragma unroll
     for (int i = 0; i < 2; i++) {
       const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(c[i], false);
@@ -157,7 +201,7 @@ __global__ __launch_bounds__(kThreads) void values_kernel(ValueParams p) {
       v[4 * i] = a[0], v[4 * i + 1] = a[1], v[4 * i + 2] = b[0], v[4 * i + 3] = b[1];
     }
   } else {
-    const unsigned c = *reinterpret_cast<const unsigned*>(p.codes + (long)unit * 4);
+    const unsigned c = *reinterpret_cast<const unsigned*>(p.codes + u.at * 4);
     const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 0);
     const auto b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 1);
     const auto d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 2);
@@ -167,7 +211,7 @@ __global__ __launch_bounds__(kThreads) void values_kernel(ValueParams p) {
   }
 #pragma unroll
   for (int i = 0; i < 8; i++) v[i] *= f;
-  store_row<TYPE, 8>(p.out, (long)row * p.dim + col, p.dim - col, v);
+  store_row<TYPE, 8>(p.out, (long)u.row * p.dim + u.col, p.dim - u.col, v);
 }
 
 template <int TYPE, int L, int V>
@@ -191,20 +235,56 @@ void norm_of_type(const RowParams& p, hipStream_t stream) {
   hipLaunchKernelGGL(norm_long_kernel<TYPE>, dim3(p.rows), dim3(kThreads), 0, stream, p);
 }
 
+template <int L>
 dim3 unit_grid(long rows, long dim) {
-  return dim3((unsigned)((rows * 16 * groups(dim) + kThreads - 1) / kThreads));
+  constexpr long kRows = kThreads / L;
+  return dim3((unsigned)((rows + kRows - 1) / kRows), (unsigned)((16 * groups(dim) + L - 1) / L));
+}
+
+// Rows of up to 512 values by 16 threads a piece, up to 2048 by 64: full lines, and few idle threads.
+template <int TYPE, int FORMAT>
+void quantize_to(const RowParams& p, hipStream_t stream) {
+  if (p.dim <= 512)
+    hipLaunchKernelGGL((quantize_kernel<TYPE, FORMAT, 16>), unit_grid<16>(p.rows, p.dim), dim3(kThreads), 0,
+                       stream, p);
+  else if (p.dim <= 2048)
+    hipLaunchKernelGGL((quantize_kernel<TYPE, FORMAT, 64>), unit_grid<64>(p.rows, p.dim), dim3(kThreads), 0,
+                       stream, p);
+  else
+    hipLaunchKernelGGL((quantize_kernel<TYPE, FORMAT, 256>), unit_grid<256>(p.rows, p.dim), dim3(kThreads),
+                       0, stream, p);
+}
+
+template <int TYPE, int FORMAT>
+void values_of(const ValueParams& p, hipStream_t stream) {
+  if (p.dim <= 512)
+    hipLaunchKernelGGL((values_kernel<TYPE, FORMAT, 16>), unit_grid<16>(p.rows, p.dim), dim3(kThreads), 0,
+                       stream, p);
+  else if (p.dim <= 2048)
+    hipLaunchKernelGGL((values_kernel<TYPE, FORMAT, 64>), unit_grid<64>(p.rows, p.dim), dim3(kThreads), 0,
+                       stream, p);
+  else
+    hipLaunchKernelGGL((values_kernel<TYPE, FORMAT, 256>), unit_grid<256>(p.rows, p.dim), dim3(kThreads), 0,
+                       stream, p);
 }
 
 }  // namespace
 
-hipError_t launch_quantize(const RowParams& p, hipStream_t stream) {
-  const dim3 grid = unit_grid(p.rows, p.dim);
-  if (p.type == kF32)
-    hipLaunchKernelGGL(quantize_kernel<kF32>, grid, dim3(kThreads), 0, stream, p);
-  else if (p.type == kF16)
-    hipLaunchKernelGGL(quantize_kernel<kF16>, grid, dim3(kThreads), 0, stream, p);
+template <int TYPE>
+static void start_quantize(const RowParams& p, hipStream_t stream) {
+  if (p.format == kFp8)
+    quantize_to<TYPE, kFp8>(p, stream);
   else
-    hipLaunchKernelGGL(quantize_kernel<kBf16>, grid, dim3(kThreads), 0, stream, p);
+    quantize_to<TYPE, kFp4>(p, stream);
+}
+
+hipError_t launch_quantize(const RowParams& p, hipStream_t stream) {
+  if (p.type == kF32)
+    start_quantize<kF32>(p, stream);
+  else if (p.type == kF16)
+    start_quantize<kF16>(p, stream);
+  else
+    start_quantize<kBf16>(p, stream);
   return hipGetLastError();
 }
 
@@ -218,14 +298,21 @@ hipError_t launch_norm(const RowParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-hipError_t launch_values(const ValueParams& p, hipStream_t stream) {
-  const dim3 grid = unit_grid(p.rows, p.dim);
-  if (p.type == kF32)
-    hipLaunchKernelGGL(values_kernel<kF32>, grid, dim3(kThreads), 0, stream, p);
-  else if (p.type == kF16)
-    hipLaunchKernelGGL(values_kernel<kF16>, grid, dim3(kThreads), 0, stream, p);
+template <int TYPE>
+static void start_values(const ValueParams& p, hipStream_t stream) {
+  if (p.format == kFp8)
+    values_of<TYPE, kFp8>(p, stream);
   else
-    hipLaunchKernelGGL(values_kernel<kBf16>, grid, dim3(kThreads), 0, stream, p);
+    values_of<TYPE, kFp4>(p, stream);
+}
+
+hipError_t launch_values(const ValueParams& p, hipStream_t stream) {
+  if (p.type == kF32)
+    start_values<kF32>(p, stream);
+  else if (p.type == kF16)
+    start_values<kF16>(p, stream);
+  else
+    start_values<kBf16>(p, stream);
   return hipGetLastError();
 }
 

@@ -5,34 +5,81 @@ namespace ancha {
 namespace mx {
 namespace {
 
-// One fragment (16 columns x 128 k) per wave: lane l quantises column l % 16, k 32 (l / 16) .. + 31.
-// The four waves of a workgroup have the four fragments of a strip and group.
+// Column and k block of value (c, k) in a strip and group; 16 bytes of codes per column and block.
+__device__ __forceinline__ long code_place(long piece, int c, int block) {
+  return piece * kStripCodes + (c >> 4) * 1024 + ((c & 15) + 16 * block) * 16;
+}
+__device__ __forceinline__ long scale_place(long pieces, long piece, int c, int block) {
+  return pieces * kStripCodes + piece * kStripScales + ((c & 15) + 16 * block) * 4 + (c >> 4);
+}
+
+// A strip (64 columns) and group (128 k) per workgroup, any layout: lane l of wave b has column l, k block
+// b. Neighbouring lanes read neighbouring columns, so [in, out] weights are read in whole lines.
 template <int TYPE>
-__global__ __launch_bounds__(256) void weight_kernel(WeightParams p) {
+__global__ __launch_bounds__(256) void weight_columns_kernel(WeightParams p) {
   typedef typename Stored<TYPE>::type T;
-  const int lane = threadIdx.x & 63, tile = threadIdx.x >> 6;
+  const int c = threadIdx.x & 63, block = threadIdx.x >> 6;
   const unsigned steps = (unsigned)groups(p.k);
   const unsigned strip = blockIdx.x / steps, step = blockIdx.x - strip * steps;
-  const int col = (int)strip * 64 + 16 * tile + (lane & 15);
-  const int k0 = (int)step * kGroup + 32 * (lane >> 4);
-  const T* x = static_cast<const T*>(p.x) + (long)col * p.ldm;
+  const int col = (int)strip * 64 + c, k0 = (int)step * kGroup + 32 * block;
+  const T* x = static_cast<const T*>(p.x) + (long)min(col, p.m - 1) * p.ldm;
+  T t[32];
+#pragma unroll
+  for (int i = 0; i < 32; i++) t[i] = x[(long)min(k0 + i, p.k - 1) * p.ldk];
   float v[32];
   unsigned top = 0;
 #pragma unroll
   for (int i = 0; i < 32; i++) {
-    v[i] = col < p.m && k0 + i < p.k ? (float)x[(long)(k0 + i) * p.ldk] : 0.f;
+    v[i] = col < p.m && k0 + i < p.k ? (float)t[i] : 0.f;
     top = max(top, magnitude(v[i]));
   }
   const unsigned s = scale_byte(top, kFp4);
   const float f = unscale(s);
 #pragma unroll
   for (int i = 0; i < 32; i++) v[i] *= f;
-  u32x4 c;
+  u32x4 q;
 #pragma unroll
-  for (int i = 0; i < 4; i++) c[i] = s == 255u ? 0u : codes_fp4(v + 8 * i);
-  const long piece = (long)blockIdx.x;
-  *reinterpret_cast<u32x4*>(p.weight + piece * kStripCodes + tile * 1024 + lane * 16) = c;
-  p.weight[(long)gridDim.x * kStripCodes + piece * kStripScales + lane * 4 + tile] = (uint8_t)s;
+  for (int i = 0; i < 4; i++) q[i] = s == 255u ? 0u : codes_fp4(v + 8 * i);
+  *reinterpret_cast<u32x4*>(p.weight + code_place(blockIdx.x, c, block)) = q;
+  p.weight[scale_place(gridDim.x, blockIdx.x, c, block)] = (uint8_t)s;
+}
+
+// The same for a weight whose columns are contiguous along k ([out, in] storage): sixteen lanes have the
+// 128 k of a column, eight neighbouring values each, a wave four columns at a time.
+template <int TYPE>
+__global__ __launch_bounds__(256) void weight_rows_kernel(WeightParams p) {
+  typedef typename Stored<TYPE>::type T;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15;
+  const unsigned steps = (unsigned)groups(p.k);
+  const unsigned strip = blockIdx.x / steps, step = blockIdx.x - strip * steps;
+  const int k = (int)step * kGroup + 8 * j;
+  T t[4][8];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int col = (int)strip * 64 + 16 * wave + 4 * i + (lane >> 4);
+    const int valid = col < p.m ? p.k - k : 0;
+    load_stored<TYPE, 8>(p.x, valid > 0 ? (long)col * p.ldm + k : 0, valid, t[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int c = 16 * wave + 4 * i + (lane >> 4);
+    float v[8];
+    unsigned top = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      v[e] = (float)t[i][e];
+      top = max(top, magnitude(v[e]));
+    }
+    top = max(top, dpp<kSwap1>(top));
+    top = max(top, dpp<kSwap2>(top));
+    const unsigned s = scale_byte(top, kFp4);
+    const float f = unscale(s);
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] *= f;
+    *reinterpret_cast<unsigned*>(p.weight + code_place(blockIdx.x, c, j >> 2) + 4 * (j & 3)) =
+        s == 255u ? 0u : codes_fp4(v);
+    if ((j & 3) == 0) p.weight[scale_place(gridDim.x, blockIdx.x, c, j >> 2)] = (uint8_t)s;
+  }
 }
 
 // A strip and group per workgroup: lane l of wave `tile` decodes its 32 values.
@@ -65,14 +112,22 @@ __global__ __launch_bounds__(256) void weight_values_kernel(WeightValueParams p)
 
 }  // namespace
 
-hipError_t launch_weight(const WeightParams& p, hipStream_t stream) {
+template <int TYPE>
+static void start_weight(const WeightParams& p, hipStream_t stream) {
   const dim3 grid((unsigned)(strips(p.m) * groups(p.k)));
-  if (p.type == kF32)
-    hipLaunchKernelGGL(weight_kernel<kF32>, grid, dim3(256), 0, stream, p);
-  else if (p.type == kF16)
-    hipLaunchKernelGGL(weight_kernel<kF16>, grid, dim3(256), 0, stream, p);
+  if (p.ldk == 1)
+    hipLaunchKernelGGL(weight_rows_kernel<TYPE>, grid, dim3(256), 0, stream, p);
   else
-    hipLaunchKernelGGL(weight_kernel<kBf16>, grid, dim3(256), 0, stream, p);
+    hipLaunchKernelGGL(weight_columns_kernel<TYPE>, grid, dim3(256), 0, stream, p);
+}
+
+hipError_t launch_weight(const WeightParams& p, hipStream_t stream) {
+  if (p.type == kF32)
+    start_weight<kF32>(p, stream);
+  else if (p.type == kF16)
+    start_weight<kF16>(p, stream);
+  else
+    start_weight<kBf16>(p, stream);
   return hipGetLastError();
 }
 
