@@ -122,9 +122,9 @@ __device__ __forceinline__ unsigned scale_byte(unsigned top, int format) {
   return e == 255 ? 255u : (unsigned)max(e - (format == kFp8 ? 8 : 2), 0);
 }
 
-// 2^(127 - s): what a value is multiplied by before it is rounded (0 for the byte of a NaN block).
-__device__ __forceinline__ float unscale(unsigned s) {
-  return s == 255u ? 0.f : __builtin_bit_cast(float, (254u - s) << 23);
+// 2^(s - 127), by which the conversions divide (not for s = 255).
+__device__ __forceinline__ float divisor(unsigned s) {
+  return __builtin_bit_cast(float, s == 0u ? 0x00400000u : s << 23);
 }
 
 // 2^(s - 127), NaN for s = 255.
@@ -132,27 +132,31 @@ __device__ __forceinline__ float scale_value(unsigned s) {
   return __builtin_bit_cast(float, s == 255u ? 0x7fc00000u : s == 0u ? 0x00400000u : s << 23);
 }
 
-// Codes of four values that are already divided by their block's scale.
-__device__ __forceinline__ unsigned codes_fp8(float a, float b, float c, float d) {
-  a = __builtin_amdgcn_fmed3f(a, -448.f, 448.f);
-  b = __builtin_amdgcn_fmed3f(b, -448.f, 448.f);
-  c = __builtin_amdgcn_fmed3f(c, -448.f, 448.f);
-  d = __builtin_amdgcn_fmed3f(d, -448.f, 448.f);
-  const int low = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-  return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, low, true);
+// e4m3 codes of four values of a block with the scale byte s (f its divisor): the conversion makes a NaN
+// of what is rounded past 448, so the values stop there first.
+__device__ __forceinline__ unsigned codes_fp8(float a, float b, float c, float d, float f) {
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  const float most = 448.f * f;
+  a = __builtin_amdgcn_fmed3f(a, -most, most);
+  b = __builtin_amdgcn_fmed3f(b, -most, most);
+  c = __builtin_amdgcn_fmed3f(c, -most, most);
+  d = __builtin_amdgcn_fmed3f(d, -most, most);
+  s16x2 w = {0, 0};
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, a, b, f, false);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, c, d, f, true);
+  return __builtin_bit_cast(unsigned, w);
 }
 
-// Codes of eight values (the conversion saturates).
-__device__ __forceinline__ unsigned codes_fp4(const float* v) {
-  unsigned r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, v[0], v[1], 1.f, 0);
-  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], 1.f, 1);
-  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[4], v[5], 1.f, 2);
-  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6], v[7], 1.f, 3);
+// e2m1 codes of eight (four) values (the conversion saturates).
+__device__ __forceinline__ unsigned codes_fp4(const float* v, float f) {
+  unsigned r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, v[0], v[1], f, 0);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], f, 1);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[4], v[5], f, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6], v[7], f, 3);
 }
-
-__device__ __forceinline__ unsigned codes_fp4x4(float a, float b, float c, float d) {
-  const unsigned r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, a, b, 1.f, 0);
-  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, c, d, 1.f, 1);
+__device__ __forceinline__ unsigned codes_fp4x4(const float* v, float f) {
+  const unsigned r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, v[0], v[1], f, 0);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], f, 1);
 }
 
 // Eight consecutive values of a row held by one lane, a block by four neighbouring lanes, a group of
@@ -170,18 +174,15 @@ __device__ __forceinline__ void store_codes(const float* v, int format, bool sto
   unsigned all = s << (8 * (lane >> 2));
   all |= dpp<kMirror8>(all);
   all |= dpp<kMirror16>(all);
-  const float f = unscale(s);
-  float q[8];
-#pragma unroll
-  for (int i = 0; i < 8; i++) q[i] = v[i] * f;
+  const float f = divisor(s);
   const bool none = s == 255u;
   if (!store) return;
   if (format == kFp8) {
-    const u32x2 c = {none ? 0u : codes_fp8(q[0], q[1], q[2], q[3]),
-                     none ? 0u : codes_fp8(q[4], q[5], q[6], q[7])};
+    const u32x2 c = {none ? 0u : codes_fp8(v[0], v[1], v[2], v[3], f),
+                     none ? 0u : codes_fp8(v[4], v[5], v[6], v[7], f)};
     __builtin_nontemporal_store(c, reinterpret_cast<u32x2*>(codes + unit * 8));
   } else {
-    __builtin_nontemporal_store(none ? 0u : codes_fp4(q), reinterpret_cast<unsigned*>(codes + unit * 4));
+    __builtin_nontemporal_store(none ? 0u : codes_fp4(v, f), reinterpret_cast<unsigned*>(codes + unit * 4));
   }
   if (lane == 0) *reinterpret_cast<unsigned*>(scales + (unit >> 4) * 4) = all;
 }

@@ -149,7 +149,7 @@ __device__ __forceinline__ unsigned encode16(const float* v, unsigned* codes) {
   const auto both = __builtin_amdgcn_permlane16_swap(top, top, false, false);
   top = max((unsigned)both[0], (unsigned)both[1]);
   const unsigned s = scale_byte(top, OUT);
-  const float f = __builtin_bit_cast(float, s == 0u ? 0x00400000u : s << 23);
+  const float f = divisor(s);
   typedef short s16x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
   for (int i = 0; i < (OUT == kFp8 ? 4 : 2); i++) {
@@ -160,10 +160,7 @@ __device__ __forceinline__ unsigned encode16(const float* v, unsigned* codes) {
       w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, v[4 * i + 2], v[4 * i + 3], f, true);
       c = __builtin_bit_cast(unsigned, w);
     } else {
-      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, v[8 * i], v[8 * i + 1], f, 0);
-      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * i + 2], v[8 * i + 3], f, 1);
-      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * i + 4], v[8 * i + 5], f, 2);
-      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * i + 6], v[8 * i + 7], f, 3);
+      c = codes_fp4(v + 8 * i, f);
     }
     codes[i] = s == 255u ? 0u : c;
   }
@@ -666,17 +663,17 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(LinearParams p) {
       top = max(top, dpp<kSwap2>(top));
       top = max(top, dpp<kMirror8>(top));
       const unsigned s = scale_byte(top, OUT);
-      const float f = unscale(s);
+      const float f = divisor(s);
       if (!here) continue;
       const long unit = row * 32 * groups(p.m) + (c >> 2);  // four values
       if ((i & 7) == 0) p.out_scales[unit >> 3] = (uint8_t)s;
       uint8_t* out = static_cast<uint8_t*>(p.out);
       if constexpr (OUT == kFp8)
         *reinterpret_cast<unsigned*>(out + unit * 4) =
-            s == 255u ? 0u : codes_fp8(v[0] * f, v[1] * f, v[2] * f, v[3] * f);
+            s == 255u ? 0u : codes_fp8(v[0], v[1], v[2], v[3], f);
       else
         *reinterpret_cast<uint16_t*>(out + unit * 2) =
-            s == 255u ? (uint16_t)0 : (uint16_t)codes_fp4x4(v[0] * f, v[1] * f, v[2] * f, v[3] * f);
+            s == 255u ? (uint16_t)0 : (uint16_t)codes_fp4x4(v, f);
     }
   }
 }

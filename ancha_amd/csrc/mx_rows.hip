@@ -48,17 +48,22 @@ __device__ __forceinline__ double sum_lanes(double s) {
 // gives what rounding d itself does.
 __device__ __forceinline__ float to_odd(double d) {
   const unsigned long long bits = __builtin_bit_cast(unsigned long long, d);
-  const unsigned hi = (unsigned)(bits >> 32) | ((unsigned)bits != 0u ? 1u : 0u);
+  const unsigned hi = (unsigned)(bits >> 32) | min((unsigned)bits, 1u);
   return (float)__builtin_bit_cast(double, (unsigned long long)hi << 32);
 }
 
 // 1 / max(sqrt(s), 1e-12) for a sum of squares s, following the division where s is not finite
 // (0 for an infinity, NaN for a NaN; on the bits, as the library is compiled without NaN semantics).
+// The hardware's estimate (about 26 bits) and two Newton steps.
 __device__ __forceinline__ double inverse_length(double s) {
   unsigned hi = (unsigned)(__builtin_bit_cast(unsigned long long, s) >> 32);
   asm("" : "+v"(hi));
   if ((hi & 0x7ff00000u) == 0x7ff00000u) return (hi & 0xfffffu) ? s : 0.0;
-  return 1.0 / fmax(sqrt(s), 1e-12);
+  if (s <= 1e-24) return 1e12;
+  double y = __builtin_amdgcn_rsq(s);
+#pragma unroll
+  for (int i = 0; i < 2; i++) y = __builtin_fma(0.5 * y, __builtin_fma(-s * y, y, 1.0), y);
+  return y;
 }
 
 template <int TYPE>
@@ -129,17 +134,20 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(RowParams p) {
   }
   ss = sum_lanes<(L < 64 ? L : 64)>(ss);
   if constexpr (L > 64) {
+    constexpr int kWaves = L / 64;  // of a row
     __shared__ double part[kThreads / 64];
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = ss;
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) part[wave] = ss;
     __syncthreads();
     ss = 0.0;
 #pragma unroll
-    for (int w = 0; w < kThreads / 64; w++) ss += part[w];
+    for (int w = 0; w < kWaves; w++) ss += part[wave / kWaves * kWaves + w];
   }
   const double inv = inverse_length(ss + (double)p.dim * p.eps);
   const long first = row * (padded / 8);
 #pragma unroll
   for (int i = 0; i < V; i++) {
+    if (8 * L * i >= padded) break;
     const int col = 8 * (at + L * i);
     float y[8];
     normed(p, h[i], inv, col, 8 * L * (i + 1) <= p.dim, y);
@@ -221,18 +229,39 @@ void start_norm(const RowParams& p, hipStream_t stream) {
                      dim3(kThreads), 0, stream, p);
 }
 
+// Rows in registers, L threads a row and V pieces of 8 L values. Measured with each form forced (us, with
+// the addition / without):
+//   96 120 x 384 fp32     16 threads  80 / 37, 64  79 / 47, 32  107 / 54
+//   30 000 x 700 bf16     32 threads  36 / 25, 64  38 / 28, 128  51 / 37
+//   30 000 x 1024 bf16    64 threads  37 / 25, 32  38 / 26, 128  43 / 31
+//   20 000 x 1800 fp32   128 threads  85 / 37, 64  87 / 40, 256  83 / 40, 32  106 / 53
+//   30 000 x 4096 bf16   256 threads 156 / 92, 128 172 / 91, 64  208 / 112
+// and, with few rows, the more threads a row the shorter the way through it: 200 x 1500 fp16 256 threads
+// 5.0 / 4.4, 64 7.1 / 5.8, 32 10.3 / 8.1; 300 x 384 fp16 64 threads 4.4 / 4.7, 16 6.1 / 5.2.
 template <int TYPE>
 void norm_of_type(const RowParams& p, hipStream_t stream) {
   const long g = groups(p.dim);
-  if (g <= 1) return start_norm<TYPE, 16, 1>(p, stream);
-  if (g <= 2) return start_norm<TYPE, 16, 2>(p, stream);
-  if (g <= 3) return start_norm<TYPE, 16, 3>(p, stream);
-  if (g <= 4) return start_norm<TYPE, 16, 4>(p, stream);
-  if (g <= 8) return start_norm<TYPE, 64, 2>(p, stream);
-  if (g <= 16) return start_norm<TYPE, 64, 4>(p, stream);
-  if (g <= 32) return start_norm<TYPE, 256, 2>(p, stream);
-  if (g <= 64) return start_norm<TYPE, 256, 4>(p, stream);
-  hipLaunchKernelGGL(norm_long_kernel<TYPE>, dim3(p.rows), dim3(kThreads), 0, stream, p);
+  const bool few = p.rows < 1024;
+  if (g > 64)
+    hipLaunchKernelGGL(norm_long_kernel<TYPE>, dim3(p.rows), dim3(kThreads), 0, stream, p);
+  else if (g > 32)
+    start_norm<TYPE, 256, 4>(p, stream);
+  else if (g > 16)
+    start_norm<TYPE, 256, 2>(p, stream);
+  else if (g > 4 && few)
+    start_norm<TYPE, 256, 1>(p, stream);
+  else if (g > 8)
+    start_norm<TYPE, 128, 2>(p, stream);
+  else if (g > 6)
+    start_norm<TYPE, 64, 2>(p, stream);
+  else if (g > 4)
+    start_norm<TYPE, 32, 3>(p, stream);
+  else if (few)
+    start_norm<TYPE, 64, 1>(p, stream);
+  else if (g > 2)
+    g > 3 ? start_norm<TYPE, 16, 4>(p, stream) : start_norm<TYPE, 16, 3>(p, stream);
+  else
+    g > 1 ? start_norm<TYPE, 16, 2>(p, stream) : start_norm<TYPE, 16, 1>(p, stream);
 }
 
 template <int L>

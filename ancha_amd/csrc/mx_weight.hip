@@ -34,12 +34,10 @@ __global__ __launch_bounds__(256) void weight_columns_kernel(WeightParams p) {
     top = max(top, magnitude(v[i]));
   }
   const unsigned s = scale_byte(top, kFp4);
-  const float f = unscale(s);
-#pragma unroll
-  for (int i = 0; i < 32; i++) v[i] *= f;
+  const float f = divisor(s);
   u32x4 q;
 #pragma unroll
-  for (int i = 0; i < 4; i++) q[i] = s == 255u ? 0u : codes_fp4(v + 8 * i);
+  for (int i = 0; i < 4; i++) q[i] = s == 255u ? 0u : codes_fp4(v + 8 * i, f);
   *reinterpret_cast<u32x4*>(p.weight + code_place(blockIdx.x, c, block)) = q;
   p.weight[scale_place(gridDim.x, blockIdx.x, c, block)] = (uint8_t)s;
 }
@@ -73,11 +71,8 @@ __global__ __launch_bounds__(256) void weight_rows_kernel(WeightParams p) {
     top = max(top, dpp<kSwap1>(top));
     top = max(top, dpp<kSwap2>(top));
     const unsigned s = scale_byte(top, kFp4);
-    const float f = unscale(s);
-#pragma unroll
-    for (int e = 0; e < 8; e++) v[e] *= f;
     *reinterpret_cast<unsigned*>(p.weight + code_place(blockIdx.x, c, j >> 2) + 4 * (j & 3)) =
-        s == 255u ? 0u : codes_fp4(v);
+        s == 255u ? 0u : codes_fp4(v, divisor(s));
     if ((j & 3) == 0) p.weight[scale_place(gridDim.x, blockIdx.x, c, j >> 2)] = (uint8_t)s;
   }
 }
