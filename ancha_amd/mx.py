@@ -21,7 +21,7 @@ import torch
 
 from . import _native
 from ._tensors import require
-from .fused import ATTENTION_HEAD_DIM, Epilogue, _ptr, _usable
+from .fused import ATTENTION_HEAD_DIM, Epilogue, _ptr
 
 BLOCK = 32
 _FORMATS = {"fp8": 8, "fp4": 4}
@@ -116,10 +116,8 @@ class Tensor:
         """The values that the codes stand for, ``shape`` in ``dtype`` (16 bits hold all but those at
         the ends of the type's range)."""
         kind = _type(dtype, "dtype")
-        if not _usable():
-            return None
         device = self.device
-        out = torch.empty(self.shape, dtype=dtype, device=device)
+        out = torch.empty(tuple(self.shape), dtype=dtype, device=device)
         codes, scales = self._pointers()
         return out if _launch(device.index, "ancha_hip_mx_values", codes, scales, self.rows,
                               self.shape[-1], _FORMATS[self.format], kind, out.data_ptr()) else None
@@ -138,8 +136,6 @@ class Weight:
     def values(self, dtype: torch.dtype = torch.float32) -> Optional[torch.Tensor]:
         """The values that the codes stand for, [k, m] in ``dtype``."""
         kind = _type(dtype, "dtype")
-        if not _usable():
-            return None
         out = torch.empty(self.shape, dtype=dtype, device=self.device)
         return out if _launch(self.device.index, "ancha_hip_mx_weight_values", self._data.data_ptr(),
                               *self.shape, kind, out.data_ptr()) else None
@@ -157,19 +153,17 @@ def _rows(t: torch.Tensor, dim: int, rows: int) -> tuple[torch.Tensor, int]:
     return flat, stride[0] if rows > 1 else dim
 
 
-def _input(x: torch.Tensor, name: str) -> Optional[int]:
+def _input(x: torch.Tensor, name: str) -> int:
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise ValueError(f"{name} must be a tensor on a GPU")
     if x.dim() == 0:
         raise ValueError(f"{name} must have at least one axis")
-    return _type(x.dtype, name) if _usable() else None
+    return _type(x.dtype, name)
 
 
 def quantize(x: torch.Tensor, format: str = "fp4") -> Optional[Tensor]:
     """``x`` [..., dim] in blocks of 32 along its last axis."""
     bits, kind = _format(format), _input(x, "x")
-    if kind is None:
-        return None
     shape = x.shape
     dim = shape[-1]
     rows = shape[:-1].numel()
@@ -182,8 +176,6 @@ def quantize(x: torch.Tensor, format: str = "fp4") -> Optional[Tensor]:
 
 def _norm(x, residual, scale, eps, format):
     bits, kind = _format(format), _input(x, "x")
-    if kind is None:
-        return None, None
     shape, device = x.shape, x.device
     dim = shape[-1]
     rows = shape[:-1].numel()
@@ -195,7 +187,7 @@ def _norm(x, residual, scale, eps, format):
     if residual is not None:
         require(residual, "residual", device, shape, x.dtype)
         residual, ldr = _rows(residual, dim, rows)
-        total = torch.empty(shape, dtype=x.dtype, device=device)
+        total = torch.empty_like(x, memory_format=torch.contiguous_format)
     out = Tensor._empty(shape, rows, format, device)
     codes, scales = out._pointers()
     done = _launch(device.index, "ancha_hip_mx_norm", flat.data_ptr(), kind, rows, dim, ld, _ptr(residual),
@@ -229,8 +221,6 @@ def weight(w: torch.Tensor) -> Optional[Weight]:
     kind = _input(w, "w")
     if w.dim() != 2:
         raise ValueError(f"w must be [k, m], got {tuple(w.shape)}")
-    if kind is None:
-        return None
     k, m = w.shape
     size = int(_native.lib().ancha_hip_mx_weight_bytes(k, m))
     if size == 0:
@@ -282,13 +272,11 @@ def linear(x: Tensor, w: Weight, epilogue: Optional[Epilogue] = None,
         if residual is not None:
             require(residual, "residual", device, shape, dtype)
             residual = residual.contiguous()
-    if not _usable():
-        return None
     if bits:
         out = Tensor._empty(shape, n, format, device)
         to, to_scales = out._pointers()
     else:
-        out = torch.empty(shape, dtype=dtype, device=device)
+        out = torch.empty(tuple(shape), dtype=dtype, device=device)
         to, to_scales = out.data_ptr(), None
     codes, scales = x._pointers()
     return out if _launch(device.index, "ancha_hip_mx_linear", codes, scales, n, k, _FORMATS[x.format],
