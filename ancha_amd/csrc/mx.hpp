@@ -101,10 +101,12 @@ __device__ __forceinline__ void store_row(void* base, long at, int valid, const 
 }
 
 // Magnitude of x as an unsigned number: ordered like |x|, infinities and NaN above every finite value
-// (the library is compiled without NaN semantics, so the comparison is made on the bits).
-__device__ __forceinline__ unsigned magnitude(float x) {
+// (the library is compiled without NaN semantics, so the comparison is made on the bits). x then comes from
+// its bits too, so that the compiler keeps one register for both.
+__device__ __forceinline__ unsigned magnitude(float& x) {
   unsigned bits = __builtin_bit_cast(unsigned, x);
   asm("" : "+v"(bits));
+  x = __builtin_bit_cast(float, bits);
   return bits & 0x7fffffffu;
 }
 
@@ -162,7 +164,7 @@ __device__ __forceinline__ unsigned codes_fp4x4(const float* v, float f) {
 // Eight consecutive values of a row held by one lane, a block by four neighbouring lanes, a group of
 // 128 by sixteen: rounds them, writes the codes of unit `unit` (eight values, counted from the start of
 // the codes) and, from one lane of sixteen, the group's four scale bytes. All sixteen lanes take part.
-__device__ __forceinline__ void store_codes(const float* v, int format, bool store, long unit,
+__device__ __forceinline__ void store_codes(float* v, int format, bool store, long unit,
                                             uint8_t* codes, uint8_t* scales) {
   unsigned top = 0;
 #pragma unroll

@@ -14,7 +14,6 @@
 #include <algorithm>
 
 #include "buffer.hpp"
-#include "gemm.hpp"
 #include "mx.hpp"
 
 namespace ancha {
@@ -47,6 +46,40 @@ __device__ __forceinline__ void split(unsigned c, unsigned& large, unsigned& sma
   const unsigned mask = __builtin_amdgcn_perm(c << 9, c << 1, 0x090b080au);
   large = c & mask;
   small = c & ~mask;
+}
+
+// erf-GELU: x Phi(x) = max(x, 0) - |x| 2^Q(|x|) with Q a polynomial for log2 Phi(-a), fitted to the least
+// largest error of the result on [0, 6] (WIDE: degree 10, [0, 7], for fp32 results; beyond, Q stays below
+// -29 and falls, so the product vanishes). Of the value, relatively: 9e-7 above x = -1, 2e-5 above -4 (WIDE
+// 5e-7, 2e-6); absolutely within the rounding of the larger results. Eight or ten fused multiply-adds and one
+// exp2 where erf costs the vector ALU, which bounds these epilogues, three times as much: 96 120 x 384 ->
+// 1536 with bias and GELU to codes 141 us (152 with erf's rational form), to fp32 162 (229 with erff).
+template <bool WIDE>
+__device__ __forceinline__ float gelu(float x) {
+  const float a = fabsf(x);
+  float q;
+  if constexpr (WIDE) {
+    q = fmaf(a, -5.376492496e-8f, 1.340385325e-6f);
+    q = fmaf(a, q, -1.47964638e-5f);
+    q = fmaf(a, q, 9.261807281e-5f);
+    q = fmaf(a, q, -3.185693058e-4f);
+    q = fmaf(a, q, 5.334966409e-5f);
+    q = fmaf(a, q, 6.907870993e-3f);
+    q = fmaf(a, q, -5.242882669e-2f);
+    q = fmaf(a, q, -4.592211545e-1f);
+    q = fmaf(a, q, -1.151104569f);
+    q = fmaf(a, q, -1.0f);
+  } else {
+    q = fmaf(a, -1.6903760525e-6f, 2.5082976208e-5f);
+    q = fmaf(a, q, -1.1446096323e-4f);
+    q = fmaf(a, q, -3.2334669959e-4f);
+    q = fmaf(a, q, 7.3333908804e-3f);
+    q = fmaf(a, q, -5.2714202553e-2f);
+    q = fmaf(a, q, -4.5911544561e-1f);
+    q = fmaf(a, q, -1.1511232853f);
+    q = fmaf(a, q, -9.9999886751e-1f);
+  }
+  return fmaf(-a, __builtin_amdgcn_exp2f(q), fmaxf(x, 0.f));
 }
 
 constexpr bool kCodes(int out) { return out == kFp8 || out == kFp4; }
@@ -125,9 +158,11 @@ __device__ __forceinline__ void store_values(const LinearParams& p, const Rows<O
   }
 }
 
-__device__ __forceinline__ unsigned bits_of(float x) {
+// The bits of x; x itself then comes from them, so that the compiler keeps one register for both.
+__device__ __forceinline__ unsigned bits_of(float& x) {
   unsigned bits = __builtin_bit_cast(unsigned, x);
   asm("" : "+v"(bits));
+  x = __builtin_bit_cast(float, bits);
   return bits;
 }
 
@@ -136,7 +171,7 @@ __device__ __forceinline__ unsigned bits_of(float x) {
 // unsigned ones (the largest negative value, if there is one), a NaN above everything. The conversion
 // divides by the scale and, with saturate() in effect, stops at the largest value.
 template <int OUT>
-__device__ __forceinline__ unsigned encode16(const float* v, unsigned* codes) {
+__device__ __forceinline__ unsigned encode16(float* v, unsigned* codes) {
   int positive = 0;
   unsigned negative = 0;
 #pragma unroll
@@ -207,7 +242,7 @@ __device__ __forceinline__ void finish_codes(const LinearParams& p, const Rows<O
   for (int i = 0; i < 16; i++) v[i] += bias[i];
   if (p.gelu)
 #pragma unroll
-    for (int i = 0; i < 16; i++) v[i] = gemm::gelu_fast(v[i]);
+    for (int i = 0; i < 16; i++) v[i] = gelu<false>(v[i]);
   if (p.rope && c < 2 * p.width) {
     const unsigned token = (unsigned)(d.row0 + r) % (unsigned)p.tokens;
     const float* table = p.rope + (c < p.width ? 0 : 2) * (long)p.tokens * 64 + token * 64ul + (c & 63);
@@ -274,7 +309,7 @@ __device__ __forceinline__ void finish_tile(const LinearParams& p, const Rows<OU
     for (int q = 0; q < 4; q++)
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        v[q][i] = OUT == kF32 ? gemm::gelu_erf(v[q][i]) : gemm::gelu_fast(v[q][i]);
+        v[q][i] = gelu<OUT == kF32>(v[q][i]);
   if (p.rope && c < 2 * p.width) {
     const float* table = p.rope + (c < p.width ? 0 : 2) * (long)p.tokens * 64 + (c & 63);
 #pragma unroll
@@ -373,12 +408,15 @@ __device__ __forceinline__ void barrier() {
 // scales go straight from memory to LDS, ST - 1 steps ahead, in ST buffers: one barrier per step, behind
 // which the buffer of the step before is free. OCC: waves per SIMD that the registers leave room for.
 //
+// KG > 1: that many such groups of waves take the steps in turn, for few tiles with a long k, where the
+// time is the chain of steps; the first adds up the sums of all.
+//
 // A row's 16-byte chunks lie in LDS at chunk ^ (row & 7) (e4m3: 128 bytes a row; e2m1: 64 bytes, chunk ^
 // (row / 2 & 3)), so that the eight lanes that are served together hit different banks; the loads to LDS
 // write in lane order, so the lanes choose their chunk in memory instead. Weight fragments are in lane
 // order already.
-template <int FORMAT, bool SPLIT, int OUT, int WM, int WN, int SM, int TN, int ST, int OCC>
-__global__ __launch_bounds__(64 * WM * WN, OCC) void tile_kernel(LinearParams p, unsigned mtiles,
+template <int FORMAT, bool SPLIT, int OUT, int WM, int WN, int SM, int TN, int ST, int OCC, int KG = 1>
+__global__ __launch_bounds__(64 * WM * WN * KG, OCC) void tile_kernel(LinearParams p, unsigned mtiles,
                                                             unsigned ntiles, int direct) {
   constexpr int W = WM * WN, STRIPS = WM * SM, ROWS = 16 * TN * WN;
   constexpr int kRow = FORMAT == kFp8 ? 128 : 64;           // bytes of a row and step
@@ -388,9 +426,10 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void tile_kernel(LinearParams p,
   constexpr int QX = ROWS / 64, Q = (QX + STRIPS + W - 1) / W;  // 256-byte pieces of scales
   static_assert(PX * W * 1024 == kX && PW * W * 1024 == kW && QX * 64 == ROWS, "whole pieces");
   constexpr int kLoads = PX + PW + Q;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[ST][kStageBytes];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[ST][KG][kStageBytes];
   const int lane = threadIdx.x & 63, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int any = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = any % W, kg = any / W;
   const int wm = wave % WM, wn = wave / WM;
 
   // Workgroups that run at the same time on an XCD share its L2: four row tiles by neighbouring column
@@ -401,7 +440,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void tile_kernel(LinearParams p,
   const unsigned mt = rest / high, nt = 4 * band + (rest - mt * high);
   const long row0 = (long)nt * ROWS;
   const int strip0 = (int)mt * STRIPS, nstrips = (int)strips(p.m);
-  const int steps = (int)groups(p.k);
+  const int steps = (int)groups(p.k), chunks = (steps + KG - 1) / KG;
 
   const uint8_t* x = p.x + row0 * steps * kRow;
   const uint8_t* xs = p.x_scales + row0 * steps * 4;
@@ -435,7 +474,9 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void tile_kernel(LinearParams p,
     qo[i] = piece < QX ? (unsigned)min(64 * piece + lane, last_row) * (unsigned)(steps * 4)
                        : (unsigned)min(piece - QX, last_strip) * (unsigned)(steps * kStripScales) + lane * 4;
   }
-  auto load = [&](int s, uint8_t* to) {
+  // Chunk c: this group's step of it (the last step again behind the end, not multiplied).
+  auto load = [&](int c, uint8_t* to) {
+    const int s = KG == 1 ? c : min(c * KG + kg, steps - 1);
 #pragma unroll
     for (int i = 0; i < PX; i++) to_lds<16>(x + (long)s * kRow, xo[i], to + (wave * PX + i) * 1024);
 #pragma unroll
@@ -467,17 +508,19 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void tile_kernel(LinearParams p,
   }
 
 #pragma unroll
-  for (int s = 0; s < ST - 1; s++)
-    if (s < steps) load(s, lds[s]);
+  for (int c = 0; c < ST - 1; c++)
+    if (c < chunks) load(c, lds[c][kg]);
   int b = 0;
-  for (int s = 0; s < steps; s++) {
-    if (s + ST - 2 < steps)
+  for (int c = 0; c < chunks; c++) {
+    if (c + ST - 2 < chunks)
       wait_loads<(ST - 2) * kLoads>();
     else
       wait_loads<0>();
     barrier();
-    if (s + ST - 1 < steps) load(s + ST - 1, lds[b == 0 ? ST - 1 : b - 1]);
-    const uint8_t* from = lds[b];
+    if (c + ST - 1 < chunks) load(c + ST - 1, lds[b == 0 ? ST - 1 : b - 1][kg]);
+    const uint8_t* from = lds[b][kg];
+    b = b == ST - 1 ? 0 : b + 1;
+    if (KG > 1 && c * KG + kg >= steps) break;  // the last chunk: no barrier follows in the loop
     // A strip's fragments are read from LDS while the strip before it is multiplied (left to the compiler,
     // all of a step's reads come first and the matrix cores wait for the last).
     const uint8_t* wl = from + kX + wm * SM * kStripCodes + lane * 16;
@@ -522,27 +565,46 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void tile_kernel(LinearParams p,
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    b = b == ST - 1 ? 0 : b + 1;
   }
-  static_assert(W * kOutStage + ROWS * 4 <= ST * kStageBytes, "the way out fits the operands' buffers");
-  int* tokens = reinterpret_cast<int*>(&lds[0][0] + W * kOutStage);
+  constexpr int kSums = W * TN * SM * 4 * 1024;  // bytes of a group's sums
+  static_assert((KG - 1) * kSums + W * kOutStage + ROWS * 4 <= ST * KG * kStageBytes,
+                "sums and results on their way out fit the operands' buffers");
+  uint8_t* free = &lds[0][0][0];
+  int* tokens = reinterpret_cast<int*>(free + (KG - 1) * kSums + W * kOutStage);
   const int rows = (int)min((long)ROWS, p.n - row0);
-  if (!kCodes(OUT)) {
-    // Every wave is done with the operands before the first one's results take their place.
+  if (KG > 1 || !kCodes(OUT)) {
+    // Every wave is done with the operands before something else takes their place.
     wait_loads<0>();
     barrier();
   }
-  if (!kCodes(OUT) && p.rope) {
-    if ((int)threadIdx.x < ROWS) tokens[threadIdx.x] = (int)((unsigned)(row0 + threadIdx.x) % (unsigned)p.tokens);
-    __syncthreads();
+  if (!kCodes(OUT) && p.rope && (int)threadIdx.x < ROWS)
+    tokens[threadIdx.x] = (int)((unsigned)(row0 + threadIdx.x) % (unsigned)p.tokens);
+  if constexpr (KG > 1) {
+    if (kg)
+#pragma unroll
+      for (int q = 0; q < TN * SM * 4; q++)
+        reinterpret_cast<f32x4*>(free + (kg - 1) * kSums)[(wave * TN * SM * 4 + q) * 64 + lane] =
+            acc[q / (SM * 4)][q / 4 % SM][q % 4];
+  }
+  if (KG > 1 || (!kCodes(OUT) && p.rope)) __syncthreads();
+  if constexpr (KG > 1) {
+    if (kg) return;
+#pragma unroll
+    for (int o = 0; o < KG - 1; o++)
+#pragma unroll
+      for (int q = 0; q < TN * SM * 4; q++)
+        acc[q / (SM * 4)][q / 4 % SM][q % 4] +=
+            reinterpret_cast<const f32x4*>(free + o * kSums)[(wave * TN * SM * 4 + q) * 64 + lane];
   }
   if (kCodes(OUT)) saturate();
   const Rows<OUT> d = rows_of<OUT>(p, row0, rows);
   const int c0 = (strip0 + wm * SM) * 64;
   if (direct)
-    finish_wave<OUT, true, SM, TN>(p, d, wn * TN * 16, c0, acc, tokens, &lds[0][0] + wave * kOutStage);
+    finish_wave<OUT, true, SM, TN>(p, d, wn * TN * 16, c0, acc, tokens,
+                                      free + (KG - 1) * kSums + wave * kOutStage);
   else
-    finish_wave<OUT, false, SM, TN>(p, d, wn * TN * 16, c0, acc, tokens, &lds[0][0] + wave * kOutStage);
+    finish_wave<OUT, false, SM, TN>(p, d, wn * TN * 16, c0, acc, tokens,
+                                      free + (KG - 1) * kSums + wave * kOutStage);
 }
 
 // Whether the rows of a workgroup are written (and the residual read) through plain pointers.
@@ -551,12 +613,12 @@ int direct_rows(const LinearParams& p, long rows) {
          (reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.residual)) % 4 != 0;
 }
 
-template <int FORMAT, bool SPLIT, int OUT, int WM, int WN, int SM, int TN, int ST, int OCC>
+template <int FORMAT, bool SPLIT, int OUT, int WM, int WN, int SM, int TN, int ST, int OCC, int KG = 1>
 void start_tiles(const LinearParams& p, hipStream_t stream) {
   const unsigned mtiles = (unsigned)((strips(p.m) + WM * SM - 1) / (WM * SM));
   const unsigned ntiles = (unsigned)(((long)p.n + 16 * TN * WN - 1) / (16 * TN * WN));
-  hipLaunchKernelGGL((tile_kernel<FORMAT, SPLIT, OUT, WM, WN, SM, TN, ST, OCC>), dim3(mtiles * ntiles),
-                     dim3(64 * WM * WN), 0, stream, p, mtiles, ntiles, direct_rows(p, 16 * TN * WN));
+  hipLaunchKernelGGL((tile_kernel<FORMAT, SPLIT, OUT, WM, WN, SM, TN, ST, OCC, KG>), dim3(mtiles * ntiles),
+                     dim3(64 * WM * WN * KG), 0, stream, p, mtiles, ntiles, direct_rows(p, 16 * TN * WN));
 }
 
 // Few rows: the weight is what has to be read. A workgroup has 32 columns and 16 TN rows; its waves (one
@@ -653,7 +715,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(LinearParams p) {
     }
     if (p.gelu)
 #pragma unroll
-      for (int e = 0; e < 4; e++) v[e] = OUT == kF32 ? gemm::gelu_erf(v[e]) : gemm::gelu_fast(v[e]);
+      for (int e = 0; e < 4; e++) v[e] = gelu<OUT == kF32>(v[e]);
     if (p.rope && here && c < 2 * p.width) {
       const float* table = p.rope + (c < p.width ? 0 : 2) * (long)p.tokens * 64 +
                            (unsigned)row % (unsigned)p.tokens * 64ul + (c & 63);
@@ -710,6 +772,8 @@ void start(const LinearParams& p, hipStream_t stream) {
   //   few rows / 64 x 64 tiles: 16 x 4096 x 4096 6.3 / 10.9, 64 x 4096 x 4096 9.8 / 11.0, 64 x 8192 x 8192
   //   30.6 / 19.9, 64 x 2048 x 512 4.4 / 6.8; with 16 / 32 rows a workgroup where 16 already fill the
   //   chip: 24 x 8192 x 8192 16.9 / 13.7 (e2m1 16.7 / 11.0);
+  //   64 x 64 tiles, the steps in one chain / in four: 128 x 4096 x 4096 11.6 / 8.9, 128 x 8192 x 8192 21.8 /
+  //   15.8, 800 x 2048 x 512 7.2 / 6.4, 512 x 1024 x 1024 5.1 / 5.3, 512 x 4096 x 4096 14.3 / 16.5;
   //   64 x 64 / 128 x 128: 512 x 4096 x 4096 14.9 / 21.7, 4096 x 2048 x 512 9.2 / 12.9, 1024 x 4096 x 4096
   //   26.2 / 25.5, 512 x 8192 x 8192 51.0 / 45.8;
   //   128 rows x 128 / 256 columns: 2048 x 4096 x 4096 35.0 / 37.7, 4096 x 4096 x 4096 61.6 / 56.1,
@@ -722,9 +786,12 @@ void start(const LinearParams& p, hipStream_t stream) {
     start_few<FORMAT, SPLIT, OUT, 2>(p, stream);
   else if ((n + 15) / 16 * columns <= 2 * cus)
     start_few<FORMAT, SPLIT, OUT, 1>(p, stream);
-  else if (narrow * high * 4 < 3 * cus)
-    start_tiles<FORMAT, SPLIT, OUT, 1, 4, 1, 1, 3, 4>(p, stream);
-  else if (wide * 32 <= narrow * 17 && wide * high >= 2 * cus)
+  else if (narrow * high * 4 < 3 * cus) {
+    if ((n + 63) / 64 * ((m + 63) / 64) <= cus && p.k >= 2048)
+      start_tiles<FORMAT, SPLIT, OUT, 1, 4, 1, 1, 3, 4, 4>(p, stream);
+    else
+      start_tiles<FORMAT, SPLIT, OUT, 1, 4, 1, 1, 3, 4>(p, stream);
+  } else if (wide * 32 <= narrow * 17 && wide * high >= 2 * cus)
     // 32 x 256 a wave where rows are split (twice the registers for a row tile), 64 x 128 otherwise (fewer
     // LDS reads): 8192 x 8192 x 8192 to fp32 629 / 709, to bf16 400 / 375.
     if constexpr (SPLIT)

@@ -204,9 +204,13 @@ def product_bound(x, w, fmt, short):
     steps = -(-k // 128)
     off = (steps + 1) * 2.0 ** -22 * (np.abs(x) @ np.abs(w))
     if short and fmt == "fp8":
-        for k0 in range(0, k, 8):
-            a, b = np.abs(x[:, k0:k0 + 8]), np.abs(w[k0:k0 + 8])
-            off += 8 * 2.0 ** -13 * (a[:, :, None] * b[None]).max(1)
+        if x.shape[0] * w.shape[1] <= 1 << 19:
+            for k0 in range(0, k, 8):
+                a, b = np.abs(x[:, k0:k0 + 8]), np.abs(w[k0:k0 + 8])
+                off += 8 * 2.0 ** -13 * (a[:, :, None] * b[None]).max(1)
+        else:  # the largest product of eight is at most the product of the eights' largest values
+            eights = lambda a: np.pad(np.abs(a), ((0, 0), (0, -k % 8))).reshape(len(a), -1, 8).max(2)  # noqa: E731
+            off += 8 * 2.0 ** -13 * (eights(x) @ eights(w.T).T)
     return off
 
 
@@ -254,6 +258,43 @@ def test_products(gpu, n, k, m, fmt, kind):
     assert got.shape == (n, m) and got.dtype == TYPES[kind]
     y, tol = expected(x, wv, fmt, kind != "f32", dtype=TYPES[kind])
     near(f"{n}x{k}x{m} {fmt} {kind}", host(got), y, tol)
+
+
+# Every form that the rule on sizes picks: steps in four chains, 128 x 128 tiles (plain and direct rows), 256
+# columns (plain and direct).
+FORMS = [(130, 2100, 2050), (2100, 200, 1549), (2100, 130, 1600), (8200, 130, 2047), (8200, 160, 2048)]
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("fmt", ["fp8", "fp4"])
+@pytest.mark.parametrize("n,k,m", FORMS)
+def test_forms(gpu, n, k, m, fmt, kind):
+    dtype = TYPES[kind]
+    t, w, x, wv = problem(gpu, n, k, m, fmt, 25)
+    b, r = dev(W.normal((m,), 26, 1.0), gpu), dev(W.normal((n, m), 27, 2.0), gpu, dtype)
+    near(f"{n}x{k}x{m} {fmt} {kind}", host(mx.linear(t, w, fused.Epilogue(bias=b, residual=r), dtype=dtype)),
+         *expected(x, wv, fmt, kind != "f32", host(b), residual=host(r), dtype=dtype))
+    tokens = max(d for d in range(1, 900) if n % d == 0)
+    table, width = W.axis_rope_packed(W.rope_freqs(), tokens), m // 128 * 64
+    near(f"rotary {n}x{k}x{m} {fmt} {kind}",
+         host(mx.linear(t, w, fused.Epilogue(rotary=(dev(table, gpu), width)), dtype=dtype)),
+         *expected(x, wv, fmt, kind != "f32", rotary=(table.astype(np.float64), width), dtype=dtype))
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "fp4"])
+@pytest.mark.parametrize("n,k,m", FORMS)
+def test_forms_to_codes(gpu, n, k, m, fmt):
+    t, w, x, wv = problem(gpu, n, k, m, fmt, 28)
+    b = dev(W.normal((m,), 29, 1.0), gpu)
+    out = "fp4" if fmt == "fp4" else "fp8"
+    tokens = max(d for d in range(1, 900) if n % d == 0)
+    table, width = W.axis_rope_packed(W.rope_freqs(), tokens), m // 128 * 64
+    got = mx.linear(t, w, fused.Epilogue(bias=b, rotary=(dev(table, gpu), width)), format=out)
+    y, tol = expected(x, wv, fmt, False, host(b), rotary=(table.astype(np.float64), width))
+    check_codes(f"{n}x{k}x{m} {fmt} -> {out}", got, y, tol, out)
+    small = mx.linear(mx.Tensor(t.codes[-40:], t.scales[-40:], fmt, (40, k)), w, fused.Epilogue(bias=b), format=out)
+    y, tol = expected(x[-40:], wv, fmt, False, host(b))
+    check_codes(f"40x{k}x{m} {fmt} -> {out}", small, y, tol, out)
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
