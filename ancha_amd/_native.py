@@ -62,16 +62,16 @@ SIGNATURES = {
     "ancha_hip_istft_workspace": (_sz, [_sz]),
     "ancha_hip_istft": (_int, [_p, _p, _sz, _sz, _sz, _int, _p, _sz, _p, _p]),
     "ancha_hip_istft_noalloc": (_int, [_p, _p, _sz, _sz, _sz, _int, _p, _p]),
-    "ancha_hip_mx_pitch": (_sz, [_sz, _int]),
-    "ancha_hip_mx_scales": (_sz, [_sz]),
-    "ancha_hip_mx_quantize": (_int, [_p, _int, _sz, _sz, _sz, _int, _p, _p, _p]),
-    "ancha_hip_mx_norm": (_int, [_p, _int, _sz, _sz, _sz, _p, _sz, _p, ctypes.c_double, _int, _p, _p,
+    "ancha_mx_pitch": (_sz, [_sz, _int]),
+    "ancha_mx_scales": (_sz, [_sz]),
+    "ancha_mx_quantize": (_int, [_p, _int, _sz, _sz, _sz, _int, _p, _p, _p]),
+    "ancha_mx_norm": (_int, [_p, _int, _sz, _sz, _sz, _p, _sz, _p, ctypes.c_double, _int, _p, _p,
                                  _p, _p]),
-    "ancha_hip_mx_values": (_int, [_p, _p, _sz, _sz, _int, _int, _p, _p]),
-    "ancha_hip_mx_weight_bytes": (_sz, [_sz, _sz]),
-    "ancha_hip_mx_weight": (_int, [_p, _int, _sz, _sz, _sz, _sz, _p, _p]),
-    "ancha_hip_mx_weight_values": (_int, [_p, _sz, _sz, _int, _p, _p]),
-    "ancha_hip_mx_linear": (_int, [_p, _p, _sz, _sz, _int, _p, _sz, _p, _int, _p, _sz, _sz, _p, _int,
+    "ancha_mx_values": (_int, [_p, _p, _sz, _sz, _int, _int, _p, _p]),
+    "ancha_mx_weight_bytes": (_sz, [_sz, _sz]),
+    "ancha_mx_weight": (_int, [_p, _int, _sz, _sz, _sz, _sz, _p, _p]),
+    "ancha_mx_weight_values": (_int, [_p, _sz, _sz, _int, _p, _p]),
+    "ancha_mx_linear": (_int, [_p, _p, _sz, _sz, _int, _p, _sz, _p, _int, _p, _sz, _sz, _p, _int,
                                    _int, _p, _p, _p]),
     "ancha_hip_check": (_int, []),
     "ancha_hip_last_error": (ctypes.c_char_p, []),

@@ -93,31 +93,31 @@ bool weight_fits(size_t k, size_t m) {
 
 extern "C" {
 
-size_t ancha_hip_mx_pitch(size_t dim, int format) {
+size_t ancha_mx_pitch(size_t dim, int format) {
   return is_format(format) && dim <= kIntMax / 2 ? static_cast<size_t>(mx::pitch(static_cast<long>(dim), format)) : 0;
 }
 
-size_t ancha_hip_mx_scales(size_t dim) {
+size_t ancha_mx_scales(size_t dim) {
   return dim <= kIntMax / 2 ? 4 * static_cast<size_t>(mx::groups(static_cast<long>(dim))) : 0;
 }
 
-int ancha_hip_mx_quantize(const void* x, int type, size_t rows, size_t dim, size_t ldx, int format,
-                          void* codes, void* scales, hipStream_t stream) {
-  return run_rows("ancha_hip_mx_quantize", x, type, rows, dim, ldx, nullptr, 0, nullptr, 0.0, false,
+int ancha_mx_quantize(const void* x, int type, size_t rows, size_t dim, size_t ldx, int format,
+                      void* codes, void* scales, hipStream_t stream) {
+  return run_rows("ancha_mx_quantize", x, type, rows, dim, ldx, nullptr, 0, nullptr, 0.0, false,
                   format, nullptr, codes, scales, stream);
 }
 
-int ancha_hip_mx_norm(const void* x, int type, size_t rows, size_t dim, size_t ldx,
-                      const void* residual, size_t ldr, const float* scale, double eps, int format,
-                      void* sum, void* codes, void* scales, hipStream_t stream) {
-  return run_rows("ancha_hip_mx_norm", x, type, rows, dim, ldx, residual, ldr, scale, eps, true, format,
+int ancha_mx_norm(const void* x, int type, size_t rows, size_t dim, size_t ldx,
+                  const void* residual, size_t ldr, const float* scale, double eps, int format,
+                  void* sum, void* codes, void* scales, hipStream_t stream) {
+  return run_rows("ancha_mx_norm", x, type, rows, dim, ldx, residual, ldr, scale, eps, true, format,
                   sum, codes, scales, stream);
 }
 
-int ancha_hip_mx_values(const void* codes, const void* scales, size_t rows, size_t dim, int format,
-                        int type, void* out, hipStream_t stream) {
+int ancha_mx_values(const void* codes, const void* scales, size_t rows, size_t dim, int format,
+                    int type, void* out, hipStream_t stream) {
   if (const int s = sticky()) return s;
-  const std::string who("ancha_hip_mx_values");
+  const std::string who("ancha_mx_values");
   if (!is_type(type) || !is_format(format))
     return fail(ANCHA_HIP_INVALID, who + ": unknown type or format");
   if (rows == 0 || dim == 0) return ANCHA_HIP_OK;
@@ -137,16 +137,16 @@ int ancha_hip_mx_values(const void* codes, const void* scales, size_t rows, size
   return e == hipSuccess ? ANCHA_HIP_OK : hip_fail(e, who);
 }
 
-size_t ancha_hip_mx_weight_bytes(size_t k, size_t m) {
+size_t ancha_mx_weight_bytes(size_t k, size_t m) {
   return k && m && weight_fits(k, m)
              ? static_cast<size_t>(mx::weight_bytes(static_cast<long>(k), static_cast<long>(m)))
              : 0;
 }
 
-int ancha_hip_mx_weight(const void* w, int type, size_t k, size_t m, size_t ldk, size_t ldm,
-                        void* weight, hipStream_t stream) {
+int ancha_mx_weight(const void* w, int type, size_t k, size_t m, size_t ldk, size_t ldm,
+                    void* weight, hipStream_t stream) {
   if (const int s = sticky()) return s;
-  const std::string who("ancha_hip_mx_weight");
+  const std::string who("ancha_mx_weight");
   if (!is_type(type)) return fail(ANCHA_HIP_INVALID, who + ": unknown type");
   if (k == 0 || m == 0 || !weight_fits(k, m))
     return fail(ANCHA_HIP_UNSUPPORTED, who + ": empty or too large a weight");
@@ -165,10 +165,10 @@ int ancha_hip_mx_weight(const void* w, int type, size_t k, size_t m, size_t ldk,
   return e == hipSuccess ? ANCHA_HIP_OK : hip_fail(e, who);
 }
 
-int ancha_hip_mx_weight_values(const void* weight, size_t k, size_t m, int type, void* out,
-                               hipStream_t stream) {
+int ancha_mx_weight_values(const void* weight, size_t k, size_t m, int type, void* out,
+                           hipStream_t stream) {
   if (const int s = sticky()) return s;
-  const std::string who("ancha_hip_mx_weight_values");
+  const std::string who("ancha_mx_weight_values");
   if (!is_type(type)) return fail(ANCHA_HIP_INVALID, who + ": unknown type");
   if (k == 0 || m == 0 || !weight_fits(k, m))
     return fail(ANCHA_HIP_UNSUPPORTED, who + ": empty or too large a weight");
@@ -185,12 +185,12 @@ int ancha_hip_mx_weight_values(const void* weight, size_t k, size_t m, int type,
   return e == hipSuccess ? ANCHA_HIP_OK : hip_fail(e, who);
 }
 
-int ancha_hip_mx_linear(const void* codes, const void* scales, size_t n, size_t k, int format,
-                        const void* weight, size_t m, const float* bias, int gelu, const float* rope,
-                        size_t tokens, size_t width, const void* residual, int type, int out_format,
-                        void* out, void* out_scales, hipStream_t stream) {
+int ancha_mx_linear(const void* codes, const void* scales, size_t n, size_t k, int format,
+                    const void* weight, size_t m, const float* bias, int gelu, const float* rope,
+                    size_t tokens, size_t width, const void* residual, int type, int out_format,
+                    void* out, void* out_scales, hipStream_t stream) {
   if (const int s = sticky()) return s;
-  const std::string who("ancha_hip_mx_linear");
+  const std::string who("ancha_mx_linear");
   if (!is_type(type) || !is_format(format) || (out_format && !is_format(out_format)))
     return fail(ANCHA_HIP_INVALID, who + ": unknown type or format");
   if (out_format && type != ANCHA_HIP_F32)

@@ -119,7 +119,7 @@ class Tensor:
         device = self.device
         out = torch.empty(tuple(self.shape), dtype=dtype, device=device)
         codes, scales = self._pointers()
-        return out if _launch(device.index, "ancha_hip_mx_values", codes, scales, self.rows,
+        return out if _launch(device.index, "ancha_mx_values", codes, scales, self.rows,
                               self.shape[-1], _FORMATS[self.format], kind, out.data_ptr()) else None
 
 
@@ -137,7 +137,7 @@ class Weight:
         """The values that the codes stand for, [k, m] in ``dtype``."""
         kind = _type(dtype, "dtype")
         out = torch.empty(self.shape, dtype=dtype, device=self.device)
-        return out if _launch(self.device.index, "ancha_hip_mx_weight_values", self._data.data_ptr(),
+        return out if _launch(self.device.index, "ancha_mx_weight_values", self._data.data_ptr(),
                               *self.shape, kind, out.data_ptr()) else None
 
 
@@ -170,7 +170,7 @@ def quantize(x: torch.Tensor, format: str = "fp4") -> Optional[Tensor]:
     flat, ld = _rows(x, dim, rows)
     out = Tensor._empty(shape, rows, format, x.device)
     codes, scales = out._pointers()
-    return out if _launch(x.get_device(), "ancha_hip_mx_quantize", flat.data_ptr(), kind, rows, dim, ld,
+    return out if _launch(x.get_device(), "ancha_mx_quantize", flat.data_ptr(), kind, rows, dim, ld,
                           bits, codes, scales) else None
 
 
@@ -190,7 +190,7 @@ def _norm(x, residual, scale, eps, format):
         total = torch.empty_like(x, memory_format=torch.contiguous_format)
     out = Tensor._empty(shape, rows, format, device)
     codes, scales = out._pointers()
-    done = _launch(device.index, "ancha_hip_mx_norm", flat.data_ptr(), kind, rows, dim, ld, _ptr(residual),
+    done = _launch(device.index, "ancha_mx_norm", flat.data_ptr(), kind, rows, dim, ld, _ptr(residual),
                    ldr, _ptr(scale), float(eps), bits, _ptr(total), codes, scales)
     return (out, total) if done else (None, None)
 
@@ -222,13 +222,13 @@ def weight(w: torch.Tensor) -> Optional[Weight]:
     if w.dim() != 2:
         raise ValueError(f"w must be [k, m], got {tuple(w.shape)}")
     k, m = w.shape
-    size = int(_native.lib().ancha_hip_mx_weight_bytes(k, m))
+    size = int(_native.lib().ancha_mx_weight_bytes(k, m))
     if size == 0:
         return None
     if min(w.stride()) < 0 or (0 in w.stride()):
         w = w.contiguous()
     data = torch.empty(size, dtype=torch.uint8, device=w.device)
-    return Weight(data, k, m) if _launch(w.get_device(), "ancha_hip_mx_weight", w.data_ptr(), kind, k, m,
+    return Weight(data, k, m) if _launch(w.get_device(), "ancha_mx_weight", w.data_ptr(), kind, k, m,
                                          *w.stride(), data.data_ptr()) else None
 
 
@@ -279,6 +279,6 @@ def linear(x: Tensor, w: Weight, epilogue: Optional[Epilogue] = None,
         out = torch.empty(tuple(shape), dtype=dtype, device=device)
         to, to_scales = out.data_ptr(), None
     codes, scales = x._pointers()
-    return out if _launch(device.index, "ancha_hip_mx_linear", codes, scales, n, k, _FORMATS[x.format],
+    return out if _launch(device.index, "ancha_mx_linear", codes, scales, n, k, _FORMATS[x.format],
                           w._data.data_ptr(), m, _ptr(bias), gelu, _ptr(table), tokens, width,
                           _ptr(residual), kind, bits, to, to_scales) else None

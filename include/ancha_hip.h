@@ -277,9 +277,9 @@ int ancha_hip_istft_noalloc(const float *spectrum, const float *masks, size_t fr
  * magnitude. A block of zeros has s = 0; one with a NaN or an infinity has s = 255, and all its values
  * are NaN.
  *
- * A tensor [rows][dim] is two arrays: codes, rows of ancha_hip_mx_pitch(dim, format) bytes (one byte per
+ * A tensor [rows][dim] is two arrays: codes, rows of ancha_mx_pitch(dim, format) bytes (one byte per
  * e4m3 value, two e2m1 values to a byte, the first in the low half), 16-byte aligned, and scales, rows of
- * ancha_hip_mx_scales(dim) bytes, 4-byte aligned. Both rows hold whole groups of 128 values; codes behind
+ * ancha_mx_scales(dim) bytes, 4-byte aligned. Both rows hold whole groups of 128 values; codes behind
  * dim are zero, and a caller who fills the arrays keeps them so. */
 #define ANCHA_HIP_F32 0
 #define ANCHA_HIP_F16 1
@@ -288,13 +288,13 @@ int ancha_hip_istft_noalloc(const float *spectrum, const float *masks, size_t fr
 #define ANCHA_HIP_MX_FP8 8
 
 /* Bytes of a row of codes / scale bytes of a row (0 for an unknown format or dim > 2^30 - 1). */
-size_t ancha_hip_mx_pitch(size_t dim, int format);
-size_t ancha_hip_mx_scales(size_t dim);
+size_t ancha_mx_pitch(size_t dim, int format);
+size_t ancha_mx_scales(size_t dim);
 
 /* codes, scales = x [rows][dim] of `type` (ANCHA_HIP_F32 / F16 / BF16), row stride ldx in elements, any
  * element alignment. */
-int ancha_hip_mx_quantize(const void *x, int type, size_t rows, size_t dim, size_t ldx, int format,
-                          void *codes, void *scales, hipStream_t stream);
+int ancha_mx_quantize(const void *x, int type, size_t rows, size_t dim, size_t ldx, int format,
+                      void *codes, void *scales, hipStream_t stream);
 
 /* The row norm into codes: h = x, or x + residual rounded to `type` and stored in sum [rows][dim]
  * (contiguous; may be x or residual itself where that is contiguous); then
@@ -302,27 +302,27 @@ int ancha_hip_mx_quantize(const void *x, int type, size_t rows, size_t dim, size
  * in 64 bits (scale [dim] fp32 or NULL for ones), and its codes and scales. eps = 0 is
  * ancha_hip_unit_norm; with scale = sqrt(dim) * gamma and eps > 0 it is the root-mean-square norm
  * gamma * h / sqrt(mean h^2 + eps). Without a residual (NULL) sum is not touched. */
-int ancha_hip_mx_norm(const void *x, int type, size_t rows, size_t dim, size_t ldx,
-                      const void *residual, size_t ldr, const float *scale, double eps, int format,
-                      void *sum, void *codes, void *scales, hipStream_t stream);
+int ancha_mx_norm(const void *x, int type, size_t rows, size_t dim, size_t ldx,
+                  const void *residual, size_t ldr, const float *scale, double eps, int format,
+                  void *sum, void *codes, void *scales, hipStream_t stream);
 
 /* out [rows][dim] of `type`, contiguous: the values that codes and scales stand for. */
-int ancha_hip_mx_values(const void *codes, const void *scales, size_t rows, size_t dim, int format,
-                        int type, void *out, hipStream_t stream);
+int ancha_mx_values(const void *codes, const void *scales, size_t rows, size_t dim, int format,
+                    int type, void *out, hipStream_t stream);
 
 /* A weight w [k][m] (element (i, j) at i * ldk + j * ldm) in e2m1 with blocks along k, laid out for
- * ancha_hip_mx_linear: ancha_hip_mx_weight_bytes(k, m) bytes (0: empty, k > 2^23 or too large), 16-byte
+ * ancha_mx_linear: ancha_mx_weight_bytes(k, m) bytes (0: empty, k > 2^23 or too large), 16-byte
  * aligned.
  * Done once, when a model is loaded. */
-size_t ancha_hip_mx_weight_bytes(size_t k, size_t m);
-int ancha_hip_mx_weight(const void *w, int type, size_t k, size_t m, size_t ldk, size_t ldm,
-                        void *weight, hipStream_t stream);
+size_t ancha_mx_weight_bytes(size_t k, size_t m);
+int ancha_mx_weight(const void *w, int type, size_t k, size_t m, size_t ldk, size_t ldm,
+                    void *weight, hipStream_t stream);
 
-/* out [k][m] of `type`, contiguous: the values of a weight made by ancha_hip_mx_weight. */
-int ancha_hip_mx_weight_values(const void *weight, size_t k, size_t m, int type, void *out,
-                               hipStream_t stream);
+/* out [k][m] of `type`, contiguous: the values of a weight made by ancha_mx_weight. */
+int ancha_mx_weight_values(const void *weight, size_t k, size_t m, int type, void *out,
+                           hipStream_t stream);
 
-/* out [n][m] = epilogue(x . w): x [n][k] in `format` as above, weight from ancha_hip_mx_weight. Products
+/* out [n][m] = epilogue(x . w): x [n][k] in `format` as above, weight from ancha_mx_weight. Products
  * of codes are exact and sums are held in fp32. The epilogue is ancha_hip_linear's, in its order: bias
  * [m] fp32; erf-GELU; rotary; residual [n][m] of `type`, contiguous (may be out). out_format 0: out is
  * [n][m] of `type`, contiguous; ANCHA_HIP_MX_FP8 / FP4: out and out_scales are the codes and scales of
@@ -330,10 +330,10 @@ int ancha_hip_mx_weight_values(const void *weight, size_t k, size_t m, int type,
  * sums are taken, 4e-6 off (rms, relative to the result, normal data); every other result is held to
  * fp32. Any k, m > 0. ANCHA_HIP_UNSUPPORTED for k == 0, m == 0 and a rotary shape that does not fit
  * (tokens == 0, n % tokens, width % 64, 2 * width > m). */
-int ancha_hip_mx_linear(const void *codes, const void *scales, size_t n, size_t k, int format,
-                        const void *weight, size_t m, const float *bias, int gelu, const float *rope,
-                        size_t tokens, size_t width, const void *residual, int type, int out_format,
-                        void *out, void *out_scales, hipStream_t stream);
+int ancha_mx_linear(const void *codes, const void *scales, size_t n, size_t k, int format,
+                    const void *weight, size_t m, const float *bias, int gelu, const float *rope,
+                    size_t tokens, size_t width, const void *residual, int type, int out_format,
+                    void *out, void *out_scales, hipStream_t stream);
 
 /* Sticky device-failure check: 0, or the first HIP error (< 0) any call has met.
  * Replaces `device::check()` (src/device.rs:30-41) for this path. */

@@ -152,7 +152,7 @@ def test_norm_layouts_and_sums_in_place(gpu):
             want = x + r
             out = mx.Tensor._empty(torch.Size((9, dim)), 9, "fp8", gpu)
             total = x if place == "x" else r
-            rc = lib.ancha_hip_mx_norm(x.data_ptr(), 0, 9, dim, dim, r.data_ptr(), dim, None, 0.0, 8,
+            rc = lib.ancha_mx_norm(x.data_ptr(), 0, 9, dim, dim, r.data_ptr(), dim, None, 0.0, 8,
                                        total.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), stream)
             assert rc == _native.OK
             assert torch.equal(total, want)
@@ -440,21 +440,21 @@ def test_nothing_beyond_the_outputs(gpu, n):
     t, w, _, _ = problem(gpu, n, k, m, "fp8", 81)
     for kind, dtype in enumerate(TYPES.values()):
         room = torch.full((n * m + 4096,), 7.0, dtype=dtype, device=gpu)
-        rc = lib.ancha_hip_mx_linear(t.codes.data_ptr(), t.scales.data_ptr(), n, k, 8, w._data.data_ptr(), m,
+        rc = lib.ancha_mx_linear(t.codes.data_ptr(), t.scales.data_ptr(), n, k, 8, w._data.data_ptr(), m,
                                      None, 0, None, 0, 0, None, kind, 0, room.data_ptr(), None, stream)
         assert rc == _native.OK and (room[n * m:] == 7).all()
         assert torch.equal(room[:n * m].view(n, m), mx.linear(t, w, dtype=dtype))
     for fmt, bits in (("fp8", 8), ("fp4", 4)):
         codes = torch.full((n * 48 * bits + 4096,), 7, dtype=torch.uint8, device=gpu)
         scales = torch.full((n * 12 + 4096,), 7, dtype=torch.uint8, device=gpu)
-        rc = lib.ancha_hip_mx_linear(t.codes.data_ptr(), t.scales.data_ptr(), n, k, 8, w._data.data_ptr(), m,
+        rc = lib.ancha_mx_linear(t.codes.data_ptr(), t.scales.data_ptr(), n, k, 8, w._data.data_ptr(), m,
                                      None, 0, None, 0, 0, None, 0, bits, codes.data_ptr(), scales.data_ptr(),
                                      stream)
         want = mx.linear(t, w, format=fmt)
         assert rc == _native.OK and (codes[n * 48 * bits:] == 7).all() and (scales[n * 12:] == 7).all()
         assert torch.equal(codes[:n * 48 * bits].view(n, -1), want.codes)
         assert torch.equal(scales[:n * 12].view(n, -1), want.scales)
-        rc = lib.ancha_hip_mx_quantize(room.data_ptr(), 2, n, 333, 333, bits, codes.data_ptr(),
+        rc = lib.ancha_mx_quantize(room.data_ptr(), 2, n, 333, 333, bits, codes.data_ptr(),
                                        scales.data_ptr(), stream)
         assert rc == _native.OK and (codes[n * 48 * bits:] == 7).all() and (scales[n * 12:] == 7).all()
 
