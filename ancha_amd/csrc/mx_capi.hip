@@ -80,10 +80,10 @@ int run_rows(const char* name, const void* x, int type, size_t rows, size_t dim,
   return e == hipSuccess ? ANCHA_HIP_OK : hip_fail(e, name);
 }
 
-// Strips and groups of a weight, one workgroup each; rows of at most 2^23 values, so that the rows of a
-// tile lie within 32 bits of its first.
+// Strips and groups of a weight, one workgroup each; at most 2^23 k and 2^24 columns, so that a tile's 128
+// rows of codes lie within 32 bits of its first, read and written.
 bool weight_fits(size_t k, size_t m) {
-  return k <= size_t(1) << 23 && m <= kIntMax / 2 &&
+  return k <= size_t(1) << 23 && m <= size_t(1) << 24 &&
          static_cast<size_t>(mx::strips(static_cast<long>(m))) *
                  static_cast<size_t>(mx::groups(static_cast<long>(k))) <
              (size_t(1) << 24);

@@ -48,14 +48,18 @@ __device__ __forceinline__ void split(unsigned c, unsigned& large, unsigned& sma
   small = c & ~mask;
 }
 
+// Whether OUT names a format of codes (or a type of values).
+constexpr bool kCodes(int out) { return out == kFp8 || out == kFp4; }
+
 // erf-GELU: x Phi(x) = max(x, 0) - |x| 2^Q(|x|) with Q a polynomial for log2 Phi(-a), fitted to the least
 // largest error of the result on [0, 6] (WIDE: degree 10, [0, 7], for fp32 results; beyond, Q stays below
 // -29 and falls, so the product vanishes). Of the value, relatively: 9e-7 above x = -1, 2e-5 above -4 (WIDE
 // 5e-7, 2e-6); absolutely within the rounding of the larger results. Eight or ten fused multiply-adds and one
 // exp2 where erf costs the vector ALU, which bounds these epilogues, three times as much: 96 120 x 384 ->
 // 1536 with bias and GELU to codes 141 us (152 with erf's rational form), to fp32 162 (229 with erff).
-template <bool WIDE>
+template <int OUT>
 __device__ __forceinline__ float gelu(float x) {
+  constexpr bool WIDE = OUT == kF32;
   const float a = fabsf(x);
   float q;
   if constexpr (WIDE) {
@@ -79,10 +83,11 @@ __device__ __forceinline__ float gelu(float x) {
     q = fmaf(a, q, -1.1511232853f);
     q = fmaf(a, q, -9.9999886751e-1f);
   }
-  return fmaf(-a, __builtin_amdgcn_exp2f(q), fmaxf(x, 0.f));
+  // An infinity times 0 would be NaN (which codes do not tell apart).
+  const float b = kCodes(OUT) ? a : fminf(a, 1e30f);
+  return fmaf(-b, __builtin_amdgcn_exp2f(q), fmaxf(x, 0.f));
 }
 
-constexpr bool kCodes(int out) { return out == kFp8 || out == kFp4; }
 
 constexpr int kOutStage = 4096;  // LDS bytes per wave for one 16 x 64 tile on its way out
 
@@ -242,7 +247,7 @@ __device__ __forceinline__ void finish_codes(const LinearParams& p, const Rows<O
   for (int i = 0; i < 16; i++) v[i] += bias[i];
   if (p.gelu)
 #pragma unroll
-    for (int i = 0; i < 16; i++) v[i] = gelu<false>(v[i]);
+    for (int i = 0; i < 16; i++) v[i] = gelu<OUT>(v[i]);
   if (p.rope && c < 2 * p.width) {
     const unsigned token = (unsigned)(d.row0 + r) % (unsigned)p.tokens;
     const float* table = p.rope + (c < p.width ? 0 : 2) * (long)p.tokens * 64 + token * 64ul + (c & 63);
@@ -309,7 +314,7 @@ __device__ __forceinline__ void finish_tile(const LinearParams& p, const Rows<OU
     for (int q = 0; q < 4; q++)
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        v[q][i] = gelu<OUT == kF32>(v[q][i]);
+        v[q][i] = gelu<OUT>(v[q][i]);
   if (p.rope && c < 2 * p.width) {
     const float* table = p.rope + (c < p.width ? 0 : 2) * (long)p.tokens * 64 + (c & 63);
 #pragma unroll
@@ -715,7 +720,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(LinearParams p) {
     }
     if (p.gelu)
 #pragma unroll
-      for (int e = 0; e < 4; e++) v[e] = gelu<OUT == kF32>(v[e]);
+      for (int e = 0; e < 4; e++) v[e] = gelu<OUT>(v[e]);
     if (p.rope && here && c < 2 * p.width) {
       const float* table = p.rope + (c < p.width ? 0 : 2) * (long)p.tokens * 64 +
                            (unsigned)row % (unsigned)p.tokens * 64ul + (c & 63);

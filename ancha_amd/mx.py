@@ -60,8 +60,8 @@ class Tensor:
     """Rows of ``shape[-1]`` values in microscaled form. ``codes`` [rows, pitch] and ``scales``
     [rows, blocks] are uint8 tensors whose rows hold whole groups of 128 values: ``pitch`` is 128 bytes
     a group for "fp8", 64 for "fp4" (two values to a byte, the first in the low half), ``blocks`` 4 a
-    group; codes behind ``shape[-1]`` are zero. A scale byte s stands for 2**(s - 127), 255 makes its
-    block NaN."""
+    group; behind ``shape[-1]`` codes are zero and scales not 255. A scale byte s stands for
+    2**(s - 127), 255 makes its block NaN."""
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, format: str, shape: Sequence[int]):
         bits = _format(format)
@@ -240,7 +240,8 @@ def linear(x: Tensor, w: Weight, epilogue: Optional[Epilogue] = None,
     product's operand. Any k, m > 0; ``None`` for an empty axis or a rotary shape that does not fit.
 
     Products of codes are exact and sums are held in 32 bits; "fp8" rows with a 16-bit ``dtype`` take
-    the matrix cores' shorter sums (4e-6 of the result on normal data, far below the type's step)."""
+    the matrix cores' shorter sums (4e-6 of the result on normal data, far below the type's step). The
+    order of a row's sums depends on n, k and m, so its last bits may differ from one n to another."""
     if not isinstance(x, Tensor) or not isinstance(w, Weight):
         raise ValueError("linear takes a microscaled Tensor and a Weight")
     kind = _type(dtype, "dtype")

@@ -279,8 +279,8 @@ int ancha_hip_istft_noalloc(const float *spectrum, const float *masks, size_t fr
  *
  * A tensor [rows][dim] is two arrays: codes, rows of ancha_mx_pitch(dim, format) bytes (one byte per
  * e4m3 value, two e2m1 values to a byte, the first in the low half), 16-byte aligned, and scales, rows of
- * ancha_mx_scales(dim) bytes, 4-byte aligned. Both rows hold whole groups of 128 values; codes behind
- * dim are zero, and a caller who fills the arrays keeps them so. */
+ * ancha_mx_scales(dim) bytes, 4-byte aligned. Both rows hold whole groups of 128 values; behind
+ * dim the codes are zero and the scales not 255, and a caller who fills the arrays keeps them so. */
 #define ANCHA_HIP_F32 0
 #define ANCHA_HIP_F16 1
 #define ANCHA_HIP_BF16 2
@@ -311,9 +311,8 @@ int ancha_mx_values(const void *codes, const void *scales, size_t rows, size_t d
                     int type, void *out, hipStream_t stream);
 
 /* A weight w [k][m] (element (i, j) at i * ldk + j * ldm) in e2m1 with blocks along k, laid out for
- * ancha_mx_linear: ancha_mx_weight_bytes(k, m) bytes (0: empty, k > 2^23 or too large), 16-byte
- * aligned.
- * Done once, when a model is loaded. */
+ * ancha_mx_linear: ancha_mx_weight_bytes(k, m) bytes (0: empty, k > 2^23, m > 2^24 or more than
+ * 2^37 values), 16-byte aligned. Done once, when a model is loaded. */
 size_t ancha_mx_weight_bytes(size_t k, size_t m);
 int ancha_mx_weight(const void *w, int type, size_t k, size_t m, size_t ldk, size_t ldm,
                     void *weight, hipStream_t stream);
@@ -328,7 +327,7 @@ int ancha_mx_weight_values(const void *weight, size_t k, size_t m, int type, voi
  * [n][m] of `type`, contiguous; ANCHA_HIP_MX_FP8 / FP4: out and out_scales are the codes and scales of
  * the fp32 result (`type` is ANCHA_HIP_F32). With e4m3 rows and a 16-bit `type` the matrix cores' own
  * sums are taken, 4e-6 off (rms, relative to the result, normal data); every other result is held to
- * fp32. Any k, m > 0. ANCHA_HIP_UNSUPPORTED for k == 0, m == 0 and a rotary shape that does not fit
+ * fp32 (below its normal range it may be 0). The order of a row's sums depends on n, k and m. Any k, m > 0. ANCHA_HIP_UNSUPPORTED for k == 0, m == 0 and a rotary shape that does not fit
  * (tokens == 0, n % tokens, width % 64, 2 * width > m). */
 int ancha_mx_linear(const void *codes, const void *scales, size_t n, size_t k, int format,
                     const void *weight, size_t m, const float *bias, int gelu, const float *rope,

@@ -57,7 +57,8 @@ def test_row_sizes(dim, groups):
 
 @pytest.mark.parametrize("k,m,size", [(1, 1, 2 * 4352), (128, 128, 2 * 4352), (129, 129, 8 * 4352),
                                       (384, 1664, 26 * 3 * 4352), (0, 5, 0), (5, 0, 0),
-                                      (1 << 20, 1 << 20, 0)])
+                                      (1 << 20, 1 << 20, 0), (128, (1 << 24) + 1, 0),
+                                      ((1 << 23) + 1, 64, 0), (128, 1 << 24, (1 << 18) * 4352)])
 def test_weight_sizes(k, m, size):
     assert _native.lib().ancha_mx_weight_bytes(k, m) == size
 
@@ -94,6 +95,7 @@ def test_entry_points_check_arguments(lib):
     assert y(k=0) == UNS and y(m=0) == UNS and y(n=0) == _native.OK
     for tok, width in ((0, 64), (3, 64), (4, 32), (4, 128)):
         assert y(rope=p, tok=tok, width=width) == UNS and "rotary" in _native.last_error()
+    assert y(m=(1 << 24) + 1) == UNS and y(k=(1 << 23) + 1) == UNS
     assert y(n=(1 << 31) - 1) == UNS and "too many" in _native.last_error()
     assert y() == UNS and "gfx950" in _native.last_error()
     assert lib.ancha_hip_check() == 0

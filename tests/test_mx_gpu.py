@@ -377,6 +377,25 @@ def test_products_not_finite(gpu, fmt):
     assert np.isnan(host(got.values())[0, 64:96]).all() and np.isfinite(host(got.values())[0, :64]).all()
 
 
+@pytest.mark.parametrize("n", [3, 3000])
+def test_gelu_of_infinities(gpu, n):
+    """Products past fp32's range: GELU(inf) = inf, GELU(-inf) = 0, NaN stays; codes mark the block."""
+    codes = torch.full((n, 128), 0x38, dtype=torch.uint8, device=gpu)  # 1.0
+    scales = torch.full((n, 4), 254, dtype=torch.uint8, device=gpu)  # 2^127
+    t = mx.Tensor(codes, scales, "fp8", (n, 128))
+    w = torch.zeros((128, 64), device=gpu)
+    w[:, 0], w[:, 1], w[:, 40] = 2.0 ** 100, -2.0 ** 100, 2.0 ** -120
+    b = torch.zeros(64, device=gpu)
+    b[2] = float("nan")
+    e = fused.Epilogue(bias=b, gelu=True)
+    for dtype in TYPES.values():
+        y = mx.linear(t, mx.weight(w), e, dtype=dtype).float()
+        assert (y[:, 0] == float("inf")).all() and (y[:, 1] == 0).all() and y[:, 2].isnan().all()
+        assert (y[:, 40] == 2.0 ** 14).all() and (y[:, 3:40] == 0).all()
+    marks = mx.linear(t, mx.weight(w), e, format="fp8").scales
+    assert (marks[:, 0] == 255).all() and (marks[:, 1] != 255).all()
+
+
 def test_zero_rows_and_empty_calls(gpu):
     w = mx.weight(dev(W.normal((100, 70), 61, 1.0), gpu))
     zero = mx.quantize(torch.zeros((5, 100), device=gpu), "fp8")
@@ -386,6 +405,18 @@ def test_zero_rows_and_empty_calls(gpu):
     three = mx.quantize(dev(W.normal((2, 3, 100), 62, 1.0), gpu), "fp4")
     flat = mx.Tensor(three.codes, three.scales, "fp4", (6, 100))
     assert torch.equal(mx.linear(three, w).reshape(6, 70), mx.linear(flat, w))
+
+
+def test_results_in_place_of_the_residual(gpu):
+    """The entry point may write over the residual that it reads, whatever the form."""
+    lib, stream = _native.lib(), torch.cuda.current_stream().cuda_stream
+    for n, k, m in ((9, 200, 77), (300, 300, 200), (130, 2100, 2050), (2100, 130, 1600)):
+        t, w, _, _ = problem(gpu, n, k, m, "fp8", 65)
+        r = dev(W.normal((n, m), 66, 1.0), gpu)
+        want = mx.linear(t, w, fused.Epilogue(residual=r))
+        rc = lib.ancha_mx_linear(*t._pointers(), n, k, 8, w._data.data_ptr(), m, None, 0, None, 0, 0,
+                                 r.data_ptr(), 0, 0, r.data_ptr(), None, stream)
+        assert rc == _native.OK and torch.equal(r, want)
 
 
 def test_refusals(gpu):
