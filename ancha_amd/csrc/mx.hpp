@@ -100,14 +100,19 @@ __device__ __forceinline__ void store_row(void* base, long at, int valid, const 
   }
 }
 
-// Magnitude of x as an unsigned number: ordered like |x|, infinities and NaN above every finite value
-// (the library is compiled without NaN semantics, so the comparison is made on the bits). x then comes from
-// its bits too, so that the compiler keeps one register for both.
-__device__ __forceinline__ unsigned magnitude(float& x) {
-  unsigned bits = __builtin_bit_cast(unsigned, x);
-  asm("" : "+v"(bits));
-  x = __builtin_bit_cast(float, bits);
-  return bits & 0x7fffffffu;
+// The exponent bits of the largest of |v[0]| .. |v[N - 1]|, 255 where one is infinite or a NaN: the
+// instruction hands a NaN on (the library is compiled without NaN semantics, so no comparison would).
+__device__ __forceinline__ float largest(float a, float b, float c) {
+  float m;
+  asm("v_maximum3_f32 %0, |%1|, |%2|, |%3|" : "=v"(m) : "v"(a), "v"(b), "v"(c));
+  return m;
+}
+template <int N>
+__device__ __forceinline__ unsigned top_exponent(const float* v) {
+  float m = largest(v[0], v[1], v[2]);
+#pragma unroll
+  for (int i = 3; i < N; i += 2) m = largest(m, v[i], v[i + 1 < N ? i + 1 : i]);
+  return __builtin_bit_cast(unsigned, m) >> 23 & 255u;
 }
 
 // Lane exchanges within 16 lanes (DPP, no LDS): the neighbour, the other pair of four lanes, the other
@@ -118,10 +123,9 @@ __device__ __forceinline__ unsigned dpp(unsigned x) {
 }
 constexpr int kSwap1 = 0xb1, kSwap2 = 0x4e, kMirror8 = 0x141, kMirror16 = 0x140;
 
-// Scale byte of a block whose largest magnitude has the bits `top`.
-__device__ __forceinline__ unsigned scale_byte(unsigned top, int format) {
-  const int e = (int)(top >> 23);
-  return e == 255 ? 255u : (unsigned)max(e - (format == kFp8 ? 8 : 2), 0);
+// Scale byte of a block whose largest magnitude has the exponent bits e.
+__device__ __forceinline__ unsigned scale_byte(unsigned e, int format) {
+  return e == 255u ? 255u : (unsigned)max((int)e - (format == kFp8 ? 8 : 2), 0);
 }
 
 // 2^(s - 127), by which the conversions divide (not for s = 255).
@@ -134,22 +138,20 @@ __device__ __forceinline__ float scale_value(unsigned s) {
   return __builtin_bit_cast(float, s == 255u ? 0x7fc00000u : s == 0u ? 0x00400000u : s << 23);
 }
 
-// e4m3 codes of four values of a block with the scale byte s (f its divisor): the conversion makes a NaN
-// of what is rounded past 448, so the values stop there first.
-__device__ __forceinline__ unsigned codes_fp8(float a, float b, float c, float d, float f) {
+// Sets MODE.FP16_OVFL: conversions to e4m3 stop at 448 instead of turning into a NaN. Conversions to fp16 stop
+// at 65504 then, and matrix instructions no longer give a NaN for the scale byte 255: only behind both.
+__device__ __forceinline__ void saturate() { __builtin_amdgcn_s_setreg(1 | 23 << 6 | 0 << 11, 1); }
+
+// e4m3 codes of four values, divided by f, with saturate() in effect.
+__device__ __forceinline__ unsigned codes_fp8(const float* v, float f) {
   typedef short s16x2 __attribute__((ext_vector_type(2)));
-  const float most = 448.f * f;
-  a = __builtin_amdgcn_fmed3f(a, -most, most);
-  b = __builtin_amdgcn_fmed3f(b, -most, most);
-  c = __builtin_amdgcn_fmed3f(c, -most, most);
-  d = __builtin_amdgcn_fmed3f(d, -most, most);
   s16x2 w = {0, 0};
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, a, b, f, false);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, c, d, f, true);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, v[0], v[1], f, false);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, v[2], v[3], f, true);
   return __builtin_bit_cast(unsigned, w);
 }
 
-// e2m1 codes of eight (four) values (the conversion saturates).
+// e2m1 codes of eight (four) values, divided by f (the conversion saturates by itself).
 __device__ __forceinline__ unsigned codes_fp4(const float* v, float f) {
   unsigned r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, v[0], v[1], f, 0);
   r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], f, 1);
@@ -163,12 +165,11 @@ __device__ __forceinline__ unsigned codes_fp4x4(const float* v, float f) {
 
 // Eight consecutive values of a row held by one lane, a block by four neighbouring lanes, a group of
 // 128 by sixteen: rounds them, writes the codes of unit `unit` (eight values, counted from the start of
-// the codes) and, from one lane of sixteen, the group's four scale bytes. All sixteen lanes take part.
-__device__ __forceinline__ void store_codes(float* v, int format, bool store, long unit,
+// the codes) and, from one lane of sixteen, the group's four scale bytes. All sixteen lanes take part, with
+// saturate() in effect.
+__device__ __forceinline__ void store_codes(const float* v, int format, bool store, long unit,
                                             uint8_t* codes, uint8_t* scales) {
-  unsigned top = 0;
-#pragma unroll
-  for (int i = 0; i < 8; i++) top = max(top, magnitude(v[i]));
+  unsigned top = top_exponent<8>(v);
   top = max(top, dpp<kSwap1>(top));
   top = max(top, dpp<kSwap2>(top));
   const unsigned s = scale_byte(top, format);
@@ -180,8 +181,7 @@ __device__ __forceinline__ void store_codes(float* v, int format, bool store, lo
   const bool none = s == 255u;
   if (!store) return;
   if (format == kFp8) {
-    const u32x2 c = {none ? 0u : codes_fp8(v[0], v[1], v[2], v[3], f),
-                     none ? 0u : codes_fp8(v[4], v[5], v[6], v[7], f)};
+    const u32x2 c = {none ? 0u : codes_fp8(v, f), none ? 0u : codes_fp8(v + 4, f)};
     __builtin_nontemporal_store(c, reinterpret_cast<u32x2*>(codes + unit * 8));
   } else {
     __builtin_nontemporal_store(none ? 0u : codes_fp4(v, f), reinterpret_cast<unsigned*>(codes + unit * 4));

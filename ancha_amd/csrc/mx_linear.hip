@@ -88,7 +88,6 @@ __device__ __forceinline__ float gelu(float x) {
   return fmaf(-b, __builtin_amdgcn_exp2f(q), fmaxf(x, 0.f));
 }
 
-
 constexpr int kOutStage = 4096;  // LDS bytes per wave for one 16 x 64 tile on its way out
 
 // Where a workgroup's rows lie: buffers over them, so that rows behind the last one read as 0 and are
@@ -163,53 +162,22 @@ __device__ __forceinline__ void store_values(const LinearParams& p, const Rows<O
   }
 }
 
-// The bits of x; x itself then comes from them, so that the compiler keeps one register for both.
-__device__ __forceinline__ unsigned bits_of(float& x) {
-  unsigned bits = __builtin_bit_cast(unsigned, x);
-  asm("" : "+v"(bits));
-  x = __builtin_bit_cast(float, bits);
-  return bits;
-}
-
-// Sixteen neighbouring values a lane, a block of 32 by lanes l and l ^ 16, to codes and the scale byte.
-// The largest magnitude is taken on the bits, as signed numbers (the largest positive value) and as
-// unsigned ones (the largest negative value, if there is one), a NaN above everything. The conversion
-// divides by the scale and, with saturate() in effect, stops at the largest value.
+// Sixteen neighbouring values a lane, a block of 32 by lanes l and l ^ 16, to codes and the scale byte,
+// with saturate() in effect.
 template <int OUT>
-__device__ __forceinline__ unsigned encode16(float* v, unsigned* codes) {
-  int positive = 0;
-  unsigned negative = 0;
-#pragma unroll
-  for (int i = 0; i < 16; i++) {
-    const unsigned b = bits_of(v[i]);
-    positive = max(positive, (int)b);
-    negative = max(negative, b);
-  }
-  unsigned top = max((unsigned)positive, negative & 0x7fffffffu);
+__device__ __forceinline__ unsigned encode16(const float* v, unsigned* codes) {
+  unsigned top = top_exponent<16>(v);
   const auto both = __builtin_amdgcn_permlane16_swap(top, top, false, false);
   top = max((unsigned)both[0], (unsigned)both[1]);
   const unsigned s = scale_byte(top, OUT);
   const float f = divisor(s);
-  typedef short s16x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
   for (int i = 0; i < (OUT == kFp8 ? 4 : 2); i++) {
-    unsigned c;
-    if constexpr (OUT == kFp8) {
-      s16x2 w = {0, 0};
-      w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, v[4 * i], v[4 * i + 1], f, false);
-      w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, v[4 * i + 2], v[4 * i + 3], f, true);
-      c = __builtin_bit_cast(unsigned, w);
-    } else {
-      c = codes_fp4(v + 8 * i, f);
-    }
+    const unsigned c = OUT == kFp8 ? codes_fp8(v + 4 * i, f) : codes_fp4(v + 8 * i, f);
     codes[i] = s == 255u ? 0u : c;
   }
   return s;
 }
-
-// Sets MODE.FP16_OVFL: conversions to e4m3 stop at 448 instead of turning into a NaN. Only behind the last
-// matrix instruction: with the mode set those no longer give a NaN for the scale byte 255.
-__device__ __forceinline__ void saturate() { __builtin_amdgcn_s_setreg(1 | 23 << 6 | 0 << 11, 1); }
 
 // Turns acc[t] of a 16 x 64 tile as the MFMAs leave it (lane l: row l % 16, columns 16 t + 4 (l / 16) ..
 // + 3) into sixteen neighbouring columns of the same row: lane l has columns 16 (l / 16) + 4 t .. + 3 in
@@ -601,7 +569,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, OCC) void tile_kernel(LinearPara
         acc[q / (SM * 4)][q / 4 % SM][q % 4] +=
             reinterpret_cast<const f32x4*>(free + o * kSums)[(wave * TN * SM * 4 + q) * 64 + lane];
   }
-  if (kCodes(OUT)) saturate();
+  if (kCodes(OUT)) saturate();  // behind the last product
   const Rows<OUT> d = rows_of<OUT>(p, row0, rows);
   const int c0 = (strip0 + wm * SM) * 64;
   if (direct)
@@ -703,6 +671,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(LinearParams p) {
       *reinterpret_cast<f32x4*>(part + wave * kPart + (16 * j + r) * 128 + (((4 * t + g) ^ (r & 7)) << 4)) =
           acc[j][t];
   __syncthreads();
+  if (kCodes(OUT)) saturate();  // behind the last product
   for (int i = (int)threadIdx.x; i < 16 * TN * 8; i += (int)blockDim.x) {
     const int tr = i >> 3, c = (int)blockIdx.x * kFewColumns + 4 * (i & 7);
     const long row = row0 + tr;
@@ -741,7 +710,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(LinearParams p) {
     } else {
 #pragma unroll
       for (int e = 0; e < 4; e++) v[e] = e < valid ? v[e] : 0.f;
-      unsigned top = max(max(magnitude(v[0]), magnitude(v[1])), max(magnitude(v[2]), magnitude(v[3])));
+      unsigned top = top_exponent<4>(v);
       top = max(top, dpp<kSwap1>(top));
       top = max(top, dpp<kSwap2>(top));
       top = max(top, dpp<kMirror8>(top));
@@ -753,7 +722,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(LinearParams p) {
       uint8_t* out = static_cast<uint8_t*>(p.out);
       if constexpr (OUT == kFp8)
         *reinterpret_cast<unsigned*>(out + unit * 4) =
-            s == 255u ? 0u : codes_fp8(v[0], v[1], v[2], v[3], f);
+            s == 255u ? 0u : codes_fp8(v, f);
       else
         *reinterpret_cast<uint16_t*>(out + unit * 2) =
             s == 255u ? (uint16_t)0 : (uint16_t)codes_fp4x4(v, f);

@@ -32,6 +32,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(RowParams p) {
   const int valid = here ? p.dim - u.col : 0;
   float v[8];
   load_row<TYPE, 8>(p.x, valid > 0 ? (long)u.row * p.ldx + u.col : 0, valid, v);
+  saturate();
   store_codes(v, FORMAT, here, u.at, p.codes, p.scales);
 }
 
@@ -48,7 +49,9 @@ __device__ __forceinline__ double sum_lanes(double s) {
 // gives what rounding d itself does.
 __device__ __forceinline__ float to_odd(double d) {
   const unsigned long long bits = __builtin_bit_cast(unsigned long long, d);
-  const unsigned hi = (unsigned)(bits >> 32) | min((unsigned)bits, 1u);
+  unsigned lost;  // one instruction where the compiler takes two
+  asm("v_min_u32 %0, 1, %1" : "=v"(lost) : "v"((unsigned)bits));
+  const unsigned hi = (unsigned)(bits >> 32) | lost;
   return (float)__builtin_bit_cast(double, (unsigned long long)hi << 32);
 }
 
@@ -64,6 +67,13 @@ __device__ __forceinline__ double inverse_length(double s) {
 #pragma unroll
   for (int i = 0; i < 2; i++) y = __builtin_fma(0.5 * y, __builtin_fma(-s * y, y, 1.0), y);
   return y;
+}
+
+// saturate() between the sums' rounding to fp16, on which inv depends, and the codes, which depend on inv.
+__device__ __forceinline__ void saturate_before(double& inv) {
+  asm volatile("" : "+v"(inv));
+  saturate();
+  asm volatile("" : "+v"(inv));
 }
 
 template <int TYPE>
@@ -143,7 +153,8 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(RowParams p) {
 #pragma unroll
     for (int w = 0; w < kWaves; w++) ss += part[wave / kWaves * kWaves + w];
   }
-  const double inv = inverse_length(ss + (double)p.dim * p.eps);
+  double inv = inverse_length(ss + (double)p.dim * p.eps);
+  saturate_before(inv);
   const long first = row * (padded / 8);
 #pragma unroll
   for (int i = 0; i < V; i++) {
@@ -181,7 +192,8 @@ __global__ __launch_bounds__(kThreads) void norm_long_kernel(RowParams p) {
   ss = 0.0;
 #pragma unroll
   for (int w = 0; w < kThreads / 64; w++) ss += part[w];
-  const double inv = inverse_length(ss + (double)p.dim * p.eps);
+  double inv = inverse_length(ss + (double)p.dim * p.eps);
+  saturate_before(inv);
   const long first = (long)row * (padded / 8);
   // The sum is read back by the thread that wrote it.
   const void* from = p.residual ? p.sum : p.x;

@@ -27,13 +27,9 @@ __global__ __launch_bounds__(256) void weight_columns_kernel(WeightParams p) {
 #pragma unroll
   for (int i = 0; i < 32; i++) t[i] = x[(long)min(k0 + i, p.k - 1) * p.ldk];
   float v[32];
-  unsigned top = 0;
 #pragma unroll
-  for (int i = 0; i < 32; i++) {
-    v[i] = col < p.m && k0 + i < p.k ? (float)t[i] : 0.f;
-    top = max(top, magnitude(v[i]));
-  }
-  const unsigned s = scale_byte(top, kFp4);
+  for (int i = 0; i < 32; i++) v[i] = col < p.m && k0 + i < p.k ? (float)t[i] : 0.f;
+  const unsigned s = scale_byte(top_exponent<32>(v), kFp4);
   const float f = divisor(s);
   u32x4 q;
 #pragma unroll
@@ -62,12 +58,9 @@ __global__ __launch_bounds__(256) void weight_rows_kernel(WeightParams p) {
   for (int i = 0; i < 4; i++) {
     const int c = 16 * wave + 4 * i + (lane >> 4);
     float v[8];
-    unsigned top = 0;
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      v[e] = (float)t[i][e];
-      top = max(top, magnitude(v[e]));
-    }
+    for (int e = 0; e < 8; e++) v[e] = (float)t[i][e];
+    unsigned top = top_exponent<8>(v);
     top = max(top, dpp<kSwap1>(top));
     top = max(top, dpp<kSwap2>(top));
     const unsigned s = scale_byte(top, kFp4);
