@@ -327,8 +327,9 @@ int ancha_mx_weight_values(const void *weight, size_t k, size_t m, int type, voi
  * [n][m] of `type`, contiguous; ANCHA_HIP_MX_FP8 / FP4: out and out_scales are the codes and scales of
  * the fp32 result (`type` is ANCHA_HIP_F32). With e4m3 rows and a 16-bit `type` the matrix cores' own
  * sums are taken, 4e-6 off (rms, relative to the result, normal data); every other result is held to
- * fp32 (below its normal range it may be 0). The order of a row's sums depends on n, k and m. Any k, m > 0. ANCHA_HIP_UNSUPPORTED for k == 0, m == 0 and a rotary shape that does not fit
- * (tokens == 0, n % tokens, width % 64, 2 * width > m). */
+ * fp32 (below its normal range it may be 0). The order of a row's sums depends on n, k and m. Any k, m > 0.
+ * ANCHA_HIP_UNSUPPORTED for k == 0, m == 0 and a rotary shape that does not fit (tokens == 0, n % tokens,
+ * width % 64, 2 * width > m). */
 int ancha_mx_linear(const void *codes, const void *scales, size_t n, size_t k, int format,
                     const void *weight, size_t m, const float *bias, int gelu, const float *rope,
                     size_t tokens, size_t width, const void *residual, int type, int out_format,
