@@ -121,7 +121,7 @@ template <int CTRL>
 __device__ __forceinline__ unsigned dpp(unsigned x) {
   return (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true);
 }
-constexpr int kSwap1 = 0xb1, kSwap2 = 0x4e, kMirror8 = 0x141, kMirror16 = 0x140;
+constexpr int kSwap1 = 0xb1, kSwap2 = 0x4e, kMirror8 = 0x141;
 
 // Scale byte of a block whose largest magnitude has the exponent bits e.
 __device__ __forceinline__ unsigned scale_byte(unsigned e, int format) {
@@ -163,20 +163,15 @@ __device__ __forceinline__ unsigned codes_fp4x4(const float* v, float f) {
   return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], f, 1);
 }
 
-// Eight consecutive values of a row held by one lane, a block by four neighbouring lanes, a group of
-// 128 by sixteen: rounds them, writes the codes of unit `unit` (eight values, counted from the start of
-// the codes) and, from one lane of sixteen, the group's four scale bytes. All sixteen lanes take part, with
-// saturate() in effect.
+// Eight consecutive values of a row held by one lane, a block by four neighbouring lanes, all of which take
+// part with saturate() in effect: rounds them, writes the codes of unit `unit` (eight values, counted from the
+// start of the codes) and, from a block's first lane, its scale byte.
 __device__ __forceinline__ void store_codes(const float* v, int format, bool store, long unit,
                                             uint8_t* codes, uint8_t* scales) {
   unsigned top = top_exponent<8>(v);
   top = max(top, dpp<kSwap1>(top));
   top = max(top, dpp<kSwap2>(top));
   const unsigned s = scale_byte(top, format);
-  const int lane = threadIdx.x & 15;
-  unsigned all = s << (8 * (lane >> 2));
-  all |= dpp<kMirror8>(all);
-  all |= dpp<kMirror16>(all);
   const float f = divisor(s);
   const bool none = s == 255u;
   if (!store) return;
@@ -186,7 +181,7 @@ __device__ __forceinline__ void store_codes(const float* v, int format, bool sto
   } else {
     __builtin_nontemporal_store(none ? 0u : codes_fp4(v, f), reinterpret_cast<unsigned*>(codes + unit * 4));
   }
-  if (lane == 0) *reinterpret_cast<unsigned*>(scales + (unit >> 4) * 4) = all;
+  if (threadIdx.x % 4 == 0) scales[unit >> 2] = (uint8_t)s;
 }
 
 // ---- parameter blocks and launchers (arguments checked by the entry points)

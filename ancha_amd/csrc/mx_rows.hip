@@ -118,15 +118,16 @@ __device__ __forceinline__ void normed(const RowParams& p, const float* h, doubl
     for (int j = 0; j < 8; j++) y[j] = col + j < p.dim ? y[j] : 0.f;
 }
 
-// One row by L threads, eight neighbouring values each, V times; a workgroup of 256 threads. A piece of 8 L
+// One row by L threads, eight neighbouring values each, V times; a workgroup of 256 threads or L. A piece of 8 L
 // columns that all exist is read and written without a mask (threads behind the last row read that one).
 // The row stays in registers, so memory is passed once. With the addition it is what bounds: 96 120 x 384 fp32
 // 80 us (481 MB, 6.0 TB/s). Without it, on 16-bit rows, the vector ALU does (91 % busy), with about 21
 // instructions a value, seven of them in 64 bits: 30 000 x 1024 bf16 23 us (4.0 TB/s).
 template <int TYPE, int L, int V>
-__global__ __launch_bounds__(kThreads) void norm_kernel(RowParams p) {
+__global__ __launch_bounds__(L > kThreads ? L : kThreads) void norm_kernel(RowParams p) {
+  constexpr int kAll = L > kThreads ? L : kThreads;
   const int at = threadIdx.x % L;
-  const unsigned mine = blockIdx.x * (unsigned)(kThreads / L) + threadIdx.x / L;
+  const unsigned mine = blockIdx.x * (unsigned)(kAll / L) + threadIdx.x / L;
   const bool here = mine < (unsigned)p.rows;
   const long row = here ? mine : p.rows - 1;
   const int padded = kGroup * (int)groups(p.dim);
@@ -167,7 +168,7 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(RowParams p) {
   ss = sum_lanes<(L < 64 ? L : 64)>(ss);
   if constexpr (L > 64) {
     constexpr int kWaves = L / 64;  // of a row
-    __shared__ double part[kThreads / 64];
+    __shared__ double part[kAll / 64];
     const int wave = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 0) part[wave] = ss;
     __syncthreads();
@@ -188,8 +189,9 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(RowParams p) {
   }
 }
 
-// Rows longer than the registers hold (more than 8192 values): read twice, the second time mostly from the
-// caches. 2000 x 12 000 bf16 with the addition 47 us (3.6 TB/s of what has to be moved).
+// Rows longer than the registers hold (more than 16 384 values): read twice, the second time mostly from the
+// caches. 2000 x 20 000 bf16 with the addition 76 us (3.7 TB/s of what has to be moved; 92 with the sum left in
+// the caches for it).
 template <int TYPE>
 __global__ __launch_bounds__(kThreads) void norm_long_kernel(RowParams p) {
   const unsigned row = blockIdx.x;
@@ -229,9 +231,9 @@ __global__ __launch_bounds__(kThreads) void norm_long_kernel(RowParams p) {
   }
 }
 
-// A unit of 16 bytes of TYPE a thread (a store instruction of a wave then writes one piece of memory: with
-// eight fp32 values a thread 96 120 x 384 took 53 us, so 27): code times 2^(s - 127), exact but for the rounding
-// to TYPE. Bound by memory: 16 384 x 8192 e2m1 to bf16 48 us (7.1 TB/s).
+// A unit of 16 bytes of TYPE a thread, so that a wave's store instruction writes one piece of memory: code times
+// 2^(s - 127), exact but for the rounding to TYPE. Bound by memory: 16 384 x 8192 e2m1 to bf16 48 us (7.1 TB/s),
+// 96 120 x 384 e4m3 to fp32 27 (6.9; 53 with eight values a thread).
 template <int TYPE>
 constexpr int kDecoded = TYPE == kF32 ? 4 : 8;
 template <int TYPE, int FORMAT>
@@ -269,13 +271,13 @@ __global__ __launch_bounds__(kThreads) void values_kernel(ValueParams p, Divide 
 
 template <int TYPE, int L, int V>
 void start_norm(const RowParams& p, hipStream_t stream) {
-  constexpr int kRows = kThreads / L;
+  constexpr int kAll = L > kThreads ? L : kThreads, kRows = kAll / L;
   hipLaunchKernelGGL((norm_kernel<TYPE, L, V>), dim3((p.rows + (long)kRows - 1) / kRows),
-                     dim3(kThreads), 0, stream, p);
+                     dim3(kAll), 0, stream, p);
 }
 
 // Rows in registers, L threads a row and V pieces of 8 L values. Measured with each form forced (us, with
-// the addition / without):
+// the addition / without; the forms taken are up to 15 % faster since, by lighter codes):
 //   96 120 x 384 fp32     16 threads  80 / 37, 64  79 / 47, 32  107 / 54
 //   30 000 x 700 bf16     32 threads  36 / 25, 64  38 / 28, 128  51 / 37
 //   30 000 x 1024 bf16    64 threads  37 / 25, 32  38 / 26, 128  43 / 31
@@ -283,12 +285,16 @@ void start_norm(const RowParams& p, hipStream_t stream) {
 //   30 000 x 4096 bf16   256 threads 156 / 92, 128 172 / 91, 64  208 / 112
 // and, with few rows, the more threads a row the shorter the way through it: 200 x 1500 fp16 256 threads
 // 5.0 / 4.4, 64 7.1 / 5.8, 32 10.3 / 8.1; 300 x 384 fp16 64 threads 4.4 / 4.7, 16 6.1 / 5.2.
+// Past 8192 values 512 threads, with the addition: 2000 x 12 000 bf16 36 (read twice 47), 2000 x 16 000 fp32 74
+// (118). Four fp32 values side by side a thread in place of eight were slower: 96 120 x 384 84 / 38 (80 / 31).
 template <int TYPE>
 void norm_of_type(const RowParams& p, hipStream_t stream) {
   const long g = groups(p.dim);
   const bool few = p.rows < 1024;
-  if (g > 64)
+  if (g > 128)
     hipLaunchKernelGGL(norm_long_kernel<TYPE>, dim3(p.rows), dim3(kThreads), 0, stream, p);
+  else if (g > 64)
+    start_norm<TYPE, 512, 4>(p, stream);
   else if (g > 32)
     start_norm<TYPE, 256, 4>(p, stream);
   else if (g > 16)

@@ -128,7 +128,7 @@ def test_norms(gpu, dim, kind):
 
 
 def test_norm_special_rows(gpu):
-    for dim in (300, 700, 3000, 9000):
+    for dim in (300, 700, 3000, 9000, 17000):
         x = W.normal((6, dim), 11, 1.0)
         x[1, 40], x[2, dim - 1], x[3] = np.inf, np.nan, 0
         x[4], x[5] = 1e-30, 3e38
@@ -136,6 +136,19 @@ def test_norm_special_rows(gpu):
         want = O.encode(O.unit_norm(x), "fp8")
         same_bytes(f"dim {dim}", got, want)
         assert want[1][1, 40 // 32] == 255 and (want[1][2, :-(-dim // 32)] == 255).all()
+
+
+@pytest.mark.parametrize("dim", [64, 700, 2500, 9000, 17000])
+def test_sums_that_overflow(gpu, dim):
+    """fp16 sums past 65504 are infinite, in the stream and for the norm, in every form of the kernel."""
+    x, r = (dev(W.normal((3, dim), seed, 1.0), gpu, torch.float16) for seed in (17, 18))
+    x[1, dim - 3] = r[1, dim - 3] = 60000
+    x[2, 5] = r[2, 5] = -60000
+    for fmt in ("fp8", "fp4"):
+        got, total = mx.add_unit_norm(x, r, None, 1e-5, fmt)
+        h = (x.float() + r.float()).half()
+        assert torch.equal(total, h) and bool(h[1:].isinf().any(1).all())
+        same_bytes(f"dim {dim}", got, O.encode(O.unit_norm(host(h), None, 1e-5), fmt))
 
 
 def test_norm_layouts_and_sums_in_place(gpu):
@@ -146,7 +159,7 @@ def test_norm_layouts_and_sums_in_place(gpu):
         got, total = mx.add_unit_norm(x, r)
         assert torch.equal(total, x + r) and total.is_contiguous()
         same_bytes("strided", got, O.encode(O.unit_norm(host(x + r)), "fp8"))
-    for dim in (384, 1549, 12000):
+    for dim in (384, 1549, 12000, 17000):
         for place in ("x", "residual"):
             x, r = dev(rows_of((9, dim), 15), gpu), dev(W.normal((9, dim), 16, 1.0), gpu)
             want = x + r
