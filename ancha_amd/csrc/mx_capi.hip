@@ -19,7 +19,8 @@ bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) %
 bool is_type(int t) { return t == ANCHA_HIP_F32 || t == ANCHA_HIP_F16 || t == ANCHA_HIP_BF16; }
 bool is_format(int f) { return f == ANCHA_HIP_MX_FP8 || f == ANCHA_HIP_MX_FP4; }
 
-// rows x dim values as units of eight, one thread each: below HIP's 2^32 threads and 65 536 column pieces.
+// rows x dim values as fewer than 2^27 stored groups, so that sixteen or 32 threads a group (a row's in the norm)
+// stay below HIP's 2^32, in rows of at most 2^26 values.
 bool units_fit(size_t rows, size_t dim) {
   return rows <= kIntMax && dim <= size_t(1) << 26 &&
          rows <= ((size_t(1) << 27) - 1024) / static_cast<size_t>(mx::groups(static_cast<long>(dim)));
