@@ -121,7 +121,7 @@ template <int CTRL>
 __device__ __forceinline__ unsigned dpp(unsigned x) {
   return (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true);
 }
-constexpr int kSwap1 = 0xb1, kSwap2 = 0x4e, kMirror8 = 0x141;
+constexpr int kSwap1 = 0xb1, kSwap2 = 0x4e, kMirror8 = 0x141, kMirror16 = 0x140;
 
 // Scale byte of a block whose largest magnitude has the exponent bits e.
 __device__ __forceinline__ unsigned scale_byte(unsigned e, int format) {
@@ -164,10 +164,10 @@ __device__ __forceinline__ unsigned codes_fp4x4(const float* v, float f) {
 }
 
 // Eight consecutive values of a row held by one lane, a block by four neighbouring lanes, all of which take
-// part with saturate() in effect: rounds them, writes the codes of unit `unit` (eight values, counted from the
-// start of the codes) and, from a block's first lane, its scale byte.
-__device__ __forceinline__ void store_codes(const float* v, int format, bool store, long unit,
-                                            uint8_t* codes, uint8_t* scales) {
+// part with saturate() in effect: rounds them, writes their codes to `codes` and, from a block's first lane,
+// its scale byte to `scale`.
+__device__ __forceinline__ void store_codes(const float* v, int format, bool store, uint8_t* codes,
+                                            uint8_t* scale) {
   unsigned top = top_exponent<8>(v);
   top = max(top, dpp<kSwap1>(top));
   top = max(top, dpp<kSwap2>(top));
@@ -177,11 +177,11 @@ __device__ __forceinline__ void store_codes(const float* v, int format, bool sto
   if (!store) return;
   if (format == kFp8) {
     const u32x2 c = {none ? 0u : codes_fp8(v, f), none ? 0u : codes_fp8(v + 4, f)};
-    __builtin_nontemporal_store(c, reinterpret_cast<u32x2*>(codes + unit * 8));
+    __builtin_nontemporal_store(c, reinterpret_cast<u32x2*>(codes));
   } else {
-    __builtin_nontemporal_store(none ? 0u : codes_fp4(v, f), reinterpret_cast<unsigned*>(codes + unit * 4));
+    __builtin_nontemporal_store(none ? 0u : codes_fp4(v, f), reinterpret_cast<unsigned*>(codes));
   }
-  if (threadIdx.x % 4 == 0) scales[unit >> 2] = (uint8_t)s;
+  if (threadIdx.x % 4 == 0) *scale = (uint8_t)s;
 }
 
 // ---- parameter blocks and launchers (arguments checked by the entry points)

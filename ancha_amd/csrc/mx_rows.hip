@@ -52,14 +52,33 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(RowParams p, Divide 
   float v[8];
   load_row<TYPE, 8>(p.x, valid > 0 ? (long)u.row * p.ldx + u.col : 0, valid, v);
   saturate();
-  store_codes(v, FORMAT, here, u.at, p.codes, p.scales);
+  store_codes(v, FORMAT, here, p.codes + u.at * (FORMAT == kFp8 ? 8 : 4), p.scales + (u.at >> 2));
 }
 
-// Sum over L lanes (a power of two up to 64) in 64 bits.
+// Sum over L = 16, 32 or 64 lanes in 64 bits, by lane exchanges without LDS.
+template <int CTRL>
+__device__ __forceinline__ double add_lane(double s) {
+  const unsigned long long b = __builtin_bit_cast(unsigned long long, s);
+  const unsigned long long hi = dpp<CTRL>((unsigned)(b >> 32)), lo = dpp<CTRL>((unsigned)b);
+  return s + __builtin_bit_cast(double, hi << 32 | lo);
+}
 template <int L>
 __device__ __forceinline__ double sum_lanes(double s) {
+  s = add_lane<kSwap1>(s);
+  s = add_lane<kSwap2>(s);
+  s = add_lane<kMirror8>(s);
+  s = add_lane<kMirror16>(s);
 #pragma unroll
-  for (int o = 1; o < L; o <<= 1) s += __shfl_xor(s, o);
+  for (int o = 16; o < L; o <<= 1) {
+    const unsigned long long b = __builtin_bit_cast(unsigned long long, s);
+    const unsigned h = (unsigned)(b >> 32), l = (unsigned)b;
+    const auto hi = o == 16 ? __builtin_amdgcn_permlane16_swap(h, h, false, false)
+                            : __builtin_amdgcn_permlane32_swap(h, h, false, false);
+    const auto lo = o == 16 ? __builtin_amdgcn_permlane16_swap(l, l, false, false)
+                            : __builtin_amdgcn_permlane32_swap(l, l, false, false);
+    s = __builtin_bit_cast(double, (unsigned long long)(unsigned)hi[0] << 32 | (unsigned)lo[0]) +
+        __builtin_bit_cast(double, (unsigned long long)(unsigned)hi[1] << 32 | (unsigned)lo[1]);
+  }
   return s;
 }
 
@@ -178,14 +197,17 @@ __global__ __launch_bounds__(L > kThreads ? L : kThreads) void norm_kernel(RowPa
   }
   double inv = inverse_length(ss + (double)p.dim * p.eps);
   saturate_before(inv);
-  const long first = row * (padded / 8);
+  const long first = row * (padded / 8) + at;
+  const int bytes = p.format == kFp8 ? 8 : 4;  // of a unit
+  uint8_t* const codes = p.codes + first * bytes;
+  uint8_t* const scales = p.scales + (first >> 2);
 #pragma unroll
   for (int i = 0; i < V; i++) {
     if (8 * L * i >= padded) break;
     const int col = 8 * (at + L * i);
     float y[8];
     normed(p, h[i], inv, col, 8 * L * (i + 1) <= p.dim, y);
-    store_codes(y, p.format, here && col < padded, first + at + L * i, p.codes, p.scales);
+    store_codes(y, p.format, here && col < padded, codes + L * i * bytes, scales + L * i / 4);
   }
 }
 
@@ -220,6 +242,7 @@ __global__ __launch_bounds__(kThreads) void norm_long_kernel(RowParams p) {
   double inv = inverse_length(ss + (double)p.dim * p.eps);
   saturate_before(inv);
   const long first = (long)row * (padded / 8);
+  const int bytes = p.format == kFp8 ? 8 : 4;  // of a unit
   // The sum is read back by the thread that wrote it.
   const void* from = p.residual ? p.sum : p.x;
   const long ld = p.residual ? p.dim : p.ldx;
@@ -227,7 +250,7 @@ __global__ __launch_bounds__(kThreads) void norm_long_kernel(RowParams p) {
     float h[8], y[8];
     load_row<TYPE, 8>(from, col < p.dim ? (long)row * ld + col : 0, p.dim - col, h);
     normed(p, h, inv, col, col + 8 <= p.dim, y);
-    store_codes(y, p.format, true, first + col / 8, p.codes, p.scales);
+    store_codes(y, p.format, true, p.codes + (first + col / 8) * bytes, p.scales + (first + col / 8) / 4);
   }
 }
 
