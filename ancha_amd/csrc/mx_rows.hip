@@ -140,8 +140,8 @@ __device__ __forceinline__ void normed(const RowParams& p, const float* h, doubl
 // One row by L threads, eight neighbouring values each, V times; a workgroup of 256 threads or L. A piece of 8 L
 // columns that all exist is read and written without a mask (threads behind the last row read that one).
 // The row stays in registers, so memory is passed once. With the addition it is what bounds: 96 120 x 384 fp32
-// 80 us (481 MB, 6.0 TB/s). Without it, on 16-bit rows, the vector ALU does (91 % busy), with about 21
-// instructions a value, seven of them in 64 bits: 30 000 x 1024 bf16 23 us (4.0 TB/s).
+// 80 us (481 MB, 6.0 TB/s). Without it, on 16-bit rows, the vector ALU does (91 % busy), with about 20
+// instructions a value, seven of them in 64 bits: 30 000 x 1024 bf16 22 us (4.3 TB/s).
 template <int TYPE, int L, int V>
 __global__ __launch_bounds__(L > kThreads ? L : kThreads) void norm_kernel(RowParams p) {
   constexpr int kAll = L > kThreads ? L : kThreads;

@@ -369,6 +369,18 @@ def test_results_in_codes(gpu, n, k, m, fmt, out):
         check_codes(f"{name} {n}x{k}x{m} {fmt} -> {out}", got, y, tol, out)
 
 
+@pytest.mark.parametrize("out", ["fp8", "fp4"])
+@pytest.mark.parametrize("n,k,m", [(6, 100, 200), (801, 128, 192), (2100, 200, 1549), (8200, 130, 512)])
+def test_rotary_results_in_codes(gpu, n, k, m, out):
+    t, w, x, wv = problem(gpu, n, k, m, "fp8", 45)
+    b, width = dev(W.normal((m,), 46, 0.5), gpu), m // 128 * 64
+    tokens = max(d for d in range(1, 300) if n % d == 0)
+    table = W.axis_rope_packed(W.rope_freqs(), tokens)
+    got = mx.linear(t, w, fused.Epilogue(bias=b, rotary=(dev(table, gpu), width)), format=out)
+    y, tol = expected(x, wv, "fp8", False, host(b), False, (table.astype(np.float64), width))
+    check_codes(f"rotary {n}x{k}x{m} -> {out}", got, y, tol, out)
+
+
 @pytest.mark.parametrize("fmt", ["fp8", "fp4"])
 def test_products_not_finite(gpu, fmt):
     """A NaN block of a row spoils that row alone, one of the weight its column alone; codes of a result
