@@ -91,6 +91,23 @@ def test_quantize_special_values(gpu):
         same_bytes("f16", half, O.encode(x.astype(np.float16).astype(np.float64), "fp8"))
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("fmt", ["fp8", "fp4"])
+def test_quantize_ends_of_the_types(gpu, fmt, kind):
+    """Infinities and NaN of every input type, its largest and its smallest values, in blocks of their own."""
+    dtype = TYPES[kind]
+    x = dev(W.normal((7, 200), 19, 1.0), gpu, dtype)
+    ends = torch.finfo(dtype)
+    x[0, 3], x[1, 40], x[2, 199], x[3, 31] = float("inf"), float("-inf"), float("nan"), -float("nan")
+    x[4, 64], x[4, 100] = ends.max, -ends.max
+    x[5, 32:64] = ends.tiny
+    x[6, 32:64] = 0
+    x[6, 40] = ends.smallest_normal * ends.eps  # the smallest of all
+    want = O.encode(host(x), fmt)
+    same_bytes(f"{fmt} {kind}", mx.quantize(x, fmt), want)
+    assert [int((want[1][r] == 255).sum()) for r in range(7)] == [1, 1, 1, 1, 0, 0, 0]
+
+
 @pytest.mark.parametrize("fmt", ["fp8", "fp4"])
 def test_quantize_layouts(gpu, fmt):
     base = dev(rows_of((40, 301), 5), gpu)
