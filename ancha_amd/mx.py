@@ -239,8 +239,8 @@ def linear(x: Tensor, w: Weight, epilogue: Optional[Epilogue] = None,
     [..., m] in ``dtype``, or with ``format`` the :class:`Tensor` of the float32 result, the next
     product's operand. Any k, m > 0; ``None`` for an empty axis or a rotary shape that does not fit.
 
-    Products of codes are exact and sums are held in 32 bits; "fp8" rows with a 16-bit ``dtype`` take
-    the matrix cores' shorter sums (4e-6 of the result on normal data, far below the type's step). The
+    Products of codes are exact and sums are held in 32 bits, whatever ``dtype`` ("fp8" rows take the
+    matrix cores two passes for that, so twice the time of "fp4" rows where these are what bounds). The
     order of a row's sums depends on n, k and m, so its last bits may differ from one n to another."""
     if not isinstance(x, Tensor) or not isinstance(w, Weight):
         raise ValueError("linear takes a microscaled Tensor and a Weight")

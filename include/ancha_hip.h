@@ -325,9 +325,8 @@ int ancha_mx_weight_values(const void *weight, size_t k, size_t m, int type, voi
  * of codes are exact and sums are held in fp32. The epilogue is ancha_hip_linear's, in its order: bias
  * [m] fp32; erf-GELU; rotary; residual [n][m] of `type`, contiguous (may be out). out_format 0: out is
  * [n][m] of `type`, contiguous; ANCHA_HIP_MX_FP8 / FP4: out and out_scales are the codes and scales of
- * the fp32 result (`type` is ANCHA_HIP_F32). With e4m3 rows and a 16-bit `type` the matrix cores' own
- * sums are taken, 4e-6 off (rms, relative to the result, normal data); every other result is held to
- * fp32 (below its normal range it may be 0). The order of a row's sums depends on n, k and m. Any k, m > 0.
+ * the fp32 result (`type` is ANCHA_HIP_F32). Sums are held to fp32 whatever `type` (below its normal range
+ * they may be 0). The order of a row's sums depends on n, k and m. Any k, m > 0.
  * ANCHA_HIP_UNSUPPORTED for k == 0, m == 0 and a rotary shape that does not fit (tokens == 0, n % tokens,
  * width % 64, 2 * width > m). */
 int ancha_mx_linear(const void *codes, const void *scales, size_t n, size_t k, int format,

@@ -1,0 +1,44 @@
+"""The product of microscaled rows where its forms and its roundings meet hard values: sums whose large
+products cancel. Oracle and tolerances: tests/test_mx_gpu.py."""
+import numpy as np
+import pytest
+import torch
+
+from ancha_amd import mx
+from oracle import mx as O
+from tests.test_mx_gpu import TYPES, dev, expected, host, near
+
+pytestmark = pytest.mark.gpu
+
+# One size for each form of the product: few rows, 64 x 64 tiles with the steps in one chain and in four, 128 x
+# 128 tiles, 256 columns.
+FORMS = [(5, 300, 40), (801, 1000, 1549), (130, 2100, 2050), (2100, 200, 1549), (8200, 130, 2048)]
+
+
+def cancelling(n, k, m):
+    """x [n, k], w [k, m] that both formats hold exactly: of every eight neighbouring products two are large and
+    add up to 0, one is small, the others are 0."""
+    rng = np.random.default_rng(n + k + m)
+    x, w = np.zeros((n, k), np.float32), np.zeros((k, m), np.float32)
+    large, small = O.grid("fp8")[-7:], O.grid("fp8")[1:41]  # 256 .. 448, 2^-9 .. 0.25
+    for k0 in range(0, k - 7, 8):
+        a, b, c = k0 + rng.choice(8, 3, replace=False)
+        x[:, a] = rng.choice(large, n)
+        x[:, b] = -x[:, a]
+        x[:, c] = rng.choice(small, n)
+        w[a] = w[b] = rng.choice((4.0, -4.0, 6.0, -6.0), m)
+        w[c] = rng.choice((0.5, 1.0, 1.5), m)
+    return x, w
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("n,k,m", FORMS)
+def test_large_products_cancel(gpu, n, k, m, kind):
+    """e4m3 sums are held in 32 bits whatever the result's type: small products beside large ones that cancel
+    are what is left."""
+    x, w = cancelling(n, k, m)
+    t, handle = mx.quantize(dev(x, gpu), "fp8"), mx.weight(dev(w, gpu))
+    xv, wv = host(t.values()), host(handle.values())
+    y, tol = expected(xv, wv, "fp8", False, dtype=TYPES[kind])
+    assert (tol < 0.25 * np.abs(y).mean()).all()
+    near(f"{n}x{k}x{m} {kind}", host(mx.linear(t, handle, dtype=TYPES[kind])), y, tol)
