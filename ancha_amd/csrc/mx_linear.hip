@@ -83,9 +83,8 @@ __device__ __forceinline__ float gelu(float x) {
     q = fmaf(a, q, -1.1511232853f);
     q = fmaf(a, q, -9.9999886751e-1f);
   }
-  // An infinity times 0 would be NaN (which codes do not tell apart).
-  const float b = kCodes(OUT) ? a : fminf(a, 1e30f);
-  return fmaf(-b, __builtin_amdgcn_exp2f(q), fmaxf(x, 0.f));
+  // An infinity times 0 would be NaN.
+  return fmaf(-fminf(a, 1e30f), __builtin_amdgcn_exp2f(q), fmaxf(x, 0.f));
 }
 
 constexpr int kOutStage = 4096;  // LDS bytes per wave for one 16 x 64 tile on its way out

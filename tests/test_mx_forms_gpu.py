@@ -1,12 +1,12 @@
 """The product of microscaled rows where its forms and its roundings meet hard values: sums whose large
-products cancel. Oracle and tolerances: tests/test_mx_gpu.py."""
+products cancel, GELU of infinities. Oracle and tolerances: tests/test_mx_gpu.py."""
 import numpy as np
 import pytest
 import torch
 
-from ancha_amd import mx
+from ancha_amd import fused, mx
 from oracle import mx as O
-from tests.test_mx_gpu import TYPES, dev, expected, host, near
+from tests.test_mx_gpu import TYPES, dev, expected, host, near, same_bytes
 
 pytestmark = pytest.mark.gpu
 
@@ -42,3 +42,33 @@ def test_large_products_cancel(gpu, n, k, m, kind):
     y, tol = expected(xv, wv, "fp8", False, dtype=TYPES[kind])
     assert (tol < 0.25 * np.abs(y).mean()).all()
     near(f"{n}x{k}x{m} {kind}", host(mx.linear(t, handle, dtype=TYPES[kind])), y, tol)
+
+
+# ---- GELU. Rows of zeros give products of exactly 0, so the bias is what GELU takes.
+
+GELU_FORMS = [(3, 200, 700), (801, 200, 1549), (130, 2100, 2050), (2100, 200, 1549), (8200, 130, 2048)]
+
+
+def on_bias(gpu, n, k, m, values):
+    zeros = mx.quantize(torch.zeros((n, k), device=gpu), "fp8")
+    bias = torch.zeros(m, device=gpu)
+    bias[:len(values)] = dev(values, gpu)
+    return zeros, mx.weight(dev(np.ones((k, m)), gpu)), fused.Epilogue(bias=bias, gelu=True), host(bias)
+
+
+@pytest.mark.parametrize("n,k,m", GELU_FORMS)
+def test_gelu_of_infinities_in_codes(gpu, n, k, m):
+    """GELU(-inf) = 0 leaves its block as it is, +inf and NaN spoil theirs."""
+    values = np.ones(160, np.float32)
+    values[5], values[32:64], values[70], values[100] = -np.inf, -np.inf, np.inf, np.nan
+    t, w, e, bias = on_bias(gpu, n, k, m, values)
+    y = np.where(bias == -np.inf, 0.0, O.gelu(np.where(np.isfinite(bias), bias, 0.0)))
+    y = np.where(np.isnan(bias) | (bias == np.inf), bias, y)
+    for fmt in ("fp8", "fp4"):
+        want = O.encode(np.repeat(y[None], n, 0), fmt)
+        assert want[1][0, :5].tolist().count(255) == 2 and want[1][0, 1] == 0
+        same_bytes(fmt, mx.linear(t, w, e, format=fmt), want)
+    for dtype in TYPES.values():
+        got = mx.linear(t, w, e, dtype=dtype).float()
+        assert (got[:, 32:64] == 0).all() and (got[:, 5] == 0).all() and (got[:, 70] == float("inf")).all()
+        assert got[:, 100].isnan().all() and int(got.isnan().sum()) == n
