@@ -1,12 +1,14 @@
 """The product of microscaled rows where its forms and its roundings meet hard values: sums whose large
-products cancel, GELU of infinities. Oracle and tolerances: tests/test_mx_gpu.py."""
+products cancel, GELU of infinities and far below zero. Oracle and tolerances: tests/test_mx_gpu.py."""
+import math
+
 import numpy as np
 import pytest
 import torch
 
 from ancha_amd import fused, mx
 from oracle import mx as O
-from tests.test_mx_gpu import TYPES, dev, expected, host, near, same_bytes
+from tests.test_mx_gpu import TYPES, check_codes, dev, expected, host, near, same_bytes
 
 pytestmark = pytest.mark.gpu
 
@@ -72,3 +74,25 @@ def test_gelu_of_infinities_in_codes(gpu, n, k, m):
         got = mx.linear(t, w, e, dtype=dtype).float()
         assert (got[:, 32:64] == 0).all() and (got[:, 5] == 0).all() and (got[:, 70] == float("inf")).all()
         assert got[:, 100].isnan().all() and int(got.isnan().sum()) == n
+
+
+def gelu_error(x, dtype):
+    """The kernel's documented error of GELU relative to its value."""
+    steps = (1e-6, 4e-6, 1e-4, 2e-3) if dtype == torch.float32 else (2.5e-6, 3e-5, 1e-3, 3e-3)
+    ends = (-2, -4, -6) if dtype == torch.float32 else (-2, -4, -8)
+    return np.select([x >= e for e in ends], steps[:3], steps[3])
+
+
+@pytest.mark.parametrize("n,k,m", GELU_FORMS)
+def test_gelu_far_below_zero(gpu, n, k, m):
+    """Results of 1e-34 to 3, neighbouring columns alike, so that blocks hold nothing but small ones."""
+    t, w, e, bias = on_bias(gpu, n, k, m, np.linspace(-12.5, 3, min(m, 1500)).astype(np.float32))
+    y = 0.5 * bias * np.array([math.erfc(-b / math.sqrt(2)) for b in bias])
+    y = np.repeat(y[None], n, 0)
+    for kind, dtype in TYPES.items():
+        type_off = torch.finfo(dtype).eps / 2 * np.abs(y) + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+        near(f"{n}x{k}x{m} {kind}", host(mx.linear(t, w, e, dtype=dtype)), y,
+             gelu_error(bias, dtype) * np.abs(y) * (1 + torch.finfo(dtype).eps) + type_off)
+    for fmt in ("fp8", "fp4"):
+        got = mx.linear(t, w, e, format=fmt)
+        check_codes(f"{n}x{k}x{m} {fmt}", got, y, gelu_error(bias, torch.bfloat16) * np.abs(y), fmt)
