@@ -57,9 +57,9 @@ constexpr bool kCodes(int out) { return out == kFp8 || out == kFp4; }
 //   x                       above -2   -4 .. -2   -6 .. -4   -8 .. -6   below
 //   fp32                    7e-7       3e-6       6e-5       8e-4       2e-3
 //   16 bits and codes       2e-6       2e-5       8e-4       9e-4       2.3e-3
-// so rows of nothing but small results have right codes and 16-bit values as well. One exp2 and the polynomial,
-// where erf costs the vector ALU, which bounds these epilogues, three times as much: 96 120 x 384 -> 1536 with bias
-// and GELU to codes 152 us (162 with erf's rational form), to fp32 173 (229 with erff).
+// so rows of nothing but small results have right codes and 16-bit values as well. One exp2 and the polynomial, as
+// the vector ALU bounds these epilogues: 96 120 x 384 -> 1536 with bias and GELU to codes 152 us (as long with
+// erf's rational form, which has no small results right), to fp32 173 (229 with erff).
 template <int OUT>
 __device__ __forceinline__ float gelu(float x) {
   constexpr bool WIDE = OUT == kF32;
