@@ -633,44 +633,37 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(LinearParams p) {
   f32x4 acc[TN][2];
 #pragma unroll
   for (int j = 0; j < TN; j++) acc[j][0] = zero4(), acc[j][1] = zero4();
-  // Four of the wave's steps at a time, all their loads in flight together (steps behind the last are
-  // loaded again, not multiplied).
-  constexpr int U = 4;
-  for (int s0 = wave; s0 < steps; s0 += U * waves) {
-    u32x4 a[U][2], lo[U][TN], hi[U][TN];
-    unsigned sa[U], sb[U][TN];
+  // A step's loads are in flight together, one step's at a time: with up to 32 waves on a CU, two or four steps' of
+  // a wave at once (all loads before the first product) gain nothing and cost registers, so workgroups: 1 x 4096 x
+  // 14 336 9.4 us (two steps 10.8, four 10.9), 16 x 14 336 x 4096 14.9 (14.9, 15.0), 1 x 4096 x 4096 4.4 (4.4, 4.4).
+  for (int s = wave; s < steps; s += waves) {
+    const u32x4 a0 = *reinterpret_cast<const u32x4*>(w + (long)s * kStripCodes);
+    const u32x4 a1 = *reinterpret_cast<const u32x4*>(w + (long)s * kStripCodes + 1024);
+    const unsigned sa = *reinterpret_cast<const uint16_t*>(ws + (long)s * kStripScales);
+    u32x4 lo[TN], hi[TN];
+    unsigned sb[TN];
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      const long s = min(s0 + u * waves, steps - 1);
-      a[u][0] = *reinterpret_cast<const u32x4*>(w + s * kStripCodes);
-      a[u][1] = *reinterpret_cast<const u32x4*>(w + s * kStripCodes + 1024);
-      sa[u] = *reinterpret_cast<const uint16_t*>(ws + s * kStripScales);
-#pragma unroll
-      for (int j = 0; j < TN; j++) {
-        lo[u][j] = *reinterpret_cast<const u32x4*>(x[j] + s * kRow);
-        hi[u][j] = FORMAT == kFp8 ? *reinterpret_cast<const u32x4*>(x[j] + s * kRow + 64) : lo[u][j];
-        sb[u][j] = xs[j][s * 4];
-      }
+    for (int j = 0; j < TN; j++) {
+      lo[j] = *reinterpret_cast<const u32x4*>(x[j] + (long)s * kRow);
+      hi[j] = FORMAT == kFp8 ? *reinterpret_cast<const u32x4*>(x[j] + (long)s * kRow + 64) : lo[j];
+      sb[j] = xs[j][s * 4l];
     }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      if (s0 + u * waves >= steps) break;
+    for (int j = 0; j < TN; j++) {
+      u32x8 large = operand<FORMAT>(lo[j], hi[j]), small = large;
+      if constexpr (FORMAT == kFp8)
 #pragma unroll
-      for (int j = 0; j < TN; j++) {
-        u32x8 large = operand<FORMAT>(lo[u][j], hi[u][j]), small = large;
-        if constexpr (FORMAT == kFp8)
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            unsigned y, z;
-            split(large[i], y, z);
-            large[i] = y, small[i] = z;
-          }
-        acc[j][0] = mfma<FORMAT, 0>(a[u][0], sa[u], large, sb[u][j], acc[j][0]);
-        acc[j][1] = mfma<FORMAT, 1>(a[u][1], sa[u], large, sb[u][j], acc[j][1]);
-        if constexpr (FORMAT == kFp8) {
-          acc[j][0] = mfma<FORMAT, 0>(a[u][0], sa[u], small, sb[u][j], acc[j][0]);
-          acc[j][1] = mfma<FORMAT, 1>(a[u][1], sa[u], small, sb[u][j], acc[j][1]);
+        for (int i = 0; i < 8; i++) {
+          unsigned y, z;
+          split(large[i], y, z);
+          large[i] = y, small[i] = z;
         }
+      acc[j][0] = mfma<FORMAT, 0>(a0, sa, large, sb[j], acc[j][0]);
+      acc[j][1] = mfma<FORMAT, 1>(a1, sa, large, sb[j], acc[j][1]);
+      if constexpr (FORMAT == kFp8) {
+        acc[j][0] = mfma<FORMAT, 0>(a0, sa, small, sb[j], acc[j][0]);
+        acc[j][1] = mfma<FORMAT, 1>(a1, sa, small, sb[j], acc[j][1]);
       }
     }
   }
