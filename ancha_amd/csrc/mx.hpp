@@ -248,5 +248,10 @@ struct LinearParams {
 };
 hipError_t launch_linear(const LinearParams& p, hipStream_t stream);
 
+// The kernel that a product takes: few rows (16 or 32 a workgroup), tiles of 64 x 64 (the steps of k in one chain
+// or four), 128 x 128 and 128 rows x 256 columns.
+enum LinearForm { kFew16, kFew32, kTiles64, kTiles64Chains, kTiles128, kTiles256 };
+LinearForm linear_form(long n, long k, long m);
+
 }  // namespace mx
 }  // namespace ancha

@@ -232,4 +232,9 @@ int ancha_mx_linear(const void* codes, const void* scales, size_t n, size_t k, i
   return e == hipSuccess ? ANCHA_HIP_OK : hip_fail(e, who);
 }
 
+// For the tests: the kernel that a product of n rows takes (mx::LinearForm).
+int ancha_amd_mx_linear_form(size_t n, size_t k, size_t m) {
+  return mx::linear_form(static_cast<long>(n), static_cast<long>(k), static_cast<long>(m));
+}
+
 }  // extern "C"

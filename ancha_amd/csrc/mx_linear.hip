@@ -606,8 +606,9 @@ void start_tiles(const LinearParams& p, hipStream_t stream) {
 
 // Few rows: the weight is what has to be read. A workgroup has 32 columns and 16 TN rows; its waves (one
 // to sixteen) take the steps of 128 k in turn, straight from memory, and add up their sums in LDS. Then
-// eight threads have a row, four neighbouring columns each. Bound by the way to memory and back: 1 x 4096 x 4096
-// 4.5 us, 24 x 8192 x 8192 (e2m1) 11 us, 36 MB at 3.3 TB/s.
+// eight threads have a row, four neighbouring columns each. Small weights are bound by the way to memory and the sum
+// over the waves, large ones by memory; the weight from memory: 1 x 4096 x 4096 5.3 us, 1 x 4096 x 28 672 17 us (3.7
+// TB/s), 1 x 4096 x 128 256 56 us (5.0 TB/s).
 constexpr int kFewColumns = 32, kFewWaves = 16;
 
 template <int FORMAT, int OUT, int TN>
@@ -746,38 +747,20 @@ void start_few(const LinearParams& p, hipStream_t stream) {
 
 template <int FORMAT, int OUT>
 void start(const LinearParams& p, hipStream_t stream) {
-  // Measured with each form forced, e4m3 -> bf16, us (n x k x m):
-  //   few rows / 64 x 64 tiles: 16 x 4096 x 4096 6.3 / 10.9, 64 x 4096 x 4096 9.8 / 11.0, 64 x 8192 x 8192
-  //   30.6 / 19.9, 64 x 2048 x 512 4.4 / 6.8; with 16 / 32 rows a workgroup where 16 already fill the
-  //   chip: 24 x 8192 x 8192 16.9 / 13.7 (e2m1 16.7 / 11.0);
-  //   64 x 64 tiles, the steps in one chain / in four: 128 x 4096 x 4096 11.6 / 8.9, 128 x 8192 x 8192 21.8 /
-  //   15.8, 800 x 2048 x 512 7.2 / 6.4, 512 x 1024 x 1024 5.1 / 5.3, 512 x 4096 x 4096 14.3 / 16.5;
-  //   64 x 64 / 128 x 128: 512 x 4096 x 4096 14.9 / 21.7, 4096 x 2048 x 512 9.2 / 12.9, 1024 x 4096 x 4096
-  //   26.2 / 25.5, 512 x 8192 x 8192 51.0 / 45.8;
-  //   128 rows x 128 / 256 columns: 2048 x 4096 x 4096 35.0 / 37.7, 4096 x 4096 x 4096 61.6 / 56.1,
-  //   8192 x 8192 x 8192 441 / 388 (all of these with e4m3 rows in one pass); where 256 columns leave a tile mostly empty (96 120 x 1536 x 384, fp32
-  //   with bias and residual) 118 / 134.
-  const long cus = device_cus(), n = p.n, m = p.m;
-  const long columns = (m + 31) / 32, narrow = (m + 127) / 128, wide = (m + 255) / 256;
-  const long high = (n + 127) / 128;
-  if (n > 16 && columns >= cus && (n + 31) / 32 * columns <= cus)
-    start_few<FORMAT, OUT, 2>(p, stream);
-  else if ((n + 15) / 16 * columns <= 2 * cus)
-    start_few<FORMAT, OUT, 1>(p, stream);
-  else if (narrow * high * 4 < 3 * cus) {
-    if ((n + 63) / 64 * ((m + 63) / 64) <= cus && p.k >= 2048)
-      start_tiles<FORMAT, OUT, 1, 4, 1, 1, 3, 4, 4>(p, stream);
-    else
-      start_tiles<FORMAT, OUT, 1, 4, 1, 1, 3, 4>(p, stream);
-  } else if (wide * 32 <= narrow * 17 && wide * high >= 2 * cus)
-    // 32 x 256 a wave where rows are split (twice the registers for a row tile), 64 x 128 otherwise (fewer
-    // LDS reads): 8192 x 8192 x 8192 e4m3 629 / 709, in one pass 400 / 375.
-    if constexpr (FORMAT == kFp8)
-      start_tiles<FORMAT, OUT, 1, 4, 4, 2, 2, 2>(p, stream);
-    else
-      start_tiles<FORMAT, OUT, 2, 2, 2, 4, 2, 2>(p, stream);
+  switch (linear_form(p.n, p.k, p.m)) {
+    case kFew16: return start_few<FORMAT, OUT, 1>(p, stream);
+    case kFew32: return start_few<FORMAT, OUT, 2>(p, stream);
+    case kTiles64: return start_tiles<FORMAT, OUT, 1, 4, 1, 1, 3, 4>(p, stream);
+    case kTiles64Chains: return start_tiles<FORMAT, OUT, 1, 4, 1, 1, 3, 4, 4>(p, stream);
+    case kTiles128: return start_tiles<FORMAT, OUT, 1, 4, 2, 2, 2, 3>(p, stream);
+    case kTiles256: break;
+  }
+  // 32 x 256 a wave where rows are split (twice the registers for a row tile), 64 x 128 otherwise (fewer
+  // LDS reads): 8192 x 8192 x 8192 e4m3 629 / 709, in one pass 400 / 375.
+  if constexpr (FORMAT == kFp8)
+    start_tiles<FORMAT, OUT, 1, 4, 4, 2, 2, 2>(p, stream);
   else
-    start_tiles<FORMAT, OUT, 1, 4, 2, 2, 2, 3>(p, stream);
+    start_tiles<FORMAT, OUT, 2, 2, 2, 4, 2, 2>(p, stream);
 }
 
 // The formats of the rows and of the result pick the kernel.
@@ -791,6 +774,55 @@ hipError_t linear_to(const LinearParams& p, hipStream_t stream) {
 }
 
 }  // namespace
+
+// Measured with each form forced, to bf16, the weights from memory, us, e4m3 / e2m1 rows (n x k x m):
+//                       16 rows      32 rows      64 x 64      in four chains
+//   1 x 4096 x 14 336   10.2 /  9.3  13.8 /  9.8  16.2 / 13.5  12.8 /  9.3
+//   16 x 4096 x 28 672  18.7 / 17.5  28.2 / 18.3  21.7 / 16.1  25.4 / 19.4
+//   1 x 4096 x 128 256  55.7 / 55.0  91.7 / 57.2  72.4 / 51.6  93.8 / 65.6
+//   24 x 4096 x 4096     6.8 /  5.8   8.5 /  7.4  15.7 / 12.7  11.5 /  8.5
+//   128 x 2048 x 512     4.5 /  4.0   5.9 /  5.0   8.9 /  6.3   7.5 /  5.8
+//   24 x 4096 x 7168     9.5 /  9.1   8.7 /  7.8  15.9 / 13.1  11.8 /  8.8
+//   64 x 4096 x 4096    10.1 /  8.4   9.5 /  7.6  15.7 / 13.2  13.5 / 11.7
+//   24 x 8192 x 8192    17.3 / 16.4  15.3 / 12.5  28.5 / 23.2  19.6 / 14.1
+//   64 x 2048 x 4096     6.8 /  5.7   6.5 /  5.5   9.4 /  8.0   8.8 /  7.4
+//   64 x 1024 x 4096     4.7 /  4.2   4.7 /  4.1   6.1 /  5.2   6.3 /  5.4
+//   128 x 384 x 1536     3.1 /  2.8   3.4 /  3.0   3.9 /  3.4   4.7 /  4.2
+//   48 x 4096 x 4128    10.1 /  8.8  13.1 / 10.2  15.7 / 12.9  12.6 / 10.0
+//   24 x 8192 x 8224    20.8 / 18.8  26.2 / 18.4  28.6 / 23.3  19.6 / 14.1
+//   24 x 4096 x 14 336  15.9 / 14.9  16.2 / 11.5  16.4 / 13.8  12.8 /  9.8
+//   64 x 4096 x 7168    17.1 / 14.9  17.3 / 12.2  16.0 / 13.5  14.0 / 12.1
+//                                                 64 x 64      in four chains  128 x 128
+//   128 x 4096 x 4096                             15.9 / 13.1  13.4 / 11.2     33.1 / 27.0
+//   512 x 2048 x 2048                              9.9 /  7.6   8.7 /  6.8     18.5 / 13.9
+//   512 x 1024 x 1024                              6.0 /  4.6   5.9 /  5.0     11.0 /  7.6
+//   128 x 4096 x 14 336                           21.9 / 18.3  25.6 / 21.5     33.4 / 27.6
+//   512 x 4096 x 4096                             22.8 / 15.9  24.7 / 19.3     33.3 / 26.2
+//   64 x 4096 x 28 672                            24.2 / 21.1  27.6 / 24.5     34.9 / 28.1
+//   64 x 4096 x 128 256                           89.1 / 82.5   109 / 92.8     99.2 / 81.3
+//   128 x 4096 x 28 672                           39.0 / 35.8  49.9 / 40.9     34.4 / 29.5
+//   1024 x 4096 x 4096                            38.2 / 28.6                  34.2 / 25.9
+//                                                              128 x 128       128 x 256
+//   2048 x 4096 x 4096                                         48.4 / 37.4     52.3 / 30.8
+//   4096 x 4096 x 4096                                         92.5 / 63.4     85.4 / 46.6
+//   8192 x 8192 x 8192                                          664 / 396       616 / 300
+//   96 120 x 384 x 1536                                         107 / 70.5      100 / 69.3
+//   96 120 x 1536 x 384 (the second tile half empty)           79.7 / 46.2     96.0 / 51.3
+LinearForm linear_form(long n, long k, long m) {
+  const long cus = device_cus();
+  const long columns = (m + 31) / 32, narrow = (m + 127) / 128, wide = (m + 255) / 256;
+  const long high = (n + 127) / 128, blocks16 = (n + 15) / 16 * columns, blocks32 = (n + 31) / 32 * columns;
+  // One tile of rows, whatever the width: the weight is read once. Also where the workgroups fit one to a CU.
+  if (n <= 16 || blocks16 <= cus) return kFew16;
+  // Twice the rows where that is what makes them fit and there is a chain of steps to save.
+  if (blocks32 <= cus && k >= 2048) return kFew32;
+  if (blocks16 <= 2 * cus) return kFew16;
+  // A tile of 128 rows half empty at best, or fewer of them than three for four CUs.
+  if (n <= 64 || narrow * high * 4 < 3 * cus)
+    return (n + 63) / 64 * ((m + 63) / 64) <= cus && k >= 2048 ? kTiles64Chains : kTiles64;
+  // 256 columns unless they leave a tile mostly empty or less than two tiles to a CU.
+  return wide * 32 <= narrow * 17 && wide * high >= 2 * cus ? kTiles256 : kTiles128;
+}
 
 hipError_t launch_linear(const LinearParams& p, hipStream_t stream) {
   switch (p.out_format ? p.out_format : p.type) {

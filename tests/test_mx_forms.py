@@ -1,0 +1,43 @@
+"""Which kernel a microscaled product takes, where that was chosen by measurement (CPU; the rule counts the CUs
+of the current device, 256 where there is none), and that the GPU tests' sizes reach every one."""
+import pytest
+
+from ancha_amd import _native
+from tests import test_mx_forms_gpu as G
+
+FEW16, FEW32, TILES64, CHAINS64, TILES128, TILES256 = range(6)
+
+
+def form(n, k, m):
+    return _native.lib().ancha_amd_mx_linear_form(n, k, m)
+
+
+RULE = [
+    # One tile of rows: the weight is read once, whatever its width.
+    (1, 128, 32, FEW16), (1, 4096, 4096, FEW16), (16, 4096, 7168, FEW16), (8, 8192, 8224, FEW16),
+    (1, 4096, 14336, FEW16), (16, 4096, 28672, FEW16), (1, 4096, 128256, FEW16), (16, 128, 1 << 24, FEW16),
+    # Few rows of few columns: sixteen rows a workgroup while these fit one to a CU, then 32 for a long k.
+    (24, 4096, 4096, FEW16), (128, 2048, 512, FEW16), (4096, 384, 32, FEW16), (17, 4096, 4128, FEW32),
+    (24, 4096, 7168, FEW32), (32, 8192, 8192, FEW32), (24, 8192, 8160, FEW32), (64, 4096, 4096, FEW32),
+    (64, 2048, 4096, FEW32), (64, 2047, 4096, FEW16), (64, 1024, 4096, FEW16), (128, 384, 1536, FEW16),
+    (48, 4096, 4128, FEW16), (33, 4096, 5120, FEW16),
+    # 64 x 64 tiles, four chains of steps while the tiles fit one to a CU and k is long.
+    (24, 8192, 8224, CHAINS64), (24, 4096, 14336, CHAINS64), (64, 4096, 7168, CHAINS64),
+    (128, 4096, 4096, CHAINS64), (512, 2048, 2048, CHAINS64), (512, 1024, 1024, TILES64),
+    (17, 4096, 28672, TILES64), (64, 4096, 128256, TILES64), (128, 4096, 14336, TILES64),
+    (512, 4096, 4096, TILES64), (801, 1000, 1549, TILES64), (2048, 1024, 1024, TILES64),
+    # Larger ones.
+    (65, 4096, 28672, TILES128), (128, 4096, 28672, TILES128), (1024, 4096, 4096, TILES128),
+    (2048, 4096, 4096, TILES128), (96120, 1536, 384, TILES128), (4096, 4096, 4096, TILES256),
+    (8192, 8192, 8192, TILES256), (96120, 384, 1536, TILES256),
+]
+
+
+@pytest.mark.parametrize("n,k,m,want", RULE)
+def test_form_of_a_product(n, k, m, want):
+    assert form(n, k, m) == want
+
+
+@pytest.mark.parametrize("sizes", ["FORMS", "GELU_FORMS"])
+def test_sizes_of_the_gpu_tests_reach_every_form(sizes):
+    assert {form(*s) for s in getattr(G, sizes)} == set(range(6))

@@ -12,9 +12,9 @@ from tests.test_mx_gpu import TYPES, check_codes, dev, expected, host, near, sam
 
 pytestmark = pytest.mark.gpu
 
-# One size for each form of the product: few rows, 64 x 64 tiles with the steps in one chain and in four, 128 x
-# 128 tiles, 256 columns.
-FORMS = [(5, 300, 40), (801, 1000, 1549), (130, 2100, 2050), (2100, 200, 1549), (8200, 130, 2048)]
+# One size for each form of the product: few rows (16 and 32 a workgroup), 64 x 64 tiles with the steps in one
+# chain and in four, 128 x 128 tiles, 256 columns.
+FORMS = [(5, 300, 40), (24, 2100, 4200), (801, 1000, 1549), (130, 2100, 2050), (2100, 200, 1549), (8200, 130, 2048)]
 
 
 def cancelling(n, k, m):
@@ -48,7 +48,7 @@ def test_large_products_cancel(gpu, n, k, m, kind):
 
 # ---- GELU. Rows of zeros give products of exactly 0, so the bias is what GELU takes.
 
-GELU_FORMS = [(3, 200, 700), (801, 200, 1549), (130, 2100, 2050), (2100, 200, 1549), (8200, 130, 2048)]
+GELU_FORMS = [(3, 200, 700), (24, 2100, 4200), (801, 200, 1549), (130, 2100, 2050), (2100, 200, 1549), (8200, 130, 2048)]
 
 
 def on_bias(gpu, n, k, m, values):
