@@ -200,6 +200,11 @@ struct RowParams {
 hipError_t launch_quantize(const RowParams& p, hipStream_t stream);
 hipError_t launch_norm(const RowParams& p, hipStream_t stream);
 
+// The form of the norm's kernel: threads a row and their pieces of eight values each, or 0 where rows are read
+// twice.
+constexpr int norm_code(int threads, int pieces) { return 8 * threads + pieces; }
+int norm_form(long rows, long dim);
+
 struct ValueParams {
   const uint8_t* codes;
   const uint8_t* scales;

@@ -237,4 +237,9 @@ int ancha_amd_mx_linear_form(size_t n, size_t k, size_t m) {
   return mx::linear_form(static_cast<long>(n), static_cast<long>(k), static_cast<long>(m));
 }
 
+// For the tests: the kernel that a norm takes, 8 x threads a row + pieces (0: rows read twice).
+int ancha_amd_mx_norm_form(size_t rows, size_t dim) {
+  return mx::norm_form(static_cast<long>(rows), static_cast<long>(dim));
+}
+
 }  // extern "C"

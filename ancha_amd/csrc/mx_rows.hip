@@ -299,43 +299,23 @@ void start_norm(const RowParams& p, hipStream_t stream) {
                      dim3(kAll), 0, stream, p);
 }
 
-// Rows in registers, L threads a row and V pieces of 8 L values. Measured with each form forced (us, with
-// the addition / without; the forms taken are up to 15 % faster since, by lighter codes):
-//   96 120 x 384 fp32     16 threads  80 / 37, 64  79 / 47, 32  107 / 54
-//   30 000 x 700 bf16     32 threads  36 / 25, 64  38 / 28, 128  51 / 37
-//   30 000 x 1024 bf16    64 threads  37 / 25, 32  38 / 26, 128  43 / 31
-//   20 000 x 1800 fp32   128 threads  85 / 37, 64  87 / 40, 256  83 / 40, 32  106 / 53
-//   30 000 x 4096 bf16   256 threads 156 / 92, 128 172 / 91, 64  208 / 112
-// and, with few rows, the more threads a row the shorter the way through it: 200 x 1500 fp16 256 threads
-// 5.0 / 4.4, 64 7.1 / 5.8, 32 10.3 / 8.1; 300 x 384 fp16 64 threads 4.4 / 4.7, 16 6.1 / 5.2.
-// Past 8192 values 512 threads, with the addition: 2000 x 12 000 bf16 36 (read twice 47), 2000 x 16 000 fp32 74
-// (118). Four fp32 values side by side a thread in place of eight were slower: 96 120 x 384 84 / 38 (80 / 31).
 template <int TYPE>
 void norm_of_type(const RowParams& p, hipStream_t stream) {
-  const long g = groups(p.dim);
-  const bool few = p.rows < 1024;
-  if (g > 128)
-    hipLaunchKernelGGL(norm_long_kernel<TYPE>, dim3(p.rows), dim3(kThreads), 0, stream, p);
-  else if (g > 64)
-    start_norm<TYPE, 512, 4>(p, stream);
-  else if (g > 32)
-    start_norm<TYPE, 256, 4>(p, stream);
-  else if (g > 16)
-    start_norm<TYPE, 256, 2>(p, stream);
-  else if (g > 4 && few)
-    start_norm<TYPE, 256, 1>(p, stream);
-  else if (g > 8)
-    start_norm<TYPE, 128, 2>(p, stream);
-  else if (g > 6)
-    start_norm<TYPE, 64, 2>(p, stream);
-  else if (g > 4)
-    start_norm<TYPE, 32, 3>(p, stream);
-  else if (few)
-    start_norm<TYPE, 64, 1>(p, stream);
-  else if (g > 2)
-    g > 3 ? start_norm<TYPE, 16, 4>(p, stream) : start_norm<TYPE, 16, 3>(p, stream);
-  else
-    g > 1 ? start_norm<TYPE, 16, 2>(p, stream) : start_norm<TYPE, 16, 1>(p, stream);
+  switch (norm_form(p.rows, p.dim)) {
+    case norm_code(16, 1): return start_norm<TYPE, 16, 1>(p, stream);
+    case norm_code(16, 2): return start_norm<TYPE, 16, 2>(p, stream);
+    case norm_code(16, 3): return start_norm<TYPE, 16, 3>(p, stream);
+    case norm_code(16, 4): return start_norm<TYPE, 16, 4>(p, stream);
+    case norm_code(32, 3): return start_norm<TYPE, 32, 3>(p, stream);
+    case norm_code(64, 1): return start_norm<TYPE, 64, 1>(p, stream);
+    case norm_code(64, 2): return start_norm<TYPE, 64, 2>(p, stream);
+    case norm_code(128, 2): return start_norm<TYPE, 128, 2>(p, stream);
+    case norm_code(256, 1): return start_norm<TYPE, 256, 1>(p, stream);
+    case norm_code(256, 2): return start_norm<TYPE, 256, 2>(p, stream);
+    case norm_code(256, 4): return start_norm<TYPE, 256, 4>(p, stream);
+    case norm_code(512, 4): return start_norm<TYPE, 512, 4>(p, stream);
+    default: hipLaunchKernelGGL(norm_long_kernel<TYPE>, dim3(p.rows), dim3(kThreads), 0, stream, p);
+  }
 }
 
 template <int TYPE, int FORMAT>
@@ -368,6 +348,31 @@ hipError_t launch_quantize(const RowParams& p, hipStream_t stream) {
   else
     start_quantize<kBf16>(p, stream);
   return hipGetLastError();
+}
+
+// Rows in registers, L threads a row and V pieces of 8 L values. Measured with each form forced (us, with
+// the addition / without; the forms taken are up to 15 % faster since, by lighter codes):
+//   96 120 x 384 fp32     16 threads  80 / 37, 64  79 / 47, 32  107 / 54
+//   30 000 x 700 bf16     32 threads  36 / 25, 64  38 / 28, 128  51 / 37
+//   30 000 x 1024 bf16    64 threads  37 / 25, 32  38 / 26, 128  43 / 31
+//   20 000 x 1800 fp32   128 threads  85 / 37, 64  87 / 40, 256  83 / 40, 32  106 / 53
+//   30 000 x 4096 bf16   256 threads 156 / 92, 128 172 / 91, 64  208 / 112
+// and, with few rows, the more threads a row the shorter the way through it: 200 x 1500 fp16 256 threads
+// 5.0 / 4.4, 64 7.1 / 5.8, 32 10.3 / 8.1; 300 x 384 fp16 64 threads 4.4 / 4.7, 16 6.1 / 5.2.
+// Past 8192 values 512 threads, with the addition: 2000 x 12 000 bf16 36 (read twice 47), 2000 x 16 000 fp32 74
+// (118). Four fp32 values side by side a thread in place of eight were slower: 96 120 x 384 84 / 38 (80 / 31).
+int norm_form(long rows, long dim) {
+  const long g = groups(dim);
+  const bool few = rows < 1024;
+  if (g > 128) return 0;
+  if (g > 64) return norm_code(512, 4);
+  if (g > 32) return norm_code(256, 4);
+  if (g > 16) return norm_code(256, 2);
+  if (few) return g > 4 ? norm_code(256, 1) : norm_code(64, 1);
+  if (g > 8) return norm_code(128, 2);
+  if (g > 6) return norm_code(64, 2);
+  if (g > 4) return norm_code(32, 3);
+  return norm_code(16, static_cast<int>(g));
 }
 
 hipError_t launch_norm(const RowParams& p, hipStream_t stream) {

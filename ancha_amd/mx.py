@@ -241,8 +241,8 @@ def linear(x: Tensor, w: Weight, epilogue: Optional[Epilogue] = None,
 
     Products of codes are exact and sums are held in 32 bits, whatever ``dtype`` ("fp8" rows take the
     matrix cores two passes for that, so twice the time of "fp4" rows where these are what bounds). GELU is
-    off by at most 3e-6 of its value for arguments above -4 and 2e-3 below (16-bit results and codes: 2e-5,
-    2.5e-3). The order of a row's sums depends on n, k and m, so its last bits may differ from one n to another."""
+    off by at most 4e-6 of its value for arguments above -4 and 2e-3 below (16-bit results and codes: 3e-5,
+    3e-3). The order of a row's sums depends on n, k and m, so its last bits may differ from one n to another."""
     if not isinstance(x, Tensor) or not isinstance(w, Weight):
         raise ValueError("linear takes a microscaled Tensor and a Weight")
     kind = _type(dtype, "dtype")

@@ -326,8 +326,8 @@ int ancha_mx_weight_values(const void *weight, size_t k, size_t m, int type, voi
  * [m] fp32; erf-GELU; rotary; residual [n][m] of `type`, contiguous (may be out). out_format 0: out is
  * [n][m] of `type`, contiguous; ANCHA_HIP_MX_FP8 / FP4: out and out_scales are the codes and scales of
  * the fp32 result (`type` is ANCHA_HIP_F32). Sums are held to fp32 whatever `type` (below its normal range
- * they may be 0); GELU is off by at most 3e-6 of its value for arguments above -4 and 2e-3 below (results of
- * 16 bits and codes: 2e-5, 2.5e-3). The order of a row's sums depends on n, k and m. Any k, m > 0.
+ * they may be 0); GELU is off by at most 4e-6 of its value for arguments above -4 and 2e-3 below (results of
+ * 16 bits and codes: 3e-5, 3e-3). The order of a row's sums depends on n, k and m. Any k, m > 0.
  * ANCHA_HIP_UNSUPPORTED for k == 0, m == 0 and a rotary shape that does not fit (tokens == 0, n % tokens,
  * width % 64, 2 * width > m). */
 int ancha_mx_linear(const void *codes, const void *scales, size_t n, size_t k, int format,

@@ -1,9 +1,10 @@
-"""Which kernel a microscaled product takes, where that was chosen by measurement (CPU; the rule counts the CUs
+"""Which kernel a microscaled product or norm takes, where that was chosen by measurement (CPU; the rule counts the CUs
 of the current device, 256 where there is none), and that the GPU tests' sizes reach every one."""
 import pytest
 
 from ancha_amd import _native
 from tests import test_mx_forms_gpu as G
+from tests import test_mx_norm_forms_gpu as N
 
 FEW16, FEW32, TILES64, CHAINS64, TILES128, TILES256 = range(6)
 
@@ -38,6 +39,24 @@ def test_form_of_a_product(n, k, m, want):
     assert form(n, k, m) == want
 
 
-@pytest.mark.parametrize("sizes", ["FORMS", "GELU_FORMS"])
+@pytest.mark.parametrize("sizes", ["FORMS", "GELU_FORMS", "EPILOGUE_SIZES"])
 def test_sizes_of_the_gpu_tests_reach_every_form(sizes):
     assert {form(*s) for s in getattr(G, sizes)} == set(range(6))
+
+
+# rows, columns, threads a row, pieces of eight values of each (0, 0: rows read twice)
+NORMS = [(1, 1, 64, 1), (1023, 512, 64, 1), (1023, 513, 256, 1), (1, 2048, 256, 1), (1, 2049, 256, 2),
+         (5000, 4096, 256, 2), (1, 4097, 256, 4), (1, 8193, 512, 4), (9999, 16384, 512, 4), (1, 16385, 0, 0),
+         (1024, 128, 16, 1), (1024, 129, 16, 2), (96120, 384, 16, 3), (1024, 512, 16, 4), (1024, 513, 32, 3),
+         (1024, 768, 32, 3), (1024, 769, 64, 2), (1024, 1024, 64, 2), (6007, 1549, 128, 2), (1024, 2048, 128, 2)]
+
+
+@pytest.mark.parametrize("rows,dim,threads,pieces", NORMS)
+def test_form_of_a_norm(rows, dim, threads, pieces):
+    assert _native.lib().ancha_amd_mx_norm_form(rows, dim) == 8 * threads + pieces
+    assert 8 * threads * pieces >= dim or not threads
+
+
+def test_shapes_of_the_gpu_tests_reach_every_norm():
+    forms = {_native.lib().ancha_amd_mx_norm_form(r, d) for r, d in N.SHAPES}
+    assert forms == {8 * t + p for _, _, t, p in NORMS}
