@@ -124,10 +124,16 @@ class Tensor:
 
 
 class Weight:
-    """A [k, m] weight in e2m1 along k, laid out for the matrix cores; made by :func:`weight`."""
+    """A [k, m] weight in e2m1 along k, laid out for the matrix cores; made by :func:`weight`. ``data`` is the
+    uint8 tensor that such a weight of the same shape holds."""
 
     def __init__(self, data: torch.Tensor, k: int, m: int):
-        self._data, self.shape = data, torch.Size((k, m))
+        size = int(_native.lib().ancha_mx_weight_bytes(k, m)) if k > 0 and m > 0 else 0
+        if size == 0:
+            raise ValueError(f"no weight has the shape [{k}, {m}]")
+        if not isinstance(data, torch.Tensor) or not data.is_cuda:
+            raise ValueError("data must be a tensor on a GPU")
+        self._data, self.shape = _bytes(data, "data", data.device, (size,), 16), torch.Size((k, m))
 
     @property
     def device(self) -> torch.device:

@@ -1,8 +1,9 @@
 """Which kernel a microscaled product or norm takes, where that was chosen by measurement (CPU; the rule counts the CUs
 of the current device, 256 where there is none), and that the GPU tests' sizes reach every one."""
 import pytest
+import torch
 
-from ancha_amd import _native
+from ancha_amd import _native, mx
 from tests import test_mx_forms_gpu as G
 from tests import test_mx_norm_forms_gpu as N
 
@@ -60,3 +61,11 @@ def test_form_of_a_norm(rows, dim, threads, pieces):
 def test_shapes_of_the_gpu_tests_reach_every_norm():
     forms = {_native.lib().ancha_amd_mx_norm_form(r, d) for r, d in N.SHAPES}
     assert forms == {8 * t + p for _, _, t, p in NORMS}
+
+
+def test_weights_check_what_they_are_made_of():
+    with pytest.raises(ValueError, match="on a GPU"):
+        mx.Weight(torch.zeros(2 * 4352, dtype=torch.uint8), 128, 64)
+    for k, m in ((0, 64), (64, 0), (-1, 64), (1 << 24, 64)):
+        with pytest.raises(ValueError, match="no weight"):
+            mx.Weight(torch.zeros(0, dtype=torch.uint8), k, m)

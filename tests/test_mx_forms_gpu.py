@@ -215,3 +215,13 @@ def test_each_product_beside_the_largest(gpu, n, m, pair):
     t, handle = mx.quantize(dev(x, gpu), "fp8"), mx.weight(dev(w, gpu))
     assert np.array_equal(host(t.values()), x) and np.array_equal(host(handle.values()), w)
     assert np.array_equal(host(mx.linear(t, handle)), np.outer(x[:, 3].astype(np.float64), w[3]))
+
+
+def test_weights_check_what_they_are_made_of(gpu):
+    w = mx.weight(dev(W.normal((130, 70), 91, 1.0), gpu))
+    t = mx.quantize(dev(W.normal((3, 130), 92, 1.0), gpu))
+    assert torch.equal(mx.linear(t, mx.Weight(w._data.clone(), 130, 70)), mx.linear(t, w))
+    for data, k, m in ((w._data[:-16], 130, 70), (w._data, 300, 70), (w._data.view(2, -1), 130, 70),
+                       (w._data.view(torch.int8), 130, 70)):
+        with pytest.raises(ValueError, match="data must"):
+            mx.Weight(data, k, m)
