@@ -15,7 +15,7 @@ __device__ __forceinline__ long scale_place(long pieces, long piece, int c, int 
 
 // A strip (64 columns) and group (128 k) per workgroup, any layout: lane l of wave b has column l, k block
 // b. Neighbouring lanes read neighbouring columns, so [in, out] weights are read in whole lines.
-// Both kernels are bound by memory and run once per weight.
+// Both kernels run once per weight and are bound by memory: 8192 x 8192 [in, out] fp32 48 us (6.4 TB/s), bf16 33.
 template <int TYPE>
 __global__ __launch_bounds__(256) void weight_columns_kernel(WeightParams p) {
   typedef typename Stored<TYPE>::type T;
