@@ -104,7 +104,7 @@ def test_gelu_far_below_zero(gpu, n, k, m):
 
 EPILOGUE_SIZES = [(5, 300, 40), (13, 300, 327), (24, 2100, 4200), (29, 2100, 4101), (801, 1000, 1549), (800, 200, 1552),
                   (130, 2100, 2050), (130, 2100, 2052), (2100, 200, 1549), (2100, 130, 1600), (8200, 130, 2047),
-                  (8200, 160, 2048)]
+                  (8200, 160, 2048), (3, 130, 20000), (16, 300, 33001), (40, 130, 30000)]
 
 
 def result(x, w, bias, gelu, residual, dtype=None):
