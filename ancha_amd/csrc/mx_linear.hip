@@ -53,7 +53,7 @@ constexpr bool kCodes(int out) { return out == kFp8 || out == kFp4; }
 
 // erf-GELU: x Phi(x) = max(x, 0) - |x| 2^Q(|x|) with Q a polynomial for log2 Phi(-a) on [0, 13.2], beyond which
 // the product is below fp32's normal range (Q goes on falling). Degree 12 for fp32 results, 10 for others. Its
-// error relative to the value, fitted to least weighted maxima (as tests hold it to, rounded up):
+// error relative to the value, fitted to least weighted maxima (tests hold it to somewhat larger ones):
 //   x                       above -2   -4 .. -2   -6 .. -4   -8 .. -6   below
 //   fp32                    7e-7       3e-6       6e-5       8e-4       2e-3
 //   16 bits and codes       2e-6       2e-5       8e-4       9e-4       2.3e-3
