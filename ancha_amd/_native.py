@@ -73,6 +73,12 @@ SIGNATURES = {
     "ancha_mx_weight_values": (_int, [_p, _sz, _sz, _int, _p, _p]),
     "ancha_mx_linear": (_int, [_p, _p, _sz, _sz, _int, _p, _sz, _p, _int, _p, _sz, _sz, _p, _int,
                                    _int, _p, _p, _p]),
+    "ancha_paged_rotary": (_int, [_p, _int, _sz, _sz, _sz, _sz, _sz, _p, _int, _p, _p, _p, _p]),
+    "ancha_paged_write": (_int, [_p, _p, _int, _sz, _sz, _sz, _sz, _sz, _p, _p, _p, _p]),
+    "ancha_paged_read": (_int, [_p, _p, _sz, _int, _p, _p, _p]),
+    "ancha_paged_attention_workspace": (_sz, [_sz, _sz, _p, _p]),
+    "ancha_paged_attention": (_int, [_p, _int, _sz, _sz, _sz, _sz, _p, _p, ctypes.c_double, _int, _sz, _p, _sz,
+                                     _p, _p]),
     "ancha_hip_check": (_int, []),
     "ancha_hip_last_error": (ctypes.c_char_p, []),
     # Not in the header: linear / norm_linear with scratch for the weight's fp16 fragments, and, for the
@@ -85,6 +91,22 @@ SIGNATURES = {
     "ancha_amd_mx_linear_form": (_int, [_sz, _sz, _sz]),
     "ancha_amd_mx_norm_form": (_int, [_sz, _sz]),
 }
+
+
+class PagedBatch(ctypes.Structure):
+    """ancha_paged_batch"""
+    _fields_ = [("starts", _p), ("lengths", _p), ("table", _p), ("sequences", _sz), ("columns", _sz)]
+
+
+class PagedCache(ctypes.Structure):
+    """ancha_paged_cache"""
+    _fields_ = [("codes", _p), ("scales", _p), ("pages", _sz), ("heads", _sz), ("page", _sz), ("dim", _sz),
+                ("format", _int)]
+
+
+class PagedPlan(ctypes.Structure):
+    """ancha_paged_plan"""
+    _fields_ = [("freqs", _p), ("width", _sz), ("interleaved", _int), ("magnitude", ctypes.c_double)]
 
 
 def lib() -> ctypes.CDLL:

@@ -184,6 +184,32 @@ __device__ __forceinline__ void store_codes(const float* v, int format, bool sto
   if (threadIdx.x % 4 == 0) *scale = (uint8_t)s;
 }
 
+// The double d with its last 32 bits folded into the one above them, as a float: truncated, with the
+// last bit set if anything was lost (rounding to odd). Rounding the result to 4 or fewer bits then
+// gives what rounding d itself does.
+__device__ __forceinline__ float to_odd(double d) {
+  const unsigned long long bits = __builtin_bit_cast(unsigned long long, d);
+  unsigned lost;  // one instruction where the compiler takes two
+  asm("v_min_u32 %0, 1, %1" : "=v"(lost) : "v"((unsigned)bits));
+  const unsigned hi = (unsigned)(bits >> 32) | lost;
+  return (float)__builtin_bit_cast(double, (unsigned long long)hi << 32);
+}
+
+// Division by a number d, a row's groups for example: n / d = n * factor >> shift for every n < 2^28, with factor = 2^shift / d + 1 and
+// 2^shift = 2^31 times the largest power of two up to d (the product is off by n d / 2^shift < 1/4 of a whole).
+struct Divide {
+  unsigned factor;
+  int shift;
+};
+inline Divide divide_by(long d) {
+  int shift = 31;
+  while (2l << (shift - 31) <= d) shift++;
+  return {(unsigned)((1ul << shift) / (unsigned long)d + 1), shift};
+}
+__device__ __forceinline__ unsigned divided(unsigned n, Divide d) {
+  return (unsigned)((unsigned long)n * d.factor >> d.shift);
+}
+
 // ---- parameter blocks and launchers (arguments checked by the entry points)
 
 struct RowParams {

@@ -8,18 +8,6 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Division by a row's groups d: n / d = n * factor >> shift for every n < 2^28, with factor = 2^shift / d + 1 and
-// 2^shift = 2^31 times the largest power of two up to d (the product is off by n d / 2^shift < 1/4 of a whole).
-struct Divide {
-  unsigned factor;
-  int shift;
-};
-Divide divide_by(long d) {
-  int shift = 31;
-  while (2l << (shift - 31) <= d) shift++;
-  return {(unsigned)((1ul << shift) / (unsigned long)d + 1), shift};
-}
-
 // The unit of N neighbouring values that a thread has: 128 / N threads a group, groups in the order in which
 // they are stored, so a workgroup reads and writes whole rows beside each other whatever their length.
 struct Unit {
@@ -32,7 +20,7 @@ __device__ __forceinline__ Unit my_unit(int dim, Divide d) {
   constexpr unsigned kLanes = kGroup / N;
   Unit u;
   const unsigned lane = threadIdx.x % kLanes, group = blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
-  u.row = (unsigned)((unsigned long)group * d.factor >> d.shift);
+  u.row = divided(group, d);
   u.col = N * (int)(kLanes * (group - u.row * (unsigned)groups(dim)) + lane);
   u.at = kLanes * (long)group + lane;
   return u;
@@ -80,17 +68,6 @@ __device__ __forceinline__ double sum_lanes(double s) {
         __builtin_bit_cast(double, (unsigned long long)(unsigned)hi[1] << 32 | (unsigned)lo[1]);
   }
   return s;
-}
-
-// The double d with its last 32 bits folded into the one above them, as a float: truncated, with the
-// last bit set if anything was lost (rounding to odd). Rounding the result to 4 or fewer bits then
-// gives what rounding d itself does.
-__device__ __forceinline__ float to_odd(double d) {
-  const unsigned long long bits = __builtin_bit_cast(unsigned long long, d);
-  unsigned lost;  // one instruction where the compiler takes two
-  asm("v_min_u32 %0, 1, %1" : "=v"(lost) : "v"((unsigned)bits));
-  const unsigned hi = (unsigned)(bits >> 32) | lost;
-  return (float)__builtin_bit_cast(double, (unsigned long long)hi << 32);
 }
 
 // 1 / max(sqrt(s), 1e-12) for a sum of squares s, following the division where s is not finite

@@ -1,0 +1,603 @@
+// Attention of new tokens over a paged, microscaled cache (gfx950). Contract: include/ancha_hip.h; layout: paged.hpp.
+//
+// For a query row r (a token and a head; the heads that share a head of the cache are rows beside each other) and the
+// keys j that it sees:  o = sum_j e^(c q.k_j) v_j / sum_j e^(c q.k_j), in one pass with a running maximum.
+//
+// Operands. A key's codes times their power of two are bf16 values without loss, so products with a bf16 query are
+// exact; a query of 16 or 32 bits that bf16 does not hold is the sum of two or three bf16 parts, a product each. The
+// weights e^.. are fp16 (fp32 results: two fp16 parts), eight times finer than bf16. So values have to be fp16 too:
+// each block of 32 columns has a reference power `ref` that all of its values are taken relative to, so that the
+// largest fits; what lies 2^-32 below it, where fp16 ends, is far below the result's own rounding. When a larger one
+// comes, the sums so far are scaled down, like those of the running maximum.
+#include "paged.hpp"
+
+namespace ancha {
+namespace paged {
+namespace {
+
+using namespace mx;
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kTile = 16;  // query rows
+constexpr int kStep = 32;  // keys
+constexpr int kWaves = 4;
+constexpr int kLeast = 2 * kWaves;  // steps that a workgroup of a split has at least
+
+__device__ __forceinline__ f32x4 mfma_bf16(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                 0);
+}
+
+// Two codes (number `pair` of those in w) as bf16 / fp16 times 2^(s - 127), f having the exponent bits s.
+template <int FORMAT>
+__device__ __forceinline__ unsigned two_bf16(unsigned w, float f, int pair) {
+  bf16x2 r;
+  if constexpr (FORMAT == kFp8)
+    r = pair ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, f, true)
+             : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, f, false);
+  else
+    r = pair == 0   ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 0)
+        : pair == 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 1)
+        : pair == 2 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 2)
+                    : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 3);
+  return __builtin_bit_cast(unsigned, r);
+}
+template <int FORMAT>
+__device__ __forceinline__ unsigned two_f16(unsigned w, float f, int pair) {
+  h16x2 r;
+  if constexpr (FORMAT == kFp8)
+    r = pair ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, f, true)
+             : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, f, false);
+  else
+    r = pair == 0   ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 0)
+        : pair == 1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 1)
+        : pair == 2 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 2)
+                    : __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 3);
+  return __builtin_bit_cast(unsigned, r);
+}
+
+__device__ __forceinline__ float power(int e) { return __builtin_bit_cast(float, (unsigned)(e + 127) << 23); }
+
+// A NaN that the compiler, which assumes there is none, cannot see.
+__device__ __forceinline__ float hidden_nan() {
+  unsigned bits = 0x7fc00000u;
+  asm volatile("" : "+v"(bits));
+  return __builtin_bit_cast(float, bits);
+}
+
+// Zeros for a first product, in registers: as the instruction's constant they leave its result free to lie over its
+// operands.
+__device__ __forceinline__ f32x4 zeros() {
+  f32x4 z = {0.f, 0.f, 0.f, 0.f};
+  asm volatile("" : "+v"(z));
+  return z;
+}
+
+// Keys [low, high) that row r of a sequence sees, r = token * group + head.
+struct Range {
+  int low, high;
+};
+__device__ __forceinline__ Range visible(const AttentionParams& p, const Sequence& s, int token) {
+  const int capacity = (int)min((long)p.batch.columns << p.cache.shift, (long)0x7fffffff);
+  const long at = (long)s.length - s.count + token;
+  const long high = p.causal ? at + 1 : s.length, low = p.window ? at - p.window + 1 : 0;
+  const int h = (int)min(max(high, 0l), (long)capacity);
+  return {(int)min(max(low, 0l), (long)h), h};
+}
+
+// Tile `id` of the call: its sequence and first row (of count * group), false behind the last one, when `id` is left
+// with its number among those.
+__device__ __forceinline__ bool find_tile(const AttentionParams& p, int group, int& id, int& i, Sequence& s, int& row) {
+  const int lane = threadIdx.x & 63;
+  for (int base = 0; base < p.batch.sequences; base += 64) {
+    Sequence mine = {0, 0, 0};
+    if (base + lane < p.batch.sequences) mine = sequence(p.batch, base + lane, p.rows);
+    const int tiles = (int)(((long)mine.count * group + kTile - 1) / kTile);
+    int sum = tiles;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int below = __shfl_up(sum, o);
+      if (lane >= o) sum += below;
+    }
+    const int all = __builtin_amdgcn_readlane(sum, 63);
+    if (id < all) {
+      const unsigned long long past = __ballot(sum > id);
+      const int at = __builtin_amdgcn_readfirstlane(__builtin_ctzll(past));
+      i = base + at;
+      s.first = __builtin_amdgcn_readlane(mine.first, at);
+      s.count = __builtin_amdgcn_readlane(mine.count, at);
+      s.length = __builtin_amdgcn_readlane(mine.length, at);
+      row = (id - (__builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(tiles, at))) * kTile;
+      return true;
+    }
+    id -= all;
+  }
+  return false;
+}
+
+// Rows of the call that are of no sequence: zeros, by the workgroups behind the last tile (`which` of `count`).
+template <typename T>
+__device__ void clear_rows(const AttentionParams& p, int which, int count) {
+  const int n = p.batch.sequences;
+  const int from = n ? min(max(p.batch.starts[0], 0), p.rows) : 0;
+  const int to = n ? min(max(p.batch.starts[n], from), p.rows) : 0;
+  const long wide = (long)p.heads * p.cache.dim;
+  T* out = static_cast<T*>(p.out);
+  for (long at = (long)which * blockDim.x + threadIdx.x; at < (p.rows - (to - from)) * wide;
+       at += (long)count * blockDim.x)
+    out[at < from * wide ? at : at + (to - from) * wide] = (T)0.f;
+}
+
+// Steps of 32 keys that the rows of a tile see, and how many of the p.splits workgroups share them.
+struct Walk {
+  int first, high, low;  // keys [first, high); the steps begin at low, a multiple of 32
+  int steps, each, splits;
+};
+__device__ __forceinline__ Walk walk_of(const AttentionParams& p, const Sequence& s, int group, int row) {
+  const int last = min(row + kTile, s.count * group) - 1;
+  const Range a = visible(p, s, row / group), b = visible(p, s, last / group);
+  Walk w;
+  w.first = a.low;
+  w.low = a.low & ~(kStep - 1);
+  w.high = b.high;
+  w.steps = w.high > w.low ? (w.high - w.low - 1) / kStep + 1 : 0;
+  w.each = max((w.steps + p.splits - 1) / p.splits, kLeast);
+  w.splits = max((w.steps + w.each - 1) / w.each, 1);
+  return w;
+}
+
+// Workspace of a split: per (tile, head of the cache, split) the rows' maxima and sums, then their results.
+template <int D>
+constexpr long kPart = kTile * (D + 2);
+
+// One tile of 16 query rows over some of its keys: every fourth step of 32 keys a wave. Lane l = 16 g + c has
+//   scores   keys 4 g + i of both 16-key halves for row c (K . Q^T), and so the weights as P . V's operand,
+//   K        key c of each half: 16 (fp8) or up to 32 (fp4) neighbouring columns at a time,
+//   V        the same eight keys as its weights, columns D / 16 * c on, transposed in registers two by two.
+// Nothing passes through LDS before the four waves' sums are joined. Bound by the reading of the cache while there are
+// few rows.
+template <int D, int FORMAT, int TYPE>
+__global__ __launch_bounds__(64 * kWaves) void attention_kernel(AttentionParams p) {
+  typedef typename Stored<TYPE>::type T;
+  constexpr int kQ = TYPE == kBf16 ? 1 : TYPE == kF16 ? 2 : 3;  // parts of a query
+  constexpr int kP = TYPE == kF32 ? 2 : 1;                      // of a weight
+  constexpr int kRow = row_bytes(D, FORMAT), kBlocks = D / kBlock;
+  constexpr int kChunk = FORMAT == kFp4 && D >= 128 ? 32 : 16;  // columns of a key that a lane has beside each other
+  constexpr int kChunks = D / (4 * kChunk);
+  constexpr int kChunkWords = kChunk * (FORMAT == kFp8 ? 8 : 4) / 32;
+  constexpr int kCols = D / 16;                                    // columns of V a lane
+  constexpr int kColBytes = FORMAT == kFp8 ? kCols : kCols / 2;    // 2 to 16
+  constexpr int kColWords = kColBytes < 4 ? 1 : kColBytes / 4;
+  constexpr int kScaleWords = (kBlocks + 3) / 4;
+  // Powers of two of a block's scale byte over its reference: as many as fp16 holds, and when the reference is taken a
+  // few less, so a block may grow by 8 (fp8) or 16 times before the sums are scaled.
+  constexpr int kMost = FORMAT == kFp8 ? 7 : 13, kTaken = FORMAT == kFp8 ? 4 : 9;
+  constexpr int kNoRef = -1000;
+  // Weights are e^.. 2^kUp: a maximum may lag 2^8 behind before the sums are scaled, and small weights keep their bits.
+  constexpr float kUp = 7.f, kLag = 8.f;
+
+  const int group = p.heads / p.cache.heads;
+  int id = blockIdx.x / (p.splits * p.cache.heads), i, row;
+  const int in_tile = blockIdx.x - id * (p.splits * p.cache.heads);
+  const int head = in_tile / p.splits, split = in_tile - head * p.splits;
+  const int tile = id;
+  Sequence s;
+  if (!find_tile(p, group, id, i, s, row)) {
+    // id tiles are behind the last one, of which p.tiles - (tile - id) there are.
+    clear_rows<T>(p, id * p.splits * p.cache.heads + in_tile, (p.tiles - (tile - id)) * p.splits * p.cache.heads);
+    return;
+  }
+  const Walk w = walk_of(p, s, group, row);
+  if (split >= w.splits) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int g = lane >> 4, c = lane & 15;
+
+  // The row of this lane and what it sees.
+  const int rows = s.count * group;
+  const int my_row = row + c, token = min(my_row, rows - 1) / group;
+  const int my_head = head * group + min(my_row, rows - 1) - token * group;
+  Range seen = visible(p, s, token);
+  if (my_row >= rows) seen = {0, 0};
+  // What all rows of the tile see: no masks there.
+  const Range first_sees = visible(p, s, row / group), last_sees = visible(p, s, (min(row + kTile, rows) - 1) / group);
+  const int all_low = last_sees.low, all_high = first_sees.high;
+
+  u32x4 q[kQ][D / 32];
+  {
+    const T* from = static_cast<const T*>(p.q) + (s.first + token) * p.ldq + my_head * p.ldqh;
+#pragma unroll
+    for (int k = 0; k < D / 32; k++) {
+      constexpr int kPer = kChunk / 8;  // of 32 columns in a chunk
+      T t[8];
+      __builtin_memcpy(t, from + k / kPer * 4 * kChunk + g * kChunk + k % kPer * 8, sizeof(t));
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[j] = (float)t[j];
+#pragma unroll
+      for (int part = 0; part < kQ; part++) {
+        bf16x8 b;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          b[j] = (__bf16)v[j];
+          v[j] -= (float)b[j];
+        }
+        q[part][k] = __builtin_bit_cast(u32x4, b);
+      }
+    }
+  }
+
+  const int shift = p.cache.shift, slots = 1 << shift;
+  const int* const table = p.batch.table + (long)i * p.batch.columns;
+  const long values = (long)p.cache.pages * p.cache.heads << shift;  // slots between a key and its value
+  // The half step of 16 keys from `key` on: the slot of its first one, or -1 where there are none.
+  const auto half_at = [&](int key) -> long {
+    if (key >= w.high) return -1;
+    const int page = __builtin_amdgcn_readfirstlane(table[key >> shift]);
+    if ((unsigned)page >= (unsigned)p.cache.pages) return -1;
+    return slot_of(p.cache, 0, page, head, key & (slots - 1));
+  };
+
+  struct Raw {
+    unsigned k[2][kChunks][kChunkWords], v[2][4][kColWords], ks[2][kScaleWords], vs[2][kBlocks];
+    bool there[2];
+  };
+  const auto fetch = [&](int key, Raw& r) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      long slot = half_at(key + 16 * h);
+      r.there[h] = slot >= 0;
+      if (slot < 0) slot = 0;
+      const uint8_t* kc = p.cache.codes + slot * kRow + c * kRow + g * (4 * kChunkWords);
+      const uint8_t* vc = p.cache.codes + (slot + values) * kRow + 4 * g * kRow + c * kColBytes;
+#pragma unroll
+      for (int n = 0; n < kChunks; n++) __builtin_memcpy(r.k[h][n], kc + n * 16 * kChunkWords, 4 * kChunkWords);
+      r.ks[h][0] = 0;
+      __builtin_memcpy(r.ks[h], p.cache.scales + (slot + c) * kBlocks, kBlocks);
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        r.v[h][j][0] = 0;
+        __builtin_memcpy(r.v[h][j], vc + j * kRow, kColBytes);
+      }
+      __builtin_memcpy(r.vs[h], p.cache.scales + (slot + values + 4 * g) * kBlocks, 4 * kBlocks);
+    }
+  };
+
+  float m = -__builtin_inff(), l = 0.f;  // of row c: a whole number near its maximum, and this lane's share of the sum
+  bool any = false;                      // whether this lane has met a key that the row sees
+  int ref = kNoRef;                      // of the block that this lane has columns of
+  f32x4 acc[kCols];                      // element i of number t: column kCols * (4 g + i) + t of row c
+#pragma unroll
+  for (int t = 0; t < kCols; t++) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // Lane whose ref is that of element i of this lane's sums.
+  const auto of_sums = [&](int i) {
+    return D == 64 ? 8 * (g >> 1) : D == 128 ? 4 * g : 4 * g + (i & 2);
+  };
+
+  const int end = w.low + kStep * min(w.steps, (split + 1) * w.each);
+  int key = w.low + kStep * (split * w.each + wave);
+  Raw raw, next;
+  if (key < end) fetch(key, next);
+  for (; key < end; key += kStep * kWaves) {
+    raw = next;
+    if (key + kStep * kWaves < end) fetch(key + kStep * kWaves, next);
+
+    float x[8];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      f32x4 sum = zeros();
+#pragma unroll
+      for (int n = 0; n < kChunks; n++) {
+        // The chunk lies in block (4 n + g) kChunk / 32.
+        const unsigned scale = kChunk == 32 ? raw.ks[h][n] >> 8 * g : raw.ks[h][n / 2] >> (16 * (n & 1) + 8 * (g >> 1));
+        const float f = __builtin_bit_cast(float, (scale & 255u) << 23);
+#pragma unroll
+        for (int e = 0; e < kChunk / 8; e++) {
+          u32x4 a;
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            a[j] = FORMAT == kFp8 ? two_bf16<FORMAT>(raw.k[h][n][2 * e + j / 2], f, j & 1)
+                                  : two_bf16<FORMAT>(raw.k[h][n][e], f, j);
+#pragma unroll
+          for (int part = kQ - 1; part >= 0; part--) sum = mfma_bf16(a, q[part][n * (kChunk / 8) + e], sum);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++) x[4 * h + j] = sum[j];
+    }
+
+    // Scale bytes of V's blocks; keys that no row sees and pages that are not there count as zeros.
+    int sv[8];
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int block = c * kCols / kBlock;
+        unsigned word;
+        if constexpr (D == 64)
+          word = raw.vs[h][j / 2] >> (16 * (j & 1) + 8 * block);
+        else if constexpr (D == 128)
+          word = raw.vs[h][j] >> 8 * block;
+        else
+          word = (block & 4 ? raw.vs[h][2 * j + 1] : raw.vs[h][2 * j]) >> 8 * (block & 3);
+        sv[4 * h + j] = word & 255u;
+      }
+    const bool whole = key >= w.first && key + kStep <= w.high && raw.there[0] && raw.there[1];
+    unsigned sees = 255u;  // a bit for each of the eight keys
+    if (!whole) {
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const int at = key + 16 * (j / 4) + 4 * g + j % 4;
+        if (raw.there[j / 4] && at >= w.first && at < w.high) continue;
+        sv[j] = 0;
+#pragma unroll
+        for (int n = 0; n < kColWords; n++) raw.v[j / 4][j % 4][n] = 0;
+      }
+    }
+    if (!whole || key < all_low || key + kStep > all_high) {
+      sees = 0;
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const int at = key + 16 * (j / 4) + 4 * g + j % 4;
+        const bool yes = raw.there[j / 4] && at >= seen.low && at < seen.high;
+        sees |= (unsigned)yes << j;
+        x[j] = yes ? x[j] : -__builtin_inff();
+      }
+    }
+    any |= sees != 0;
+
+    float top = fmaxf(x[0], x[1]);
+#pragma unroll
+    for (int j = 2; j < 8; j++) top = fmaxf(top, x[j]);
+    top *= p.scale;
+    if (__any(top > m + kLag)) {
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float to = fmaxf(m, __builtin_ceilf(top));
+      const float f = m == -__builtin_inff() ? 0.f : fast_exp2(m - to);
+      m = to;
+      l *= f;
+#pragma unroll
+      for (int t = 0; t < kCols; t++) acc[t] *= f;
+    }
+    const float base = m == -__builtin_inff() ? 0.f : kUp - m;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      x[j] = fast_exp2(__builtin_fmaf(x[j], p.scale, base));
+      l += x[j];
+    }
+    u32x4 weight[kP];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const unsigned two = pack_h2(x[2 * j], x[2 * j + 1]);
+      weight[0][j] = two;
+      if constexpr (kP == 2) {
+        const h16x2 high = __builtin_bit_cast(h16x2, two);
+        weight[1][j] = pack_h2(x[2 * j] - (float)high[0], x[2 * j + 1] - (float)high[1]);
+      }
+    }
+
+    // Blocks that hold a NaN (scale byte 255): NaN in those columns of the rows that see the key, in no other.
+    int largest = 0;
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      bad |= sv[j] == 255;
+      largest = max(largest, sv[j] == 255 ? 0 : sv[j]);
+    }
+    if (__any(bad)) {
+      u32x4 nan, see;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        nan[j] = (sv[2 * j] == 255 ? 0x3c00u : 0u) | (sv[2 * j + 1] == 255 ? 0x3c000000u : 0u);
+        see[j] = (sees >> 2 * j & 1u ? 0x3c00u : 0u) | (sees >> (2 * j + 1) & 1u ? 0x3c000000u : 0u);
+      }
+      const f32x4 met = mfma16x16x32(nan, see, zeros());
+      const float none = hidden_nan();
+#pragma unroll
+      for (int t = 0; t < kCols; t++)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (met[j] > 0.5f) acc[t][j] = none;
+#pragma unroll
+      for (int j = 0; j < 8; j++) sv[j] = sv[j] == 255 ? 0 : sv[j];
+    }
+    if (__any(largest > ref + kMost)) {
+      largest = max(largest, __shfl_xor(largest, 16));
+      largest = max(largest, __shfl_xor(largest, 32));
+      const int to = largest > ref + kMost ? largest - kTaken : ref, down = ref - to;
+      ref = to;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int d = __shfl(down, of_sums(j));
+        const float f = d < -126 ? 0.f : power(d);
+#pragma unroll
+        for (int t = 0; t < kCols; t++) acc[t][j] *= f;
+      }
+    }
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) f[j] = __builtin_bit_cast(float, (unsigned)max(sv[j] - ref + 127, 0) << 23);
+#pragma unroll
+    for (int u = 0; u < kCols / 2; u++) {
+      unsigned two[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        two[j] = FORMAT == kFp8 ? two_f16<FORMAT>(raw.v[j / 4][j % 4][u / 2], f[j], u & 1)
+                                : two_f16<FORMAT>(raw.v[j / 4][j % 4][u / 4], f[j], u & 3);
+      u32x4 even, odd;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        even[j] = __builtin_amdgcn_perm(two[2 * j + 1], two[2 * j], 0x05040100u);
+        odd[j] = __builtin_amdgcn_perm(two[2 * j + 1], two[2 * j], 0x07060302u);
+      }
+#pragma unroll
+      for (int part = kP - 1; part >= 0; part--) {
+        acc[2 * u] = mfma16x16x32(even, weight[part], acc[2 * u]);
+        acc[2 * u + 1] = mfma16x16x32(odd, weight[part], acc[2 * u + 1]);
+      }
+    }
+  }
+
+  // The waves' sums joined: rows' maxima and sums, and the values, into LDS.
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  int met = any;
+  met |= __shfl_xor(met, 16);
+  met |= __shfl_xor(met, 32);
+  // Nothing but scores of minus infinity: 0 / 0, where a row that sees no key is 0.
+  if (met && !(l > 0.f)) l = hidden_nan();
+  // Divided before the power of two comes back: the mean of values is in their range, their sum may not be.
+  const float mean = l == 0.f ? 0.f : 1.f / l;
+  __shared__ float tops[kWaves][kTile], sums[kWaves][kTile];
+  __shared__ __attribute__((aligned(16))) float outs[kWaves][kTile][D + 4];
+  if (g == 0) {
+    tops[wave][c] = m;
+    sums[wave][c] = l;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const int e = __shfl(ref, of_sums(j)) - 127;
+#pragma unroll
+    for (int t = 0; t < kCols; t++) outs[wave][c][kCols * (4 * g + j) + t] = __builtin_ldexpf(acc[t][j] * mean, e);
+  }
+  __syncthreads();
+  const int r = threadIdx.x / 16, part = threadIdx.x % 16;  // columns kCols * part on of row r
+  float top = tops[0][r];
+#pragma unroll
+  for (int v = 1; v < kWaves; v++) top = fmaxf(top, tops[v][r]);
+  float sum = 0.f, share[kWaves], o[kCols];
+#pragma unroll
+  for (int t = 0; t < kCols; t++) o[t] = 0.f;
+#pragma unroll
+  for (int v = 0; v < kWaves; v++) {
+    share[v] = (tops[v][r] == -__builtin_inff() ? 0.f : fast_exp2(tops[v][r] - top)) * sums[v][r];
+    sum += share[v];
+  }
+  const float over = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int v = 0; v < kWaves; v++)
+#pragma unroll
+    for (int t = 0; t < kCols; t++) o[t] = __builtin_fmaf(share[v] * over, outs[v][r][kCols * part + t], o[t]);
+  if (w.splits > 1) {
+    float* to = p.parts + (((long)tile * p.cache.heads + head) * p.splits + split) * kPart<D>;
+    if (part == 0) {
+      to[r] = top;
+      to[kTile + r] = sum;
+    }
+    __builtin_memcpy(to + 2 * kTile + r * D + kCols * part, o, sizeof(o));
+  } else if (row + r < rows) {
+    const int token = (row + r) / group, at_head = head * group + row + r - token * group;
+    store_row<TYPE, kCols>(p.out, ((long)(s.first + token) * p.heads + at_head) * D + kCols * part, kCols, o);
+  }
+}
+
+// The parts of split tiles joined: a wave a row.
+template <int D, int TYPE>
+__global__ __launch_bounds__(256) void join_kernel(AttentionParams p) {
+  constexpr int N = D / 64;
+  const int group = p.heads / p.cache.heads, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+  const int r = wave % kTile, head = wave / kTile % p.cache.heads;
+  int id = wave / kTile / p.cache.heads, i, row;
+  const int tile = id;
+  Sequence s;
+  if (!find_tile(p, group, id, i, s, row) || row + r >= s.count * group) return;
+  const Walk w = walk_of(p, s, group, row);
+  if (w.splits == 1) return;
+  const float* parts = p.parts + ((long)tile * p.cache.heads + head) * p.splits * kPart<D>;
+  float top = -__builtin_inff();
+  for (int j = lane; j < w.splits; j += 64) top = fmaxf(top, parts[j * kPart<D> + r]);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+  const auto share = [&](int j) {
+    const float m = parts[j * kPart<D> + r];
+    return (m == -__builtin_inff() ? 0.f : fast_exp2(m - top)) * parts[j * kPart<D> + kTile + r];
+  };
+  float sum = 0.f, v[N];
+  for (int j = lane; j < w.splits; j += 64) sum += share(j);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
+  const float over = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int n = 0; n < N; n++) v[n] = 0.f;
+  for (int base = 0; base < w.splits; base += 64) {
+    const float weight = base + lane < w.splits ? share(base + lane) * over : 0.f;
+    const int count = min(64, w.splits - base);
+    for (int j = 0; j < count; j += 8) {  // eight reads in flight; behind the last part its own again, without weight
+      float o[8][N];
+#pragma unroll
+      for (int k = 0; k < 8; k++)
+        __builtin_memcpy(o[k], parts + (base + min(j + k, count - 1)) * kPart<D> + 2 * kTile + r * D + lane * N,
+                         sizeof(o[k]));
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        const float f = __shfl(weight, min(j + k, 63));
+        if (j + k < count)
+#pragma unroll
+          for (int n = 0; n < N; n++) v[n] = __builtin_fmaf(f, o[k][n], v[n]);
+      }
+    }
+  }
+  const int token = (row + r) / group, at_head = head * group + row + r - token * group;
+  store_row<TYPE, N>(p.out, ((long)(s.first + token) * p.heads + at_head) * D + lane * N, N, v);
+}
+
+template <int D, int FORMAT, int TYPE>
+void start(const AttentionParams& p, hipStream_t stream) {
+  const unsigned blocks = (unsigned)((long)p.tiles * p.cache.heads * p.splits);
+  hipLaunchKernelGGL((attention_kernel<D, FORMAT, TYPE>), dim3(blocks), dim3(64 * kWaves), 0, stream, p);
+  if (p.splits > 1)
+    hipLaunchKernelGGL((join_kernel<D, TYPE>), dim3((unsigned)((long)p.tiles * p.cache.heads * kTile / 4)), dim3(256),
+                       0, stream, p);
+}
+
+template <int D, int FORMAT>
+void start_type(const AttentionParams& p, hipStream_t stream) {
+  if (p.type == kF32)
+    start<D, FORMAT, kF32>(p, stream);
+  else if (p.type == kF16)
+    start<D, FORMAT, kF16>(p, stream);
+  else
+    start<D, FORMAT, kBf16>(p, stream);
+}
+
+template <int D>
+void start_format(const AttentionParams& p, hipStream_t stream) {
+  if (p.cache.format == kFp8)
+    start_type<D, kFp8>(p, stream);
+  else
+    start_type<D, kFp4>(p, stream);
+}
+
+}  // namespace
+
+AttentionForm attention_form(const AttentionParams& p) {
+  AttentionForm f;
+  const long group = p.heads / p.cache.heads;
+  // Sequences fill their last tiles in part; one tile more for rows of no sequence.
+  f.tiles = (p.rows * group + (long)min(p.batch.sequences, p.rows) * (kTile - 1)) / kTile + 1;
+  // Workgroups share a tile's keys until there are 512, two a CU.
+  const long steps = ((long)p.batch.columns << p.cache.shift) / kStep + 1;
+  f.splits = (int)min(max(512 / (f.tiles * p.cache.heads), 1l), min((steps + kLeast - 1) / kLeast, 256l));
+  const long part = (long)kTile * (p.cache.dim + 2);
+  f.bytes = f.splits > 1 ? (size_t)(f.tiles * p.cache.heads * f.splits * part * 4) : 0;
+  return f;
+}
+
+hipError_t launch_attention(AttentionParams p, hipStream_t stream) {
+  const AttentionForm f = attention_form(p);
+  p.tiles = (int)f.tiles;
+  p.splits = f.splits;
+  if (p.cache.dim == 64)
+    start_format<64>(p, stream);
+  else if (p.cache.dim == 128)
+    start_format<128>(p, stream);
+  else
+    start_format<256>(p, stream);
+  return hipGetLastError();
+}
+
+}  // namespace paged
+}  // namespace ancha

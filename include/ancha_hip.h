@@ -335,6 +335,75 @@ int ancha_mx_linear(const void *codes, const void *scales, size_t n, size_t k, i
                     size_t tokens, size_t width, const void *residual, int type, int out_format,
                     void *out, void *out_scales, hipStream_t stream);
 
+/* ---- Paged operators: rotary positions, a cache of keys and values in pages of microscaled codes, and attention of
+ * new tokens over it. No counterpart in the reference; they stand beside ancha_hip_attention and the microscaled
+ * operators, whose formats the cache has.
+ *
+ * A batch are the sequences of one call, in device memory: the rows starts[i] .. starts[i + 1] - 1 of q, k and v are
+ * the new tokens of sequence i, of which the last has position lengths[i] - 1; its tokens lie in the pages table[i][0],
+ * table[i][1], ... The kernels check what they read there: rows outside every sequence are of none, a page number
+ * outside [0, pages) (and a column behind the last) is a page that is not there, and a position below 0 is no place.
+ * starts must not decrease, and no two tokens of a call may have the same place when they are written.
+ *
+ * A cache is [2][pages][heads][page][dim] (keys, then values): codes, dim (e4m3) or dim / 2 (e2m1, the first value in
+ * the low half) bytes a token, and scales, dim / 32 bytes a token, by the rule of the microscaled operators; both
+ * 16-byte aligned. What a page holds where nothing was written is never part of a result. */
+typedef struct {
+  const int *starts;  /* [sequences + 1] */
+  const int *lengths; /* [sequences] */
+  const int *table;   /* [sequences][columns] */
+  size_t sequences, columns;
+} ancha_paged_batch;
+
+typedef struct {
+  void *codes;
+  void *scales;
+  size_t pages, heads, page, dim; /* page: tokens, a power of two from 16 to 65536; dim: 64, 128 or 256 */
+  int format;                     /* ANCHA_HIP_MX_FP8 / FP4 */
+} ancha_paged_cache;
+
+/* Rotary positions: the first `width` columns of a head turn by position * freqs[i] (pair i: columns i and
+ * i + width / 2, or with `interleaved` 2 i and 2 i + 1), times `magnitude`; the others stay as they are. */
+typedef struct {
+  const double *freqs; /* [width / 2], device */
+  size_t width;        /* even, 2 .. 2048 */
+  int interleaved;
+  double magnitude;
+} ancha_paged_plan;
+
+/* out [rows][heads][dim] contiguous = x rotated; element (row, head, d) of x at row * ldx + head * ldh + d. positions
+ * [rows] of 4 or 8 bytes each (`position_bytes`), or NULL: those of `batch` (rows of no sequence give zeros; otherwise
+ * `batch` may be NULL). Angles are taken in 64 bits, the rest in 32. out must not overlap
+ * x. */
+int ancha_paged_rotary(const void *x, int type, size_t rows, size_t heads, size_t dim, size_t ldx, size_t ldh,
+                       const void *positions, int position_bytes, const ancha_paged_batch *batch,
+                       const ancha_paged_plan *plan, void *out, hipStream_t stream);
+
+/* The rows' keys (rotated, if plan is not NULL) and values into their places: rotation in 64 bits, so the rounding to
+ * the codes is the only one. Rows without a place are left out. Element (row, head, d) of k at row * ldk + head * ldkh
+ * + d, of v likewise. */
+int ancha_paged_write(const void *k, const void *v, int type, size_t rows, size_t ldk, size_t ldkh, size_t ldv,
+                      size_t ldvh, const ancha_paged_batch *batch, const ancha_paged_plan *plan,
+                      const ancha_paged_cache *cache, hipStream_t stream);
+
+/* k, v [sequences][size][heads][dim] of `type`, contiguous: tokens 0 .. size - 1 of each sequence as values, zeros
+ * behind its length and where its page is not there. `starts` is not read (may be NULL). */
+int ancha_paged_read(const ancha_paged_cache *cache, const ancha_paged_batch *batch, size_t size, int type, void *k,
+                     void *v, hipStream_t stream);
+
+/* out [rows][heads][dim] of `type`, contiguous: softmax(scale q.k) v of each row over its sequence's cached tokens,
+ * heads / cache heads neighbouring heads of q for each head of the cache; element (row, head, d) of q at row * ldq +
+ * head * ldqh + d. A row at position t sees the tokens up to t (with `causal`, otherwise all of its sequence) and, with
+ * window > 0, none before t - window + 1. Rows that see no token and rows of no sequence are 0. Scores of any q are
+ * exact to fp32, weights are fp16 (`type` fp32: 22 bits), sums fp32. A NaN in the cache reaches the rows that see it.
+ * workspace: ancha_paged_attention_workspace bytes (of the same arguments; may be 0 and NULL), 16-byte aligned, not
+ * shared with a call that may run at the same time. */
+size_t ancha_paged_attention_workspace(size_t rows, size_t heads, const ancha_paged_cache *cache,
+                                       const ancha_paged_batch *batch);
+int ancha_paged_attention(const void *q, int type, size_t rows, size_t heads, size_t ldq, size_t ldqh,
+                          const ancha_paged_cache *cache, const ancha_paged_batch *batch, double scale, int causal,
+                          size_t window, void *workspace, size_t workspace_bytes, void *out, hipStream_t stream);
+
 /* Sticky device-failure check: 0, or the first HIP error (< 0) any call has met.
  * Replaces `device::check()` (src/device.rs:30-41) for this path. */
 int ancha_hip_check(void);
