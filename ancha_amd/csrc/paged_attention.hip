@@ -9,148 +9,15 @@
 // each block of 32 columns has a reference power `ref` that all of its values are taken relative to, so that the
 // largest fits; what lies 2^-32 below it, where fp16 ends, is far below the result's own rounding. When a larger one
 // comes, the sums so far are scaled down, like those of the running maximum.
-#include "paged.hpp"
+#include "paged_attention.hpp"
 
 namespace ancha {
 namespace paged {
 namespace {
 
-using namespace mx;
-
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-
 constexpr int kTile = 16;  // query rows
 constexpr int kStep = 32;  // keys
 constexpr int kWaves = 4;
-constexpr int kLeast = 2 * kWaves;  // steps that a workgroup of a split has at least
-
-__device__ __forceinline__ f32x4 mfma_bf16(u32x4 a, u32x4 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
-                                                 0);
-}
-
-// Two codes (number `pair` of those in w) as bf16 / fp16 times 2^(s - 127), f having the exponent bits s.
-template <int FORMAT>
-__device__ __forceinline__ unsigned two_bf16(unsigned w, float f, int pair) {
-  bf16x2 r;
-  if constexpr (FORMAT == kFp8)
-    r = pair ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, f, true)
-             : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, f, false);
-  else
-    r = pair == 0   ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 0)
-        : pair == 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 1)
-        : pair == 2 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 2)
-                    : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 3);
-  return __builtin_bit_cast(unsigned, r);
-}
-template <int FORMAT>
-__device__ __forceinline__ unsigned two_f16(unsigned w, float f, int pair) {
-  h16x2 r;
-  if constexpr (FORMAT == kFp8)
-    r = pair ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, f, true)
-             : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, f, false);
-  else
-    r = pair == 0   ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 0)
-        : pair == 1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 1)
-        : pair == 2 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 2)
-                    : __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 3);
-  return __builtin_bit_cast(unsigned, r);
-}
-
-__device__ __forceinline__ float power(int e) { return __builtin_bit_cast(float, (unsigned)(e + 127) << 23); }
-
-// A NaN that the compiler, which assumes there is none, cannot see.
-__device__ __forceinline__ float hidden_nan() {
-  unsigned bits = 0x7fc00000u;
-  asm volatile("" : "+v"(bits));
-  return __builtin_bit_cast(float, bits);
-}
-
-// Zeros for a first product, in registers: as the instruction's constant they leave its result free to lie over its
-// operands.
-__device__ __forceinline__ f32x4 zeros() {
-  f32x4 z = {0.f, 0.f, 0.f, 0.f};
-  asm volatile("" : "+v"(z));
-  return z;
-}
-
-// Keys [low, high) that row r of a sequence sees, r = token * group + head.
-struct Range {
-  int low, high;
-};
-__device__ __forceinline__ Range visible(const AttentionParams& p, const Sequence& s, int token) {
-  const int capacity = (int)min((long)p.batch.columns << p.cache.shift, (long)0x7fffffff);
-  const long at = (long)s.length - s.count + token;
-  const long high = p.causal ? at + 1 : s.length, low = p.window ? at - p.window + 1 : 0;
-  const int h = (int)min(max(high, 0l), (long)capacity);
-  return {(int)min(max(low, 0l), (long)h), h};
-}
-
-// Tile `id` of the call: its sequence and first row (of count * group), false behind the last one, when `id` is left
-// with its number among those.
-__device__ __forceinline__ bool find_tile(const AttentionParams& p, int group, int& id, int& i, Sequence& s, int& row) {
-  const int lane = threadIdx.x & 63;
-  for (int base = 0; base < p.batch.sequences; base += 64) {
-    Sequence mine = {0, 0, 0};
-    if (base + lane < p.batch.sequences) mine = sequence(p.batch, base + lane, p.rows);
-    const int tiles = (int)(((long)mine.count * group + kTile - 1) / kTile);
-    int sum = tiles;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int below = __shfl_up(sum, o);
-      if (lane >= o) sum += below;
-    }
-    const int all = __builtin_amdgcn_readlane(sum, 63);
-    if (id < all) {
-      const unsigned long long past = __ballot(sum > id);
-      const int at = __builtin_amdgcn_readfirstlane(__builtin_ctzll(past));
-      i = base + at;
-      s.first = __builtin_amdgcn_readlane(mine.first, at);
-      s.count = __builtin_amdgcn_readlane(mine.count, at);
-      s.length = __builtin_amdgcn_readlane(mine.length, at);
-      row = (id - (__builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(tiles, at))) * kTile;
-      return true;
-    }
-    id -= all;
-  }
-  return false;
-}
-
-// Rows of the call that are of no sequence: zeros, by the workgroups behind the last tile (`which` of `count`).
-template <typename T>
-__device__ void clear_rows(const AttentionParams& p, int which, int count) {
-  const int n = p.batch.sequences;
-  const int from = n ? min(max(p.batch.starts[0], 0), p.rows) : 0;
-  const int to = n ? min(max(p.batch.starts[n], from), p.rows) : 0;
-  const long wide = (long)p.heads * p.cache.dim;
-  T* out = static_cast<T*>(p.out);
-  for (long at = (long)which * blockDim.x + threadIdx.x; at < (p.rows - (to - from)) * wide;
-       at += (long)count * blockDim.x)
-    out[at < from * wide ? at : at + (to - from) * wide] = (T)0.f;
-}
-
-// Steps of 32 keys that the rows of a tile see, and how many of the p.splits workgroups share them.
-struct Walk {
-  int first, high, low;  // keys [first, high); the steps begin at low, a multiple of 32
-  int steps, each, splits;
-};
-__device__ __forceinline__ Walk walk_of(const AttentionParams& p, const Sequence& s, int group, int row) {
-  const int last = min(row + kTile, s.count * group) - 1;
-  const Range a = visible(p, s, row / group), b = visible(p, s, last / group);
-  Walk w;
-  w.first = a.low;
-  w.low = a.low & ~(kStep - 1);
-  w.high = b.high;
-  w.steps = w.high > w.low ? (w.high - w.low - 1) / kStep + 1 : 0;
-  w.each = max((w.steps + p.splits - 1) / p.splits, kLeast);
-  w.splits = max((w.steps + w.each - 1) / w.each, 1);
-  return w;
-}
-
-// Workspace of a split: per (tile, head of the cache, split) the rows' maxima and sums, then their results.
-template <int D>
-constexpr long kPart = kTile * (D + 2);
 
 // One tile of 16 query rows over some of its keys: every fourth step of 32 keys a wave. Lane l = 16 g + c has
 //   scores   keys 4 g + i of both 16-key halves for row c (K . Q^T), and so the weights as P . V's operand,
@@ -184,12 +51,12 @@ __global__ __launch_bounds__(64 * kWaves) void attention_kernel(AttentionParams 
   const int head = in_tile / p.splits, split = in_tile - head * p.splits;
   const int tile = id;
   Sequence s;
-  if (!find_tile(p, group, id, i, s, row)) {
+  if (!find_tile(p, group, kTile, id, i, s, row)) {
     // id tiles are behind the last one, of which p.tiles - (tile - id) there are.
     clear_rows<T>(p, id * p.splits * p.cache.heads + in_tile, (p.tiles - (tile - id)) * p.splits * p.cache.heads);
     return;
   }
-  const Walk w = walk_of(p, s, group, row);
+  const Walk w = walk_of(p, s, group, row, kTile, kStep);
   if (split >= w.splits) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int g = lane >> 4, c = lane & 15;
@@ -266,6 +133,7 @@ __global__ __launch_bounds__(64 * kWaves) void attention_kernel(AttentionParams 
 
   float m = -__builtin_inff(), l = 0.f;  // of row c: a whole number near its maximum, and this lane's share of the sum
   bool any = false;                      // whether this lane has met a key that the row sees
+  unsigned none = 0;                     // a bit for each element of its sums in which the row sees a NaN
   int ref = kNoRef;                      // of the block that this lane has columns of
   f32x4 acc[kCols];                      // element i of number t: column kCols * (4 g + i) + t of row c
 #pragma unroll
@@ -394,12 +262,8 @@ __global__ __launch_bounds__(64 * kWaves) void attention_kernel(AttentionParams 
         see[j] = (sees >> 2 * j & 1u ? 0x3c00u : 0u) | (sees >> (2 * j + 1) & 1u ? 0x3c000000u : 0u);
       }
       const f32x4 met = mfma16x16x32(nan, see, zeros());
-      const float none = hidden_nan();
 #pragma unroll
-      for (int t = 0; t < kCols; t++)
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-          if (met[j] > 0.5f) acc[t][j] = none;
+      for (int j = 0; j < 4; j++) none |= (unsigned)(met[j] > 0.5f) << j;
 #pragma unroll
       for (int j = 0; j < 8; j++) sv[j] = sv[j] == 255 ? 0 : sv[j];
     }
@@ -447,7 +311,8 @@ __global__ __launch_bounds__(64 * kWaves) void attention_kernel(AttentionParams 
   met |= __shfl_xor(met, 16);
   met |= __shfl_xor(met, 32);
   // Nothing but scores of minus infinity: 0 / 0, where a row that sees no key is 0.
-  if (met && !(l > 0.f)) l = hidden_nan();
+  const float nan = hidden_nan();
+  if (met && !(l > 0.f)) l = nan;
   // Divided before the power of two comes back: the mean of values is in their range, their sum may not be.
   const float mean = l == 0.f ? 0.f : 1.f / l;
   __shared__ float tops[kWaves][kTile], sums[kWaves][kTile];
@@ -460,7 +325,7 @@ __global__ __launch_bounds__(64 * kWaves) void attention_kernel(AttentionParams 
   for (int j = 0; j < 4; j++) {
     const int e = __shfl(ref, of_sums(j)) - 127;
 #pragma unroll
-    for (int t = 0; t < kCols; t++) outs[wave][c][kCols * (4 * g + j) + t] = __builtin_ldexpf(acc[t][j] * mean, e);
+    for (int t = 0; t < kCols; t++) outs[wave][c][kCols * (4 * g + j) + t] = none >> j & 1u ? nan : __builtin_ldexpf(acc[t][j] * mean, e);
   }
   __syncthreads();
   const int r = threadIdx.x / 16, part = threadIdx.x % 16;  // columns kCols * part on of row r
@@ -481,7 +346,7 @@ __global__ __launch_bounds__(64 * kWaves) void attention_kernel(AttentionParams 
 #pragma unroll
     for (int t = 0; t < kCols; t++) o[t] = __builtin_fmaf(share[v] * over, outs[v][r][kCols * part + t], o[t]);
   if (w.splits > 1) {
-    float* to = p.parts + (((long)tile * p.cache.heads + head) * p.splits + split) * kPart<D>;
+    float* to = p.parts + (((long)tile * p.cache.heads + head) * p.splits + split) * part_floats(kTile, D);
     if (part == 0) {
       to[r] = top;
       to[kTile + r] = sum;
@@ -493,27 +358,28 @@ __global__ __launch_bounds__(64 * kWaves) void attention_kernel(AttentionParams 
   }
 }
 
-// The parts of split tiles joined: a wave a row.
+// The parts of split tiles of `rows` rows and steps of `keys` keys joined: a wave a row.
 template <int D, int TYPE>
-__global__ __launch_bounds__(256) void join_kernel(AttentionParams p) {
+__global__ __launch_bounds__(256) void join_kernel(AttentionParams p, int rows, int keys) {
   constexpr int N = D / 64;
+  const long kPart = part_floats(rows, D);
   const int group = p.heads / p.cache.heads, lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-  const int r = wave % kTile, head = wave / kTile % p.cache.heads;
-  int id = wave / kTile / p.cache.heads, i, row;
+  const int r = wave % rows, head = wave / rows % p.cache.heads;
+  int id = wave / rows / p.cache.heads, i, row;
   const int tile = id;
   Sequence s;
-  if (!find_tile(p, group, id, i, s, row) || row + r >= s.count * group) return;
-  const Walk w = walk_of(p, s, group, row);
+  if (!find_tile(p, group, rows, id, i, s, row) || row + r >= s.count * group) return;
+  const Walk w = walk_of(p, s, group, row, rows, keys);
   if (w.splits == 1) return;
-  const float* parts = p.parts + ((long)tile * p.cache.heads + head) * p.splits * kPart<D>;
+  const float* parts = p.parts + ((long)tile * p.cache.heads + head) * p.splits * kPart;
   float top = -__builtin_inff();
-  for (int j = lane; j < w.splits; j += 64) top = fmaxf(top, parts[j * kPart<D> + r]);
+  for (int j = lane; j < w.splits; j += 64) top = fmaxf(top, parts[j * kPart + r]);
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
   const auto share = [&](int j) {
-    const float m = parts[j * kPart<D> + r];
-    return (m == -__builtin_inff() ? 0.f : fast_exp2(m - top)) * parts[j * kPart<D> + kTile + r];
+    const float m = parts[j * kPart + r];
+    return (m == -__builtin_inff() ? 0.f : fast_exp2(m - top)) * parts[j * kPart + rows + r];
   };
   float sum = 0.f, v[N];
   for (int j = lane; j < w.splits; j += 64) sum += share(j);
@@ -529,7 +395,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionParams p) {
       float o[8][N];
 #pragma unroll
       for (int k = 0; k < 8; k++)
-        __builtin_memcpy(o[k], parts + (base + min(j + k, count - 1)) * kPart<D> + 2 * kTile + r * D + lane * N,
+        __builtin_memcpy(o[k], parts + (base + min(j + k, count - 1)) * kPart + 2 * rows + r * D + lane * N,
                          sizeof(o[k]));
 #pragma unroll
       for (int k = 0; k < 8; k++) {
@@ -544,45 +410,50 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionParams p) {
   store_row<TYPE, N>(p.out, ((long)(s.first + token) * p.heads + at_head) * D + lane * N, N, v);
 }
 
-template <int D, int FORMAT, int TYPE>
-void start(const AttentionParams& p, hipStream_t stream) {
-  const unsigned blocks = (unsigned)((long)p.tiles * p.cache.heads * p.splits);
-  hipLaunchKernelGGL((attention_kernel<D, FORMAT, TYPE>), dim3(blocks), dim3(64 * kWaves), 0, stream, p);
-  if (p.splits > 1)
-    hipLaunchKernelGGL((join_kernel<D, TYPE>), dim3((unsigned)((long)p.tiles * p.cache.heads * kTile / 4)), dim3(256),
-                       0, stream, p);
-}
-
 template <int D, int FORMAT>
-void start_type(const AttentionParams& p, hipStream_t stream) {
+void start_tiles(const AttentionParams& p, hipStream_t stream) {
+  const dim3 grid((unsigned)((long)p.tiles * p.cache.heads * p.splits)), block(64 * kWaves);
   if (p.type == kF32)
-    start<D, FORMAT, kF32>(p, stream);
+    hipLaunchKernelGGL((attention_kernel<D, FORMAT, kF32>), grid, block, 0, stream, p);
   else if (p.type == kF16)
-    start<D, FORMAT, kF16>(p, stream);
+    hipLaunchKernelGGL((attention_kernel<D, FORMAT, kF16>), grid, block, 0, stream, p);
   else
-    start<D, FORMAT, kBf16>(p, stream);
+    hipLaunchKernelGGL((attention_kernel<D, FORMAT, kBf16>), grid, block, 0, stream, p);
 }
 
 template <int D>
-void start_format(const AttentionParams& p, hipStream_t stream) {
-  if (p.cache.format == kFp8)
-    start_type<D, kFp8>(p, stream);
+void start(const AttentionParams& p, hipStream_t stream) {
+  if (p.chunk)
+    launch_chunk(p, stream);
+  else if (p.cache.format == kFp8)
+    start_tiles<D, kFp8>(p, stream);
   else
-    start_type<D, kFp4>(p, stream);
+    start_tiles<D, kFp4>(p, stream);
+  if (p.splits == 1) return;
+  const int rows = p.chunk ? chunk_rows(D, p.type) : kTile, keys = p.chunk ? chunk_keys(D) : kStep;
+  const dim3 grid((unsigned)((long)p.tiles * p.cache.heads * rows / 4)), block(256);
+  if (p.type == kF32)
+    hipLaunchKernelGGL((join_kernel<D, kF32>), grid, block, 0, stream, p, rows, keys);
+  else if (p.type == kF16)
+    hipLaunchKernelGGL((join_kernel<D, kF16>), grid, block, 0, stream, p, rows, keys);
+  else
+    hipLaunchKernelGGL((join_kernel<D, kBf16>), grid, block, 0, stream, p, rows, keys);
 }
 
 }  // namespace
 
 AttentionForm attention_form(const AttentionParams& p) {
-  AttentionForm f;
-  const long group = p.heads / p.cache.heads;
+  AttentionForm f{};
+  const long group = p.heads / p.cache.heads, rows = p.rows * group, some = min(p.batch.sequences, p.rows);
+  f.chunk = rows >= 64 * some;
+  const int of = f.chunk ? chunk_rows(p.cache.dim, p.type) : kTile;
   // Sequences fill their last tiles in part; one tile more for rows of no sequence.
-  f.tiles = (p.rows * group + (long)min(p.batch.sequences, p.rows) * (kTile - 1)) / kTile + 1;
-  // Workgroups share a tile's keys until there are 512, two a CU.
-  const long steps = ((long)p.batch.columns << p.cache.shift) / kStep + 1;
-  f.splits = (int)min(max(512 / (f.tiles * p.cache.heads), 1l), min((steps + kLeast - 1) / kLeast, 256l));
-  const long part = (long)kTile * (p.cache.dim + 2);
-  f.bytes = f.splits > 1 ? (size_t)(f.tiles * p.cache.heads * f.splits * part * 4) : 0;
+  f.tiles = (rows + some * (of - 1)) / of + 1;
+  // Workgroups share a tile's keys until there are 512, two a CU (256 of eight waves).
+  const long keys = (long)p.batch.columns << p.cache.shift;
+  const long want = f.chunk && chunk_waves(p.cache.dim, p.type) == 8 ? 256 : 512;
+  f.splits = (int)min(max(want / (f.tiles * p.cache.heads), 1l), min(keys / kLeastKeys + 1, 256l));
+  f.bytes = f.splits > 1 ? (size_t)(f.tiles * p.cache.heads * f.splits * part_floats(of, p.cache.dim) * 4) : 0;
   return f;
 }
 
@@ -590,12 +461,13 @@ hipError_t launch_attention(AttentionParams p, hipStream_t stream) {
   const AttentionForm f = attention_form(p);
   p.tiles = (int)f.tiles;
   p.splits = f.splits;
+  p.chunk = f.chunk;
   if (p.cache.dim == 64)
-    start_format<64>(p, stream);
+    start<64>(p, stream);
   else if (p.cache.dim == 128)
-    start_format<128>(p, stream);
+    start<128>(p, stream);
   else
-    start_format<256>(p, stream);
+    start<256>(p, stream);
   return hipGetLastError();
 }
 

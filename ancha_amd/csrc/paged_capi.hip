@@ -203,8 +203,8 @@ int ancha_paged_attention(const void* q, int type, size_t rows, size_t heads, si
   p.rows = static_cast<int>(rows);
   p.heads = static_cast<int>(heads);
   const paged::AttentionForm form = paged::attention_form(p);
-  // Both kernels below HIP's 2^32 threads.
-  if (form.tiles * static_cast<long>(cache->heads) * (form.splits > 4 ? form.splits : 4) >= 1l << 24)
+  // Below HIP's 2^32 threads, up to 512 a workgroup (and few tiles where there are several workgroups a tile).
+  if (form.tiles * static_cast<long>(cache->heads) * form.splits >= 1l << 23)
     return fail(ANCHA_HIP_UNSUPPORTED, who + ": too many rows and heads");
   if (workspace_bytes < form.bytes || (form.bytes && (!workspace || !aligned(workspace, 16))))
     return fail(ANCHA_HIP_INVALID, who + ": the workspace is null, too small or not 16-byte aligned");

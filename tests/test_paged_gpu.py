@@ -7,7 +7,8 @@ from 64 bits: the oracle's bytes.
 Attention, with A = sum_j w_j |v_j| of a row: scores are sums of exact products, D / 32 instructions a part of q, each
 of which adds at most one step (2^-23) of the largest of its terms twice; three parts hold 24 bits of q. With R the largest
 scale sum |q k|, a score is within e = (D / 32 * parts + 4) 2^-22 R, and so the result within 2 e A. Exponentials are
-good to 2^-21, weights to half a step of fp16 (fp32 results: 2^-21). Each weight that is less than fp16 holds is off by
+good to 2^-21, weights to half a step of fp16 (fp32 results: 2^-21), in the products and in the sum that divides them:
+2^-11 (A + |o|). Each weight that is less than fp16 holds is off by
 2^-25 where the largest is 2^6 to 2^15, so by 2^-31 of it: 2^-31 sum_j |v_j| in all. Values are off by 2^-25 where the
 largest of their block is 2^11 or more, less than 2^-32 of it. Then the result's type: half its eps, and
 below its normal values, where its steps no longer shrink, half of their step (fp16: 2^-25).
@@ -235,7 +236,7 @@ def check_attention(gpu, kind, heads, cache, codes, scales, batch, plain, rows, 
     e = (cache.dim // 32 * PARTS[kind] + 4) * 2.0 ** -22 * reach
     weights = 2.0 ** -21 if kind == "f32" else torch.finfo(torch.float16).eps / 2
     held = np.exp2(np.where(scales == 255, 0, scales).max() - 127.0) * (448 if cache.format == "fp8" else 6)
-    tol = size * (2 * e + weights + 2.0 ** -21) + rounding(want, dtype) + held * 2.0 ** -32
+    tol = size * (2 * e + weights + 2.0 ** -21) + np.abs(want) * weights + rounding(want, dtype) + held * 2.0 ** -32
     tol = tol + total * 2.0 ** -31
     close(f"attention {kind} {how}", got, want, tol)
     return got
@@ -341,7 +342,8 @@ def test_attention_blocks_and_scores_of_any_size(gpu, kind):
             e = (dim // 32 * PARTS[kind] + 4) * 2.0 ** -22 * reach
             # A value is off by 2^-32 of the largest of its own block of columns, however large the others are.
             weights = 2.0 ** -21 if kind == "f32" else 2.0 ** -11
-            tol = size * (2 * np.minimum(e, 1) + weights + 2.0 ** -21) + rounding(want, TYPES[kind])
+            tol = size * (2 * np.minimum(e, 1) + weights + 2.0 ** -21) + np.abs(want) * weights
+            tol = tol + rounding(want, TYPES[kind])
             blocks = np.exp2(scales[1].max((0, 1, 2)) - 127.0).repeat(32) * (448 if fmt == "fp8" else 6)
             got = paged.attention(q, cache, batch)
             tol = tol + total * 2.0 ** -31 + blocks * 2.0 ** -32
