@@ -122,25 +122,27 @@ struct AttentionParams {
   long ldq, ldqh;
   int rows, heads, type, causal, window;  // window 0: none
   float scale;                            // of the scores, times log2(e)
-  int tiles, splits, chunk;               // of attention_form
+  int tiles, splits, form;                // of attention_form
 };
 hipError_t launch_attention(AttentionParams p, hipStream_t stream);
 void launch_chunk(const AttentionParams& p, hipStream_t stream);
 
-// How a call is laid out: whether by the chunk kernel; query tiles (an upper bound, the kernels count the real ones);
-// the workgroups that share the keys of a tile; bytes of workspace.
+// How a call is laid out: tiles of 16 query rows by four or eight waves, or the chunk kernel's; tiles (an upper bound,
+// the kernels count the real ones); the workgroups that share the keys of a tile; bytes of workspace.
+enum { kTiles4, kTiles8, kChunk };
 struct AttentionForm {
-  int chunk;
+  int form;
   long tiles;
   int splits;
   size_t bytes;
 };
 AttentionForm attention_form(const AttentionParams& p);
 
-// The chunk kernel's waves, with 32 query rows each, and the keys of a step.
+// The chunk kernel takes heads of 64 or 128 columns; its waves have 32 query rows each and walk in steps of kChunkKeys.
+// (fp32 queries of 128 columns are 96 registers in three parts, which leaves room for one wave a SIMD.)
+constexpr int kChunkKeys = 64;
 constexpr int chunk_waves(int dim, int type) { return dim == 128 && type != kF32 ? 8 : 4; }
 constexpr int chunk_rows(int dim, int type) { return 32 * chunk_waves(dim, type); }
-constexpr int chunk_keys(int dim) { return dim == 256 ? 32 : 64; }
 
 }  // namespace paged
 }  // namespace ancha

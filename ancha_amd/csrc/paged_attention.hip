@@ -17,17 +17,17 @@ namespace {
 
 constexpr int kTile = 16;  // query rows
 constexpr int kStep = 32;  // keys
-constexpr int kWaves = 4;
 
-// One tile of 16 query rows over some of its keys: every fourth step of 32 keys a wave. Lane l = 16 g + c has
+// One tile of 16 query rows over some of its keys: every WAVES-th step of 32 keys a wave. Lane l = 16 g + c has
 //   scores   keys 4 g + i of both 16-key halves for row c (K . Q^T), and so the weights as P . V's operand,
 //   K        key c of each half: 16 (fp8) or up to 32 (fp4) neighbouring columns at a time,
 //   V        the same eight keys as its weights, columns D / 16 * c on, transposed in registers two by two.
-// Nothing passes through LDS before the four waves' sums are joined. Bound by the reading of the cache while there are
+// Nothing passes through LDS before the waves' sums are joined. Bound by the reading of the cache while there are
 // few rows.
-template <int D, int FORMAT, int TYPE>
-__global__ __launch_bounds__(64 * kWaves) void attention_kernel(AttentionParams p) {
+template <int D, int FORMAT, int TYPE, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void attention_kernel(AttentionParams p) {
   typedef typename Stored<TYPE>::type T;
+  constexpr int kWaves = WAVES;
   constexpr int kQ = TYPE == kBf16 ? 1 : TYPE == kF16 ? 2 : 3;  // parts of a query
   constexpr int kP = TYPE == kF32 ? 2 : 1;                      // of a weight
   constexpr int kRow = row_bytes(D, FORMAT), kBlocks = D / kBlock;
@@ -53,10 +53,12 @@ __global__ __launch_bounds__(64 * kWaves) void attention_kernel(AttentionParams 
   Sequence s;
   if (!find_tile(p, group, kTile, id, i, s, row)) {
     // id tiles are behind the last one, of which p.tiles - (tile - id) there are.
+    note_tile(p, tile, head, split, {0, 0, 0, 0});
     clear_rows<T>(p, id * p.splits * p.cache.heads + in_tile, (p.tiles - (tile - id)) * p.splits * p.cache.heads);
     return;
   }
   const Walk w = walk_of(p, s, group, row, kTile, kStep);
+  note_tile(p, tile, head, split, {w.splits, s.first, row, min(kTile, s.count * group - row)});
   if (split >= w.splits) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int g = lane >> 4, c = lane & 15;
@@ -98,11 +100,20 @@ __global__ __launch_bounds__(64 * kWaves) void attention_kernel(AttentionParams 
   const int shift = p.cache.shift, slots = 1 << shift;
   const int* const table = p.batch.table + (long)i * p.batch.columns;
   const long values = (long)p.cache.pages * p.cache.heads << shift;  // slots between a key and its value
-  // The half step of 16 keys from `key` on: the slot of its first one, or -1 where there are none.
-  const auto half_at = [&](int key) -> long {
-    if (key >= w.high) return -1;
-    const int page = __builtin_amdgcn_readfirstlane(table[key >> shift]);
-    if ((unsigned)page >= (unsigned)p.cache.pages) return -1;
+  // The pages of both half steps of 16 keys from `key` on, and the slot of a half's first key, or -1 where there are
+  // none.
+  struct Pages {
+    int of[2];
+  };
+  const auto pages_at = [&](int key) {
+    Pages g;
+#pragma unroll
+    for (int h = 0; h < 2; h++) g.of[h] = table[min(key + 16 * h, w.high - 1) >> shift];
+    return g;
+  };
+  const auto half_at = [&](int key, int of) -> long {
+    const int page = __builtin_amdgcn_readfirstlane(of);
+    if (key >= w.high || (unsigned)page >= (unsigned)p.cache.pages) return -1;
     return slot_of(p.cache, 0, page, head, key & (slots - 1));
   };
 
@@ -110,10 +121,10 @@ __global__ __launch_bounds__(64 * kWaves) void attention_kernel(AttentionParams 
     unsigned k[2][kChunks][kChunkWords], v[2][4][kColWords], ks[2][kScaleWords], vs[2][kBlocks];
     bool there[2];
   };
-  const auto fetch = [&](int key, Raw& r) {
+  const auto fetch = [&](int key, const Pages& pages, Raw& r) {
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-      long slot = half_at(key + 16 * h);
+      long slot = half_at(key + 16 * h, pages.of[h]);
       r.there[h] = slot >= 0;
       if (slot < 0) slot = 0;
       const uint8_t* kc = p.cache.codes + slot * kRow + c * kRow + g * (4 * kChunkWords);
@@ -145,11 +156,22 @@ __global__ __launch_bounds__(64 * kWaves) void attention_kernel(AttentionParams 
 
   const int end = w.low + kStep * min(w.steps, (split + 1) * w.each);
   int key = w.low + kStep * (split * w.each + wave);
+  // Codes one step ahead, page numbers two.
+  constexpr int kStride = kStep * kWaves;
   Raw raw, next;
-  if (key < end) fetch(key, next);
-  for (; key < end; key += kStep * kWaves) {
+  Pages pages;
+  if (key < end) {
+    pages = pages_at(key);
+    fetch(key, pages, next);
+    pages = pages_at(key + kStride);
+  }
+  for (; key < end; key += kStride) {
     raw = next;
-    if (key + kStep * kWaves < end) fetch(key + kStep * kWaves, next);
+    if (key + kStride < end) {
+      const Pages now = pages;
+      pages = pages_at(key + 2 * kStride);
+      fetch(key + kStride, now, next);
+    }
 
     float x[8];
 #pragma unroll
@@ -328,6 +350,7 @@ __global__ __launch_bounds__(64 * kWaves) void attention_kernel(AttentionParams 
     for (int t = 0; t < kCols; t++) outs[wave][c][kCols * (4 * g + j) + t] = none >> j & 1u ? nan : __builtin_ldexpf(acc[t][j] * mean, e);
   }
   __syncthreads();
+  if (WAVES > 4 && threadIdx.x >= 256) return;
   const int r = threadIdx.x / 16, part = threadIdx.x % 16;  // columns kCols * part on of row r
   float top = tops[0][r];
 #pragma unroll
@@ -346,7 +369,7 @@ __global__ __launch_bounds__(64 * kWaves) void attention_kernel(AttentionParams 
 #pragma unroll
     for (int t = 0; t < kCols; t++) o[t] = __builtin_fmaf(share[v] * over, outs[v][r][kCols * part + t], o[t]);
   if (w.splits > 1) {
-    float* to = p.parts + (((long)tile * p.cache.heads + head) * p.splits + split) * part_floats(kTile, D);
+    float* to = part_of(p, tile, head, split, kTile, D);
     if (part == 0) {
       to[r] = top;
       to[kTile + r] = sum;
@@ -358,21 +381,17 @@ __global__ __launch_bounds__(64 * kWaves) void attention_kernel(AttentionParams 
   }
 }
 
-// The parts of split tiles of `rows` rows and steps of `keys` keys joined: a wave a row.
+// The parts of split tiles of `rows` rows joined: a wave a row.
 template <int D, int TYPE>
-__global__ __launch_bounds__(256) void join_kernel(AttentionParams p, int rows, int keys) {
+__global__ __launch_bounds__(256) void join_kernel(AttentionParams p, int rows) {
   constexpr int N = D / 64;
   const long kPart = part_floats(rows, D);
-  const int group = p.heads / p.cache.heads, lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-  const int r = wave % rows, head = wave / rows % p.cache.heads;
-  int id = wave / rows / p.cache.heads, i, row;
-  const int tile = id;
-  Sequence s;
-  if (!find_tile(p, group, rows, id, i, s, row) || row + r >= s.count * group) return;
-  const Walk w = walk_of(p, s, group, row, rows, keys);
-  if (w.splits == 1) return;
-  const float* parts = p.parts + ((long)tile * p.cache.heads + head) * p.splits * kPart;
+  const int r = wave % rows, at = wave / rows, head = at % p.cache.heads;
+  const Joined w = reinterpret_cast<const Joined*>(p.parts)[at];
+  if (r >= w.rows || w.splits == 1) return;
+  const float* parts = part_of(p, at / p.cache.heads, head, 0, rows, D);
   float top = -__builtin_inff();
   for (int j = lane; j < w.splits; j += 64) top = fmaxf(top, parts[j * kPart + r]);
 #pragma unroll
@@ -406,38 +425,46 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionParams p, int rows, 
       }
     }
   }
-  const int token = (row + r) / group, at_head = head * group + row + r - token * group;
-  store_row<TYPE, N>(p.out, ((long)(s.first + token) * p.heads + at_head) * D + lane * N, N, v);
+  const int group = p.heads / p.cache.heads, token = (w.row + r) / group;
+  const int at_head = head * group + w.row + r - token * group;
+  store_row<TYPE, N>(p.out, ((long)(w.first + token) * p.heads + at_head) * D + lane * N, N, v);
+}
+
+template <int D, int FORMAT, int WAVES>
+void start_tiles(const AttentionParams& p, hipStream_t stream) {
+  const dim3 grid((unsigned)((long)p.tiles * p.cache.heads * p.splits)), block(64 * WAVES);
+  if (p.type == kF32)
+    hipLaunchKernelGGL((attention_kernel<D, FORMAT, kF32, WAVES>), grid, block, 0, stream, p);
+  else if (p.type == kF16)
+    hipLaunchKernelGGL((attention_kernel<D, FORMAT, kF16, WAVES>), grid, block, 0, stream, p);
+  else
+    hipLaunchKernelGGL((attention_kernel<D, FORMAT, kBf16, WAVES>), grid, block, 0, stream, p);
 }
 
 template <int D, int FORMAT>
-void start_tiles(const AttentionParams& p, hipStream_t stream) {
-  const dim3 grid((unsigned)((long)p.tiles * p.cache.heads * p.splits)), block(64 * kWaves);
-  if (p.type == kF32)
-    hipLaunchKernelGGL((attention_kernel<D, FORMAT, kF32>), grid, block, 0, stream, p);
-  else if (p.type == kF16)
-    hipLaunchKernelGGL((attention_kernel<D, FORMAT, kF16>), grid, block, 0, stream, p);
-  else
-    hipLaunchKernelGGL((attention_kernel<D, FORMAT, kBf16>), grid, block, 0, stream, p);
+void start_format(const AttentionParams& p, hipStream_t stream) {
+  if constexpr (D < 256)
+    if (p.form == kTiles8) return start_tiles<D, FORMAT, 8>(p, stream);
+  start_tiles<D, FORMAT, 4>(p, stream);
 }
 
 template <int D>
 void start(const AttentionParams& p, hipStream_t stream) {
-  if (p.chunk)
+  if (p.form == kChunk)
     launch_chunk(p, stream);
   else if (p.cache.format == kFp8)
-    start_tiles<D, kFp8>(p, stream);
+    start_format<D, kFp8>(p, stream);
   else
-    start_tiles<D, kFp4>(p, stream);
+    start_format<D, kFp4>(p, stream);
   if (p.splits == 1) return;
-  const int rows = p.chunk ? chunk_rows(D, p.type) : kTile, keys = p.chunk ? chunk_keys(D) : kStep;
+  const int rows = p.form == kChunk ? chunk_rows(D, p.type) : kTile;
   const dim3 grid((unsigned)((long)p.tiles * p.cache.heads * rows / 4)), block(256);
   if (p.type == kF32)
-    hipLaunchKernelGGL((join_kernel<D, kF32>), grid, block, 0, stream, p, rows, keys);
+    hipLaunchKernelGGL((join_kernel<D, kF32>), grid, block, 0, stream, p, rows);
   else if (p.type == kF16)
-    hipLaunchKernelGGL((join_kernel<D, kF16>), grid, block, 0, stream, p, rows, keys);
+    hipLaunchKernelGGL((join_kernel<D, kF16>), grid, block, 0, stream, p, rows);
   else
-    hipLaunchKernelGGL((join_kernel<D, kBf16>), grid, block, 0, stream, p, rows, keys);
+    hipLaunchKernelGGL((join_kernel<D, kBf16>), grid, block, 0, stream, p, rows);
 }
 
 }  // namespace
@@ -445,15 +472,18 @@ void start(const AttentionParams& p, hipStream_t stream) {
 AttentionForm attention_form(const AttentionParams& p) {
   AttentionForm f{};
   const long group = p.heads / p.cache.heads, rows = p.rows * group, some = min(p.batch.sequences, p.rows);
-  f.chunk = rows >= 64 * some;
-  const int of = f.chunk ? chunk_rows(p.cache.dim, p.type) : kTile;
+  const bool chunk = p.cache.dim < 256 && rows >= 64 * some;
+  const int of = chunk ? chunk_rows(p.cache.dim, p.type) : kTile;
   // Sequences fill their last tiles in part; one tile more for rows of no sequence.
   f.tiles = (rows + some * (of - 1)) / of + 1;
-  // Workgroups share a tile's keys until there are 512, two a CU (256 of eight waves).
+  const long groups = f.tiles * p.cache.heads;
+  f.form = chunk ? kChunk : p.cache.dim < 256 && groups < 1024 ? kTiles8 : kTiles4;
+  // Workgroups share a tile's keys until there are 512 (256 of the chunk kernel's with eight waves).
+  const long want = chunk && chunk_waves(p.cache.dim, p.type) == 8 ? 256 : 512;
   const long keys = (long)p.batch.columns << p.cache.shift;
-  const long want = f.chunk && chunk_waves(p.cache.dim, p.type) == 8 ? 256 : 512;
-  f.splits = (int)min(max(want / (f.tiles * p.cache.heads), 1l), min(keys / kLeastKeys + 1, 256l));
-  f.bytes = f.splits > 1 ? (size_t)(f.tiles * p.cache.heads * f.splits * part_floats(of, p.cache.dim) * 4) : 0;
+  f.splits = (int)min(max(want / groups, 1l), min(keys / kLeastKeys + 1, 256l));
+  if (f.splits > 1)
+    f.bytes = 4 * (size_t)(joined_floats(f.tiles, p.cache.heads) + groups * f.splits * part_floats(of, p.cache.dim));
   return f;
 }
 
@@ -461,7 +491,7 @@ hipError_t launch_attention(AttentionParams p, hipStream_t stream) {
   const AttentionForm f = attention_form(p);
   p.tiles = (int)f.tiles;
   p.splits = f.splits;
-  p.chunk = f.chunk;
+  p.form = f.form;
   if (p.cache.dim == 64)
     start<64>(p, stream);
   else if (p.cache.dim == 128)

@@ -82,11 +82,17 @@ __device__ __forceinline__ bool find_tile(const AttentionParams& p, int group, i
     Sequence mine = {0, 0, 0};
     if (base + lane < p.batch.sequences) mine = sequence(p.batch, base + lane, p.rows);
     const int tiles = (int)(((long)mine.count * group + rows - 1) / rows);
-    int sum = tiles;
+    int sum;  // of the tiles up to this lane's
+    if (!__any(tiles > 1)) {
+      const unsigned long long some = __ballot(tiles != 0);
+      sum = tiles + (int)__builtin_amdgcn_mbcnt_hi((unsigned)(some >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)some, 0u));
+    } else {
+      sum = tiles;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int below = __shfl_up(sum, o);
-      if (lane >= o) sum += below;
+      for (int o = 1; o < 64; o <<= 1) {
+        const int below = __shfl_up(sum, o);
+        if (lane >= o) sum += below;
+      }
     }
     const int all = __builtin_amdgcn_readlane(sum, 63);
     if (id < all) {
@@ -137,8 +143,22 @@ __device__ __forceinline__ Walk walk_of(const AttentionParams& p, const Sequence
   return w;
 }
 
-// Workspace of a split: per (tile, head of the cache, split) the rows' maxima and sums, then their results.
+// Workspace of a split: per (tile, head of the cache) what the parts are of, then per (tile, head, split) the rows'
+// maxima and sums and their results.
+struct Joined {
+  int splits, first, row, rows;  // parts; the sequence's first row of the call; the tile's first and its number of rows
+};
 __host__ __device__ constexpr long part_floats(int rows, int dim) { return (long)rows * (dim + 2); }
+__host__ __device__ constexpr long joined_floats(long tiles, int heads) { return tiles * heads * 4; }
+__device__ __forceinline__ float* part_of(const AttentionParams& p, int tile, int head, int split, int rows, int dim) {
+  const long at = ((long)tile * p.cache.heads + head) * p.splits + split;
+  return p.parts + joined_floats(p.tiles, p.cache.heads) + at * part_floats(rows, dim);
+}
+// By the first workgroup of every (tile, head), also where there is no tile (rows 0).
+__device__ __forceinline__ void note_tile(const AttentionParams& p, int tile, int head, int split, Joined j) {
+  if (p.splits > 1 && split == 0 && threadIdx.x == 0)
+    reinterpret_cast<Joined*>(p.parts)[(long)tile * p.cache.heads + head] = j;
+}
 
 }  // namespace paged
 }  // namespace ancha

@@ -1,12 +1,14 @@
 // Attention of many new tokens over a paged, microscaled cache (gfx950): chunks and whole prompts. The operation and its
-// operands are those of paged_attention.hip; here 128 or 256 query rows share the keys that a workgroup reads.
+// operands are those of paged_attention.hip; here 128 or 256 query rows share
+// the keys that a workgroup reads. Heads of 64 or 128 columns.
 #include "paged_attention.hpp"
 
 namespace ancha {
 namespace paged {
 namespace {
 
-constexpr int kBuffers = 3;  // steps of keys and values in LDS
+constexpr int kBuffers = 3;         // steps of keys and values in LDS
+constexpr int kKeys = kChunkKeys;  // of a step
 
 __device__ __forceinline__ f32x16 mfma32_bf16(u32x4 a, u32x4 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
@@ -24,34 +26,31 @@ struct Shape {
   static constexpr int kQ = TYPE == kBf16 ? 1 : TYPE == kF16 ? 2 : 3;  // bf16 parts of a query
   static constexpr int kP = TYPE == kF32 ? 2 : 1;                      // fp16 parts of a weight
   static constexpr int kWaves = chunk_waves(D, TYPE), kThreads = 64 * kWaves, kRows = 32 * kWaves;
-  static constexpr int kKeys = D == 256 ? 32 : 64;      // of a step
   static constexpr int kScales = D / kBlock;            // scale bytes a token
   static constexpr int kBuffer = 2 * kKeys * D * 2;     // LDS bytes of a step's keys and values
   // A wave's own: the powers of two of a step's values, and for every buffer which blocks of a token are NaN.
-  static constexpr int kPowers = kKeys * kScales * 4, kPrivate = kPowers + kBuffers * 64;
+  static constexpr int kPowers = kKeys * kScales * 4, kPrivate = kPowers + kBuffers * kKeys;
   static constexpr int kLds = kBuffers * kBuffer + kWaves * kPrivate;
 };
 
-// A workgroup has 32 query rows a wave and walks over the keys in steps of 64 (32): its threads bring a step's codes to
+// A workgroup has 32 query rows a wave and walks over the keys in steps of 64: its threads bring a step's codes to
 // bf16 (keys) and fp16 (values) once and leave them in LDS in the order in which the matrix instructions take them, two
 // steps ahead. With l = 32 h + r, a lane has
 //   scores   element 4 q + e: key 8 q + 4 h + e of 32 for row r (K . Q^T), so the weights are the operand of V^T . P
 //            as they are, if V's keys come in the same order: 16 s + 4 h + (0..3) and 8 further on,
 //   sums     element 4 q + e of block b: column 32 b + 8 q + 4 h + e of row r.
-// A block of 32 columns is one of the cache's own, so its reference power is one number a workgroup. The scores of the
-// next 32 keys are multiplied beside the exponentials of these.
+// A block of 32 columns is one of the cache's own, so its reference power is one number a workgroup.
 template <int D, int FORMAT, int TYPE>
 __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void chunk_kernel(AttentionParams p) {
   typedef typename Stored<TYPE>::type T;
   typedef Shape<D, FORMAT, TYPE> S;
   constexpr int kQ = S::kQ, kP = S::kP, kScales = S::kScales, kRow = row_bytes(D, FORMAT);
-  constexpr int kKeys = S::kKeys, kHalves = kKeys / 32, kWaves = S::kWaves, kThreads = S::kThreads;
+  constexpr int kWaves = S::kWaves, kThreads = S::kThreads;
   // As many blocks of keys as groups of eight values x four columns: one of each a thread, or half the waves have either.
   constexpr int kUnits = kKeys * kScales;
   static_assert(kUnits == kThreads || 2 * kUnits == kThreads, "a unit a thread");
   constexpr bool kApart = kUnits < kThreads;
   constexpr int kBlockWords = FORMAT == kFp8 ? 8 : 4;
-  constexpr int kScaleWords = (kScales + 3) / 4;
   constexpr int kTurn = 8 / kScales;                                             // see slot_of_key
   constexpr int kMost = FORMAT == kFp8 ? 7 : 13, kTaken = FORMAT == kFp8 ? 4 : 9;  // see paged_attention.hip
   constexpr int kNoRef = -1000;
@@ -66,11 +65,13 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
   const int tile = id, split = in_head % p.splits;
   Sequence s;
   if (!find_tile(p, group, S::kRows, id, i, s, row)) {
+    note_tile(p, tile, head, split, {0, 0, 0, 0});
     clear_rows<T>(p, (id * p.cache.heads + head) * p.splits + split,
                   (p.tiles - (tile - id)) * p.cache.heads * p.splits);
     return;
   }
   const Walk w = walk_of(p, s, group, row, S::kRows, kKeys);
+  note_tile(p, tile, head, split, {w.splits, s.first, row, min(S::kRows, s.count * group - row)});
   if (split >= w.splits) return;
   const int begin = split * w.each, end = min(w.steps, begin + w.each);  // steps of this workgroup
   const int thread = threadIdx.x, lane = thread & 63, h = lane >> 5, r = lane & 31;
@@ -135,17 +136,17 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
     int scale, key, value;
   };
   struct Raw {
-    unsigned k[kBlockWords], v[8], vs[kScaleWords], ks;
+    unsigned k[kBlockWords], v[8], vs, ks;
     int page;  // of key `lane`
   };
   const auto fetch_pages = [&](int key, Pages& g) {
-    g.scale = page_at(key + lane % kKeys);
+    g.scale = page_at(key + lane);
     if (has_key) g.key = page_at(key + my_key);
     if (has_value) g.value = page_at(key + 16 * (half / 2));
   };
   const auto fetch = [&](int key, const Pages& g, Raw& w) {
-    w.vs[0] = 0;
-    __builtin_memcpy(w.vs, p.cache.scales + (slot_at(g.scale, key + lane % kKeys) + values) * kScales, kScales);
+    w.vs = 0;
+    __builtin_memcpy(&w.vs, p.cache.scales + (slot_at(g.scale, key + lane) + values) * kScales, kScales);
     w.page = g.scale;
     if (has_key) {
       const long at = slot_at(g.key, key + my_key);
@@ -174,7 +175,7 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
 #pragma unroll
   for (int c = 0; c < kScales; c++) sum_ref[c] = next_ref[c] = ref[c] = kNoRef;
   // Tokens that are there and whether any of them has a NaN among its values, in the same order.
-  constexpr unsigned long long kAll = kKeys == 64 ? ~0ull : ~0ull >> 32;
+  constexpr unsigned long long kAll = ~0ull;
   unsigned long long there = 0, next_there = 0, last_there = 0;
   bool bad = false, next_bad = false, last_bad = false;
 
@@ -185,13 +186,13 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
     uint8_t* const keys = lds + to * S::kBuffer;
     uint8_t* const vals = keys + kKeys * D * 2;
     const int at_key = key + lane;
-    const bool here = lane < kKeys && (unsigned)w_.page < (unsigned)p.cache.pages && at_key >= w.first && at_key < w.high;
+    const bool here = (unsigned)w_.page < (unsigned)p.cache.pages && at_key >= w.first && at_key < w.high;
     last_there = __ballot(here);
     int e[kScales];
     bool over = false;  // a block that is larger than its reference allows, or NaN
 #pragma unroll
     for (int c = 0; c < kScales; c++) {
-      e[c] = here ? (int)(w_.vs[c / 4] >> 8 * (c % 4) & 255u) : 0;
+      e[c] = here ? (int)(w_.vs >> 8 * c & 255u) : 0;
       over |= e[c] > ref[c] + kMost;
     }
     last_bad = false;
@@ -208,9 +209,9 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
         ref[c] = x > ref[c] + kMost ? x - kTaken : ref[c];
       }
       last_bad = __any(nan != 0);
-      mine[S::kPowers + to * 64 + lane] = nan;
+      mine[S::kPowers + to * kKeys + lane] = nan;
     }
-    if (has_value && lane < kKeys) {
+    if (has_value) {
 #pragma unroll
       for (int c = 0; c < kScales; c++)
         powers[c * kKeys + lane] = __builtin_bit_cast(float, (unsigned)max(e[c] - ref[c] + 127, 0) << 23);
@@ -293,7 +294,6 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
     }
   }
   __syncthreads();
-  f32x16 x = zero;
   for (int step = begin, from = 0; step < end; step++) {
     const int key = key_at(step), after = from == 2 ? 0 : from + 1, last = after == 2 ? 0 : after + 1;
     there = next_there, bad = next_bad;
@@ -314,10 +314,10 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
     const uint8_t* const vals = lds + from * S::kBuffer + kKeys * D * 2 + slot_of_value(lane) * 16;
     const bool active = step >= wave_begin && step < wave_end;
     const bool plain = there == kAll && key >= wave_last.low && key + kKeys <= wave_first.high;
-    if (step == wave_begin) x = scores(from, 0);
 #pragma unroll
-    for (int u = 0; u < kHalves; u++) {
+    for (int u = 0; u < 2; u++) {
       if (active) {
+        f32x16 x = scores(from, u);
         unsigned sees = 0x0f0f0f0fu;  // bit 8 q + e: whether the row sees the key of element 4 q + e
         if (!plain) {
           asm volatile("");
@@ -332,7 +332,7 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
         if (bad) {
 #pragma unroll
           for (int j = 0; j < 16; j++) {
-            const unsigned nan = mine[S::kPowers + from * 64 + 32 * u + j / 4 * 8 + 4 * h + j % 4];
+            const unsigned nan = mine[S::kPowers + from * kKeys + 32 * u + j / 4 * 8 + 4 * h + j % 4];
             none |= sees >> (j / 4 * 8 + j % 4) & 1u ? nan : 0u;
           }
         }
@@ -350,7 +350,6 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
           for (int c = 0; c < kScales; c++) acc[c] *= f;
         }
         const float base = m == -__builtin_inff() ? 0.f : kUp - m;
-        const f32x16 ahead = u + 1 < kHalves ? scores(from, u + 1) : scores(after, 0);
         u32x4 weight[kP][2];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
@@ -368,7 +367,6 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
             l += b;
           }
         }
-        x = ahead;
 #pragma unroll
         for (int v = 0; v < 2; v++)
 #pragma unroll
@@ -395,7 +393,7 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
   const float nan = hidden_nan();
   if (met && !(sum > 0.f)) sum = nan;  // nothing but scores of minus infinity
   const float over = sum == 0.f ? 0.f : 1.f / sum;
-  float* const part = p.parts + (((long)tile * p.cache.heads + head) * p.splits + split) * part_floats(S::kRows, D);
+  float* const part = part_of(p, tile, head, split, S::kRows, D);
   if (w.splits > 1 && h == 0) {
     part[32 * wave + r] = m;
     part[S::kRows + 32 * wave + r] = sum;
@@ -421,7 +419,6 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
 template <int D, int FORMAT, int TYPE>
 void start(const AttentionParams& p, hipStream_t stream) {
   typedef Shape<D, FORMAT, TYPE> S;
-  static_assert(S::kRows == chunk_rows(D, TYPE) && S::kKeys == chunk_keys(D), "the form's own numbers");
   hipLaunchKernelGGL((chunk_kernel<D, FORMAT, TYPE>), dim3((unsigned)((long)p.tiles * p.cache.heads * p.splits)),
                      dim3(S::kThreads), S::kLds, stream, p);
 }
@@ -446,10 +443,8 @@ void start_format(const AttentionParams& p, hipStream_t stream) {
 void launch_chunk(const AttentionParams& p, hipStream_t stream) {
   if (p.cache.dim == 64)
     start_format<64>(p, stream);
-  else if (p.cache.dim == 128)
-    start_format<128>(p, stream);
   else
-    start_format<256>(p, stream);
+    start_format<128>(p, stream);
 }
 
 }  // namespace paged

@@ -3,8 +3,10 @@ before a launch."""
 import ctypes
 import math
 import os
+import re
 import subprocess
 import sys
+import tempfile
 import textwrap
 
 import numpy as np
@@ -14,6 +16,7 @@ import torch
 from ancha_amd import _native, paged
 from oracle import mx as OM
 from oracle import paged as O
+from tests.test_wide_stores import OBJDUMP, code_objects
 
 
 @pytest.fixture(scope="module")
@@ -207,6 +210,28 @@ def test_wrappers_reject_host_tensors_and_names():
                        (lambda: paged.Rotary(torch.ones(4), "pairs"), "layout")):
         with pytest.raises(ValueError, match=text):
             call()
+
+
+def test_kernels_keep_their_registers():
+    """No kernel of the paged operators spills. (Where a group of sixteen accumulation registers is spilled in parts,
+    this compiler has been seen to leave one of them out when it brings the group back.)"""
+    readelf = os.path.join(os.path.dirname(OBJDUMP), "llvm-readelf")
+    if not os.path.exists(readelf):
+        pytest.skip("llvm-readelf is not installed")
+    found = 0
+    for code in code_objects(_native.LIB_PATH):
+        if b"paged" not in code:
+            continue
+        with tempfile.NamedTemporaryFile(suffix=".co") as f:
+            f.write(code)
+            f.flush()
+            notes = subprocess.run([readelf, "--notes", f.name], capture_output=True, text=True, check=True).stdout
+        for kernel in notes.split("- .agpr_count:")[1:]:
+            name = re.search(r"\.name:\s+(\S+)", kernel)[1]
+            found += 1
+            for what in ("vgpr_spill_count", "sgpr_spill_count", "private_segment_fixed_size"):
+                assert int(re.search(rf"\.{what}:\s+(\d+)", kernel)[1]) == 0, f"{name}: {what}"
+    assert found > 40
 
 
 _CHILD = textwrap.dedent("""

@@ -49,7 +49,8 @@ def rounding(want, dtype):
 def close(name, got, want, tol):
     got = host(got)
     assert got.shape == want.shape, f"{name}: shape {got.shape}, expected {want.shape}"
-    assert np.array_equal(np.isnan(got), np.isnan(want)), f"{name}: NaN in other places"
+    other = np.argwhere(np.isnan(got) != np.isnan(want))
+    assert not len(other), f"{name}: NaN in {len(other)} other places, the first {other[0]}"
     with np.errstate(invalid="ignore"):
         off = np.nan_to_num(np.abs(got - want), nan=0.0) / np.nan_to_num(np.broadcast_to(tol, want.shape), nan=1.0)
     worst = off.max(initial=0.0)
