@@ -76,7 +76,7 @@ SIGNATURES = {
     "ancha_paged_rotary": (_int, [_p, _int, _sz, _sz, _sz, _sz, _sz, _p, _int, _p, _p, _p, _p]),
     "ancha_paged_write": (_int, [_p, _p, _int, _sz, _sz, _sz, _sz, _sz, _p, _p, _p, _p]),
     "ancha_paged_read": (_int, [_p, _p, _sz, _int, _p, _p, _p]),
-    "ancha_paged_attention_workspace": (_sz, [_sz, _sz, _p, _p]),
+    "ancha_paged_attention_workspace": (_sz, [_int, _sz, _sz, _p, _p]),
     "ancha_paged_attention": (_int, [_p, _int, _sz, _sz, _sz, _sz, _p, _p, ctypes.c_double, _int, _sz, _p, _sz,
                                      _p, _p]),
     "ancha_hip_check": (_int, []),

@@ -49,22 +49,19 @@ __device__ __forceinline__ Sequence sequence(const Batch& b, int i, int rows) {
   return {from, to - from, max(b.lengths[i], 0)};
 }
 
-// The sequence that row r is of, and its position (false: of none).
+// The sequence that row r is of, and its position (false: of none); a wave's lanes look together, r is the same in all.
 __device__ __forceinline__ bool place(const Batch& b, int r, int& i, int& position) {
-  int low = 0, high = b.sequences;  // starts[low] <= r < starts[high], if r is of a sequence
-  if (high == 0) return false;
-  while (high - low > 1) {
-    const int mid = low + (high - low) / 2;
-    if (b.starts[mid] <= r)
-      low = mid;
-    else
-      high = mid;
+  const int lane = threadIdx.x & 63;
+  i = 0;  // starts[i] <= r < starts[i + 1], if r is of a sequence: as many ends as are not behind r
+  for (int base = 0; base < b.sequences; base += 64) {
+    const int more = __popcll(__ballot(base + lane < b.sequences && b.starts[base + lane + 1] <= r));
+    i += more;
+    if (more < 64) break;
   }
-  const int from = b.starts[low], to = b.starts[low + 1];
-  if (r < from || r >= to) return false;
-  i = low;
-  position = max(b.lengths[low], 0) - (to - r);
-  return true;
+  if (i >= b.sequences) return false;
+  const int from = b.starts[i], to = b.starts[i + 1];
+  position = max(b.lengths[i], 0) - (to - r);
+  return r >= from && r < to;
 }
 
 // The page that holds the token at `position` >= 0 of sequence i, or -1.
@@ -122,10 +119,8 @@ struct AttentionParams {
   long ldq, ldqh;
   int rows, heads, type, causal, window;  // window 0: none
   float scale;                            // of the scores, times log2(e)
-  int tiles, splits, form;                // of attention_form
+  int tiles, splits, form;                // of its AttentionForm
 };
-hipError_t launch_attention(AttentionParams p, hipStream_t stream);
-void launch_chunk(const AttentionParams& p, hipStream_t stream);
 
 // How a call is laid out: tiles of 16 query rows by four or eight waves, or the chunk kernel's; tiles (an upper bound,
 // the kernels count the real ones); the workgroups that share the keys of a tile; bytes of workspace.
@@ -136,7 +131,9 @@ struct AttentionForm {
   int splits;
   size_t bytes;
 };
-AttentionForm attention_form(const AttentionParams& p);
+AttentionForm attention_form(const AttentionParams& p);  // of the type, the sizes and the batch's
+hipError_t launch_attention(AttentionParams p, const AttentionForm& form, hipStream_t stream);
+void launch_chunk(const AttentionParams& p, hipStream_t stream);
 
 // The chunk kernel takes heads of 64 or 128 columns; its waves have 32 query rows each and walk in steps of kChunkKeys.
 // (fp32 queries of 128 columns are 96 registers in three parts, which leaves room for one wave a SIMD.)

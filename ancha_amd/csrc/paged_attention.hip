@@ -381,53 +381,51 @@ __global__ __launch_bounds__(64 * WAVES) void attention_kernel(AttentionParams p
   }
 }
 
-// The parts of split tiles of `rows` rows joined: a wave a row.
+// The parts of split tiles of `rows` rows joined: D / 4 lanes a row, four columns each, which also share the parts'
+// maxima and sums.
 template <int D, int TYPE>
 __global__ __launch_bounds__(256) void join_kernel(AttentionParams p, int rows) {
-  constexpr int N = D / 64;
+  constexpr int kLanes = D / 4, kRows = 256 / kLanes;  // of a workgroup, all in one tile
   const long kPart = part_floats(rows, D);
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-  const int r = wave % rows, at = wave / rows, head = at % p.cache.heads;
+  const int lane = threadIdx.x % kLanes;
+  const int at = blockIdx.x * kRows / rows, r = blockIdx.x * kRows % rows + threadIdx.x / kLanes;
+  const int head = at % p.cache.heads;
   const Joined w = reinterpret_cast<const Joined*>(p.parts)[at];
   if (r >= w.rows || w.splits == 1) return;
   const float* parts = part_of(p, at / p.cache.heads, head, 0, rows, D);
   float top = -__builtin_inff();
-  for (int j = lane; j < w.splits; j += 64) top = fmaxf(top, parts[j * kPart + r]);
+  for (int j = lane; j < w.splits; j += kLanes) top = fmaxf(top, parts[j * kPart + r]);
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+  for (int o = 1; o < kLanes; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
   const auto share = [&](int j) {
     const float m = parts[j * kPart + r];
     return (m == -__builtin_inff() ? 0.f : fast_exp2(m - top)) * parts[j * kPart + rows + r];
   };
-  float sum = 0.f, v[N];
-  for (int j = lane; j < w.splits; j += 64) sum += share(j);
+  float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int j = lane; j < w.splits; j += kLanes) sum += share(j);
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
+  for (int o = 1; o < kLanes; o <<= 1) sum += __shfl_xor(sum, o);
   const float over = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-  for (int n = 0; n < N; n++) v[n] = 0.f;
-  for (int base = 0; base < w.splits; base += 64) {
+  for (int base = 0; base < w.splits; base += kLanes) {
     const float weight = base + lane < w.splits ? share(base + lane) * over : 0.f;
-    const int count = min(64, w.splits - base);
+    const int count = min(kLanes, w.splits - base);
     for (int j = 0; j < count; j += 8) {  // eight reads in flight; behind the last part its own again, without weight
-      float o[8][N];
+      float o[8][4];
 #pragma unroll
       for (int k = 0; k < 8; k++)
-        __builtin_memcpy(o[k], parts + (base + min(j + k, count - 1)) * kPart + 2 * rows + r * D + lane * N,
-                         sizeof(o[k]));
+        __builtin_memcpy(o[k], parts + (base + min(j + k, count - 1)) * kPart + 2 * rows + r * D + lane * 4, 16);
 #pragma unroll
       for (int k = 0; k < 8; k++) {
-        const float f = __shfl(weight, min(j + k, 63));
+        const float f = __shfl(weight, min(j + k, kLanes - 1), kLanes);
         if (j + k < count)
 #pragma unroll
-          for (int n = 0; n < N; n++) v[n] = __builtin_fmaf(f, o[k][n], v[n]);
+          for (int n = 0; n < 4; n++) v[n] = __builtin_fmaf(f, o[k][n], v[n]);
       }
     }
   }
   const int group = p.heads / p.cache.heads, token = (w.row + r) / group;
   const int at_head = head * group + w.row + r - token * group;
-  store_row<TYPE, N>(p.out, ((long)(w.first + token) * p.heads + at_head) * D + lane * N, N, v);
+  store_row<TYPE, 4>(p.out, ((long)(w.first + token) * p.heads + at_head) * D + lane * 4, 4, v);
 }
 
 template <int D, int FORMAT, int WAVES>
@@ -458,7 +456,7 @@ void start(const AttentionParams& p, hipStream_t stream) {
     start_format<D, kFp4>(p, stream);
   if (p.splits == 1) return;
   const int rows = p.form == kChunk ? chunk_rows(D, p.type) : kTile;
-  const dim3 grid((unsigned)((long)p.tiles * p.cache.heads * rows / 4)), block(256);
+  const dim3 grid((unsigned)((long)p.tiles * p.cache.heads * rows * (D / 4) / 256)), block(256);
   if (p.type == kF32)
     hipLaunchKernelGGL((join_kernel<D, kF32>), grid, block, 0, stream, p, rows);
   else if (p.type == kF16)
@@ -487,8 +485,7 @@ AttentionForm attention_form(const AttentionParams& p) {
   return f;
 }
 
-hipError_t launch_attention(AttentionParams p, hipStream_t stream) {
-  const AttentionForm f = attention_form(p);
+hipError_t launch_attention(AttentionParams p, const AttentionForm& f, hipStream_t stream) {
   p.tiles = (int)f.tiles;
   p.splits = f.splits;
   p.form = f.form;

@@ -165,13 +165,14 @@ int ancha_paged_read(const ancha_paged_cache* cache, const ancha_paged_batch* ba
   return e == hipSuccess ? ANCHA_HIP_OK : hip_fail(e, who);
 }
 
-size_t ancha_paged_attention_workspace(size_t rows, size_t heads, const ancha_paged_cache* cache,
+size_t ancha_paged_attention_workspace(int type, size_t rows, size_t heads, const ancha_paged_cache* cache,
                                        const ancha_paged_batch* batch) {
   paged::AttentionParams p{};
-  if (!cache || !batch || !cache->heads || !heads || heads % cache->heads || rows == 0 || rows > kIntMax ||
+  if (!is_type(type) || !cache || !batch || !cache->heads || !heads || heads % cache->heads || rows == 0 || rows > kIntMax ||
       heads > kIntMax || rows * heads > kIntMax || cache->page < 16 || cache->page > 65536 ||
       batch->sequences >= kIntMax || batch->columns > kIntMax)
     return 0;
+  p.type = type;
   p.rows = static_cast<int>(rows);
   p.heads = static_cast<int>(heads);
   p.cache.heads = static_cast<int>(cache->heads);
@@ -200,6 +201,7 @@ int ancha_paged_attention(const void* q, int type, size_t rows, size_t heads, si
   if (!q || !out) return fail(ANCHA_HIP_INVALID, who + ": null tensor");
   if (rows > kIntMax || heads > 65536 || rows * heads > kIntMax || !strides_fit(rows, ldq, heads, ldqh))
     return fail(ANCHA_HIP_UNSUPPORTED, who + ": too many rows or heads");
+  p.type = type;
   p.rows = static_cast<int>(rows);
   p.heads = static_cast<int>(heads);
   const paged::AttentionForm form = paged::attention_form(p);
@@ -214,11 +216,10 @@ int ancha_paged_attention(const void* q, int type, size_t rows, size_t heads, si
   p.parts = static_cast<float*>(workspace);
   p.ldq = static_cast<long>(ldq);
   p.ldqh = static_cast<long>(ldqh);
-  p.type = type;
   p.causal = causal ? 1 : 0;
   p.window = static_cast<int>(window < kIntMax ? window : 0);
   p.scale = static_cast<float>(scale * 1.4426950408889634);
-  const hipError_t e = paged::launch_attention(p, stream);
+  const hipError_t e = paged::launch_attention(p, form, stream);
   return e == hipSuccess ? ANCHA_HIP_OK : hip_fail(e, who);
 }
 

@@ -9,7 +9,8 @@ namespace {
 using namespace mx;
 
 constexpr int kThreads = 256;
-constexpr int kTrig = 1024;  // angles of a workgroup's rows
+constexpr int kTrig = 1024;     // angles of a workgroup's rows
+constexpr int kMostRows = 64;   // of a workgroup
 
 // cos and sin of angle a to fp32: the multiple of a right angle is taken off in 64 bits, so far positions lose nothing.
 __device__ __forceinline__ float2 cos_sin(double a) {
@@ -22,85 +23,110 @@ __device__ __forceinline__ float2 cos_sin(double a) {
   return make_float2(turn == 1 || turn == 2 ? -x : x, turn & 2 ? -y : y);
 }
 
+// Threads for the rotated columns of a head, V values at a time.
+template <bool HALF>
+__host__ __device__ constexpr int turned_units(int pairs, int V) {
+  return ((HALF ? pairs : 2 * pairs) + V - 1) / V;
+}
+
 // Rows of heads at their positions. A workgroup has `rows` rows: their cosines and sines once, into LDS, then all of
-// the heads' pairs, as many a thread as 16 bytes hold (HALF: from two places of the head, otherwise neighbours);
-// columns behind the rotated ones are copied as they are. Bound by memory.
+// the heads' columns, 16 bytes a thread (HALF: of both halves), so that an instruction of a wave writes one piece of
+// memory; columns behind the rotated ones are copied as they are. The first values are on their way while the angles
+// are taken. Bound by memory.
 template <int TYPE, bool HALF>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryParams p, int rows, Divide by_row, Divide by_head) {
   constexpr int V = 16 / (int)sizeof(typename Stored<TYPE>::type);
   __shared__ float2 trig[kTrig];
-  __shared__ int of_none[kThreads];
+  __shared__ long at_row[kMostRows];
+  __shared__ bool of_none[kMostRows];
   const int pairs = p.plan.width / 2;
   const long first = (long)blockIdx.x * rows;
   const int mine = (int)min((long)rows, p.rows - first);
-  for (int i = threadIdx.x; i < mine * pairs; i += kThreads) {
-    const int r = i / pairs, j = i - r * pairs;
-    long at;
-    bool there = true;
-    if (p.positions) {
-      at = p.wide ? static_cast<const long*>(p.positions)[first + r] : static_cast<const int*>(p.positions)[first + r];
-    } else {
-      int s, position = 0;
-      there = place(p.batch, (int)first + r, s, position);
-      at = position;
+  const int turned = turned_units<HALF>(pairs, V), units = turned + (p.dim - p.plan.width + V - 1) / V;  // of a head
+  const int total = mine * p.heads * units;
+  struct Unit {
+    int row, u, col_a, col_b, valid_a, valid_b;
+    long from, to;
+    float a[V], b[V];
+  };
+  const auto load = [&](int i, Unit& x) {
+    x.row = (int)divided(i, by_row);
+    const int in_row = i - x.row * p.heads * units;
+    const int head = (int)divided(in_row, by_head);
+    x.u = in_row - head * units;
+    x.from = (first + x.row) * p.ld + head * p.ldh, x.to = ((first + x.row) * p.heads + head) * p.dim;
+    const bool copied = x.u >= turned;
+    x.col_a = copied ? p.plan.width + (x.u - turned) * V : x.u * V;
+    x.valid_a = (copied ? p.dim : HALF ? pairs : p.plan.width) - x.col_a;
+    x.col_b = HALF && !copied ? pairs + x.col_a : x.col_a;
+    x.valid_b = HALF && !copied ? x.valid_a : 0;  // 0: nothing is read or written there
+    load_row<TYPE, V>(p.x, x.from + x.col_a, x.valid_a, x.a);
+    load_row<TYPE, V>(p.x, x.from + x.col_b, x.valid_b, x.b);
+  };
+  Unit x;
+  if ((int)threadIdx.x < total) load(threadIdx.x, x);
+  if (p.positions) {
+    if ((int)threadIdx.x < mine) {
+      const long r = first + threadIdx.x;
+      at_row[threadIdx.x] = p.wide ? static_cast<const long*>(p.positions)[r] : static_cast<const int*>(p.positions)[r];
+      of_none[threadIdx.x] = false;
     }
-    const float2 t = cos_sin((double)at * p.plan.freqs[j]);
-    const float m = (float)p.plan.magnitude;
-    trig[i] = make_float2(m * t.x, m * t.y);
-    if (j == 0) of_none[r] = !there;
+  } else {
+    for (int r = threadIdx.x / 64; r < mine; r += kThreads / 64) {
+      int s, position = 0;
+      const bool there = place(p.batch, (int)first + r, s, position);
+      at_row[r] = position;
+      of_none[r] = !there;
+    }
   }
   __syncthreads();
-  const int turned = (pairs + V - 1) / V, rest = p.dim - p.plan.width;
-  const int units = turned + (rest + 2 * V - 1) / (2 * V);  // of a head
-  const int total = mine * p.heads * units;
-  for (int i = threadIdx.x; i < total; i += kThreads) {
-    const int r = (int)divided(i, by_row), in_row = i - r * p.heads * units;
-    const int head = (int)divided(in_row, by_head), u = in_row - head * units;
-    const long from = (first + r) * p.ld + head * p.ldh, to = ((first + r) * p.heads + head) * p.dim;
-    float a[V], b[V];
-    int col_a, col_b, valid_a, valid_b;
-    if (u >= turned) {
-      const int at = (u - turned) * 2 * V;
-      col_a = p.plan.width + at, valid_a = rest - at;
-      col_b = col_a + V, valid_b = valid_a - V;
-    } else if (HALF) {
-      col_a = u * V, col_b = pairs + col_a;
-      valid_a = valid_b = pairs - col_a;
-    } else {
-      col_a = 2 * V * u, col_b = col_a + V;
-      valid_a = p.plan.width - col_a, valid_b = valid_a - V;
-    }
-    if (valid_b <= 0) col_b = col_a;  // nothing is read or written there
-    load_row<TYPE, V>(p.x, from + col_a, valid_a, a);
-    load_row<TYPE, V>(p.x, from + col_b, valid_b, b);
-    if (u < turned) {
-      const float2* t = trig + r * pairs + u * V;
+  for (int i = threadIdx.x; i < mine * pairs; i += kThreads) {
+    const int r = i / pairs;
+    const float2 t = cos_sin((double)at_row[r] * p.plan.freqs[i - r * pairs]);
+    const float m = (float)p.plan.magnitude;
+    trig[i] = make_float2(m * t.x, m * t.y);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < total;) {
+    if (x.u < turned) {
+      constexpr int kPairs = HALF ? V : V / 2;
+      const float2* t = trig + x.row * pairs + x.u * kPairs;
 #pragma unroll
-      for (int j = 0; j < V; j++) {
-        if (u * V + j >= pairs) break;
+      for (int j = 0; j < kPairs; j++) {
+        if (x.u * kPairs + j >= pairs) break;
         const float2 cs = t[j];
-        float& x = HALF ? a[j] : j < V / 2 ? a[2 * j] : b[2 * j - V];
-        float& y = HALF ? b[j] : j < V / 2 ? a[2 * j + 1] : b[2 * j + 1 - V];
-        const float x0 = x;
-        x = __builtin_fmaf(x0, cs.x, -(y * cs.y));
-        y = __builtin_fmaf(y, cs.x, x0 * cs.y);
+        float& y0 = HALF ? x.a[j] : x.a[2 * j];
+        float& y1 = HALF ? x.b[j] : x.a[2 * j + 1];
+        const float y = y0;
+        y0 = __builtin_fmaf(y, cs.x, -(y1 * cs.y));
+        y1 = __builtin_fmaf(y1, cs.x, y * cs.y);
       }
     }
-    if (of_none[r])
+    if (of_none[x.row])
 #pragma unroll
-      for (int j = 0; j < V; j++) a[j] = b[j] = 0.f;
-    store_row<TYPE, V>(p.out, to + col_a, valid_a, a);
-    store_row<TYPE, V>(p.out, to + col_b, valid_b, b);
+      for (int j = 0; j < V; j++) x.a[j] = x.b[j] = 0.f;
+    store_row<TYPE, V>(p.out, x.to + x.col_a, x.valid_a, x.a);
+    store_row<TYPE, V>(p.out, x.to + x.col_b, x.valid_b, x.b);
+    i += kThreads;
+    if (i < total) load(i, x);
   }
 }
 
 // Eight columns from col on of a key, rotated in 64 bits: the rounding to the codes is the only one. x: the columns
-// themselves, `row` the key's first value, trig those of the row's pairs.
-template <int TYPE>
-__device__ __forceinline__ void turn_key(const Plan& plan, const typename Stored<TYPE>::type* row, int col,
-                                         const double2* trig, float* x) {
+// themselves, other: for HALF the other values of their pairs; trig the pairs of the key's row.
+template <bool HALF>
+__device__ __forceinline__ void turn_key(const Plan& plan, int col, const double2* trig, const float* other, float* x) {
   const int pairs = plan.width / 2;
-  if (plan.interleaved) {
+  if (HALF) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const int d = col + j;
+      if (d >= plan.width) break;
+      const double2 t = trig[d < pairs ? d : d - pairs];
+      const double a = x[j], b = other[j];
+      x[j] = d < pairs ? to_odd(a * t.x - b * t.y) : to_odd(a * t.x + b * t.y);
+    }
+  } else {
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
       if (col + j >= plan.width) break;
@@ -109,72 +135,73 @@ __device__ __forceinline__ void turn_key(const Plan& plan, const typename Stored
       x[j] = to_odd(a * t.x - b * t.y);
       x[j + 1] = to_odd(b * t.x + a * t.y);
     }
-    return;
-  }
-  // The other value of each pair: eight neighbours, unless the eight cross from one half to the other.
-  float other[8];
-  const bool low = col < pairs;
-  if (pairs % 8 == 0) {
-    load_row<TYPE, 8>(row, low ? col + pairs : col - pairs, 8, other);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const int d = col + j;
-      other[j] = d < plan.width ? (float)row[d < pairs ? d + pairs : d - pairs] : 0.f;
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < 8; j++) {
-    const int d = col + j;
-    if (d >= plan.width) break;
-    const double2 t = trig[d < pairs ? d : d - pairs];
-    const double a = x[j], b = other[j];
-    x[j] = d < pairs ? to_odd(a * t.x - b * t.y) : to_odd(a * t.x + b * t.y);
   }
 }
 
 // New keys and values into their pages. A workgroup has `rows` rows: their places and their pairs' cosines and sines
-// once (in 64 bits), then eight columns a thread, four threads a block of codes. Rows without a place are left out.
-template <int TYPE, int FORMAT>
+// once (in 64 bits), then eight columns a thread, four threads a block of codes. Rows without a place are left out. The
+// first values are on their way while the places are found and the angles taken.
+template <int TYPE, int FORMAT, bool HALF>
 __global__ __launch_bounds__(kThreads) void write_kernel(WriteParams p, int rows, Divide by_row) {
-  __shared__ double2 trig[kTrig];
-  __shared__ int2 places[kThreads];  // page (or -1) and slot
+  typedef typename Stored<TYPE>::type T;
+  __shared__ double2 trig[kTrig / 2];
+  __shared__ int2 places[kMostRows];  // page (or -1) and position
   const int pairs = p.plan.freqs ? p.plan.width / 2 : 0;
   const long first = (long)blockIdx.x * rows;
   const int mine = (int)min((long)rows, p.rows - first);
-  for (int r = threadIdx.x; r < mine; r += kThreads) {
+  const int dim = p.cache.dim, heads = p.cache.heads;
+  const int units = dim / 8;  // of a head; a multiple of 4, so a block's threads stay together
+  const int total = mine * 2 * heads * units;
+  struct Unit {
+    int row, which, head, col;
+    float x[8], other[8];
+  };
+  const auto load = [&](int i, Unit& u) {
+    u.row = (int)divided(i, by_row);
+    const int in_row = i - u.row * 2 * heads * units, both = in_row / units;
+    u.col = 8 * (in_row - both * units);
+    u.which = both >= heads, u.head = both - u.which * heads;
+    const T* row = u.which ? static_cast<const T*>(p.v) + (first + u.row) * p.ldv + u.head * p.ldvh
+                           : static_cast<const T*>(p.k) + (first + u.row) * p.ldk + u.head * p.ldkh;
+    load_row<TYPE, 8>(row, u.col, 8, u.x);
+    if (!HALF || u.which || u.col >= 2 * pairs) return;
+    // Eight neighbours, unless the eight cross from one half to the other.
+    if (pairs % 8 == 0) {
+      load_row<TYPE, 8>(row, u.col < pairs ? u.col + pairs : u.col - pairs, 8, u.other);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const int d = u.col + j;
+        u.other[j] = d < 2 * pairs ? (float)row[d < pairs ? d + pairs : d - pairs] : 0.f;
+      }
+    }
+  };
+  Unit u;
+  if ((int)threadIdx.x < total) load(threadIdx.x, u);
+  for (int r = threadIdx.x / 64; r < mine; r += kThreads / 64) {
     int s = 0, position = 0, page = -1;
     if (place(p.batch, (int)first + r, s, position) && position >= 0) page = page_of(p.batch, p.cache, s, position);
-    places[r] = make_int2(page, position & ((1 << p.cache.shift) - 1));
+    places[r] = make_int2(page, position);
   }
+  __syncthreads();
   for (int i = threadIdx.x; i < mine * pairs; i += kThreads) {
     const int r = i / pairs;
-    int s = 0, position = 0;
-    place(p.batch, (int)first + r, s, position);
     double sine, cosine;
-    sincos((double)position * p.plan.freqs[i - r * pairs], &sine, &cosine);
+    sincos((double)places[r].y * p.plan.freqs[i - r * pairs], &sine, &cosine);
     trig[i] = make_double2(p.plan.magnitude * cosine, p.plan.magnitude * sine);
   }
   __syncthreads();
   saturate();
-  const int dim = p.cache.dim, heads = p.cache.heads;
-  const int units = dim / 8;  // of a head; a multiple of 4, so a block's threads stay together
-  const int total = mine * 2 * heads * units;
-  for (int i = threadIdx.x; i < total; i += kThreads) {
-    const int r = (int)divided(i, by_row), in_row = i - r * 2 * heads * units;
-    const int both = in_row / units, col = 8 * (in_row - both * units);
-    const int which = both >= heads, head = both - which * heads;
-    const int2 to = places[r];
-    if (to.x < 0) continue;
-    typedef typename Stored<TYPE>::type T;
-    const T* row = which ? static_cast<const T*>(p.v) + (first + r) * p.ldv + head * p.ldvh
-                         : static_cast<const T*>(p.k) + (first + r) * p.ldk + head * p.ldkh;
-    float x[8];
-    load_row<TYPE, 8>(row, col, 8, x);
-    if (!which && col < 2 * pairs) turn_key<TYPE>(p.plan, row, col, trig + r * pairs, x);
-    const long slot = slot_of(p.cache, which, to.x, head, to.y);
-    store_codes(x, FORMAT, true, p.cache.codes + slot * row_bytes(dim, FORMAT) + (FORMAT == kFp8 ? col : col / 2),
-                p.cache.scales + slot * (dim / kBlock) + col / kBlock);
+  for (int i = threadIdx.x; i < total;) {
+    const int2 to = places[u.row];
+    if (to.x >= 0) {
+      if (!u.which && u.col < 2 * pairs) turn_key<HALF>(p.plan, u.col, trig + u.row * pairs, u.other, u.x);
+      const long slot = slot_of(p.cache, u.which, to.x, u.head, to.y & ((1 << p.cache.shift) - 1));
+      store_codes(u.x, FORMAT, true, p.cache.codes + slot * row_bytes(dim, FORMAT) + (FORMAT == kFp8 ? u.col : u.col / 2),
+                  p.cache.scales + slot * (dim / kBlock) + u.col / kBlock);
+    }
+    i += kThreads;
+    if (i < total) load(i, u);
   }
 }
 
@@ -182,7 +209,7 @@ __global__ __launch_bounds__(kThreads) void write_kernel(WriteParams p, int rows
 template <int TYPE, int FORMAT>
 __global__ __launch_bounds__(kThreads) void read_kernel(ReadParams p, int tokens, Divide by_token) {
   constexpr int N = 16 / (int)sizeof(typename Stored<TYPE>::type);
-  __shared__ int2 places[kThreads];
+  __shared__ int2 places[kMostRows];
   const int blocks = (p.size + tokens - 1) / tokens;
   const int s = blockIdx.x / blocks, first = (int)(blockIdx.x - (unsigned)s * blocks) * tokens;
   const int mine = min(tokens, p.size - first);
@@ -241,7 +268,8 @@ void start_rotary(const RotaryParams& p, hipStream_t stream) {
   const int pairs = p.plan.width / 2;
   // As many rows as fill the workgroup with angles, but two workgroups a CU first.
   const int rows = max(1, min(min(kThreads / pairs, 32), p.rows / 512));
-  const int units = (pairs + V - 1) / V + (p.dim - p.plan.width + 2 * V - 1) / (2 * V);
+  const int turned = p.plan.interleaved ? turned_units<false>(pairs, V) : turned_units<true>(pairs, V);
+  const int units = turned + (p.dim - p.plan.width + V - 1) / V;
   const dim3 grid((unsigned)((p.rows + (long)rows - 1) / rows));
   const Divide by_row = divide_by((long)p.heads * units), by_head = divide_by(units);
   if (p.plan.interleaved)
@@ -250,27 +278,26 @@ void start_rotary(const RotaryParams& p, hipStream_t stream) {
     hipLaunchKernelGGL((rotary_kernel<TYPE, true>), grid, dim3(kThreads), 0, stream, p, rows, by_row, by_head);
 }
 
-template <int TYPE>
+template <int TYPE, int FORMAT>
 void start_write(const WriteParams& p, hipStream_t stream) {
   const int units = 2 * p.cache.heads * p.cache.dim / 8;
   const int rows = max(1, min(min(4, 4096 / units), p.rows / 512));
   const dim3 grid((unsigned)((p.rows + (long)rows - 1) / rows));
-  if (p.cache.format == kFp8)
-    hipLaunchKernelGGL((write_kernel<TYPE, kFp8>), grid, dim3(kThreads), 0, stream, p, rows, divide_by(units));
+  if (p.plan.interleaved)
+    hipLaunchKernelGGL((write_kernel<TYPE, FORMAT, false>), grid, dim3(kThreads), 0, stream, p, rows, divide_by(units));
   else
-    hipLaunchKernelGGL((write_kernel<TYPE, kFp4>), grid, dim3(kThreads), 0, stream, p, rows, divide_by(units));
+    hipLaunchKernelGGL((write_kernel<TYPE, FORMAT, true>), grid, dim3(kThreads), 0, stream, p, rows, divide_by(units));
 }
 
-template <int TYPE>
+template <int TYPE, int FORMAT>
 void start_read(const ReadParams& p, hipStream_t stream) {
   constexpr int N = 16 / (int)sizeof(typename Stored<TYPE>::type);
   const int units = 2 * p.cache.heads * p.cache.dim / N;
-  const int tokens = max(1, min(2048 / units, 64));
+  // Up to eight units a thread, but eight workgroups a CU first.
+  const long all = (long)p.size * p.batch.sequences;
+  const int tokens = (int)max(1l, min(min(2048 / units, kMostRows) + 0l, all / 2048));
   const dim3 grid((unsigned)(((p.size + (long)tokens - 1) / tokens) * p.batch.sequences));
-  if (p.cache.format == kFp8)
-    hipLaunchKernelGGL((read_kernel<TYPE, kFp8>), grid, dim3(kThreads), 0, stream, p, tokens, divide_by(units));
-  else
-    hipLaunchKernelGGL((read_kernel<TYPE, kFp4>), grid, dim3(kThreads), 0, stream, p, tokens, divide_by(units));
+  hipLaunchKernelGGL((read_kernel<TYPE, FORMAT>), grid, dim3(kThreads), 0, stream, p, tokens, divide_by(units));
 }
 
 }  // namespace
@@ -286,22 +313,24 @@ hipError_t launch_rotary(const RotaryParams& p, hipStream_t stream) {
 }
 
 hipError_t launch_write(const WriteParams& p, hipStream_t stream) {
+  const bool fp8 = p.cache.format == kFp8;
   if (p.type == kF32)
-    start_write<kF32>(p, stream);
+    fp8 ? start_write<kF32, kFp8>(p, stream) : start_write<kF32, kFp4>(p, stream);
   else if (p.type == kF16)
-    start_write<kF16>(p, stream);
+    fp8 ? start_write<kF16, kFp8>(p, stream) : start_write<kF16, kFp4>(p, stream);
   else
-    start_write<kBf16>(p, stream);
+    fp8 ? start_write<kBf16, kFp8>(p, stream) : start_write<kBf16, kFp4>(p, stream);
   return hipGetLastError();
 }
 
 hipError_t launch_read(const ReadParams& p, hipStream_t stream) {
+  const bool fp8 = p.cache.format == kFp8;
   if (p.type == kF32)
-    start_read<kF32>(p, stream);
+    fp8 ? start_read<kF32, kFp8>(p, stream) : start_read<kF32, kFp4>(p, stream);
   else if (p.type == kF16)
-    start_read<kF16>(p, stream);
+    fp8 ? start_read<kF16, kFp8>(p, stream) : start_read<kF16, kFp4>(p, stream);
   else
-    start_read<kBf16>(p, stream);
+    fp8 ? start_read<kBf16, kFp8>(p, stream) : start_read<kBf16, kFp4>(p, stream);
   return hipGetLastError();
 }
 

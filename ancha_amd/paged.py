@@ -273,7 +273,7 @@ def attention(q: torch.Tensor, cache: Cache, batch: Batch, scale: Optional[float
     if not rows:
         return out
     q = _heads(q, "q")
-    need = _native.lib().ancha_paged_attention_workspace(rows, heads, cache._at, batch._at)
+    need = _native.lib().ancha_paged_attention_workspace(kind, rows, heads, cache._at, batch._at)
     workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     return out if _launch(device.index, "ancha_paged_attention", q.data_ptr(), kind, rows, heads, q.stride(0),
                           q.stride(1), cache._at, batch._at, scale, int(causal), window or 0,

@@ -398,7 +398,7 @@ int ancha_paged_read(const ancha_paged_cache *cache, const ancha_paged_batch *ba
  * exact to fp32, weights are fp16 (`type` fp32: 22 bits), sums fp32. A NaN in the cache reaches the rows that see it.
  * workspace: ancha_paged_attention_workspace bytes (of the same arguments; may be 0 and NULL), 16-byte aligned, not
  * shared with a call that may run at the same time. */
-size_t ancha_paged_attention_workspace(size_t rows, size_t heads, const ancha_paged_cache *cache,
+size_t ancha_paged_attention_workspace(int type, size_t rows, size_t heads, const ancha_paged_cache *cache,
                                        const ancha_paged_batch *batch);
 int ancha_paged_attention(const void *q, int type, size_t rows, size_t heads, size_t ldq, size_t ldqh,
                           const ancha_paged_cache *cache, const ancha_paged_batch *batch, double scale, int causal,

@@ -182,18 +182,23 @@ def test_entry_points_check_arguments(lib):
     refused(attention(rows=1 << 30), UNS, "too many")
     refused(attention(rows=1 << 26, heads=16), UNS, "too many")
     assert attention(rows=0) == OK
-    # Two rows of long sequences are shared out: that takes a workspace.
-    long = dict(b_columns=4096)
-    b, c, _ = structures(p, **long)
-    need = lib.ancha_paged_attention_workspace(3, 4, ref(c), ref(b))
-    assert need > 0
-    refused(attention(size=need - 1, **long), INV, "workspace")
-    refused(attention(ws=None, **long), INV, "workspace")
-    refused(attention(ws=p + 8, **long), INV, "workspace")
-    refused(attention(size=need, **long), UNS, "gfx950")
-    for rows, heads in ((0, 4), (3, 3), (3, 0)):
-        assert lib.ancha_paged_attention_workspace(rows, heads, ref(c), ref(b)) == 0
-    assert lib.ancha_paged_attention_workspace(3, 4, None, ref(b)) == 0
+    # Long sequences are shared out, which takes a workspace: as much as the call itself asks for, of every type, whatever
+    # kernel the sizes lead to (a tile of rows is another one for other types).
+    for dim, rows, sequences, columns in ((64, 3, 2, 4096), (128, 32, 8, 64), (128, 64, 2, 512), (64, 100, 1, 512),
+                                          (256, 9, 3, 512), (128, 300, 2, 512)):
+        how = dict(b_columns=columns, b_sequences=sequences, c_dim=dim)
+        b, c, _ = structures(p, **how)
+        for t in (0, 1, 2):
+            need = lib.ancha_paged_attention_workspace(t, rows, 8, ref(c), ref(b))
+            assert need > 0
+            call = dict(how, t=t, rows=rows, heads=8, ld=8 * dim, ldh=dim)
+            refused(attention(size=need - 1, **call), INV, "workspace")
+            refused(attention(ws=None, **call), INV, "workspace")
+            refused(attention(ws=p + 8, **call), INV, "workspace")
+            refused(attention(size=need, **call), UNS, "gfx950")
+    for t, rows, heads in ((0, 0, 4), (0, 3, 3), (0, 3, 0), (3, 3, 4)):
+        assert lib.ancha_paged_attention_workspace(t, rows, heads, ref(c), ref(b)) == 0
+    assert lib.ancha_paged_attention_workspace(0, 3, 4, None, ref(b)) == 0
     assert lib.ancha_hip_check() == 0
 
 
