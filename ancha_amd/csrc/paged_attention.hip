@@ -470,16 +470,19 @@ void start(const AttentionParams& p, hipStream_t stream) {
 AttentionForm attention_form(const AttentionParams& p) {
   AttentionForm f{};
   const long group = p.heads / p.cache.heads, rows = p.rows * group, some = min(p.batch.sequences, p.rows);
-  const bool chunk = p.cache.dim < 256 && rows >= 64 * some;
-  const int of = chunk ? chunk_rows(p.cache.dim, p.type) : kTile;
+  const long keys = (long)p.batch.columns << p.cache.shift;
+  const int high = p.cache.dim < 256 ? chunk_rows(p.cache.dim, p.type) : 0;
+  const bool chunk = high && 4 * rows >= 3 * high * some && rows * p.cache.heads >= (1l << 24) / max(keys, 1l);
+  const int of = chunk ? high : kTile;
   // Sequences fill their last tiles in part; one tile more for rows of no sequence.
   f.tiles = (rows + some * (of - 1)) / of + 1;
   const long groups = f.tiles * p.cache.heads;
   f.form = chunk ? kChunk : p.cache.dim < 256 && groups < 1024 ? kTiles8 : kTiles4;
-  // Workgroups share a tile's keys until there are 512 (256 of the chunk kernel's with eight waves).
-  const long want = chunk && chunk_waves(p.cache.dim, p.type) == 8 ? 256 : 512;
-  const long keys = (long)p.batch.columns << p.cache.shift;
-  f.splits = (int)min(max(want / groups, 1l), min(keys / kLeastKeys + 1, 256l));
+  // Workgroups share a tile's keys as long as all of them run at once: one of eight waves a CU, two of four. Rows are
+  // taken to be spread evenly over the sequences.
+  const long slots = (chunk ? chunk_waves(p.cache.dim, p.type) == 8 : f.form == kTiles8) ? 256 : 512;
+  const long full = some ? some * ((rows + some * of - 1) / (some * of)) : 1;
+  f.splits = (int)min(max(slots / (full * p.cache.heads), 1l), min(keys / kLeastKeys + 1, 256l));
   if (f.splits > 1)
     f.bytes = 4 * (size_t)(joined_floats(f.tiles, p.cache.heads) + groups * f.splits * part_floats(of, p.cache.dim));
   return f;
