@@ -29,7 +29,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_kernel(AttentionParams p
   typedef typename Stored<TYPE>::type T;
   constexpr int kWaves = WAVES;
   constexpr int kQ = TYPE == kBf16 ? 1 : TYPE == kF16 ? 2 : 3;  // parts of a query
-  constexpr int kP = TYPE == kF32 ? 2 : 1;                      // of a weight
+  constexpr int kP = TYPE == kBf16 ? 1 : 2;                      // of a weight
   constexpr int kRow = row_bytes(D, FORMAT), kBlocks = D / kBlock;
   constexpr int kChunk = FORMAT == kFp4 && D >= 128 ? 32 : 16;  // columns of a key that a lane has beside each other
   constexpr int kChunks = D / (4 * kChunk);

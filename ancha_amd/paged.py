@@ -122,9 +122,7 @@ def rotary_plan(width: int, base: float = 10000.0, layout: str = "half", scaling
     return Rotary(torch.tensor(freqs, dtype=torch.float64, device=device), layout, magnitude)
 
 
-def _heads(x: torch.Tensor, name: str) -> torch.Tensor:
-    """x [rows, heads, dim] with neighbouring columns (a copy where they are not)."""
-    return x if x.stride(2) == 1 or x.shape[2] == 1 else x.contiguous()
+_POSITIONS = {torch.int32: 4, torch.int64: 8}
 
 
 def _take(x: torch.Tensor, name: str) -> int:
@@ -134,11 +132,21 @@ def _take(x: torch.Tensor, name: str) -> int:
     return kind
 
 
-def _on(owner, name: str, kind: type, device: torch.device):
+def _strides(x: torch.Tensor) -> tuple[torch.Tensor, int, int]:
+    """x [rows, heads, dim] with neighbouring columns (a copy where they are not), its strides of rows and heads."""
+    row, head, column = x.stride()
+    if column == 1 or x.shape[2] == 1:
+        return x, row, head
+    x = x.contiguous()
+    return x, x.stride(0), x.stride(1)
+
+
+def _on(owner, name: str, kind: type, device: torch.device) -> None:
+    if isinstance(owner, kind) and owner.device == device:
+        return
     if not isinstance(owner, kind):
         raise ValueError(f"{name} must be a paged.{kind.__name__}")
-    if owner.device != device:
-        raise ValueError(f"{name} must be on {device}, got {owner.device}")
+    raise ValueError(f"{name} must be on {device}, got {owner.device}")
 
 
 def rotary(x: torch.Tensor, positions: Union[torch.Tensor, Batch], plan: Rotary) -> Optional[torch.Tensor]:
@@ -158,17 +166,19 @@ def rotary(x: torch.Tensor, positions: Union[torch.Tensor, Batch], plan: Rotary)
         _on(positions, "positions", Batch, device)
         batch = positions._at
     else:
-        if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64):
+        wide = _POSITIONS.get(getattr(positions, "dtype", None), 0)
+        if not wide:
             raise ValueError("positions must be an int32 or int64 tensor or a paged.Batch")
-        require(positions, "positions", device, (rows,), positions.dtype)
+        if positions.shape != (rows,) or positions.device != device:
+            require(positions, "positions", device, (rows,), positions.dtype)
         positions = positions.contiguous()
-        at, wide = positions.data_ptr(), positions.element_size()
-    out = torch.empty((rows, heads, dim), dtype=x.dtype, device=device)
+        at = positions.data_ptr()
+    out = torch.empty_like(x, memory_format=torch.contiguous_format)
     if not out.numel():
         return out
-    x = _heads(x, "x")
-    return out if _launch(device.index, "ancha_paged_rotary", x.data_ptr(), kind, rows, heads, dim, x.stride(0),
-                          x.stride(1), at, wide, batch, plan._at, out.data_ptr()) else None
+    x, row, head = _strides(x)
+    return out if _launch(device.index, "ancha_paged_rotary", x.data_ptr(), kind, rows, heads, dim, row, head, at, wide,
+                          batch, plan._at, out.data_ptr()) else None
 
 
 class Cache:
@@ -226,10 +236,10 @@ class Cache:
                 raise ValueError(f"the plan turns {plan.width} columns, the heads have {self.dim}")
         if not k.numel():
             return self
-        k, v = _heads(k, "k"), _heads(v, "v")
-        done = _launch(self.device.index, "ancha_paged_write", k.data_ptr(), v.data_ptr(), kind, k.shape[0],
-                       k.stride(0), k.stride(1), v.stride(0), v.stride(1), batch._at,
-                       None if plan is None else plan._at, self._at)
+        k, ldk, ldkh = _strides(k)
+        v, ldv, ldvh = _strides(v)
+        done = _launch(self.device.index, "ancha_paged_write", k.data_ptr(), v.data_ptr(), kind, k.shape[0], ldk, ldkh,
+                       ldv, ldvh, batch._at, None if plan is None else plan._at, self._at)
         return self if done else None
 
     def read(self, batch: Batch, size: int,
@@ -240,7 +250,8 @@ class Cache:
         _on(batch, "batch", Batch, self.device)
         if size < 0:
             raise ValueError(f"size must be >= 0, got {size}")
-        k, v = (torch.empty((len(batch), size, self.heads, self.dim), dtype=dtype, device=self.device) for _ in (0, 1))
+        k = torch.empty((len(batch), size, self.heads, self.dim), dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
         if not k.numel():
             return k, v
         return (k, v) if _launch(self.device.index, "ancha_paged_read", self._at, batch._at, size, kind, k.data_ptr(),
@@ -269,12 +280,12 @@ def attention(q: torch.Tensor, cache: Cache, batch: Batch, scale: Optional[float
     if window is not None and window < 1:
         raise ValueError(f"window must be >= 1, got {window}")
     scale = dim ** -0.5 if scale is None else float(scale)
-    out = torch.empty((rows, heads, dim), dtype=q.dtype, device=device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if not rows:
         return out
-    q = _heads(q, "q")
+    q, row, head = _strides(q)
     need = _native.lib().ancha_paged_attention_workspace(kind, rows, heads, cache._at, batch._at)
     workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    return out if _launch(device.index, "ancha_paged_attention", q.data_ptr(), kind, rows, heads, q.stride(0),
-                          q.stride(1), cache._at, batch._at, scale, int(causal), window or 0,
+    return out if _launch(device.index, "ancha_paged_attention", q.data_ptr(), kind, rows, heads, row, head,
+                          cache._at, batch._at, scale, int(causal), window or 0,
                           None if workspace is None else workspace.data_ptr(), need, out.data_ptr()) else None
