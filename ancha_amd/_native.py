@@ -82,14 +82,15 @@ SIGNATURES = {
     "ancha_hip_check": (_int, []),
     "ancha_hip_last_error": (ctypes.c_char_p, []),
     # Not in the header: linear / norm_linear with scratch for the weight's fp16 fragments, and, for the
-    # tests, the attention kernels' split and the forms of microscaled
-    # products and norms.
+    # tests, the attention kernels' split and the forms of microscaled products and norms and of attention over a
+    # paged cache.
     "ancha_amd_linear_workspace": (_sz, [_sz, _sz, _sz]),
     "ancha_amd_linear": (_int, [_p, _sz, _sz, _sz, _p, _sz, _p, _int, _p, _sz, _sz, _p, _int, _p,
                                 _sz, _p, _p]),
     "ancha_amd_attention_queries": (_int, [_sz, _sz, _sz, _int, _int]),
     "ancha_amd_mx_linear_form": (_int, [_sz, _sz, _sz]),
     "ancha_amd_mx_norm_form": (_int, [_sz, _sz]),
+    "ancha_amd_paged_form": (_int, [_int, _sz, _sz, _sz, _sz, _sz, _sz]),
 }
 
 

@@ -347,7 +347,8 @@ __global__ __launch_bounds__(64 * WAVES) void attention_kernel(AttentionParams p
   for (int j = 0; j < 4; j++) {
     const int e = __shfl(ref, of_sums(j)) - 127;
 #pragma unroll
-    for (int t = 0; t < kCols; t++) outs[wave][c][kCols * (4 * g + j) + t] = none >> j & 1u ? nan : __builtin_ldexpf(acc[t][j] * mean, e);
+    for (int t = 0; t < kCols; t++)
+      outs[wave][c][kCols * (4 * g + j) + t] = none >> j & 1u ? nan : __builtin_ldexpf(acc[t][j] * mean, e);
   }
   __syncthreads();
   if (WAVES > 4 && threadIdx.x >= 256) return;

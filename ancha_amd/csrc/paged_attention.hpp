@@ -66,7 +66,8 @@ struct Range {
   int low, high;
 };
 __device__ __forceinline__ Range visible(const AttentionParams& p, const Sequence& s, int token) {
-  const int capacity = (int)min((long)p.batch.columns << p.cache.shift, (long)0x7fffffff);
+  // Some steps below 2^31, so that a step ahead of the last one is still a number.
+  const int capacity = (int)min((long)p.batch.columns << p.cache.shift, 0x7fff0000l);
   const long at = (long)s.length - s.count + token;
   const long high = p.causal ? at + 1 : s.length, low = p.window ? at - p.window + 1 : 0;
   const int h = (int)min(max(high, 0l), (long)capacity);
@@ -81,11 +82,13 @@ __device__ __forceinline__ bool find_tile(const AttentionParams& p, int group, i
   for (int base = 0; base < p.batch.sequences; base += 64) {
     Sequence mine = {0, 0, 0};
     if (base + lane < p.batch.sequences) mine = sequence(p.batch, base + lane, p.rows);
-    const int tiles = (int)(((long)mine.count * group + rows - 1) / rows);
+    // At most 2^24 (a call has fewer): starts that do not ascend cannot make the sums overflow.
+    const int tiles = (int)min(((long)mine.count * group + rows - 1) / rows, 1l << 24);
     int sum;  // of the tiles up to this lane's
     if (!__any(tiles > 1)) {
       const unsigned long long some = __ballot(tiles != 0);
-      sum = tiles + (int)__builtin_amdgcn_mbcnt_hi((unsigned)(some >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)some, 0u));
+      const unsigned low = __builtin_amdgcn_mbcnt_lo((unsigned)some, 0u);
+      sum = tiles + (int)__builtin_amdgcn_mbcnt_hi((unsigned)(some >> 32), low);
     } else {
       sum = tiles;
 #pragma unroll
@@ -118,6 +121,7 @@ __device__ void clear_rows(const AttentionParams& p, int which, int count) {
   const int to = n ? min(max(p.batch.starts[n], from), p.rows) : 0;
   const long wide = (long)p.heads * p.cache.dim;
   T* out = static_cast<T*>(p.out);
+  count = max(count, 1);
   for (long at = (long)which * blockDim.x + threadIdx.x; at < (p.rows - (to - from)) * wide;
        at += (long)count * blockDim.x)
     out[at < from * wide ? at : at + (to - from) * wide] = (T)0.f;

@@ -64,7 +64,8 @@ int check_plan(const std::string& who, const ancha_paged_plan* p, size_t dim, pa
   if (!p->freqs || !aligned(p->freqs, 8)) return fail(ANCHA_HIP_INVALID, who + ": freqs is null or not 8-byte aligned");
   if (p->width == 0 || p->width % 2 || p->width > dim)
     return fail(ANCHA_HIP_INVALID, who + ": the rotated width is even, above 0 and at most the head's");
-  if (!above(p->magnitude, 0.0)) return fail(ANCHA_HIP_INVALID, who + ": magnitude is not a number > 0");
+  if (!above(p->magnitude, 0.0) || p->magnitude > 3.4e38)
+    return fail(ANCHA_HIP_INVALID, who + ": magnitude is not an fp32 number > 0");
   to = {p->freqs, static_cast<int>(p->width), p->interleaved ? 1 : 0, p->magnitude};
   return 0;
 }
@@ -168,8 +169,8 @@ int ancha_paged_read(const ancha_paged_cache* cache, const ancha_paged_batch* ba
 size_t ancha_paged_attention_workspace(int type, size_t rows, size_t heads, const ancha_paged_cache* cache,
                                        const ancha_paged_batch* batch) {
   paged::AttentionParams p{};
-  if (!is_type(type) || !cache || !batch || !cache->heads || !heads || heads % cache->heads || rows == 0 || rows > kIntMax ||
-      heads > kIntMax || rows * heads > kIntMax || cache->page < 16 || cache->page > 65536 ||
+  if (!is_type(type) || !cache || !batch || !cache->heads || !heads || heads % cache->heads || rows == 0 ||
+      rows > kIntMax || heads > kIntMax || rows * heads > kIntMax || cache->page < 16 || cache->page > 65536 ||
       batch->sequences >= kIntMax || batch->columns > kIntMax)
     return 0;
   p.type = type;
@@ -221,6 +222,22 @@ int ancha_paged_attention(const void* q, int type, size_t rows, size_t heads, si
   p.scale = static_cast<float>(scale * 1.4426950408889634);
   const hipError_t e = paged::launch_attention(p, form, stream);
   return e == hipSuccess ? ANCHA_HIP_OK : hip_fail(e, who);
+}
+
+// For the tests: how a call is laid out, 3 x splits + its kernel (paged::AttentionForm).
+int ancha_amd_paged_form(int type, size_t rows, size_t heads, size_t cache_heads, size_t dim, size_t sequences,
+                         size_t keys) {
+  paged::AttentionParams p{};
+  p.type = type;
+  p.rows = static_cast<int>(rows);
+  p.heads = static_cast<int>(heads);
+  p.cache.heads = static_cast<int>(cache_heads);
+  p.cache.dim = static_cast<int>(dim);
+  p.batch.sequences = static_cast<int>(sequences);
+  p.batch.columns = static_cast<int>((keys + 15) / 16);
+  p.cache.shift = 4;
+  const paged::AttentionForm f = paged::attention_form(p);
+  return 3 * f.splits + f.form;
 }
 
 }  // extern "C"

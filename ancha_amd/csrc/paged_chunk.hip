@@ -1,6 +1,6 @@
-// Attention of many new tokens over a paged, microscaled cache (gfx950): chunks and whole prompts. The operation and its
-// operands are those of paged_attention.hip; here 128 or 256 query rows share
-// the keys that a workgroup reads. Heads of 64 or 128 columns.
+// Attention of many new tokens over a paged, microscaled cache (gfx950): chunks and whole prompts. The operation and
+// its operands are those of paged_attention.hip; here 128 or 256 query rows share the keys that a workgroup reads.
+// Heads of 64 or 128 columns.
 #include "paged_attention.hpp"
 
 namespace ancha {
@@ -46,7 +46,8 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
   typedef Shape<D, FORMAT, TYPE> S;
   constexpr int kQ = S::kQ, kP = S::kP, kScales = S::kScales, kRow = row_bytes(D, FORMAT);
   constexpr int kWaves = S::kWaves, kThreads = S::kThreads;
-  // As many blocks of keys as groups of eight values x four columns: one of each a thread, or half the waves have either.
+  // As many blocks of keys as groups of eight values x four columns: one of each a thread, or half the waves have
+  // either.
   constexpr int kUnits = kKeys * kScales;
   static_assert(kUnits == kThreads || 2 * kUnits == kThreads, "a unit a thread");
   constexpr bool kApart = kUnits < kThreads;
@@ -121,7 +122,8 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
     const bool there = (unsigned)page < (unsigned)p.cache.pages;
     return slot_of(p.cache, 0, there ? page : 0, head, there ? key & ((1 << shift) - 1) : key & 15);
   };
-  // What this thread brings: the scale bytes of key `lane` (every wave for itself), a block of a key, a group of values.
+  // What this thread brings: the scale bytes of key `lane` (every wave for itself), a block of a key, a group of
+  // values.
   const bool has_key = !kApart || wave < kWaves / 2, has_value = !kApart || wave >= kWaves / 2;
   const int unit = thread % kUnits;
   const int my_key = unit / kScales, key_block = unit % kScales;
@@ -136,9 +138,10 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
     int scale, key, value;
   };
   struct Raw {
-    unsigned k[kBlockWords], v[8], vs, ks;
-    int page;  // of key `lane`
+    unsigned codes[kApart ? 8 : 16], vs, ks;  // of a key (block by block), of eight values; the same place where apart
+    int page;                                 // of key `lane`
   };
+  constexpr int kValues = kApart ? 0 : 8;  // where the values' are
   const auto fetch_pages = [&](int key, Pages& g) {
     g.scale = page_at(key + lane);
     if (has_key) g.key = page_at(key + my_key);
@@ -151,15 +154,15 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
     if (has_key) {
       const long at = slot_at(g.key, key + my_key);
       w.ks = p.cache.scales[at * kScales + key_block];
-      __builtin_memcpy(w.k, p.cache.codes + at * kRow + key_block * 4 * kBlockWords, 4 * kBlockWords);
+      __builtin_memcpy(w.codes, p.cache.codes + at * kRow + key_block * 4 * kBlockWords, 4 * kBlockWords);
     }
     if (has_value) {
       const uint8_t* from = p.cache.codes + (slot_at(g.value, key + 16 * (half / 2)) + values) * kRow +
                             col * (FORMAT == kFp8 ? 4 : 2);
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        w.v[j] = 0;
-        __builtin_memcpy(&w.v[j], from + (value_of(j) & 15) * kRow, FORMAT == kFp8 ? 4 : 2);
+        w.codes[kValues + j] = 0;
+        __builtin_memcpy(&w.codes[kValues + j], from + (value_of(j) & 15) * kRow, FORMAT == kFp8 ? 4 : 2);
       }
     }
   };
@@ -224,7 +227,8 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
         u32x4 x;
 #pragma unroll
         for (int n = 0; n < 4; n++)
-          x[n] = FORMAT == kFp8 ? two_bf16<FORMAT>(w_.k[2 * j + n / 2], f, n & 1) : two_bf16<FORMAT>(w_.k[j], f, n);
+          x[n] = FORMAT == kFp8 ? two_bf16<FORMAT>(w_.codes[2 * j + n / 2], f, n & 1)
+                                : two_bf16<FORMAT>(w_.codes[j], f, n);
         const int at = (my_key / 32 * (D / 16) + 2 * key_block + j / 2) * 64;
         *reinterpret_cast<u32x4*>(keys + (at + slot_of_key(32 * (j & 1) + my_key % 32, key_block)) * 16) = x;
       }
@@ -234,7 +238,7 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
         asm volatile("");  // a branch, not eight selections every time
 #pragma unroll
         for (int j = 0; j < 8; j++)
-          if (!(last_there >> value_of(j) & 1)) w_.v[j] = 0;
+          if (!(last_there >> value_of(j) & 1)) w_.codes[kValues + j] = 0;
       }
       float f[8];
       __builtin_memcpy(f, powers + value_block * kKeys + value_of(0), 16);
@@ -243,7 +247,7 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
 #pragma unroll
       for (int u = 0; u < 2; u++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) two[u][j] = two_f16<FORMAT>(w_.v[j], f[j], u);
+        for (int j = 0; j < 8; j++) two[u][j] = two_f16<FORMAT>(w_.codes[kValues + j], f[j], u);
 #pragma unroll
       for (int d = 0; d < 4; d++) {
         u32x4 x;

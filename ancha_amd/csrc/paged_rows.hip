@@ -197,7 +197,8 @@ __global__ __launch_bounds__(kThreads) void write_kernel(WriteParams p, int rows
     if (to.x >= 0) {
       if (!u.which && u.col < 2 * pairs) turn_key<HALF>(p.plan, u.col, trig + u.row * pairs, u.other, u.x);
       const long slot = slot_of(p.cache, u.which, to.x, u.head, to.y & ((1 << p.cache.shift) - 1));
-      store_codes(u.x, FORMAT, true, p.cache.codes + slot * row_bytes(dim, FORMAT) + (FORMAT == kFp8 ? u.col : u.col / 2),
+      uint8_t* const codes = p.cache.codes + slot * row_bytes(dim, FORMAT);
+      store_codes(u.x, FORMAT, true, codes + (FORMAT == kFp8 ? u.col : u.col / 2),
                   p.cache.scales + slot * (dim / kBlock) + u.col / kBlock);
     }
     i += kThreads;

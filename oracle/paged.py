@@ -1,6 +1,7 @@
 """The paged operators in numpy, 64 bits, token by token: rotary positions, a cache of microscaled codes in pages and
 attention over it. Arrays as ``ancha_amd.paged`` has them: codes [2, pages, heads, page, bytes], scales
-[2, pages, heads, page, dim / 32]; a batch is (starts, lengths, table), and a page number outside the cache is a page that is not there.
+[2, pages, heads, page, dim / 32]; a batch is (starts, lengths, table), and a page number outside the cache is a page
+that is not there.
 """
 from __future__ import annotations
 

@@ -1,5 +1,5 @@
-"""The paged operators without a GPU: frequencies, the oracle against a dense computation, and every refusal that is made
-before a launch."""
+"""The paged operators without a GPU: frequencies, the oracle against a dense computation, every refusal that is made
+before a launch, and what the built kernels keep in registers."""
 import ctypes
 import math
 import os
@@ -40,7 +40,8 @@ def test_frequencies():
     assert abs(g[2] - f[2] * (share + (1 - share) / 4)) < 1e-17 and abs(m - (0.1 * math.log(4) + 1)) < 1e-15
     assert paged.frequencies(2, 500.0) == ([1.0], 1.0)
     for how, text in (((0,), "width"), ((3,), "width"), ((8, -1.0), "base"), ((8, float("inf")), "base"),
-                      ((8, 1e4, "dynamic"), "scaling"), ((8, 1e4, "linear", 0.5), "factor"), ((8, 1e4, None, 2.0), "factor"),
+                      ((8, 1e4, "dynamic"), "scaling"), ((8, 1e4, "linear", 0.5), "factor"),
+                      ((8, 1e4, None, 2.0), "factor"),
                       ((8, 1e4, "yarn", float("nan"), 5), "factor"), ((8, 1e4, "yarn", 2.0), "original"),
                       ((2, 1e4, "ntk", 2.0), "ntk")):
         with pytest.raises(ValueError, match=text):
@@ -96,7 +97,8 @@ def test_entry_points_check_arguments(lib):
     INV, UNS, OK = _native.INVALID, _native.UNSUPPORTED, _native.OK
     ref = ctypes.byref
 
-    def rotary(x=p, t=0, rows=3, heads=2, dim=64, ld=128, ldh=64, at=p, size=4, out=p, batch=True, plan=True, **changes):
+    def rotary(x=p, t=0, rows=3, heads=2, dim=64, ld=128, ldh=64, at=p, size=4, out=p, batch=True, plan=True,
+               **changes):
         b, _, f = structures(p, **changes)
         return lib.ancha_paged_rotary(x, t, rows, heads, dim, ld, ldh, at, size, ref(b) if batch else None,
                                       ref(f) if plan else None, out, None)
@@ -110,11 +112,11 @@ def test_entry_points_check_arguments(lib):
         b, c, _ = structures(p, **changes)
         return lib.ancha_paged_read(ref(c) if cache else None, ref(b) if batch else None, size, t, k, v, None)
 
-    def attention(q=p, t=0, rows=3, heads=4, ld=256, ldh=64, scale=0.125, window=0, ws=p, size=1 << 40, out=p, batch=True,
-                  cache=True, **changes):
+    def attention(q=p, t=0, rows=3, heads=4, ld=256, ldh=64, scale=0.125, window=0, ws=p, size=1 << 40, out=p,
+                  batch=True, cache=True, **changes):
         b, c, _ = structures(p, **changes)
-        return lib.ancha_paged_attention(q, t, rows, heads, ld, ldh, ref(c) if cache else None, ref(b) if batch else None,
-                                         scale, 1, window, ws, size, out, None)
+        return lib.ancha_paged_attention(q, t, rows, heads, ld, ldh, ref(c) if cache else None,
+                                         ref(b) if batch else None, scale, 1, window, ws, size, out, None)
 
     def refused(rc, code, text):
         assert rc == code and text in _native.last_error(), (rc, _native.last_error())
@@ -147,7 +149,7 @@ def test_entry_points_check_arguments(lib):
             refused(call(**change), INV, "freqs")
         for width in (0, 3, 66):
             refused(call(f_width=width), INV, "width")
-        for m in (0.0, -1.0, float("nan"), float("inf")):
+        for m in (0.0, -1.0, float("nan"), float("inf"), 1e39):
             refused(call(f_magnitude=m), INV, "magnitude")
         refused(call(ld=1 << 62), UNS, "too many")
         refused(call(rows=1 << 24), UNS, "too many")
@@ -182,8 +184,8 @@ def test_entry_points_check_arguments(lib):
     refused(attention(rows=1 << 30), UNS, "too many")
     refused(attention(rows=1 << 26, heads=16), UNS, "too many")
     assert attention(rows=0) == OK
-    # Long sequences are shared out, which takes a workspace: as much as the call itself asks for, of every type, whatever
-    # kernel the sizes lead to (a tile of rows is another one for other types).
+    # Long sequences are shared out, which takes a workspace: as much as the call itself asks for, of every type,
+    # whatever kernel the sizes lead to (a tile of rows is another one for other types).
     for dim, rows, sequences, columns in ((64, 3, 2, 4096), (128, 32, 8, 64), (128, 64, 2, 512), (64, 100, 1, 512),
                                           (256, 9, 3, 512), (128, 300, 2, 512)):
         how = dict(b_columns=columns, b_sequences=sequences, c_dim=dim)

@@ -5,9 +5,9 @@ products and their sum (2^-24 each): within (|x| + |y|) m 2^-21 and the result's
 from 64 bits: the oracle's bytes.
 
 Attention, with A = sum_j w_j |v_j| of a row: scores are sums of exact products, D / 32 instructions a part of q, each
-of which adds at most one step (2^-23) of the largest of its terms twice; three parts hold 24 bits of q. With R the largest
-scale sum |q k|, a score is within e = (D / 32 * parts + 4) 2^-22 R, and so the result within 2 e A. Exponentials are
-good to 2^-21, weights to half a step of fp16 (fp32 results: 2^-21), in the products and in the sum that divides them:
+of which adds at most one step (2^-23) of the largest of its terms twice; three parts hold 24 bits of q. With R the
+largest scale sum |q k|, a score is within e = (D / 32 * parts + 4) 2^-22 R, and so the result within 2 e A.
+Exponentials are good to 2^-21, weights to half a step of fp16 (fp32 results: 2^-21), in the products and in the sum that divides them:
 2^-11 (A + |o|). Each weight that is less than fp16 holds is off by
 2^-25 where the largest is 2^6 to 2^15, so by 2^-31 of it: 2^-31 sum_j |v_j| in all. Values are off by 2^-25 where the
 largest of their block is 2^11 or more, less than 2^-32 of it. Then the result's type: half its eps, and
@@ -17,7 +17,7 @@ import numpy as np
 import pytest
 import torch
 
-from ancha_amd import fused, mx, paged
+from ancha_amd import _native, fused, mx, paged
 from ancha_amd import workload as W
 from oracle import mx as OM
 from oracle import paged as O
@@ -284,21 +284,71 @@ def test_attention_of_many_sequences(gpu, kind):
     check_attention(gpu, kind, 6, cache, codes, scales, batch, plain, rows, 64)
 
 
-@pytest.mark.parametrize("kind", ["f16", "bf16"])
-@pytest.mark.parametrize("dim,fmt", [(64, "fp4"), (128, "fp8"), (256, "fp8")])
-def test_attention_of_chunks(gpu, dim, fmt, kind):
-    """Many rows: whole prompts and chunks, odd lengths on both sides."""
-    cache, codes, scales = some_cache(gpu, 40, 32, 2, dim, fmt, 71)
-    batch, plain, rows = some_batch(gpu, [257, 130, 1], [257, 411, 300], 32, 40, 72)
+TILES4, TILES8, CHUNK = 0, 1, 2
+
+
+def form(kind, rows, heads, cache, batch):
+    """(kernel, workgroups that may share a tile's keys) of a call."""
+    got = _native.lib().ancha_amd_paged_form(list(TYPES).index(kind), rows, heads, cache.heads, cache.dim, len(batch),
+                                             batch.table.shape[1] * cache.page)
+    return got % 3, got // 3
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("dim,fmt", [(64, "fp8"), (64, "fp4"), (128, "fp8"), (128, "fp4"), (256, "fp8")])
+@pytest.mark.parametrize("new,lengths,heads,kv,page,columns", [
+    ([257, 130, 1], [257, 411, 300], 4, 2, 32, 20),       # tiles of 16 rows
+    ([257, 130, 80], [257, 411, 300], 4, 2, 32, 600),     # room for long sequences: the chunk kernel, shared keys
+    ([64, 100], [900, 100], 16, 2, 16, 1200),             # shared by several, the last part short
+    ([100, 0, 37, 90], [64, 50, 1100, 90], 21, 3, 64, 500),  # rows without keys, sevens of heads
+])
+def test_attention_of_chunks(gpu, new, lengths, heads, kv, page, columns, dim, fmt, kind):
+    pages = sum(-(-n // page) for n in lengths) + 1
+    cache, codes, scales = some_cache(gpu, pages, page, kv, dim, fmt, 71)
+    batch, plain, rows = some_batch(gpu, new, lengths, page, pages, 72, columns=columns, pad=2, first=1)
+    kernel, shares = form(kind, rows, heads, cache, batch)
+    assert kernel == (CHUNK if dim < 256 and columns > 100 else TILES8 if dim < 256 else TILES4)
+    assert shares > 1 or dim == 256
     for how in ({}, {"window": 100}, {"causal": False}):
-        check_attention(gpu, kind, 4, cache, codes, scales, batch, plain, rows, 73, **how)
+        check_attention(gpu, kind, heads, cache, codes, scales, batch, plain, rows, 73, **how)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_attention_of_whole_prompts(gpu, kind):
+    """As many tiles as run at once: nobody shares their keys."""
+    cache, codes, scales = some_cache(gpu, 34, 16, 32, 64, "fp8", 75)
+    batch, plain, rows = some_batch(gpu, [270, 200], [270, 210], 16, 34, 76, columns=1000)
+    assert form(kind, rows, 128, cache, batch) == (CHUNK, 1)
+    q = dev(W.normal((rows, 128, 64), 77, 1.0), gpu, TYPES[kind])
+    few = slice(0, 128, 29)  # the oracle on some heads: 0, 29, .. read heads 0, 7, .. of the cache
+    heads = [h // 4 for h in range(0, 128, 29)]
+    got = paged.attention(q, cache, batch)[:, few]
+    part = np.ascontiguousarray(codes[:, :, heads]), np.ascontiguousarray(scales[:, :, heads])
+    want, size, total, reach = O.attention(host(q[:, few]), *part, "fp8", plain)
+    e = (2 * PARTS[kind] + 4) * 2.0 ** -22 * reach
+    tol = size * (2 * e + 2.0 ** -11 + 2.0 ** -21) + np.abs(want) * 2.0 ** -11 + rounding(want, TYPES[kind])
+    close("prompts", got, want, tol + total * 2.0 ** -31 + np.exp2(scales.max() - 127.0) * 448 * 2.0 ** -32)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("dim,fmt", [(64, "fp4"), (128, "fp8")])
+def test_attention_of_a_thousand_tiles(gpu, dim, fmt, kind):
+    rng = np.random.default_rng(65)
+    lengths = rng.integers(0, 40, 140).tolist()
+    cache, codes, scales = some_cache(gpu, 420, 16, 8, dim, fmt, 66)
+    batch, plain, rows = some_batch(gpu, [1] * 140, lengths, 16, 420, 67)
+    assert form(kind, rows, 8, cache, batch)[0] == TILES4
+    check_attention(gpu, kind, 8, cache, codes, scales, batch, plain, rows, 68)
 
 
 def test_attention_what_was_not_written_is_not_seen(gpu):
     """NaN codes and scales behind the sequences' ends, before the window and in pages of nobody."""
-    for dim, fmt in ((64, "fp8"), (128, "fp4"), (256, "fp8")):
+    for dim, fmt, new, columns in ((64, "fp8", 1, None), (128, "fp4", 1, None), (256, "fp8", 1, None),
+                                   (64, "fp8", 30, 9000), (128, "fp4", 30, 9000)):
         cache, codes, scales = some_cache(gpu, 12, 16, 2, dim, fmt, 81)
-        batch, plain, rows = some_batch(gpu, [1, 20], [37, 50], 16, 12, 82)
+        batch, plain, rows = some_batch(gpu, [new, 20], [37, 50], 16, 12, 82, columns=columns)
+        heads = 2 if columns is None else 20
+        assert form("bf16", rows, heads, cache, batch)[0] == (CHUNK if columns else TILES4 if dim > 128 else TILES8)
         used = np.zeros((12, 16), bool)
         for i, length in enumerate(plain[1]):
             for t in range(length):
@@ -306,13 +356,17 @@ def test_attention_what_was_not_written_is_not_seen(gpu):
         codes.transpose(1, 3, 0, 2, 4)[~used], scales.transpose(1, 3, 0, 2, 4)[~used] = 0x7f, 255
         cache = paged.Cache(torch.from_numpy(codes.copy()).to(gpu), torch.from_numpy(scales.copy()).to(gpu), fmt)
         for how in ({}, {"window": 6}, {"causal": False}):
-            check_attention(gpu, "bf16", 4, cache, codes, scales, batch, plain, rows, 83, **how)
+            check_attention(gpu, "bf16", heads, cache, codes, scales, batch, plain, rows, 83, **how)
 
 
-@pytest.mark.parametrize("dim,fmt", [(64, "fp8"), (64, "fp4"), (128, "fp8"), (128, "fp4"), (256, "fp8"), (256, "fp4")])
-def test_attention_a_nan_reaches_the_rows_that_see_it(gpu, dim, fmt):
+@pytest.mark.parametrize("dim,fmt,heads,columns", [
+    (64, "fp8", 4, None), (64, "fp4", 4, None), (128, "fp8", 4, None), (128, "fp4", 4, None), (256, "fp8", 4, None),
+    (256, "fp4", 4, None), (64, "fp8", 20, 4000), (64, "fp4", 20, 4000), (128, "fp8", 20, 4000),
+    (128, "fp4", 20, 4000)])
+def test_attention_a_nan_reaches_the_rows_that_see_it(gpu, dim, fmt, heads, columns):
     cache, codes, scales = some_cache(gpu, 12, 16, 2, dim, fmt, 91)
-    batch, plain, rows = some_batch(gpu, [40, 1], [70, 90], 16, 12, 92)
+    batch, plain, rows = some_batch(gpu, [40, 1], [70, 90], 16, 12, 92, columns=columns)
+    assert (form("bf16", rows, heads, cache, batch)[0] == CHUNK) == bool(columns)
     page, slot = O.place(plain, 0, 45, 12, 16)  # seen by the rows from position 45 on
     for which, head, block in ((0, 0, 1), (1, 1, 0), (1, 1, dim // 32 - 1)):
         scales[which, page, head, slot, block], codes[which, page, head, slot].reshape(dim // 32, -1)[block] = 255, 0
@@ -321,16 +375,18 @@ def test_attention_a_nan_reaches_the_rows_that_see_it(gpu, dim, fmt):
     cache = paged.Cache(torch.from_numpy(codes.copy()).to(gpu), torch.from_numpy(scales.copy()).to(gpu), fmt)
     for kind in TYPES:
         for how in ({}, {"window": 10}, {"causal": False}):
-            got = check_attention(gpu, kind, 4, cache, codes, scales, batch, plain, rows, 93, **how)
+            got = check_attention(gpu, kind, heads, cache, codes, scales, batch, plain, rows, 93, **how)
             assert torch.isnan(got).any() and not torch.isnan(got).all()
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
-def test_attention_blocks_and_scores_of_any_size(gpu, kind):
+@pytest.mark.parametrize("heads,columns", [(2, None), (12, 9000)])
+def test_attention_blocks_and_scores_of_any_size(gpu, heads, columns, kind):
     """Values whose blocks grow by powers of two along the sequence, up and down, and scores that leave one key all."""
     for fmt, dim in (("fp8", 128), ("fp4", 64)):
         cache, codes, scales = some_cache(gpu, 20, 16, 1, dim, fmt, 101)
-        batch, plain, rows = some_batch(gpu, [3, 50], [150, 160], 16, 20, 102)
+        batch, plain, rows = some_batch(gpu, [3, 50], [150, 160], 16, 20, 102, columns=columns)
+        assert (form(kind, rows, heads, cache, batch)[0] == CHUNK) == bool(columns)
         for i in (0, 1):
             for t in range(int(plain[1][i])):
                 page, slot = O.place(plain, i, t, 20, 16)
@@ -338,7 +394,7 @@ def test_attention_blocks_and_scores_of_any_size(gpu, kind):
                 scales[1, page, :, slot, 1] = 100 + (t * 7919) % 40
         cache = paged.Cache(torch.from_numpy(codes.copy()).to(gpu), torch.from_numpy(scales.copy()).to(gpu), fmt)
         for sharp in (0.01, 1.0, 300.0):
-            q = dev(sharp * W.normal((rows, 2, dim), 103, 1.0), gpu, TYPES[kind])
+            q = dev(sharp * W.normal((rows, heads, dim), 103, 1.0), gpu, TYPES[kind])
             want, size, total, reach = O.attention(host(q), codes, scales, fmt, plain)
             e = (dim // 32 * PARTS[kind] + 4) * 2.0 ** -22 * reach
             # A value is off by 2^-32 of the largest of its own block of columns, however large the others are.
