@@ -5,7 +5,8 @@
 //
 // Operands. A key's codes times their power of two are bf16 values without loss, so products with a bf16 query are
 // exact; a query of 16 or 32 bits that bf16 does not hold is the sum of two or three bf16 parts, a product each. The
-// weights e^.. are fp16 (fp32 results: two fp16 parts), eight times finer than bf16. So values have to be fp16 too:
+// weights e^.. are fp16, eight times finer than bf16, in two parts where the result's own rounding is no coarser and
+// the products are not what bounds the kernel: for fp32, and for fp16 in the tiles here. So values have to be fp16 too:
 // each block of 32 columns has a reference power `ref` that all of its values are taken relative to, so that the
 // largest fits; what lies 2^-32 below it, where fp16 ends, is far below the result's own rounding. When a larger one
 // comes, the sums so far are scaled down, like those of the running maximum.
@@ -23,7 +24,11 @@ constexpr int kStep = 32;  // keys
 //   K        key c of each half: 16 (fp8) or up to 32 (fp4) neighbouring columns at a time,
 //   V        the same eight keys as its weights, columns D / 16 * c on, transposed in registers two by two.
 // Nothing passes through LDS before the waves' sums are joined. Bound by the reading of the cache while there are
-// few rows.
+// few rows: with 8 heads of 128 for 32 of q, 64 sequences of up to 8192 tokens in e4m3 (558 MB) take 119 us, 4.7 TB/s,
+// one of 131 072 in e2m1 (143 MB) 32 us and 6 to join its parts, one of 801 tokens 8 us and 4, which is the latency of
+// a few dependent reads. A page's number is read two steps ahead and codes one: with both one step ahead the first took
+// 183 us, not 142, and the second 77, not 57; codes two steps ahead changed nothing. With eight waves, twice the reads
+// in flight, they took 137 and 43 us, and 32 sequences of 8192 with heads of 64 in fp32 51 instead of 77.
 template <int D, int FORMAT, int TYPE, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void attention_kernel(AttentionParams p) {
   typedef typename Stored<TYPE>::type T;
@@ -383,7 +388,8 @@ __global__ __launch_bounds__(64 * WAVES) void attention_kernel(AttentionParams p
 }
 
 // The parts of split tiles of `rows` rows joined: D / 4 lanes a row, four columns each, which also share the parts'
-// maxima and sums.
+// maxima and sums. A tile's workgroups have left a note of its rows and parts, so no workgroup looks for its sequence:
+// with a search in each, one workgroup a row, the parts of 4 times 801 rows of 8 heads of 64 took 20.7 us, now 5.7.
 template <int D, int TYPE>
 __global__ __launch_bounds__(256) void join_kernel(AttentionParams p, int rows) {
   constexpr int kLanes = D / 4, kRows = 256 / kLanes;  // of a workgroup, all in one tile
@@ -472,15 +478,23 @@ AttentionForm attention_form(const AttentionParams& p) {
   AttentionForm f{};
   const long group = p.heads / p.cache.heads, rows = p.rows * group, some = min(p.batch.sequences, p.rows);
   const long keys = (long)p.batch.columns << p.cache.shift;
+  // Chunks are for sequences that fill three quarters of one, where the rows read enough to pay for its longer start.
+  // Both measured, 32 heads over 8 of 128 in bf16 (tiles / chunks): 8 sequences of 64 rows over 8192 keys 253 / 173 us,
+  // of 32 rows 127 / 143, 8 of 128 rows over 1024 78 / 48, of 64 43 / 41; one of 64 over 8192 53 / 42, of 128 over 1024
+  // 15 / 28. In fp32, 8 heads of 64, 8 sequences: 128 rows over 8192 97 / 83, 64 rows 53 / 79. Heads of 256 columns do
+  // not fit its registers.
   const int high = p.cache.dim < 256 ? chunk_rows(p.cache.dim, p.type) : 0;
   const bool chunk = high && 4 * rows >= 3 * high * some && rows * p.cache.heads >= (1l << 24) / max(keys, 1l);
   const int of = chunk ? high : kTile;
   // Sequences fill their last tiles in part; one tile more for rows of no sequence.
   f.tiles = (rows + some * (of - 1)) / of + 1;
   const long groups = f.tiles * p.cache.heads;
+  // Eight waves a tile read more at once, but have twice the sums to join: with 1024 workgroups the CUs are full either
+  // way, and 256 sequences of 1024 keys took 77 us with four and 93 with eight. Heads of 256 would spill: 42 and 97.
   f.form = chunk ? kChunk : p.cache.dim < 256 && groups < 1024 ? kTiles8 : kTiles4;
   // Workgroups share a tile's keys as long as all of them run at once: one of eight waves a CU, two of four. Rows are
-  // taken to be spread evenly over the sequences.
+  // taken to be spread evenly over the sequences. 8 sequences of 128 rows over 8192 keys took 312 us with one workgroup
+  // a tile, 190 so; 256 over 16 384 115 and 100.
   const long slots = (chunk ? chunk_waves(p.cache.dim, p.type) == 8 : f.form == kTiles8) ? 256 : 512;
   const long full = some ? some * ((rows + some * of - 1) / (some * of)) : 1;
   f.splits = (int)min(max(slots / (full * p.cache.heads), 1l), min(keys / kLeastKeys + 1, 256l));

@@ -186,6 +186,24 @@ def test_write_and_read(gpu, heads, dim, page, width, layout, fmt, kind):
     assert cache.read(batch, 0)[0].shape == (5, 0, heads, dim)
 
 
+def test_write_turns_by_any_angle(gpu):
+    """Angles within rounding of a right angle's multiples, small ones, and beyond 2^40, where another way takes over."""
+    cache, codes, scales = some_cache(gpu, 4, 64, 2, 64, "fp8", 24)
+    quarter = np.pi / 2
+    freqs = [quarter, np.nextafter(quarter, 2), -quarter / 2, 1e-9, 0.0, 1.0, -3.7, 512.5, 1e6, 2.0 ** 33 + 0.3, 1e12,
+             3e15]
+    plan = paged.Rotary(torch.tensor(freqs, dtype=torch.float64, device=gpu))
+    batch, plain, rows = some_batch(gpu, [200], [230], 64, 4, 25)
+    k = dev(W.normal((rows, 2, 64), 26, 1.0), gpu)
+    cache.write(k, k, batch, plan)
+    at = np.zeros(rows)
+    for r, _, position in O.rows_of(plain, rows):
+        at[r] = position
+    O.write(codes, scales, "fp8", O.rotate(host(k), at, freqs), host(k), plain)
+    assert np.array_equal(cache.scales.cpu().numpy(), scales)
+    assert np.array_equal(cache.codes.cpu().numpy(), codes)
+
+
 @pytest.mark.parametrize("fmt", ["fp8", "fp4"])
 def test_write_special_values_and_layouts(gpu, fmt):
     cache, codes, scales = some_cache(gpu, 4, 16, 2, 64, fmt, 21)
