@@ -25,15 +25,10 @@ __device__ __forceinline__ float2 cos_sin(double a) {
 }
 
 // The same for keys that are written, within 2^-52 of one: half pi is taken off in two parts by fused multiply-adds,
-// the rest, at most pi / 4, goes through the Taylor series to its 15th and 16th power. With the library's function,
-// which reduces any angle, 16 384 keys of 8 x 128 took 72 us to write and read, so 66; it serves angles from 2^40 on,
-// which frequencies up to 512 never reach.
+// the rest, at most pi / 4, goes through the Taylor series to its 15th and 16th power. That holds below 2^51, which
+// positions and frequencies up to 2^20 do not pass. With the library's function, which reduces any angle, 16 384 keys
+// of 8 x 128 took 72 us to write and read, so 66; with a branch to it for larger angles, 76.
 __device__ __forceinline__ double2 cos_sin_64(double a) {
-  if (!(__builtin_fabs(a) < 0x1p40)) {
-    double sine, cosine;
-    sincos(a, &sine, &cosine);
-    return make_double2(cosine, sine);
-  }
   const double whole = __builtin_rint(a * 0.6366197723675813430755);
   double r = __builtin_fma(-whole, 1.5707963267948965579990, a);
   r = __builtin_fma(-whole, 6.1232339957367660358688e-17, r);
@@ -179,7 +174,7 @@ __device__ __forceinline__ void turn_key(const Plan& plan, int col, const double
 // New keys and values into their pages. A workgroup has `rows` rows: their places and their pairs' cosines and sines
 // once (in 64 bits), then eight columns a thread, four threads a block of codes. Rows without a place are left out. The
 // first values are on their way while the places are found and the angles taken. 16 384 tokens of 8 heads of 128 in
-// bf16, 101 MB, take 42 us, of which 20 are the memory's and 6 the rotation in 64 bits: the rest is the latency of one chain (place, angle, values, codes), which one, two or eight rows a workgroup, rows dealt
+// bf16, 101 MB, take 36 us, of which 20 are the memory's and 6 the rotation in 64 bits: the rest is the latency of one chain (place, angle, values, codes), which one, two or eight rows a workgroup, rows dealt
 // by XCD, or the next values fetched ahead did not shorten. 32 tokens take 5 us.
 template <int TYPE, int FORMAT, bool HALF>
 __global__ __launch_bounds__(kThreads) void write_kernel(WriteParams p, int rows, Divide by_row) {

@@ -68,7 +68,7 @@ class Batch:
 
 class Rotary:
     """Rotary positions, made by :func:`rotary_plan` or of frequencies of one's own: ``freqs`` [width / 2] float64 on
-    the GPU, radians a position of each pair. The first ``width`` columns of a head are turned, in pairs
+    the GPU, radians a position of each pair, at most 2**20 in magnitude. The first ``width`` columns of a head are turned, in pairs
     (i, i + width / 2) for the layout "half" and (2 i, 2 i + 1) for "interleaved", and multiplied by ``magnitude``."""
 
     def __init__(self, freqs: torch.Tensor, layout: str = "half", magnitude: float = 1.0):
@@ -104,6 +104,8 @@ def frequencies(width: int, base: float = 10000.0, scaling: Optional[str] = None
         if width == 2:
             raise ValueError("'ntk' takes a width above 2")
         base = base * factor ** (width / (width - 2))
+    if math.log2(base) * (2 - width) / width > 20:
+        raise ValueError(f"base {base} makes frequencies above 2**20")
     freqs = [base ** (-2 * i / width) for i in range(width // 2)]
     if scaling == "linear":
         return [f / factor for f in freqs], 1.0

@@ -365,7 +365,7 @@ typedef struct {
 /* Rotary positions: the first `width` columns of a head turn by position * freqs[i] (pair i: columns i and
  * i + width / 2, or with `interleaved` 2 i and 2 i + 1), times `magnitude`; the others stay as they are. */
 typedef struct {
-  const double *freqs; /* [width / 2], device */
+  const double *freqs; /* [width / 2], device, of at most 2^20 in magnitude */
   size_t width;        /* even, 2 .. 2048 */
   int interleaved;
   double magnitude;
@@ -373,8 +373,7 @@ typedef struct {
 
 /* out [rows][heads][dim] contiguous = x rotated; element (row, head, d) of x at row * ldx + head * ldh + d. positions
  * [rows] of 4 or 8 bytes each (`position_bytes`), or NULL: those of `batch` (rows of no sequence give zeros; otherwise
- * `batch` may be NULL). Angles are taken in 64 bits, the rest in 32. out must not overlap
- * x. */
+ * `batch` may be NULL). Angles are taken in 64 bits, the rest in 32. out must not overlap x. */
 int ancha_paged_rotary(const void *x, int type, size_t rows, size_t heads, size_t dim, size_t ldx, size_t ldh,
                        const void *positions, int position_bytes, const ancha_paged_batch *batch,
                        const ancha_paged_plan *plan, void *out, hipStream_t stream);

@@ -40,6 +40,7 @@ def test_frequencies():
     assert abs(g[2] - f[2] * (share + (1 - share) / 4)) < 1e-17 and abs(m - (0.1 * math.log(4) + 1)) < 1e-15
     assert paged.frequencies(2, 500.0) == ([1.0], 1.0)
     for how, text in (((0,), "width"), ((3,), "width"), ((8, -1.0), "base"), ((8, float("inf")), "base"),
+                      ((64, 2.0 ** -21), "2\\*\\*20"),
                       ((8, 1e4, "dynamic"), "scaling"), ((8, 1e4, "linear", 0.5), "factor"),
                       ((8, 1e4, None, 2.0), "factor"),
                       ((8, 1e4, "yarn", float("nan"), 5), "factor"), ((8, 1e4, "yarn", 2.0), "original"),

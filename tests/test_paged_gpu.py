@@ -187,11 +187,10 @@ def test_write_and_read(gpu, heads, dim, page, width, layout, fmt, kind):
 
 
 def test_write_turns_by_any_angle(gpu):
-    """Angles within rounding of a right angle's multiples, small ones, and beyond 2^40, where another way takes over."""
+    """Angles within rounding of a right angle's multiples, small ones, and up to 2^28."""
     cache, codes, scales = some_cache(gpu, 4, 64, 2, 64, "fp8", 24)
     quarter = np.pi / 2
-    freqs = [quarter, np.nextafter(quarter, 2), -quarter / 2, 1e-9, 0.0, 1.0, -3.7, 512.5, 1e6, 2.0 ** 33 + 0.3, 1e12,
-             3e15]
+    freqs = [quarter, np.nextafter(quarter, 2), -quarter / 2, 1e-9, 0.0, 1.0, -3.7, 512.5, 1e6, 2.0 ** 20 - 0.3]
     plan = paged.Rotary(torch.tensor(freqs, dtype=torch.float64, device=gpu))
     batch, plain, rows = some_batch(gpu, [200], [230], 64, 4, 25)
     k = dev(W.normal((rows, 2, 64), 26, 1.0), gpu)
