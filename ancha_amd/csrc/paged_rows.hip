@@ -27,7 +27,7 @@ __device__ __forceinline__ float2 cos_sin(double a) {
 // The same for keys that are written, within 2^-52 of one: half pi is taken off in two parts by fused multiply-adds,
 // the rest, at most pi / 4, goes through the Taylor series to its 15th and 16th power. That holds below 2^51, which
 // positions and frequencies up to 2^20 do not pass. With the library's function, which reduces any angle, 16 384 keys
-// of 8 x 128 took 72 us to write and read, so 66; with a branch to it for larger angles, 76.
+// of 8 x 128 were written in 40 us instead of 35; with a branch to it for larger angles in 43.
 __device__ __forceinline__ double2 cos_sin_64(double a) {
   const double whole = __builtin_rint(a * 0.6366197723675813430755);
   double r = __builtin_fma(-whole, 1.5707963267948965579990, a);
@@ -145,17 +145,38 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryParams p, int ro
   }
 }
 
+// Place of a pair's cosine and sine in LDS: one free behind every eight, so that lanes eight pairs apart meet different
+// banks.
+__host__ __device__ constexpr int trig_at(int pair) { return pair + pair / 8; }
+
 // Eight columns from col on of a key, rotated in 64 bits: the rounding to the codes is the only one. x: the columns
-// themselves, other: for HALF the other values of their pairs; trig the pairs of the key's row.
+// themselves, other: for HALF the other values of their pairs; trig the pairs of the key's row. Where the eight are all
+// rotated, and for HALF of one half, which is so for most widths, no column is looked at by itself.
 template <bool HALF>
 __device__ __forceinline__ void turn_key(const Plan& plan, int col, const double2* trig, const float* other, float* x) {
   const int pairs = plan.width / 2;
-  if (HALF) {
+  if (HALF && pairs % 8 == 0) {
+    const bool second = col >= pairs;
+    const double2* t = trig + trig_at(second ? col - pairs : col);
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const double s = second ? t[j].y : -t[j].y;
+      x[j] = to_odd(__builtin_fma((double)x[j], t[j].x, (double)other[j] * s));
+    }
+  } else if (!HALF && pairs % 4 == 0) {
+    const double2* t = trig + trig_at(col / 2);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const double a = x[2 * j], b = x[2 * j + 1];
+      x[2 * j] = to_odd(__builtin_fma(a, t[j].x, -(b * t[j].y)));
+      x[2 * j + 1] = to_odd(__builtin_fma(b, t[j].x, a * t[j].y));
+    }
+  } else if (HALF) {
 #pragma unroll
     for (int j = 0; j < 8; j++) {
       const int d = col + j;
       if (d >= plan.width) break;
-      const double2 t = trig[d < pairs ? d : d - pairs];
+      const double2 t = trig[trig_at(d < pairs ? d : d - pairs)];
       const double a = x[j], b = other[j];
       x[j] = d < pairs ? to_odd(a * t.x - b * t.y) : to_odd(a * t.x + b * t.y);
     }
@@ -163,7 +184,7 @@ __device__ __forceinline__ void turn_key(const Plan& plan, int col, const double
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
       if (col + j >= plan.width) break;
-      const double2 t = trig[(col + j) / 2];
+      const double2 t = trig[trig_at((col + j) / 2)];
       const double a = x[j], b = x[j + 1];
       x[j] = to_odd(a * t.x - b * t.y);
       x[j + 1] = to_odd(b * t.x + a * t.y);
@@ -174,35 +195,43 @@ __device__ __forceinline__ void turn_key(const Plan& plan, int col, const double
 // New keys and values into their pages. A workgroup has `rows` rows: their places and their pairs' cosines and sines
 // once (in 64 bits), then eight columns a thread, four threads a block of codes. Rows without a place are left out. The
 // first values are on their way while the places are found and the angles taken. 16 384 tokens of 8 heads of 128 in
-// bf16, 101 MB, take 36 us, of which 20 are the memory's and 6 the rotation in 64 bits: the rest is the latency of one chain (place, angle, values, codes), which one, two or eight rows a workgroup, rows dealt
-// by XCD, or the next values fetched ahead did not shorten. 32 tokens take 5 us.
+// bf16, 101 MB, take 30 us, of which 20 are the memory's; the vector instructions bound it (with a decision for every
+// column and sines side by side in LDS 35 us, then 90 % busy). One, two or eight rows a workgroup, rows dealt by XCD, or
+// the next values fetched ahead changed nothing. 32 tokens take 5 us.
 template <int TYPE, int FORMAT, bool HALF>
-__global__ __launch_bounds__(kThreads) void write_kernel(WriteParams p, int rows, Divide by_row) {
+__global__ __launch_bounds__(kThreads) void write_kernel(WriteParams p, int rows, Divide by_row, Divide by_pair) {
   typedef typename Stored<TYPE>::type T;
-  __shared__ double2 trig[kTrig / 2];
+  __shared__ double2 trig[trig_at(kTrig / 2)];
   __shared__ int2 places[kMostRows];  // page (or -1) and position
   const int pairs = p.plan.freqs ? p.plan.width / 2 : 0;
   const long first = (long)blockIdx.x * rows;
   const int mine = (int)min((long)rows, p.rows - first);
   const int dim = p.cache.dim, heads = p.cache.heads;
-  const int units = dim / 8;  // of a head; a multiple of 4, so a block's threads stay together
+  const int units = dim / 8;  // of a head; 8, 16 or 32, so a block's threads stay together
+  const int shift = __builtin_ctz(units);
   const int total = mine * 2 * heads * units;
   struct Unit {
     int row, which, head, col;
     float x[8], other[8];
   };
+  const auto eight = [](const T* from, float* x) {
+    T t[8];
+    __builtin_memcpy(t, from, sizeof(t));
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = (float)t[j];
+  };
   const auto load = [&](int i, Unit& u) {
     u.row = (int)divided(i, by_row);
-    const int in_row = i - u.row * 2 * heads * units, both = in_row / units;
-    u.col = 8 * (in_row - both * units);
+    const int in_row = i - u.row * 2 * heads * units, both = in_row >> shift;
+    u.col = 8 * (in_row & (units - 1));
     u.which = both >= heads, u.head = both - u.which * heads;
     const T* row = u.which ? static_cast<const T*>(p.v) + (first + u.row) * p.ldv + u.head * p.ldvh
                            : static_cast<const T*>(p.k) + (first + u.row) * p.ldk + u.head * p.ldkh;
-    load_row<TYPE, 8>(row, u.col, 8, u.x);
+    eight(row + u.col, u.x);
     if (!HALF || u.which || u.col >= 2 * pairs) return;
     // Eight neighbours, unless the eight cross from one half to the other.
     if (pairs % 8 == 0) {
-      load_row<TYPE, 8>(row, u.col < pairs ? u.col + pairs : u.col - pairs, 8, u.other);
+      eight(row + (u.col < pairs ? u.col + pairs : u.col - pairs), u.other);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; j++) {
@@ -220,16 +249,16 @@ __global__ __launch_bounds__(kThreads) void write_kernel(WriteParams p, int rows
   }
   __syncthreads();
   for (int i = threadIdx.x; i < mine * pairs; i += kThreads) {
-    const int r = i / pairs;
-    const double2 t = cos_sin_64((double)places[r].y * p.plan.freqs[i - r * pairs]);
-    trig[i] = make_double2(p.plan.magnitude * t.x, p.plan.magnitude * t.y);
+    const int r = (int)divided(i, by_pair), pair = i - r * pairs;
+    const double2 t = cos_sin_64((double)places[r].y * p.plan.freqs[pair]);
+    trig[r * trig_at(pairs) + trig_at(pair)] = make_double2(p.plan.magnitude * t.x, p.plan.magnitude * t.y);
   }
   __syncthreads();
   saturate();
   for (int i = threadIdx.x; i < total;) {
     const int2 to = places[u.row];
     if (to.x >= 0) {
-      if (!u.which && u.col < 2 * pairs) turn_key<HALF>(p.plan, u.col, trig + u.row * pairs, u.other, u.x);
+      if (!u.which && u.col < 2 * pairs) turn_key<HALF>(p.plan, u.col, trig + u.row * trig_at(pairs), u.other, u.x);
       const long slot = slot_of(p.cache, u.which, to.x, u.head, to.y & ((1 << p.cache.shift) - 1));
       uint8_t* const codes = p.cache.codes + slot * row_bytes(dim, FORMAT);
       store_codes(u.x, FORMAT, true, codes + (FORMAT == kFp8 ? u.col : u.col / 2),
@@ -256,11 +285,11 @@ __global__ __launch_bounds__(kThreads) void read_kernel(ReadParams p, int tokens
     places[t] = make_int2(page, at & ((1 << p.cache.shift) - 1));
   }
   __syncthreads();
-  const int dim = p.cache.dim, heads = p.cache.heads, units = dim / N;
+  const int dim = p.cache.dim, heads = p.cache.heads, units = dim / N, shift = __builtin_ctz(units);
   const int total = mine * 2 * heads * units;
   for (int i = threadIdx.x; i < total; i += kThreads) {
     const int t = (int)divided(i, by_token), in_token = i - t * 2 * heads * units;
-    const int both = in_token / units, col = N * (in_token - both * units);
+    const int both = in_token >> shift, col = N * (in_token & (units - 1));
     const int which = both >= heads, head = both - which * heads;
     const int2 from = places[t];
     float v[N];
@@ -320,10 +349,11 @@ void start_write(const WriteParams& p, hipStream_t stream) {
   const int units = 2 * p.cache.heads * p.cache.dim / 8;
   const int rows = max(1, min(min(4, 4096 / units), p.rows / 512));
   const dim3 grid((unsigned)((p.rows + (long)rows - 1) / rows));
+  const Divide by_row = divide_by(units), by_pair = divide_by(max(p.plan.freqs ? p.plan.width / 2 : 1, 1));
   if (p.plan.interleaved)
-    hipLaunchKernelGGL((write_kernel<TYPE, FORMAT, false>), grid, dim3(kThreads), 0, stream, p, rows, divide_by(units));
+    hipLaunchKernelGGL((write_kernel<TYPE, FORMAT, false>), grid, dim3(kThreads), 0, stream, p, rows, by_row, by_pair);
   else
-    hipLaunchKernelGGL((write_kernel<TYPE, FORMAT, true>), grid, dim3(kThreads), 0, stream, p, rows, divide_by(units));
+    hipLaunchKernelGGL((write_kernel<TYPE, FORMAT, true>), grid, dim3(kThreads), 0, stream, p, rows, by_row, by_pair);
 }
 
 template <int TYPE, int FORMAT>

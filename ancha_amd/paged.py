@@ -68,8 +68,9 @@ class Batch:
 
 class Rotary:
     """Rotary positions, made by :func:`rotary_plan` or of frequencies of one's own: ``freqs`` [width / 2] float64 on
-    the GPU, radians a position of each pair, at most 2**20 in magnitude. The first ``width`` columns of a head are turned, in pairs
-    (i, i + width / 2) for the layout "half" and (2 i, 2 i + 1) for "interleaved", and multiplied by ``magnitude``."""
+    the GPU, radians a position of each pair, at most 2**20 in magnitude. The first ``width`` columns of a head are
+    turned, in pairs (i, i + width / 2) for the layout "half" and (2 i, 2 i + 1) for "interleaved", and multiplied by
+    ``magnitude``."""
 
     def __init__(self, freqs: torch.Tensor, layout: str = "half", magnitude: float = 1.0):
         if layout not in _LAYOUTS:

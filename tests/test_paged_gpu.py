@@ -7,11 +7,11 @@ from 64 bits: the oracle's bytes.
 Attention, with A = sum_j w_j |v_j| of a row: scores are sums of exact products, D / 32 instructions a part of q, each
 of which adds at most one step (2^-23) of the largest of its terms twice; three parts hold 24 bits of q. With R the
 largest scale sum |q k|, a score is within e = (D / 32 * parts + 4) 2^-22 R, and so the result within 2 e A.
-Exponentials are good to 2^-21, weights to half a step of fp16 (fp32 results: 2^-21), in the products and in the sum that divides them:
-2^-11 (A + |o|). Each weight that is less than fp16 holds is off by
-2^-25 where the largest is 2^6 to 2^15, so by 2^-31 of it: 2^-31 sum_j |v_j| in all. Values are off by 2^-25 where the
-largest of their block is 2^11 or more, less than 2^-32 of it. Then the result's type: half its eps, and
-below its normal values, where its steps no longer shrink, half of their step (fp16: 2^-25).
+Exponentials are good to 2^-21, weights to half a step of fp16 (fp32 results: 2^-21), in the products and in the sum
+that divides them: 2^-11 (A + |o|). Each weight that is less than fp16 holds is off by 2^-25 where the largest is 2^6
+to 2^15, so by 2^-31 of it: 2^-31 sum_j |v_j| in all. Values are off by 2^-25 where the largest of their block is 2^11
+or more, less than 2^-32 of it. Then the result's type: half its eps, and below its normal values, where its steps no
+longer shrink, half of their step (fp16: 2^-25).
 """
 import numpy as np
 import pytest
