@@ -196,8 +196,8 @@ __device__ __forceinline__ void turn_key(const Plan& plan, int col, const double
 // once (in 64 bits), then eight columns a thread, four threads a block of codes. Rows without a place are left out. The
 // first values are on their way while the places are found and the angles taken. 16 384 tokens of 8 heads of 128 in
 // bf16, 101 MB, take 30 us, of which 20 are the memory's; the vector instructions bound it (with a decision for every
-// column and sines side by side in LDS 35 us, then 90 % busy). One, two or eight rows a workgroup, rows dealt by XCD, or
-// the next values fetched ahead changed nothing. 32 tokens take 5 us.
+// column and sines side by side in LDS 35 us, then 90 % busy). One, two or eight rows a workgroup, rows dealt by XCD,
+// or the next values fetched ahead changed nothing. 32 tokens take 5 us.
 template <int TYPE, int FORMAT, bool HALF>
 __global__ __launch_bounds__(kThreads) void write_kernel(WriteParams p, int rows, Divide by_row, Divide by_pair) {
   typedef typename Stored<TYPE>::type T;
