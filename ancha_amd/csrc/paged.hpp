@@ -40,13 +40,13 @@ struct Plan {
   double magnitude;
 };
 
-// New tokens [first, first + count) of the rows, of which the last has position length - 1.
+// New tokens [first, first + count) of the rows, the first at position `at`; the sequence has `length` with them.
 struct Sequence {
-  int first, count, length;
+  int first, count, length, at;
 };
 __device__ __forceinline__ Sequence sequence(const Batch& b, int i, int rows) {
-  const int from = min(max(b.starts[i], 0), rows), to = min(max(b.starts[i + 1], from), rows);
-  return {from, to - from, max(b.lengths[i], 0)};
+  const int from = min(max(b.starts[i], 0), rows), end = max(b.starts[i + 1], from), length = max(b.lengths[i], 0);
+  return {from, min(end, rows) - from, length, length - (end - from)};
 }
 
 // The sequence that row r is of, and its position (false: of none); a wave's lanes look together, r is the same in all.

@@ -68,7 +68,7 @@ struct Range {
 __device__ __forceinline__ Range visible(const AttentionParams& p, const Sequence& s, int token) {
   // Some steps below 2^31, so that a step ahead of the last one is still a number.
   const int capacity = (int)min((long)p.batch.columns << p.cache.shift, 0x7fff0000l);
-  const long at = (long)s.length - s.count + token;
+  const long at = (long)s.at + token;
   const long high = p.causal ? at + 1 : s.length, low = p.window ? at - p.window + 1 : 0;
   const int h = (int)min(max(high, 0l), (long)capacity);
   return {(int)min(max(low, 0l), (long)h), h};
@@ -80,7 +80,7 @@ __device__ __forceinline__ bool find_tile(const AttentionParams& p, int group, i
                                           int& row) {
   const int lane = threadIdx.x & 63;
   for (int base = 0; base < p.batch.sequences; base += 64) {
-    Sequence mine = {0, 0, 0};
+    Sequence mine = {0, 0, 0, 0};
     if (base + lane < p.batch.sequences) mine = sequence(p.batch, base + lane, p.rows);
     // At most 2^24 (a call has fewer): starts that do not ascend cannot make the sums overflow.
     const int tiles = (int)min(((long)mine.count * group + rows - 1) / rows, 1l << 24);
@@ -105,6 +105,7 @@ __device__ __forceinline__ bool find_tile(const AttentionParams& p, int group, i
       s.first = __builtin_amdgcn_readlane(mine.first, at);
       s.count = __builtin_amdgcn_readlane(mine.count, at);
       s.length = __builtin_amdgcn_readlane(mine.length, at);
+      s.at = __builtin_amdgcn_readlane(mine.at, at);
       row = (id - (__builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(tiles, at))) * rows;
       return true;
     }

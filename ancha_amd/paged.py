@@ -290,5 +290,5 @@ def attention(q: torch.Tensor, cache: Cache, batch: Batch, scale: Optional[float
     need = _native.lib().ancha_paged_attention_workspace(kind, rows, heads, cache._at, batch._at)
     workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     return out if _launch(device.index, "ancha_paged_attention", q.data_ptr(), kind, rows, heads, row, head,
-                          cache._at, batch._at, scale, int(causal), window or 0,
+                          cache._at, batch._at, scale, int(causal), min(window or 0, 2 ** 31),
                           None if workspace is None else workspace.data_ptr(), need, out.data_ptr()) else None

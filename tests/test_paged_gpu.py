@@ -452,6 +452,25 @@ def test_attention_infinite_queries(gpu):
     assert torch.isnan(got).any(2).cpu().equal(nan)
 
 
+@pytest.mark.parametrize("rows", [1, 9, 40, 170])
+def test_a_batch_of_more_rows_than_there_are(gpu, rows):
+    """The first rows of a batch's: each at the position that the batch gives it, in a write, a turn and attention."""
+    cache, codes, scales = some_cache(gpu, 40, 16, 2, 64, "fp8", 71)
+    batch, plain, _ = some_batch(gpu, [8, 0, 30, 200], [100, 5, 30, 210], 16, 40, 72)
+    plan = paged.rotary_plan(64, device=gpu)
+    k, v = dev(W.normal((rows, 2, 64), 73, 1.0), gpu), dev(W.normal((rows, 2, 64), 74, 1.0), gpu)
+    at = np.zeros(rows)
+    for r, _, position in O.rows_of(plain, rows):
+        at[r] = position
+    turned = O.rotate(host(k), at, plan.freqs.tolist())
+    cache.write(k, v, batch, plan)
+    O.write(codes, scales, "fp8", turned, host(v), plain)
+    assert np.array_equal(cache.codes.cpu().numpy(), codes) and np.array_equal(cache.scales.cpu().numpy(), scales)
+    close("rotary", paged.rotary(k, batch, plan), turned, rotary_tolerance(host(k), plan, turned, torch.float32))
+    for causal, window in ((True, None), (False, None), (True, 7), (True, 2 ** 70)):
+        check_attention(gpu, "bf16", 8, cache, codes, scales, batch, plain, rows, 75, causal=causal, window=window)
+
+
 def test_attention_of_nothing(gpu):
     cache, _, _ = some_cache(gpu, 4, 16, 2, 64, "fp8", 131)
     none = paged.Batch(ints([0], gpu), ints([], gpu), torch.zeros((0, 3), dtype=torch.int32, device=gpu))
