@@ -25,7 +25,7 @@ constexpr int kStep = 32;  // keys
 //   V        the same eight keys as its weights, columns D / 16 * c on, transposed in registers two by two.
 // Nothing passes through LDS before the waves' sums are joined. Bound by the reading of the cache while there are
 // few rows: with 8 heads of 128 for 32 of q, 64 sequences of up to 8192 tokens in e4m3 (558 MB) take 119 us, 4.7 TB/s,
-// one of 131 072 in e2m1 (143 MB) 32 us and 6 to join its parts, one of 801 tokens 8 us and 4, which is the latency of
+// one of 131 072 in e2m1 (143 MB) 32 us and 6 to join its parts, one of 2048 tokens 8 us and 3, which is the latency of
 // a few dependent reads. A page's number is read two steps ahead and codes one: with both one step ahead the first took
 // 183 us, not 142, and the second 77, not 57; codes two steps ahead changed nothing. With eight waves, twice the reads
 // in flight, they took 137 and 43 us, and 32 sequences of 8192 with heads of 64 in fp32 51 instead of 77.
@@ -498,6 +498,10 @@ AttentionForm attention_form(const AttentionParams& p) {
   const long slots = (chunk ? chunk_waves(p.cache.dim, p.type) == 8 : f.form == kTiles8) ? 256 : 512;
   const long full = some ? some * ((rows + some * of - 1) / (some * of)) : 1;
   f.splits = (int)min(max(slots / (full * p.cache.heads), 1l), min(keys / kLeastKeys + 1, 256l));
+  // Sharing saves a tile's waves these keys and costs a second launch. Both measured (shared / not), one row a head: 400
+  // keys 10.9 / 9.5 us, 801 11.0 / 11.6 (heads of 64 in fp32 10.5 / 9.7), 1100 11.1 / 13.2; 16 sequences of 801 keys
+  // 16.5 / 12.7, of 2048 21.6 / 23.2.
+  if (!chunk && keys * (f.splits - 1) < (f.form == kTiles8 ? 640 : 320) * f.splits) f.splits = 1;
   if (f.splits > 1)
     f.bytes = 4 * (size_t)(joined_floats(f.tiles, p.cache.heads) + groups * f.splits * part_floats(of, p.cache.dim));
   return f;

@@ -314,7 +314,7 @@ def form(kind, rows, heads, cache, batch):
 @pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("dim,fmt", [(64, "fp8"), (64, "fp4"), (128, "fp8"), (128, "fp4"), (256, "fp8")])
 @pytest.mark.parametrize("new,lengths,heads,kv,page,columns", [
-    ([257, 130, 1], [257, 411, 300], 4, 2, 32, 20),       # tiles of 16 rows
+    ([257, 130, 1], [257, 411, 300], 4, 2, 32, 44),       # tiles of 16 rows
     ([257, 130, 80], [257, 411, 300], 4, 2, 32, 600),     # room for long sequences: the chunk kernel, shared keys
     ([64, 100], [900, 100], 16, 2, 16, 1200),             # shared by several, the last part short
     ([100, 0, 37, 90], [64, 50, 1100, 90], 21, 3, 64, 500),  # rows without keys, sevens of heads
