@@ -225,8 +225,8 @@ class Cache:
               plan: Optional[Rotary] = None) -> Optional["Cache"]:
         """The rows' keys and values [rows, heads, dim] into the places that ``batch`` gives them, keys first turned by
         ``plan`` where there is one. Rotated in 64 bits, so the rounding to the codes is the only one; a NaN or an
-        infinity makes its block of 32 NaN. Rows of no sequence, in a page that is not there or at a position below 0
-        are left out. No two rows may have the same place."""
+        infinity (2**128 or more) makes its block of 32 NaN. Rows of no sequence, in a page that is not there or at a
+        position below 0 are left out. No two rows may have the same place."""
         kind = _take(k, "k")
         require(v, "v", self.device, k.shape, k.dtype)
         if k.device != self.device or k.shape[1:] != (self.heads, self.dim):

@@ -379,8 +379,8 @@ int ancha_paged_rotary(const void *x, int type, size_t rows, size_t heads, size_
                        const ancha_paged_plan *plan, void *out, hipStream_t stream);
 
 /* The rows' keys (rotated, if plan is not NULL) and values into their places: rotation in 64 bits, so the rounding to
- * the codes is the only one. Rows without a place are left out. Element (row, head, d) of k at row * ldk + head * ldkh
- * + d, of v likewise. */
+ * the codes is the only one (2^128 and more count as infinite). Rows without a place are left out. Element (row, head,
+ * d) of k at row * ldk + head * ldkh + d, of v likewise. */
 int ancha_paged_write(const void *k, const void *v, int type, size_t rows, size_t ldk, size_t ldkh, size_t ldv,
                       size_t ldvh, const ancha_paged_batch *batch, const ancha_paged_plan *plan,
                       const ancha_paged_cache *cache, hipStream_t stream);

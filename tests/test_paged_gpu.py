@@ -222,6 +222,31 @@ def test_write_special_values_and_layouts(gpu, fmt):
                                                                                            device=gpu))) is cache
 
 
+@pytest.mark.parametrize("fmt", ["fp8", "fp4"])
+@pytest.mark.parametrize("layout,width", [("half", 64), ("half", 40), ("interleaved", 64), ("interleaved", 36)])
+def test_write_turns_special_values(gpu, layout, width, fmt):
+    """NaN, infinities and sums of 2^128 or more in a turned key make their blocks NaN, no others."""
+    cache, codes, scales = some_cache(gpu, 4, 16, 3, 64, fmt, 27)
+    batch, plain, rows = some_batch(gpu, [9], [21], 16, 4, 28)
+    plan = paged.rotary_plan(width, layout=layout, device=gpu)
+    k = dev(W.normal((rows, 3, 64), 29, 1.0), gpu)
+    k[0, 0, 0], k[1, 1, 33], k[2, 2, 5], k[3, 0, 63] = float("nan"), float("inf"), float("-inf"), float("inf")
+    k[4, 1] = 3.3e38
+    k[5, 2] *= 2.0 ** -130
+    k[6, 0] = 0.0
+    at = np.zeros(rows)
+    for r, _, position in O.rows_of(plain, rows):
+        at[r] = position
+    with np.errstate(invalid="ignore"):
+        turned = O.rotate(host(k), at, plan.freqs.tolist(), layout)
+    turned[np.abs(turned) >= 2.0 ** 128] = np.inf
+    assert np.isinf(turned[4, 1]).any() and np.isfinite(turned[4, 1]).any()
+    cache.write(k, -k.flip(2), batch, plan)
+    O.write(codes, scales, fmt, turned, host(-k.flip(2)), plain)
+    assert np.array_equal(cache.scales.cpu().numpy(), scales)
+    assert np.array_equal(cache.codes.cpu().numpy(), codes)
+
+
 def test_pages_that_are_not_there(gpu):
     """Numbers outside the cache, columns behind the table and places below 0: not written, read as zeros, not seen."""
     cache, codes, scales = some_cache(gpu, 6, 16, 2, 64, "fp8", 31)
