@@ -201,7 +201,7 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
     const bool here = (unsigned)w_.page < (unsigned)p.cache.pages && at_key >= w.first && at_key < w.high;
     last_there = __ballot(here);
     int e[kScales];
-    bool over = false;  // a block that is larger than its reference allows, or NaN
+    bool over = false;  // a block that is larger than its reference allows, or NaN (255)
 #pragma unroll
     for (int c = 0; c < kScales; c++) {
       e[c] = here ? (int)(w_.vs >> 8 * c & 255u) : 0;
@@ -218,7 +218,8 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) x = max(x, __shfl_xor(x, o));
         x = __builtin_amdgcn_readfirstlane(x);
-        ref[c] = x > ref[c] + kMost ? x - kTaken : ref[c];
+        // At most 254 - kMost, which has room for the largest byte of a number and leaves 255 above it.
+        ref[c] = x > ref[c] + kMost ? min(x - kTaken, 254 - kMost) : ref[c];
       }
       last_bad = __any(nan != 0);
       mine[S::kPowers + to * kKeys + lane] = nan;
