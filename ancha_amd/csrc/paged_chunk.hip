@@ -24,7 +24,7 @@ __device__ __forceinline__ void wave_sync() {
 template <int D, int FORMAT, int TYPE>
 struct Shape {
   static constexpr int kQ = TYPE == kBf16 ? 1 : TYPE == kF16 ? 2 : 3;  // bf16 parts of a query
-  static constexpr int kP = TYPE == kF32 ? 2 : 1;                      // fp16 parts of a weight
+  static constexpr int kP = 2;                                         // fp16 parts of a weight
   static constexpr int kWaves = chunk_waves(D, TYPE), kThreads = 64 * kWaves, kRows = 32 * kWaves;
   static constexpr int kScales = D / kBlock;            // scale bytes a token
   static constexpr int kBuffer = 2 * kKeys * D * 2;     // LDS bytes of a step's keys and values
@@ -42,13 +42,14 @@ struct Shape {
 // A block of 32 columns is one of the cache's own, so its reference power is one number a workgroup.
 //
 // Bound by the matrix units and what runs beside them: a prompt of 8192 tokens, 32 heads over 8 of 128 in bf16, is 0.55
-// TFLOP and takes 612 to 630 us replayed, 0.88 PFLOP/s, where a library product of 8192^3 reaches 1.3 on the same card;
-// 4 times 801 rows of 8 heads of 64 over 4096 keys, in fp32, 68 us and 6 to join. For the prompt, with the products
-// alone it is 389 us, without bringing the codes 513, without the exponentials 611. What did not help, against 655 us
-// at that time: 64 rows a wave with one wave a SIMD 946; both halves of a step at once 636; four reads ahead of the
-// products 698; groups given to the scheduler 700; wave priorities 690; sums by adds 675 or by a product with ones 655;
-// the next half's scores ahead of these weights, codes two steps ahead: no change. fp16 results have weights of one
-// part, 11 bits as they have themselves: a second would be half as many products again.
+// TFLOP and takes 793 us replayed, 0.69 PFLOP/s; with the weights' second part it is 0.82 TFLOP of products, 1.04
+// PFLOP/s, where a library product of 8192^3 reaches 1.3 on the same card. 4 times 801 rows of 8 heads of 64 over 4096
+// keys, in fp32, take 68 us and 6 to join. With weights of one part, 11 bits, the prompt took 615 us; of that build:
+// with the products alone 389 us, without bringing the codes 513, without the exponentials 611. What did not help an
+// earlier one of 655 us: 64 rows a wave with one wave a SIMD 946; four reads ahead of the products 698; groups given to
+// the scheduler 700; wave priorities 690; sums by adds 675 or by a product with ones 655; the next half's scores ahead
+// of these weights, codes two steps ahead: no change. Both halves of a step at once made that one 3 % faster, 636, and
+// have not been tried on this one.
 template <int D, int FORMAT, int TYPE>
 __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void chunk_kernel(AttentionParams p) {
   typedef typename Stored<TYPE>::type T;
@@ -371,15 +372,10 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
           const float b = fast_exp2(__builtin_fmaf(x[2 * j + 1], p.scale, base));
           const unsigned two = pack_h2(a, b);
           weight[0][j / 4][j % 4] = two;
-          if constexpr (kP == 1) {
-            // The sum of the rounded weights, so that they are a mean's.
-            l = __builtin_amdgcn_fdot2(__builtin_bit_cast(h16x2, two), h16x2{1, 1}, l, false);
-          } else {
-            const h16x2 high = __builtin_bit_cast(h16x2, two);
-            weight[1][j / 4][j % 4] = pack_h2(a - (float)high[0], b - (float)high[1]);
-            l += a;
-            l += b;
-          }
+          const h16x2 high = __builtin_bit_cast(h16x2, two);
+          weight[1][j / 4][j % 4] = pack_h2(a - (float)high[0], b - (float)high[1]);
+          l += a;
+          l += b;
         }
 #pragma unroll
         for (int v = 0; v < 2; v++)

@@ -1,5 +1,5 @@
 """Attention over a paged cache where its numbers are at their limits, against the 64-bit oracle: values and NaN in the
-cache of any size. Both kernels, tiles and chunks.
+cache of any size, weights to 22 bits. Both kernels, tiles and chunks.
 """
 import numpy as np
 import pytest
@@ -8,7 +8,7 @@ import torch
 from ancha_amd import paged
 from ancha_amd import workload as W
 from oracle import paged as O
-from tests.test_paged_gpu import CHUNK, TYPES, dev, form, host, some_batch, some_cache
+from tests.test_paged_gpu import CHUNK, PARTS, TYPES, close, dev, form, host, rounding, some_batch, some_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +53,28 @@ def test_a_nan_is_seen_behind_any_scale(gpu, byte, heads, columns):
     want = np.zeros(got.shape, bool)
     want[150:, heads // 2:, :32] = True
     assert np.array_equal(got, want), f"NaN in {got.sum()} places, not {want.sum()}"
+
+
+def tight(kind, want, size, total, reach, dim, blocks, small=31):
+    """What scores in 32 bits, weights in two fp16 parts and one rounding to the type leave: each weight is off by 2^-22
+    of itself, in the products and in the sum that divides them, or by 2^-small of its row's largest. blocks: the largest
+    value of each column's block."""
+    e = (dim // 32 * PARTS[kind] + 4) * 2.0 ** -22 * reach
+    tol = size * (2 * e + 2.0 ** -20) + np.abs(want) * 2.0 ** -21 + rounding(want, TYPES[kind])
+    return tol + total * 2.0 ** -small + blocks * 2.0 ** -32
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("dim,fmt", [(64, "fp8"), (64, "fp4"), (128, "fp8"), (128, "fp4"), (256, "fp8"), (256, "fp4")])
+@pytest.mark.parametrize("new,lengths,heads,columns", [([1, 1, 1], [300, 17, 2100], 8, None), ([3, 1], [700, 90], 6, 600),
+                                                       ([100, 130], [300, 130], 20, 2000)])
+def test_results_are_rounded_once(gpu, new, lengths, heads, columns, dim, fmt, kind):
+    """Whatever the kernel: nothing but the result's type rounds to fewer than 22 bits."""
+    pages = sum(-(-n // 16) for n in lengths) + 1
+    cache, codes, scales = some_cache(gpu, pages, 16, 2, dim, fmt, 221, big=0.0)
+    batch, plain, rows = some_batch(gpu, new, lengths, 16, pages, 222, columns=columns)
+    assert (form(kind, rows, heads, cache, batch)[0] == CHUNK) == (columns == 2000 and dim < 256)
+    q = dev(0.1 * W.normal((rows, heads, dim), 223, 1.0), gpu, TYPES[kind])
+    want, size, total, reach = O.attention(host(q), codes, scales, fmt, plain)
+    blocks = np.exp2(scales[1].max((0, 1, 2)) - 127.0).repeat(32) * (448 if fmt == "fp8" else 6)
+    close("once", paged.attention(q, cache, batch), want, tight(kind, want, size, total, reach, dim, blocks))
