@@ -49,8 +49,11 @@ __global__ __launch_bounds__(64 * WAVES) void attention_kernel(AttentionParams p
   // few less, so a block may grow by 8 (fp8) or 16 times before the sums are scaled.
   constexpr int kMost = FORMAT == kFp8 ? 7 : 13, kTaken = FORMAT == kFp8 ? 4 : 9;
   constexpr int kNoRef = -1000;
-  // Weights are e^.. 2^kUp: a maximum may lag 2^8 behind before the sums are scaled, and small weights keep their bits.
-  constexpr float kUp = 7.f, kLag = 8.f;
+  // Weights are e^.. 2^kUp: a maximum may lag 2^2 behind before the sums are scaled. The row's largest is 2^12 or more
+  // and fp16's second part ends at 2^-25, so a weight is off by 2^-37 of it where that is more than its own 22 bits. With
+  // 2^7 and a lag of 2^8 it was 2^-31, and a first token that took the scores but had no value left 250 others e^-23 of
+  // it with none; a prompt of 8192 tokens took 814 us then and 818 now, with a lag of 2^1 826.
+  constexpr float kUp = 13.f, kLag = 2.f;
 
   const int group = p.heads / p.cache.heads;
   int id = blockIdx.x / (p.splits * p.cache.heads), i, row;

@@ -65,7 +65,7 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
   constexpr int kTurn = 8 / kScales;                                             // see slot_of_key
   constexpr int kMost = FORMAT == kFp8 ? 7 : 13, kTaken = FORMAT == kFp8 ? 4 : 9;  // see paged_attention.hip
   constexpr int kNoRef = -1000;
-  constexpr float kUp = 7.f, kLag = 8.f;
+  constexpr float kUp = 13.f, kLag = 2.f;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
 
   const int group = p.heads / p.cache.heads;

@@ -269,10 +269,11 @@ def attention(q: torch.Tensor, cache: Cache, batch: Batch, scale: Optional[float
     all of its sequence (an encoder's states), and with ``window`` none before ``t - window + 1``. Rows that see no
     token and rows of no sequence are 0. ``scale`` > 0 is 1 / sqrt(dim) if not given.
 
-    Scores are exact to 32 bits for every type of q; the weights are held to 22 bits and sums in 32, so a result is
-    rounded to its type once. Values more than 2**30 below the largest of their head's block of 32 columns may be
-    rounded. A NaN in the cache reaches the rows that see its token, no others. How the keys are shared out depends on
-    shapes and lengths alone, so a call gives the same bits every time."""
+    Scores are exact to 32 bits for every type of q; weights are off by 2**-21 of themselves at most or by 2**-37 of
+    their row's largest, and sums are held in 32, so a result is rounded to its type once. Values more than 2**30 below
+    the largest of their head's block of 32 columns may be rounded. A NaN in the cache reaches the rows that see its
+    token, no others. How the keys are shared out depends on shapes and lengths alone, so a call gives the same bits
+    every time."""
     kind = _take(q, "q")
     device = q.device
     _on(cache, "cache", Cache, device)

@@ -394,8 +394,8 @@ int ancha_paged_read(const ancha_paged_cache *cache, const ancha_paged_batch *ba
  * heads / cache heads neighbouring heads of q for each head of the cache; element (row, head, d) of q at row * ldq +
  * head * ldqh + d. A row at position t sees the tokens up to t (with `causal`, otherwise all of its sequence) and, with
  * window > 0, none before t - window + 1. Rows that see no token and rows of no sequence are 0. Scores of any q are
- * exact to fp32, weights have 22 bits, sums are fp32, and the result is rounded to its type once. A NaN in the cache
- * reaches the rows that see it.
+ * exact to fp32, weights are off by 2^-21 of themselves at most or by 2^-37 of their row's largest, sums are fp32, and
+ * the result is rounded to its type once. A NaN in the cache reaches the rows that see it.
  * workspace: ancha_paged_attention_workspace bytes (of the same arguments; may be 0 and NULL), 16-byte aligned, not
  * shared with a call that may run at the same time. */
 size_t ancha_paged_attention_workspace(int type, size_t rows, size_t heads, const ancha_paged_cache *cache,

@@ -1,5 +1,5 @@
 """Attention over a paged cache where its numbers are at their limits, against the 64-bit oracle: values and NaN in the
-cache of any size, weights to 22 bits. Both kernels, tiles and chunks.
+cache of any size, weights to 22 bits and small ones. Both kernels, tiles and chunks.
 """
 import numpy as np
 import pytest
@@ -78,3 +78,28 @@ def test_results_are_rounded_once(gpu, new, lengths, heads, columns, dim, fmt, k
     want, size, total, reach = O.attention(host(q), codes, scales, fmt, plain)
     blocks = np.exp2(scales[1].max((0, 1, 2)) - 127.0).repeat(32) * (448 if fmt == "fp8" else 6)
     close("once", paged.attention(q, cache, batch), want, tight(kind, want, size, total, reach, dim, blocks))
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("heads,columns", FORMS)
+@pytest.mark.parametrize("gap", [10.0, 17.0, 23.0])
+@pytest.mark.parametrize("length", [250, 4100])
+def test_many_small_weights_beside_a_large_one(gpu, length, gap, heads, columns, kind):
+    """A first token that takes the scores but has no value, and others `gap` below it, all alike, so that what their
+    weights lose does not cancel: 2^-37 of the first one's each."""
+    cache, codes, scales = some_cache(gpu, 65, 64, 2, 64, "fp8", 231)
+    batch, plain, rows = some_batch(gpu, [40], [length], 64, 65, 232, columns=columns)
+    assert (form(kind, rows, heads, cache, batch)[0] == CHUNK) == bool(columns)
+    codes[0], scales[0] = 0, 0
+    codes[1] &= 0x7f  # values of one sign, so that their sum does not cancel either
+    page, slot = O.place(plain, 0, 0, 65, 64)
+    codes[0, page, :, slot, 0], scales[0, page, :, slot, 0], codes[1, page, :, slot] = 0x38, 127, 0
+    cache = on(gpu, codes, scales, "fp8")
+    q = torch.zeros((rows, heads, 64), device=gpu, dtype=TYPES[kind])
+    q[:, :, 0] = gap
+    want, size, total, reach = O.attention(host(q), codes, scales, "fp8", plain, scale=1.0)
+    blocks = np.exp2(scales[1].max((0, 1, 2)) - 127.0).repeat(32) * 448
+    # The values' own error comes with the weights of those that have one: `length` of size / total at most.
+    blocks = blocks * np.minimum(1, length * size / np.maximum(total, 1e-30))
+    tol = tight(kind, want, size, total, reach, 64, blocks, 37)
+    close("small", paged.attention(q, cache, batch, scale=1.0), want, tol)
