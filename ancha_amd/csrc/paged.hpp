@@ -118,7 +118,7 @@ struct AttentionParams {
   float* parts;  // workspace of a split, see attention_form
   long ldq, ldqh;
   int rows, heads, type, causal, window;  // window 0: none
-  float scale;                            // of the scores, times log2(e)
+  float scale, unscale;                   // of the scores, times log2(e), and its inverse
   int tiles, splits, form;                // of its AttentionForm
 };
 

@@ -153,6 +153,8 @@ __global__ __launch_bounds__(64 * WAVES) void attention_kernel(AttentionParams p
   };
 
   float m = -__builtin_inff(), l = 0.f;  // of row c: a whole number near its maximum, and this lane's share of the sum
+  float base = 0.f;                      // what its scores get to be the exponents of its weights
+  bool far = false;                      // whether any row's maximum is, see is_far
   bool any = false;                      // whether this lane has met a key that the row sees
   unsigned none = 0;                     // a bit for each element of its sums in which the row sees a NaN
   int ref = kNoRef;                      // of the block that this lane has columns of
@@ -251,7 +253,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_kernel(AttentionParams p
 #pragma unroll
     for (int j = 2; j < 8; j++) top = fmaxf(top, x[j]);
     top *= p.scale;
-    if (__any(top > m + kLag)) {
+    if (__any(top > m + kLag) || far) {
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
       const float to = fmaxf(m, __builtin_ceilf(top));
@@ -260,8 +262,12 @@ __global__ __launch_bounds__(64 * WAVES) void attention_kernel(AttentionParams p
       l *= f;
 #pragma unroll
       for (int t = 0; t < kCols; t++) acc[t] *= f;
+      base = base_of(m, kUp);
+      far = __any(is_far(m));
+      if (far)
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = is_far(m) ? behind(p, x[j], m) : x[j];
     }
-    const float base = m == -__builtin_inff() ? 0.f : kUp - m;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
       x[j] = fast_exp2(__builtin_fmaf(x[j], p.scale, base));

@@ -53,6 +53,20 @@ __device__ __forceinline__ float hidden_nan() {
   return __builtin_bit_cast(float, bits);
 }
 
+// The exponent of a weight, up + scale x - m for a row's maximum m, is one fused multiply-add: scale x + base. Its
+// product is exact and the one that m was taken from is rounded, which up to 2^22 leaves at most 1/4 between them.
+// Beyond, that would be up to half of the score's last place, 2^7 at 2^31, and the largest weight no number of fp16:
+// there scores are first replaced by what their own rounded products leave of m, over scale, and base is `up`.
+__device__ __forceinline__ bool is_far(float m) { return __builtin_fabsf(m) >= 4194304.f && m != -__builtin_inff(); }
+__device__ __forceinline__ float base_of(float m, float up) {
+  return m == -__builtin_inff() ? 0.f : is_far(m) ? up : up - m;
+}
+__device__ __forceinline__ float behind(const AttentionParams& p, float x, float m) {
+#pragma clang fp contract(off)
+  const float t = x * p.scale;
+  return (t - m) * p.unscale;
+}
+
 // Zeros for a first product, in registers: as the instruction's constant they leave its result free to lie over its
 // operands.
 __device__ __forceinline__ f32x4 zeros() {

@@ -220,6 +220,7 @@ int ancha_paged_attention(const void* q, int type, size_t rows, size_t heads, si
   p.causal = causal ? 1 : 0;
   p.window = static_cast<int>(window < kIntMax ? window : 0);
   p.scale = static_cast<float>(scale * 1.4426950408889634);
+  p.unscale = 1.f / p.scale;
   const hipError_t e = paged::launch_attention(p, form, stream);
   return e == hipSuccess ? ANCHA_HIP_OK : hip_fail(e, who);
 }

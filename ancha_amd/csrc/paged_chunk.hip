@@ -178,6 +178,8 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
   };
 
   float m = -__builtin_inff(), l = 0.f;  // of row r: a whole number near its maximum; this lane's share of its sum
+  float base = 0.f;                      // what its scores get to be the exponents of its weights
+  bool far = false;                      // whether any row's maximum is, see is_far
   bool any = false;                      // whether this lane has met a key that the row sees
   unsigned none = 0;                     // a bit for each block of columns in which the row sees a NaN
   f32x16 acc[kScales];
@@ -355,7 +357,7 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
 #pragma unroll
         for (int j = 2; j < 16; j++) top = fmaxf(top, x[j]);
         top *= p.scale;
-        if (__any(top > m + kLag)) {
+        if (__any(top > m + kLag) || far) {
           top = fmaxf(top, __shfl_xor(top, 32));
           const float to = fmaxf(m, __builtin_ceilf(top));
           const float f = m == -__builtin_inff() ? 0.f : fast_exp2(m - to);
@@ -363,8 +365,12 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
           l *= f;
 #pragma unroll
           for (int c = 0; c < kScales; c++) acc[c] *= f;
+          base = base_of(m, kUp);
+          far = __any(is_far(m));
+          if (far)
+#pragma unroll
+            for (int j = 0; j < 16; j++) x[j] = is_far(m) ? behind(p, x[j], m) : x[j];
         }
-        const float base = m == -__builtin_inff() ? 0.f : kUp - m;
         u32x4 weight[kP][2];
 #pragma unroll
         for (int j = 0; j < 8; j++) {

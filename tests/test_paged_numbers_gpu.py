@@ -1,5 +1,5 @@
 """Attention over a paged cache where its numbers are at their limits, against the 64-bit oracle: values and NaN in the
-cache of any size, weights to 22 bits and small ones. Both kernels, tiles and chunks.
+cache of any size, weights to 22 bits and small ones, large scores. Both kernels, tiles and chunks.
 """
 import numpy as np
 import pytest
@@ -103,3 +103,22 @@ def test_many_small_weights_beside_a_large_one(gpu, length, gap, heads, columns,
     blocks = blocks * np.minimum(1, length * size / np.maximum(total, 1e-30))
     tol = tight(kind, want, size, total, reach, 64, blocks, 37)
     close("small", paged.attention(q, cache, batch, scale=1.0), want, tol)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,columns", FORMS)
+@pytest.mark.parametrize("size", [2.0 ** 20, 2.0 ** 27, 2.0 ** 29, 2.0 ** 33, 2.0 ** 60])
+def test_scores_far_from_zero(gpu, size, heads, columns, kind):
+    """One key, or equal ones, whose scores are large numbers, of either sign: the values' mean."""
+    cache, codes, scales = some_cache(gpu, 20, 16, 2, 64, "fp8", 241)
+    codes[0], scales[0] = 0, 0
+    codes[0, ..., 0], scales[0, ..., 0] = 0x38, 127  # keys of (1, 0, ...)
+    batch, plain, rows = some_batch(gpu, [70, 3], [170, 90], 16, 20, 242, columns=columns)
+    cache = on(gpu, codes, scales, "fp8")
+    rng = np.random.default_rng(243)
+    q = size * (1 + rng.random((rows, heads, 64))) * rng.choice((-1, 1), (rows, heads, 1))
+    q = dev(q, gpu, TYPES[kind])
+    for window in (1, 37, None):
+        want, mean, total, _ = O.attention(host(q), codes, scales, "fp8", plain, window=window)
+        tol = (mean + np.abs(want)) * 2.0 ** -20 + rounding(want, TYPES[kind])
+        close(f"{size} {window}", paged.attention(q, cache, batch, window=window), want, tol + total * 2.0 ** -31)
