@@ -95,15 +95,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_kernel(AttentionParams p
 #pragma unroll
       for (int j = 0; j < 8; j++) v[j] = (float)t[j];
 #pragma unroll
-      for (int part = 0; part < kQ; part++) {
-        bf16x8 b;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          b[j] = (__bf16)v[j];
-          v[j] -= (float)b[j];
-        }
-        q[part][k] = __builtin_bit_cast(u32x4, b);
-      }
+      for (int part = 0; part < kQ; part++) q[part][k] = upper_bits(v);
     }
   }
 

@@ -53,6 +53,21 @@ __device__ __forceinline__ float hidden_nan() {
   return __builtin_bit_cast(float, bits);
 }
 
+// The upper 8 bits of eight values as bf16, which are taken off them: three times leaves nothing of 24 bits. Cut off, not
+// rounded, so that the largest number does not become an infinity, and the parts of one value have its sign, so that
+// products beyond fp32 are infinities of one sign too.
+__device__ __forceinline__ u32x4 upper_bits(float* v) {
+  u32x4 r;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const unsigned a = __builtin_bit_cast(unsigned, v[2 * j]), b = __builtin_bit_cast(unsigned, v[2 * j + 1]);
+    r[j] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    v[2 * j] -= __builtin_bit_cast(float, a & 0xffff0000u);
+    v[2 * j + 1] -= __builtin_bit_cast(float, b & 0xffff0000u);
+  }
+  return r;
+}
+
 // The exponent of a weight, up + scale x - m for a row's maximum m, is one fused multiply-add: scale x + base. Its
 // product is exact and the one that m was taken from is rounded, which up to 2^22 leaves at most 1/4 between them.
 // Beyond, that would be up to half of the score's last place, 2^7 at 2^31, and the largest weight no number of fp16:

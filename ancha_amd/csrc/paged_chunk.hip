@@ -109,15 +109,7 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
 #pragma unroll
       for (int j = 0; j < 8; j++) v[j] = (float)t[j];
 #pragma unroll
-      for (int part = 0; part < kQ; part++) {
-        bf16x8 x;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          x[j] = (__bf16)v[j];
-          v[j] -= (float)x[j];
-        }
-        q[part][k] = __builtin_bit_cast(u32x4, x);
-      }
+      for (int part = 0; part < kQ; part++) q[part][k] = upper_bits(v);
     }
   }
 

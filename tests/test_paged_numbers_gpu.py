@@ -1,5 +1,6 @@
 """Attention over a paged cache where its numbers are at their limits, against the 64-bit oracle: values and NaN in the
-cache of any size, weights to 22 bits and small ones, large scores. Both kernels, tiles and chunks.
+cache of any size, weights to 22 bits and small ones, large scores and queries.
+Both kernels, tiles and chunks.
 """
 import numpy as np
 import pytest
@@ -122,3 +123,21 @@ def test_scores_far_from_zero(gpu, size, heads, columns, kind):
         want, mean, total, _ = O.attention(host(q), codes, scales, "fp8", plain, window=window)
         tol = (mean + np.abs(want)) * 2.0 ** -20 + rounding(want, TYPES[kind])
         close(f"{size} {window}", paged.attention(q, cache, batch, window=window), want, tol + total * 2.0 ** -31)
+
+
+@pytest.mark.parametrize("heads,columns", FORMS)
+def test_queries_up_to_the_largest_number(gpu, heads, columns):
+    """fp32 queries at the end of their range over keys as small as scale bytes make them."""
+    for low in (3, 8):
+        cache, codes, scales = some_cache(gpu, 20, 16, 2, 64, "fp8", 261)
+        codes[0] = codes[0] & 0x8f | 0x30  # 2^-1 to 2^-0.1, both signs
+        scales[0] = low
+        batch, plain, rows = some_batch(gpu, [70, 3], [170, 90], 16, 20, 262, columns=columns)
+        cache = on(gpu, codes, scales, "fp8")
+        q = dev(W.normal((rows, heads, 64), 263, 1.0), gpu) * 2.0 ** (127 - low)
+        q[:, :, ::7] = torch.finfo(torch.float32).max * 2.0 ** (3 - low)
+        q[::2, :, 1::7] = -torch.finfo(torch.float32).max * 2.0 ** (3 - low)
+        assert torch.isfinite(q).all()
+        want, size, total, reach = O.attention(host(q), codes, scales, "fp8", plain)
+        blocks = np.exp2(scales[1].max((0, 1, 2)) - 127.0).repeat(32) * 448
+        close(f"{low}", paged.attention(q, cache, batch), want, tight("f32", want, size, total, reach, 64, blocks))
