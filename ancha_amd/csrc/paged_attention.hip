@@ -338,11 +338,10 @@ __global__ __launch_bounds__(64 * WAVES) void attention_kernel(AttentionParams p
   int met = any;
   met |= __shfl_xor(met, 16);
   met |= __shfl_xor(met, 32);
-  // Nothing but scores of minus infinity: 0 / 0, where a row that sees no key is 0.
   const float nan = hidden_nan();
-  if (met && !(l > 0.f)) l = nan;
   // Divided before the power of two comes back: the mean of values is in their range, their sum may not be.
   const float mean = l == 0.f ? 0.f : 1.f / l;
+  if (met && is_zero(l)) l = kLost;
   __shared__ float tops[kWaves][kTile], sums[kWaves][kTile];
   __shared__ __attribute__((aligned(16))) float outs[kWaves][kTile][D + 4];
   if (g == 0) {
@@ -363,13 +362,16 @@ __global__ __launch_bounds__(64 * WAVES) void attention_kernel(AttentionParams p
 #pragma unroll
   for (int v = 1; v < kWaves; v++) top = fmaxf(top, tops[v][r]);
   float sum = 0.f, share[kWaves], o[kCols];
+  bool lost = false;
 #pragma unroll
   for (int t = 0; t < kCols; t++) o[t] = 0.f;
 #pragma unroll
   for (int v = 0; v < kWaves; v++) {
     share[v] = (tops[v][r] == -__builtin_inff() ? 0.f : fast_exp2(tops[v][r] - top)) * sums[v][r];
     sum += share[v];
+    lost |= sums[v][r] == kLost;
   }
+  lost &= is_zero(sum);
   const float over = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
   for (int v = 0; v < kWaves; v++)
@@ -379,10 +381,13 @@ __global__ __launch_bounds__(64 * WAVES) void attention_kernel(AttentionParams p
     float* to = part_of(p, tile, head, split, kTile, D);
     if (part == 0) {
       to[r] = top;
-      to[kTile + r] = sum;
+      to[kTile + r] = lost ? kLost : sum;
     }
     __builtin_memcpy(to + 2 * kTile + r * D + kCols * part, o, sizeof(o));
   } else if (row + r < rows) {
+    if (lost)
+#pragma unroll
+      for (int t = 0; t < kCols; t++) o[t] = nan;
     const int token = (row + r) / group, at_head = head * group + row + r - token * group;
     store_row<TYPE, kCols>(p.out, ((long)(s.first + token) * p.heads + at_head) * D + kCols * part, kCols, o);
   }
@@ -410,9 +415,16 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionParams p, int rows) 
     return (m == -__builtin_inff() ? 0.f : fast_exp2(m - top)) * parts[j * kPart + rows + r];
   };
   float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int j = lane; j < w.splits; j += kLanes) sum += share(j);
+  int lost = 0;
+  for (int j = lane; j < w.splits; j += kLanes) {
+    sum += share(j);
+    lost |= parts[j * kPart + rows + r] == kLost;
+  }
 #pragma unroll
-  for (int o = 1; o < kLanes; o <<= 1) sum += __shfl_xor(sum, o);
+  for (int o = 1; o < kLanes; o <<= 1) {
+    sum += __shfl_xor(sum, o);
+    lost |= __shfl_xor(lost, o);
+  }
   const float over = sum == 0.f ? 0.f : 1.f / sum;
   for (int base = 0; base < w.splits; base += kLanes) {
     const float weight = base + lane < w.splits ? share(base + lane) * over : 0.f;
@@ -431,6 +443,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionParams p, int rows) 
       }
     }
   }
+  if (lost && is_zero(sum)) v[0] = v[1] = v[2] = v[3] = hidden_nan();
   const int group = p.heads / p.cache.heads, token = (w.row + r) / group;
   const int at_head = head * group + w.row + r - token * group;
   store_row<TYPE, 4>(p.out, ((long)(w.first + token) * p.heads + at_head) * D + lane * 4, 4, v);

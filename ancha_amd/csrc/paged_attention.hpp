@@ -90,6 +90,15 @@ __device__ __forceinline__ f32x4 zeros() {
   return z;
 }
 
+// In place of a part's sum: the row has met keys there, all with scores of minus infinity. They weigh nothing beside
+// others; where a row has no others its result is 0 / 0, a NaN, while a row that sees no key at all is 0.
+constexpr float kLost = -1.f;
+__device__ __forceinline__ bool is_zero(float x) {  // on the bits: a NaN is none
+  unsigned bits = __builtin_bit_cast(unsigned, x);
+  asm volatile("" : "+v"(bits));
+  return (bits & 0x7fffffffu) == 0;
+}
+
 // Keys [low, high) that row r of a sequence sees, r = token * group + head.
 struct Range {
   int low, high;

@@ -394,17 +394,18 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
     __syncthreads();
   }
 
-  float sum = l + __shfl_xor(l, 32);
+  const float sum = l + __shfl_xor(l, 32);
   int met = any;
   met |= __shfl_xor(met, 32);
   none |= __shfl_xor(none, 32);
   const float nan = hidden_nan();
-  if (met && !(sum > 0.f)) sum = nan;  // nothing but scores of minus infinity
   const float over = sum == 0.f ? 0.f : 1.f / sum;
+  const bool lost = met && is_zero(sum);
+  if (lost && w.splits == 1) none = ~0u;
   float* const part = part_of(p, tile, head, split, S::kRows, D);
   if (w.splits > 1 && h == 0) {
     part[32 * wave + r] = m;
-    part[S::kRows + 32 * wave + r] = sum;
+    part[S::kRows + 32 * wave + r] = lost ? kLost : sum;
   }
   if (my_row >= rows) return;
   const long to = ((long)(s.first + token) * p.heads + my_head) * D;

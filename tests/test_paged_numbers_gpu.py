@@ -1,6 +1,6 @@
 """Attention over a paged cache where its numbers are at their limits, against the 64-bit oracle: values and NaN in the
-cache of any size, weights to 22 bits and small ones, large scores and queries.
-Both kernels, tiles and chunks.
+cache of any size, weights to 22 bits and small ones, large and infinite scores,
+large queries. Both kernels, tiles and chunks.
 """
 import numpy as np
 import pytest
@@ -141,3 +141,40 @@ def test_queries_up_to_the_largest_number(gpu, heads, columns):
         want, size, total, reach = O.attention(host(q), codes, scales, "fp8", plain)
         blocks = np.exp2(scales[1].max((0, 1, 2)) - 127.0).repeat(32) * 448
         close(f"{low}", paged.attention(q, cache, batch), want, tight("f32", want, size, total, reach, 64, blocks))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,columns", [(4, None), (4, 600), (40, 9000)])
+@pytest.mark.parametrize("first,last", [(0, 1024), (700, 1500), (0, 33)])
+def test_scores_below_every_number(gpu, first, last, heads, columns, kind):
+    """Keys whose scores pass fp32 to minus infinity have no weight, also where some waves or workgroups have no other."""
+    cache, codes, scales = some_cache(gpu, 110, 16, 2, 64, "fp8", 251, big=0.0)
+    batch, plain, rows = some_batch(gpu, [20], [1600], 16, 110, 252, columns=columns)
+    codes[0] &= 0x7f
+    for t in range(1600):
+        page, slot = O.place(plain, 0, t, 110, 16)
+        scales[0, page, :, slot] = 127 + 40 if first <= t < last else 127 - 106
+    cache = on(gpu, codes, scales, "fp8")
+    q = dev(-np.abs(W.normal((rows, heads, 64), 253, 1.0)) * 2.0 ** 100, gpu, TYPES[kind])
+    for window in (None, 1200):
+        want, size, total, _ = O.attention(host(q), codes, scales, "fp8", plain, window=window)
+        assert np.isfinite(want).all()
+        # The largest scale sum |q k| of the keys that count: 64 products of 4.5 * 448 * 2^-6, over 8.
+        tol = tight(kind, want, size, total, np.float64(256.0), 64, 448 * np.exp2(scales[1].max() - 127.0))
+        close(f"{window}", paged.attention(q, cache, batch, window=window), want, tol)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("heads,columns", [(4, None), (4, 600), (40, 9000)])
+def test_nothing_but_scores_of_minus_infinity_is_a_nan(gpu, heads, columns, kind):
+    """0 / 0, whether or not a row's keys are shared; rows beside it are as they were, and one without keys is 0."""
+    cache, codes, scales = some_cache(gpu, 110, 16, 2, 64, "fp8", 255, big=0.0)
+    codes[0] = codes[0] & 0x7f | 8  # keys above 0
+    cache = on(gpu, codes, scales, "fp8")
+    batch, plain, rows = some_batch(gpu, [20, 3], [1600, 2], 16, 110, 256, columns=columns)
+    q = dev(W.normal((rows, heads, 64), 257, 1.0), gpu, TYPES[kind])
+    q[5, 1, 7] = q[20, 0, 0] = q[21, heads - 1, 3] = float("-inf")  # row 20 is before the second sequence's first token
+    got = torch.isnan(paged.attention(q, cache, batch)).cpu().numpy()
+    want = np.zeros(got.shape, bool)
+    want[5, 1] = want[21, heads - 1] = True
+    assert np.array_equal(got, want)
