@@ -104,6 +104,9 @@ def frequencies(width: int, base: float = 10000.0, scaling: Optional[str] = None
     if scaling == "ntk":
         if width == 2:
             raise ValueError("'ntk' takes a width above 2")
+        # By logarithms, as the power may pass the range of a float.
+        if math.log(base) + width / (width - 2) * math.log(factor) >= 709:
+            raise ValueError(f"factor {factor} makes a base beyond 64-bit numbers")
         base = base * factor ** (width / (width - 2))
     if math.log2(base) * (2 - width) / width > 20:
         raise ValueError(f"base {base} makes frequencies above 2**20")
@@ -112,7 +115,7 @@ def frequencies(width: int, base: float = 10000.0, scaling: Optional[str] = None
         return [f / factor for f in freqs], 1.0
     if scaling != "yarn":
         return freqs, 1.0
-    if original < 1:
+    if not 1 <= original <= 2 ** 53:
         raise ValueError("'yarn' takes the original length in tokens")
     keep = [min(1.0, max(0.0, (original * f / (2 * math.pi) - 1) / 31)) for f in freqs]
     return [f * (g + (1 - g) / factor) for f, g in zip(freqs, keep)], 0.1 * math.log(factor) + 1
