@@ -178,3 +178,17 @@ def test_nothing_but_scores_of_minus_infinity_is_a_nan(gpu, heads, columns, kind
     want = np.zeros(got.shape, bool)
     want[5, 1] = want[21, heads - 1] = True
     assert np.array_equal(got, want)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("heads,columns", [(4, None), (4, 600), (20, 9000)])
+def test_a_nan_in_a_query_is_its_rows_alone(gpu, heads, columns, dim, kind):
+    cache, codes, scales = some_cache(gpu, 80, 16, 2, dim, "fp8", 271)
+    batch, plain, rows = some_batch(gpu, [30, 1], [1100, 40], 16, 80, 272, columns=columns)
+    q = dev(W.normal((rows, heads, dim), 273, 1.0), gpu, TYPES[kind])
+    want, size, total, reach = O.attention(host(q), codes, scales, "fp8", plain)
+    q[7, 1, 5], q[30, heads - 1, dim - 1] = float("nan"), float("nan")
+    want[7, 1] = want[30, heads - 1] = float("nan")
+    blocks = np.exp2(scales[1].max((0, 1, 2)) - 127.0).repeat(32) * 448
+    close("nan", paged.attention(q, cache, batch), want, tight(kind, want, size, total, reach, dim, blocks))
