@@ -8,6 +8,7 @@ import torch
 
 from ancha_amd import paged
 from ancha_amd import workload as W
+from oracle import mx as OM
 from oracle import paged as O
 from tests.test_paged_gpu import CHUNK, PARTS, TYPES, close, dev, form, host, rounding, some_batch, some_cache
 
@@ -192,3 +193,27 @@ def test_a_nan_in_a_query_is_its_rows_alone(gpu, heads, columns, dim, kind):
     want[7, 1] = want[30, heads - 1] = float("nan")
     blocks = np.exp2(scales[1].max((0, 1, 2)) - 127.0).repeat(32) * 448
     close("nan", paged.attention(q, cache, batch), want, tight(kind, want, size, total, reach, dim, blocks))
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_write_turns_by_angles_up_to_the_limit(gpu, layout):
+    """Positions up to 2^31 - 1 and frequencies up to 2^20: the oracle's codes."""
+    freqs = [2.0 ** 20, -2.0 ** 20 + 0.5, 1e6 / 3, 2.0 ** 17 + 0.1, 2.0 ** 16 - 0.7, 777.7, 1.0, np.pi / 2, 1e-3, 2.0 ** -31]
+    plan = paged.Rotary(torch.tensor(freqs, dtype=torch.float64, device=gpu), layout)
+    page = 65536
+    for length in (2 ** 31 - 1, 2 ** 30 + 12345, 2 ** 28 + 7):
+        column = (length - 1) // page
+        table = np.full((1, column + 1), -1, np.int32)
+        table[0, column] = 0
+        cache = paged.Cache.empty(1, page, 1, 64, "fp8", gpu)
+        rows = 3000
+        batch = paged.Batch(*(torch.from_numpy(a.copy()).to(gpu) for a in (
+            np.array([0, rows], np.int32), np.array([length], np.int32), table)))
+        k = dev(W.normal((rows, 1, 64), 281, 1.0), gpu)
+        cache.write(k, k, batch, plan)
+        at = np.arange(length - rows, length)
+        here = at // page == column
+        want, scales = OM.encode(O.rotate(host(k), at, freqs, layout).reshape(rows, 64)[here], "fp8")
+        slots = torch.from_numpy(at[here] % page).to(gpu)
+        assert np.array_equal(cache.scales[0, 0, 0, slots].cpu().numpy(), scales[:, :2])
+        assert np.array_equal(cache.codes[0, 0, 0, slots].cpu().numpy(), want[:, :64])
