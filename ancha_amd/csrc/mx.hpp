@@ -196,8 +196,8 @@ __device__ __forceinline__ float to_odd(double d) {
 }
 
 // Division by a number d, a row's groups for example: n / d = n * factor >> shift for every n < 2^28, with factor =
-// 2^shift / d + 1 and 2^shift = 2^31 times the largest power of two up to d (the product is off by n d / 2^shift < 1/4 of
-// a whole).
+// 2^shift / d + 1 and 2^shift = 2^31 times the largest power of two up to d (the product is off by n d / 2^shift < 1/4
+// of a whole).
 struct Divide {
   unsigned factor;
   int shift;

@@ -3,15 +3,15 @@
 // For a query row r (a token and a head; the heads that share a head of the cache are rows beside each other) and the
 // keys j that it sees:  o = sum_j e^(c q.k_j) v_j / sum_j e^(c q.k_j), in one pass with a running maximum.
 //
-// Operands. A key's codes times their power of two are bf16 values without loss, so products with a bf16 query are
-// exact; a query of 16 or 32 bits that bf16 does not hold is the sum of two or three bf16 parts, a product each. The
-// weights e^.. are the sum of two fp16 parts, 22 bits, for results of every type and in both kernels: with one part the
-// distance of fp16 results from the exact ones was 1.4 times that of their own rounding (2.9e-4 instead of 2.1e-4 of
-// their size), and of bf16 ones 1.006 times. The second part costs 1 to 5 % where the cache bounds a call and 30 % where
-// the products do (see chunk_kernel). So values have to be fp16 too: each block of 32 columns has a reference power `ref`
-// that all of its values are taken relative to, so that the largest fits; what lies 2^-32 below it, where fp16 ends, is
-// far below the result's own rounding. When a larger one comes, the sums so far are scaled down, like those of the
-// running maximum.
+// Operands. A key's codes times their power of two are bf16 values without loss (of scale bytes below 3 to within
+// 2^-134), so products with a bf16 query are exact; a query of 16 or 32 bits that bf16 does not hold is the sum of
+// two or three bf16 parts, a product each. The weights e^.. are the sum of two fp16 parts, 22 bits, for results of
+// every type and in both kernels: with one part the distance of fp16 results from the exact ones was 1.4 times that
+// of their own rounding (2.9e-4 instead of 2.1e-4 of their size), and of bf16 ones 1.006 times. The second part costs
+// 1 to 5 % where the cache bounds a call and 30 to 35 % where the products do (see chunk_kernel). So values have to
+// be fp16 too: each block of 32 columns has a reference power `ref` that all of its values are taken relative to, so
+// that the largest fits; what lies 2^-32 below it, where fp16 ends, is far below the result's own rounding. When a
+// larger one comes, the sums so far are scaled down, like those of the running maximum.
 #include "paged_attention.hpp"
 
 namespace ancha {
@@ -25,12 +25,13 @@ constexpr int kStep = 32;  // keys
 //   scores   keys 4 g + i of both 16-key halves for row c (K . Q^T), and so the weights as P . V's operand,
 //   K        key c of each half: 16 (fp8) or up to 32 (fp4) neighbouring columns at a time,
 //   V        the same eight keys as its weights, columns D / 16 * c on, transposed in registers two by two.
-// Nothing passes through LDS before the waves' sums are joined. Bound by the reading of the cache while there are
-// few rows: with 8 heads of 128 for 32 of q, 64 sequences of up to 8192 tokens in e4m3 (558 MB) take 119 us, 4.7 TB/s,
-// one of 131 072 in e2m1 (143 MB) 32 us and 6 to join its parts, one of 2048 tokens 8 us and 3, which is the latency of
-// a few dependent reads. A page's number is read two steps ahead and codes one: with both one step ahead the first took
-// 183 us, not 142, and the second 77, not 57; codes two steps ahead changed nothing. With eight waves, twice the reads
-// in flight, they took 137 and 43 us, and 32 sequences of 8192 with heads of 64 in fp32 51 instead of 77.
+// Nothing passes through LDS before the waves' sums are joined. Bound by the reading of the cache while there are few
+// rows: with 8 heads of 128 for 32 of q, 64 sequences of up to 8192 tokens in e4m3 (558 MB) take 122 us, 4.6 TB/s,
+// one of 131 072 in e2m1 (143 MB) 35 us and 6 to join its parts, one of 2048 tokens 12 us with the join, which is the
+// latency of a few dependent reads. A page's number is read two steps ahead and codes one: in the first build, of
+// four waves and weights of one part, both one step ahead made the first 183 us, not 142, and the second 77, not 57;
+// codes two steps ahead changed nothing. Eight waves, twice the reads in flight, then brought them to 137 and 43 us,
+// and 32 sequences of 8192 with heads of 64 in fp32 from 77 to 51.
 template <int D, int FORMAT, int TYPE, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void attention_kernel(AttentionParams p) {
   typedef typename Stored<TYPE>::type T;
@@ -49,10 +50,10 @@ __global__ __launch_bounds__(64 * WAVES) void attention_kernel(AttentionParams p
   // few less, so a block may grow by 8 (fp8) or 16 times before the sums are scaled.
   constexpr int kMost = FORMAT == kFp8 ? 7 : 13, kTaken = FORMAT == kFp8 ? 4 : 9;
   constexpr int kNoRef = -1000;
-  // Weights are e^.. 2^kUp: a maximum may lag 2^2 behind before the sums are scaled. The row's largest is 2^12 or more
-  // and fp16's second part ends at 2^-25, so a weight is off by 2^-37 of it where that is more than its own 22 bits. With
-  // 2^7 and a lag of 2^8 it was 2^-31, and a first token that took the scores but had no value left 250 others e^-23 of
-  // it with none; a prompt of 8192 tokens took 814 us then and 818 now, with a lag of 2^1 826.
+  // Weights are e^.. 2^kUp: a maximum may lag 2^2 behind before the sums are scaled. The row's largest is 2^12 or
+  // more and fp16's second part ends at 2^-25, so a weight is off by 2^-37 of it where that is more than its own 22
+  // bits. With 2^7 and a lag of 2^8 it was 2^-31, and a first token that took the scores but had no value left 250
+  // others e^-23 of it with none; a prompt of 8192 tokens took 814 us then and 818 so, with a lag of 2^1 826.
   constexpr float kUp = 13.f, kLag = 2.f;
 
   const int group = p.heads / p.cache.heads;
@@ -493,10 +494,12 @@ AttentionForm attention_form(const AttentionParams& p) {
   const long group = p.heads / p.cache.heads, rows = p.rows * group, some = min(p.batch.sequences, p.rows);
   const long keys = (long)p.batch.columns << p.cache.shift;
   // Chunks are for sequences that fill three quarters of one, where the rows read enough to pay for its longer start.
-  // Both measured, 32 heads over 8 of 128 in bf16 (tiles / chunks): 8 sequences of 64 rows over 8192 keys 253 / 173 us,
-  // of 32 rows 127 / 143, 8 of 128 rows over 1024 78 / 48, of 64 43 / 41; one of 64 over 8192 53 / 42, of 128 over 1024
-  // 15 / 28. In fp32, 8 heads of 64, 8 sequences: 128 rows over 8192 97 / 83, 64 rows 53 / 79. Heads of 256 columns do
-  // not fit its registers.
+  // Both measured, 32 heads over 8 of 128 in bf16 (tiles / chunks): 8 sequences of 64 rows over 8192 keys 274 / 141
+  // us, of 16 rows 74 / 85, 8 of 128 rows over 1024 85 / 56, of 64 46 / 41, of 32 30 / 33; one of 64 over 8192 43 /
+  // 41, of 128 over 1024 16 / 32. In fp32, 8 heads of 64, 8 sequences: 128 rows over 8192 98 / 71, 64 rows 52 / 59.
+  // Between, 32 rows over 8192 in bf16, half a chunk, would be faster in chunks, 131 / 97, where half a chunk of fp32
+  // is not. `keys` is what the table has room for: 128 rows over 1024 keys take 17 us, but 34 with a table for 131
+  // 072. Heads of 256 columns have no chunks: three buffers of 64 of their keys and values are 192 KiB of LDS.
   const int high = p.cache.dim < 256 ? chunk_rows(p.cache.dim, p.type) : 0;
   const bool chunk = high && 4 * rows >= 3 * high * some && rows * p.cache.heads >= (1l << 24) / max(keys, 1l);
   const int of = chunk ? high : kTile;
@@ -504,19 +507,20 @@ AttentionForm attention_form(const AttentionParams& p) {
   f.tiles = (rows + some * (of - 1)) / of + 1;
   const long groups = f.tiles * p.cache.heads;
   // Eight waves a tile read more at once, but have twice the sums to join: with 1024 workgroups the CUs are full either
-  // way, and 256 sequences of 1024 keys took 77 us with four and 93 with eight. Heads of 256 would spill: 42 and 97.
+  // way, and 256 sequences of 1024 keys take 81 us with four and 96 with eight. Heads of 256 would spill.
   f.form = chunk ? kChunk : p.cache.dim < 256 && groups < 1024 ? kTiles8 : kTiles4;
   // Workgroups share a tile's keys as long as all of them run at once: one of eight waves a CU, two of four. Rows are
-  // taken to be spread evenly over the sequences. 8 sequences of 128 rows over 8192 keys took 312 us with one workgroup
-  // a tile, 190 so; 256 over 16 384 115 and 100. Twice as many shares of chunks gained up to 18 % where sequences differ
-  // in length (the same 8, ragged: 162 and 133) and lost as much as 37 % where they do not (16 of 100 over 2048: 91 and
-  // 125).
+  // taken to be spread evenly over the sequences. 8 sequences of 128 rows over 8192 keys take 375 us with one workgroup
+  // a tile, 240 so; one of 512 over 16 384 725 and 225. Twice as many shares of chunks gain up to 18 % where sequences
+  // differ in length (the same 8, ragged: 204 and 167) and lose as much as 28 % where they do not (16 of 100 over 2048:
+  // 117 and 150). One long sequence among many short ones is not shared at all: 131 072 keys and 31 times 500 take 880
+  // us, the long one alone 70.
   const long slots = (chunk ? chunk_waves(p.cache.dim, p.type) == 8 : f.form == kTiles8) ? 256 : 512;
   const long full = some ? some * ((rows + some * of - 1) / (some * of)) : 1;
   f.splits = (int)min(max(slots / (full * p.cache.heads), 1l), min(keys / kLeastKeys + 1, 256l));
-  // Sharing saves a tile's waves these keys and costs a second launch. Both measured (shared / not), one row a head: 400
-  // keys 10.9 / 9.5 us, 801 11.0 / 11.6 (heads of 64 in fp32 10.5 / 9.7), 1100 11.1 / 13.2; 16 sequences of 801 keys
-  // 16.5 / 12.7, of 2048 21.6 / 23.2.
+  // Sharing saves a tile's waves these keys and costs a second launch. Both measured (shared / not), one row a head,
+  // calls in a stream with their launches: 400 keys 11.7 / 9.5 us, 801 11.4 / 11.7 (heads of 64 in fp32 11.4 / 9.4),
+  // 1100 11.4 / 13.6; kernels alone, 16 sequences of 801 keys 16.9 / 13.5, of 2048 21.9 / 22.2.
   if (!chunk && keys * (f.splits - 1) < (f.form == kTiles8 ? 640 : 320) * f.splits) f.splits = 1;
   if (f.splits > 1)
     f.bytes = 4 * (size_t)(joined_floats(f.tiles, p.cache.heads) + groups * f.splits * part_floats(of, p.cache.dim));

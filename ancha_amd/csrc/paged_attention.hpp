@@ -53,9 +53,9 @@ __device__ __forceinline__ float hidden_nan() {
   return __builtin_bit_cast(float, bits);
 }
 
-// The upper 8 bits of eight values as bf16, which are taken off them: three times leaves nothing of 24 bits. Cut off, not
-// rounded, so that the largest number does not become an infinity, and the parts of one value have its sign, so that
-// products beyond fp32 are infinities of one sign too.
+// The upper 8 bits of eight values as bf16, which are taken off them: three times leaves nothing of 24 bits. Cut off,
+// not rounded, so that the largest number does not become an infinity, and the parts of one value have its sign, so
+// that products beyond fp32 are infinities of one sign too.
 __device__ __forceinline__ u32x4 upper_bits(float* v) {
   u32x4 r;
 #pragma unroll

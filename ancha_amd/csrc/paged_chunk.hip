@@ -41,15 +41,15 @@ struct Shape {
 //   sums     element 4 q + e of block b: column 32 b + 8 q + 4 h + e of row r.
 // A block of 32 columns is one of the cache's own, so its reference power is one number a workgroup.
 //
-// Bound by the matrix units and what runs beside them: a prompt of 8192 tokens, 32 heads over 8 of 128 in bf16, is 0.55
-// TFLOP and takes 793 us replayed, 0.69 PFLOP/s; with the weights' second part it is 0.82 TFLOP of products, 1.04
-// PFLOP/s, where a library product of 8192^3 reaches 1.3 on the same card. 4 times 801 rows of 8 heads of 64 over 4096
-// keys, in fp32, take 68 us and 6 to join. With weights of one part, 11 bits, the prompt took 615 us; of that build:
-// with the products alone 389 us, without bringing the codes 513, without the exponentials 611. What did not help an
-// earlier one of 655 us: 64 rows a wave with one wave a SIMD 946; four reads ahead of the products 698; groups given to
-// the scheduler 700; wave priorities 690; sums by adds 675 or by a product with ones 655; the next half's scores ahead
-// of these weights, codes two steps ahead: no change. Both halves of a step at once made that one 3 % faster, 636, and
-// have not been tried on this one.
+// Bound by the matrix units and what runs beside them: a prompt of 8192 tokens, 32 heads over 8 of 128 in bf16, is
+// 0.55 TFLOP and takes 793 to 878 us replayed on one card and another, 0.63 to 0.69 PFLOP/s; with the weights' second
+// part it is 0.82 TFLOP of products, 0.94 to 1.04 PFLOP/s, where a library product of 8192^3 reaches 1.3. 4 times 801
+// rows of 8 heads of 64 over 4096 keys, in fp32, take 69 us and 6 to join. With weights of one part, 11 bits, the
+// prompt took 615 to 653 us on the same cards; of that build: with the products alone 389 us, without bringing the
+// codes 513, without the exponentials 611. What did not help an earlier one of 655 us: 64 rows a wave with one wave a
+// SIMD 946; four reads ahead of the products 698; groups given to the scheduler 700; wave priorities 690; sums by
+// adds 675 or by a product with ones 655; the next half's scores ahead of these weights, codes two steps ahead: no
+// change. Both halves of a step at once made that one 3 % faster, 636, and have not been tried on this one.
 template <int D, int FORMAT, int TYPE>
 __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void chunk_kernel(AttentionParams p) {
   typedef typename Stored<TYPE>::type T;
@@ -69,7 +69,8 @@ __global__ __launch_bounds__(64 * chunk_waves(D, TYPE), D == 64 ? 2 : 1) void ch
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
 
   const int group = p.heads / p.cache.heads;
-  // Workgroups beside each other on an XCD share a head; the last tiles, which see the most keys, go first.
+  // Workgroups beside each other on an XCD share a head. Tiles go from the last to the first, so that of one sequence
+  // those that see the most keys begin first (of several, the last sequence's, however long it is).
   const int place = xcd_remap(blockIdx.x, p.tiles * p.cache.heads * p.splits);
   const int head = place / (p.tiles * p.splits), in_head = place - head * (p.tiles * p.splits);
   int id = p.tiles - 1 - in_head / p.splits, i, row;

@@ -24,13 +24,13 @@ __device__ __forceinline__ float2 cos_sin(double a) {
   return make_float2(turn == 1 || turn == 2 ? -x : x, turn & 2 ? -y : y);
 }
 
-// The same for keys that are written: half pi is taken off in two parts by fused multiply-adds, the rest, about pi / 4 at
-// most, goes through the Taylor series to its 15th and 16th power. Within 2^-52 for angles below 2^48. Beyond, a * 2 / pi
-// is itself rounded by up to an eighth of a quarter turn and more, so the rest leaves the series' range: within 2^-49 below
-// 2^50 and 2^-45 below 2^51, which positions and frequencies up to 2^20 do not pass; a code has 4 bits. (Largest of
-// 200 000 angles of each octave against 113-bit ones, in the same steps on the CPU: 0.87, 1.5, 5.5 and 85 times 2^-52 up
-// to 2^48, 2^49, 2^50 and 2^51.) With the library's function, which reduces any angle, 16 384 keys of 8 x 128 are written
-// in 35 us instead of 30.
+// The same for keys that are written: half pi is taken off in two parts by fused multiply-adds, the rest, about pi /
+// 4 at most, goes through the Taylor series to its 15th and 16th power. Within 2^-52 for angles below 2^48. Beyond, a
+// * 2 / pi is itself rounded by up to an eighth of a quarter turn and more, so the rest leaves the series' range:
+// within 2^-49 below 2^50 and 2^-45 below 2^51, which positions and frequencies up to 2^20 do not pass; a code has 4
+// bits. (Largest of 200 000 angles of each octave against 113-bit ones, in the same steps on the CPU: 0.87, 1.5, 5.5
+// and 85 times 2^-52 up to 2^48, 2^49, 2^50 and 2^51.) With the library's function, which reduces any angle, 16 384
+// keys of 8 x 128 are written in 35 us instead of 30.
 __device__ __forceinline__ double2 cos_sin_64(double a) {
   const double whole = __builtin_rint(a * 0.6366197723675813430755);
   double r = __builtin_fma(-whole, 1.5707963267948965579990, a);
@@ -196,11 +196,13 @@ __device__ __forceinline__ void turn_key(const Plan& plan, int col, const double
 }
 
 // New keys and values into their pages. A workgroup has `rows` rows: their places and their pairs' cosines and sines
-// once (in 64 bits), then eight columns a thread, four threads a block of codes. Rows without a place are left out. The
-// first values are on their way while the places are found and the angles taken. 16 384 tokens of 8 heads of 128 in
-// bf16, 101 MB, take 30 us, of which 20 are the memory's; the vector instructions bound it (with a decision for every
-// column and sines side by side in LDS 35 us, then 90 % busy). One, two or eight rows a workgroup, rows dealt by XCD,
-// or the next values fetched ahead changed nothing. 32 tokens take 5 us.
+// once (in 64 bits), then eight columns a thread, four threads a block of codes. Rows without a place are left out.
+// The first values are on their way while the places are found and the angles taken. 16 384 tokens of 8 heads of 128
+// in bf16, 101 MB, take 30 us, of which 20 are the memory's; the vector instructions bound it, 84 % busy. About one
+// in seven of them is of the 64 bits of the sines and the turn; the rest are loads' conversions, blocks' largest
+// values, codes and addresses. (With a decision for every column and sines side by side in LDS it was 35 us, 90 %
+// busy.) One, two or eight rows a workgroup, rows dealt by XCD, or the next values fetched ahead changed nothing. 32
+// tokens take 5 us.
 template <int TYPE, int FORMAT, bool HALF>
 __global__ __launch_bounds__(kThreads) void write_kernel(WriteParams p, int rows, Divide by_row, Divide by_pair) {
   typedef typename Stored<TYPE>::type T;

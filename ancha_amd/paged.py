@@ -195,8 +195,8 @@ class Cache:
     :mod:`ancha_amd.mx` with blocks of 32 along the head. ``page`` tokens a page, a power of two from 16 to 65536;
     ``dim`` 64, 128 or 256. Pages are the caller's: any page may be given to any sequence, be shared by several that
     only read it, or be copied (``cache.codes[:, to] = cache.codes[:, at]``, and the scales). Codes of one's own have to
-    be numbers, as :meth:`write` makes them: a NaN is told by its block's scale byte, 255, and e4m3's own NaN codes (0x7f
-    and 0xff) among a token's values would reach rows that do not see it."""
+    be numbers, as :meth:`write` makes them: a NaN is told by its block's scale byte, 255, and e4m3's own NaN codes
+    (0x7f and 0xff) among a token's values would reach rows that do not see it."""
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, format: str):
         bits = _format(format)
@@ -278,8 +278,8 @@ def attention(q: torch.Tensor, cache: Cache, batch: Batch, scale: Optional[float
 
     Scores are exact to 32 bits for every type of q; weights are off by 2**-21 of themselves at most or by 2**-37 of
     their row's largest, and sums are held in 32, so a result is rounded to its type once. Values more than 2**30 below
-    the largest of their head's block of 32 columns, of any token that this row or those beside it see, may be rounded. A
-    score beyond float32 is infinite: minus infinity weighs nothing, plus infinity makes its row NaN, as does a row of
+    the largest of their head's block of 32 columns, of any token that this row or those beside it see, may be rounded.
+    A score beyond float32 is infinite: minus infinity weighs nothing, plus infinity makes its row NaN, as does a row of
     nothing but minus infinity. A NaN in the cache (scale byte 255) reaches the rows that see its token, no others. How
     the keys are shared out depends on shapes and lengths alone, so a call gives the same bits
     every time."""

@@ -348,8 +348,8 @@ int ancha_mx_linear(const void *codes, const void *scales, size_t n, size_t k, i
  * A cache is [2][pages][heads][page][dim] (keys, then values): codes, dim (e4m3) or dim / 2 (e2m1, the first value in
  * the low half) bytes a token, and scales, dim / 32 bytes a token, by the rule of the microscaled operators; both
  * 16-byte aligned. What a page holds where nothing was written is never part of a result. A NaN is told by its block's
- * scale byte, 255: a caller's own codes of tokens that are seen hold no NaN codes of e4m3 (0x7f, 0xff), which would reach
- * rows that do not see the token. */
+ * scale byte, 255: a caller's own codes of tokens that are seen hold no NaN codes of e4m3 (0x7f, 0xff), which would
+ * reach rows that do not see the token. */
 typedef struct {
   const int *starts;  /* [sequences + 1] */
   const int *lengths; /* [sequences] */
@@ -397,10 +397,10 @@ int ancha_paged_read(const ancha_paged_cache *cache, const ancha_paged_batch *ba
  * head * ldqh + d. A row at position t sees the tokens up to t (with `causal`, otherwise all of its sequence) and, with
  * window > 0, none before t - window + 1. Rows that see no token and rows of no sequence are 0. Scores of any q are
  * exact to fp32, weights are off by 2^-21 of themselves at most or by 2^-37 of their row's largest, sums are fp32, and
- * the result is rounded to its type once. Values more than 2^30 below the largest of their head's block of 32 columns, of
- * any token that the row or those beside it see, may be rounded. A score beyond fp32 is infinite: minus infinity weighs
- * nothing, plus infinity makes its row NaN, as does a row of nothing but minus infinity. A NaN in the cache (scale byte
- * 255) reaches the rows that see it.
+ * the result is rounded to its type once. Values more than 2^30 below the largest of their head's block of 32 columns,
+ * of any token that the row or those beside it see, may be rounded. A score beyond fp32 is infinite: minus infinity
+ * weighs nothing, plus infinity makes its row NaN, as does a row of nothing but minus infinity. A NaN in the cache
+ * (scale byte 255) reaches the rows that see it.
  * workspace: ancha_paged_attention_workspace bytes (of the same arguments; may be 0 and NULL), 16-byte aligned, not
  * shared with a call that may run at the same time. */
 size_t ancha_paged_attention_workspace(int type, size_t rows, size_t heads, const ancha_paged_cache *cache,

@@ -59,8 +59,8 @@ def test_a_nan_is_seen_behind_any_scale(gpu, byte, heads, columns):
 
 def tight(kind, want, size, total, reach, dim, blocks, small=31):
     """What scores in 32 bits, weights in two fp16 parts and one rounding to the type leave: each weight is off by 2^-22
-    of itself, in the products and in the sum that divides them, or by 2^-small of its row's largest. blocks: the largest
-    value of each column's block."""
+    of itself, in the products and in the sum that divides them, or by 2^-small of its row's largest. blocks: the
+    largest value of each column's block."""
     e = (dim // 32 * PARTS[kind] + 4) * 2.0 ** -22 * reach
     tol = size * (2 * e + 2.0 ** -20) + np.abs(want) * 2.0 ** -21 + rounding(want, TYPES[kind])
     return tol + total * 2.0 ** -small + blocks * 2.0 ** -32
@@ -68,7 +68,8 @@ def tight(kind, want, size, total, reach, dim, blocks, small=31):
 
 @pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("dim,fmt", [(64, "fp8"), (64, "fp4"), (128, "fp8"), (128, "fp4"), (256, "fp8"), (256, "fp4")])
-@pytest.mark.parametrize("new,lengths,heads,columns", [([1, 1, 1], [300, 17, 2100], 8, None), ([3, 1], [700, 90], 6, 600),
+@pytest.mark.parametrize("new,lengths,heads,columns", [([1, 1, 1], [300, 17, 2100], 8, None),
+                                                       ([3, 1], [700, 90], 6, 600),
                                                        ([100, 130], [300, 130], 20, 2000)])
 def test_results_are_rounded_once(gpu, new, lengths, heads, columns, dim, fmt, kind):
     """Whatever the kernel: nothing but the result's type rounds to fewer than 22 bits."""
@@ -148,7 +149,7 @@ def test_queries_up_to_the_largest_number(gpu, heads, columns):
 @pytest.mark.parametrize("heads,columns", [(4, None), (4, 600), (40, 9000)])
 @pytest.mark.parametrize("first,last", [(0, 1024), (700, 1500), (0, 33)])
 def test_scores_below_every_number(gpu, first, last, heads, columns, kind):
-    """Keys whose scores pass fp32 to minus infinity have no weight, also where some waves or workgroups have no other."""
+    """Keys whose scores pass fp32 to minus infinity have no weight, also where waves or workgroups have no other."""
     cache, codes, scales = some_cache(gpu, 110, 16, 2, 64, "fp8", 251, big=0.0)
     batch, plain, rows = some_batch(gpu, [20], [1600], 16, 110, 252, columns=columns)
     codes[0] &= 0x7f
@@ -198,7 +199,7 @@ def test_a_nan_in_a_query_is_its_rows_alone(gpu, heads, columns, dim, kind):
 @pytest.mark.parametrize("layout", ["half", "interleaved"])
 def test_write_turns_by_angles_up_to_the_limit(gpu, layout):
     """Positions up to 2^31 - 1 and frequencies up to 2^20: the oracle's codes."""
-    freqs = [2.0 ** 20, -2.0 ** 20 + 0.5, 1e6 / 3, 2.0 ** 17 + 0.1, 2.0 ** 16 - 0.7, 777.7, 1.0, np.pi / 2, 1e-3, 2.0 ** -31]
+    freqs = [2.0 ** 20, -2.0 ** 20 + 0.5, 1e6 / 3, 2.0 ** 17 + 0.1, 2.0 ** 16 - 0.7, 777.7, 1.0, np.pi / 2, 1e-3]
     plan = paged.Rotary(torch.tensor(freqs, dtype=torch.float64, device=gpu), layout)
     page = 65536
     for length in (2 ** 31 - 1, 2 ** 30 + 12345, 2 ** 28 + 7):
