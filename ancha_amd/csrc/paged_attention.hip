@@ -498,8 +498,8 @@ AttentionForm attention_form(const AttentionParams& p) {
   // us, of 16 rows 74 / 85, 8 of 128 rows over 1024 85 / 56, of 64 46 / 41, of 32 30 / 33; one of 64 over 8192 43 /
   // 41, of 128 over 1024 16 / 32. In fp32, 8 heads of 64, 8 sequences: 128 rows over 8192 98 / 71, 64 rows 52 / 59.
   // Between, 32 rows over 8192 in bf16, half a chunk, would be faster in chunks, 131 / 97, where half a chunk of fp32
-  // is not. `keys` is what the table has room for: 128 rows over 1024 keys take 17 us, but 34 with a table for 131
-  // 072. Heads of 256 columns have no chunks: three buffers of 64 of their keys and values are 192 KiB of LDS.
+  // is not. `keys` is what the table has room for: 128 rows over 1024 keys take 17 us, but 34 with a table for 2^17.
+  // Heads of 256 columns have no chunks: three buffers of 64 of their keys and values are 192 KiB of LDS.
   const int high = p.cache.dim < 256 ? chunk_rows(p.cache.dim, p.type) : 0;
   const bool chunk = high && 4 * rows >= 3 * high * some && rows * p.cache.heads >= (1l << 24) / max(keys, 1l);
   const int of = chunk ? high : kTile;
